@@ -100,7 +100,8 @@ def draw(rng):
         kept = rng.randint(1, groups)
         K = rng.randint(1, min(16, kept * (E // groups)))
         return _route(_log_int(rng, 1, 16384), E, K, groups, kept, rng.choice(["sigmoid", "softmax"]),
-                      rng.choice(["top2", "max"]), bias=rng.random() < 0.6, renorm=rng.random() < 0.6,
+                      rng.choice(["top2", "max"]), bias=rng.random() < 0.6,
+                      renorm=K > 1 and rng.random() < 0.6,  # a single renormalised weight is 1, without a gradient
                       scale=rng.choice([1.0, 2.5]), logits=rng.choice(["fp32", "bf16"]), train=rng.random() < 0.4)
     if kind in ("norm", "combine"):
         o = dict(gate=rng.choice(["none", "token", "channel", "full"]), act=rng.choice(["identity", "sigmoid"]),
