@@ -168,6 +168,84 @@ int ttamd_router_route(const void* x, const void* w_router,
                        void* gemm_plan, size_t gemm_plan_bytes,
                        void* workspace, size_t workspace_bytes, void* stream);
 
+/* Value of a group of experts in the group-limited selection: the sum of its
+ * two largest selection values, or its largest one. */
+enum { TTAMD_GROUP_TOP2 = 0, TTAMD_GROUP_MAX = 1 };
+
+/*
+ * Group-limited router top-k over given logits [T, E] (fp32, or bf16 when
+ * logits_are_bf16).  No counterpart in the reference, whose router picks among
+ * all experts; it stands beside ttamd_router_topk.
+ *   s = softmax(logits) or sigmoid(logits);  v = s + expert_bias (nullable,
+ *   fp32 [E], for the selection only), in 64 bits;
+ *   the experts are num_groups runs of E / num_groups consecutive ids; the
+ *   topk_groups groups of largest value are kept (ties: lower group), a
+ *   group's value being the sum of its min(2, E / num_groups) largest v
+ *   (TTAMD_GROUP_TOP2) or its largest v (TTAMD_GROUP_MAX);
+ *   the topk experts of the kept groups with the largest v, descending (ties
+ *   to the lower id; NaN before every number, -inf after every finite value:
+ *   an expert masked with a -inf bias is picked only when the kept groups
+ *   hold too few others).  Values within 2^-42 of each other count as equal;
+ *   logits below -700 count as -700.
+ *   top_scores fp32 [T, topk] = s of the picks; renorm: divided by (their sum
+ *   + renorm_eps); times route_scale.  top_indices int64 [T, topk].
+ * Requires T <= 2^24, E <= 1024, num_groups <= 64 dividing E, 1 <= topk <=
+ * min(16, topk_groups * E / num_groups).
+ */
+int ttamd_router_topk_grouped(const void* logits, int logits_are_bf16,
+                              const float* expert_bias, int64_t num_tokens,
+                              int num_experts, int topk, int num_groups,
+                              int topk_groups, int group_score, int score_func,
+                              int renorm, float renorm_eps, float route_scale,
+                              float* top_scores, int64_t* top_indices,
+                              void* stream);
+
+/*
+ * Gradient of the routing weights of ttamd_router_topk and
+ * ttamd_router_topk_grouped with respect to the logits (the selection has
+ * none, so groups and bias do not enter):
+ *   ds as in ttamd_router_backward; softmax: dz = s * (ds - <ds, s>);
+ *   sigmoid: dz = ds * s * (1 - s), for every expert.
+ * grad_top_scores fp32 [T, K], top_indices int64 [T, K] (an index outside
+ * [0, E) contributes nothing), logits as given to the forward; grad_logits
+ * [T, E] in the logits' type.  1 <= K <= min(16, E), E <= 1024, T <= 2^24.
+ */
+int ttamd_router_topk_backward(const float* grad_top_scores,
+                               const int64_t* top_indices, const void* logits,
+                               int logits_are_bf16, int64_t num_tokens,
+                               int num_experts, int topk, int score_func,
+                               int renorm, float renorm_eps, float route_scale,
+                               void* grad_logits, void* stream);
+
+/*
+ * ttamd_router_fused and ttamd_router_route with the selection of
+ * ttamd_router_topk_grouped on the bf16 logits; every other argument, output,
+ * limit (E <= 256) and workspace as there.  ttamd_router_backward is the
+ * backward of both.
+ */
+int ttamd_router_fused_grouped(const void* x, const void* w_router,
+                               const float* expert_bias, int64_t num_tokens,
+                               int num_experts, int64_t dim, int topk,
+                               int num_groups, int topk_groups,
+                               int group_score, int score_func, int renorm,
+                               float renorm_eps, float route_scale,
+                               float* top_scores, int64_t* top_indices,
+                               void* logits_out, void* workspace,
+                               size_t workspace_bytes, void* stream);
+int ttamd_router_route_grouped(const void* x, const void* w_router,
+                               const float* expert_bias, int64_t num_tokens,
+                               int num_experts, int64_t dim, int topk,
+                               int num_groups, int topk_groups,
+                               int group_score, int score_func, int renorm,
+                               float renorm_eps, float route_scale,
+                               float* top_scores, int64_t* top_indices,
+                               int32_t* counts, int32_t* offsets,
+                               int32_t* sorted_indices, int32_t* inverse,
+                               float* sorted_scores, float* tokens_per_expert,
+                               void* gemm_plan, size_t gemm_plan_bytes,
+                               void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 /* Bytes of device workspace ttamd_moe_route / ttamd_moe_token_permute need. */
 size_t ttamd_route_workspace_bytes(int64_t num_flat, int num_experts);
 

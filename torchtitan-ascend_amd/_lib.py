@@ -47,6 +47,26 @@ SIGNATURES: dict[str, tuple] = {
          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p, _sz,
          _c_void_p],
     ),
+    "ttamd_router_topk_grouped": (
+        _i32,
+        [_c_void_p, _i32, _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _f32, _c_void_p,
+         _c_void_p, _c_void_p],
+    ),
+    "ttamd_router_topk_backward": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _f32, _c_void_p, _c_void_p],
+    ),
+    "ttamd_router_fused_grouped": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _f32,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p],
+    ),
+    "ttamd_router_route_grouped": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _f32,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz,
+         _c_void_p, _sz, _c_void_p],
+    ),
     "ttamd_route_workspace_bytes": (_sz, [_i64, _i32]),
     "ttamd_moe_route": (
         _i32,

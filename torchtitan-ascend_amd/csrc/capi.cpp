@@ -88,6 +88,92 @@ int check_ws(const char* fn, const void* ws, size_t have, size_t need) {
     if (_rc != TTAMD_OK) return _rc; \
   } while (0)
 
+// Group-limited selection: equal groups, enough experts in the kept ones.
+int check_groups(const char* fn, int E, int K, int groups, int kept, int group_score) {
+  REQUIRE(E >= 1 && groups >= 1 && groups <= 64 && E % groups == 0,
+          "%s: num_groups must be in [1, 64] and divide num_experts (%d groups, %d experts)", fn, groups, E);
+  REQUIRE(kept >= 1 && kept <= groups, "%s: topk_groups must be in [1, num_groups] (got %d)", fn, kept);
+  REQUIRE(K >= 1 && K <= 16 && K <= kept * (E / groups),
+          "%s: topk must be in [1, min(16, topk_groups * E / num_groups)] (got %d)", fn, K);
+  REQUIRE(group_score == TTAMD_GROUP_TOP2 || group_score == TTAMD_GROUP_MAX, "%s: unknown group_score %d", fn,
+          group_score);
+  return TTAMD_OK;
+}
+
+// The gate GEMM + selection of the plain and the grouped entry point.
+int router_fused(const char* fn, const ttamd::RouterGroups* groups, const void* x, const void* w_router, const float* expert_bias,
+                       int64_t num_tokens, int num_experts, int64_t dim, int topk, int score_func,
+                       int renorm, float renorm_eps, float route_scale, float* top_scores,
+                       int64_t* top_indices, void* logits_out, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  REQUIRE(num_tokens >= 0 && num_tokens <= (1 << 24), "%s: num_tokens out of range", fn);
+  REQUIRE(num_experts >= 1 && num_experts <= 256, "%s: num_experts must be in [1, 256]", fn);
+  REQUIRE(topk >= 1 && topk <= 16 && topk <= num_experts, "%s: topk must be in [1, min(16, E)]",
+          fn);
+  REQUIRE(score_func == TTAMD_SCORE_SOFTMAX || score_func == TTAMD_SCORE_SIGMOID,
+          "%s: unknown score_func %d", fn, score_func);
+  REQUIRE(dim >= 64 && dim % 64 == 0 && dim <= (1 << 20), "%s: dim must be a positive multiple of 64",
+          fn);
+  REQUIRE((int64_t)num_experts * dim * 2 < kI32Max && 128 * dim * 2 < kI32Max,
+          "%s: router weight too large", fn);
+  if (num_tokens == 0) return TTAMD_OK;
+  REQUIRE(x && w_router && top_scores && top_indices, "%s: null pointer argument", fn);
+  REQUIRE(aligned16(x) && aligned16(w_router), "%s: x and w_router must be 16-byte aligned", fn);
+  TRY(check_ws(fn, workspace, workspace_bytes, ttamd::router_workspace_bytes(num_tokens, num_experts, dim)));
+  return check_hip(ttamd::launch_router_fused(x, w_router, expert_bias, (int)num_tokens, num_experts,
+                                              (int)dim, topk, score_func, renorm, renorm_eps,
+                                              route_scale, top_scores, top_indices, logits_out, workspace,
+                                              (hipStream_t)stream, groups),
+                   fn);
+}
+
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// The same followed by the dispatch order.
+int router_route(const char* fn, const ttamd::RouterGroups* groups, const void* x, const void* w_router, const float* expert_bias, int64_t num_tokens,
+                       int num_experts, int64_t dim, int topk, int score_func, int renorm, float renorm_eps,
+                       float route_scale, float* top_scores, int64_t* top_indices, int32_t* counts,
+                       int32_t* offsets, int32_t* sorted_indices, int32_t* inverse, float* sorted_scores,
+                       float* tokens_per_expert, void* gemm_plan, size_t gemm_plan_bytes, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  REQUIRE(num_tokens >= 0 && num_tokens <= (1 << 24), "%s: num_tokens out of range", fn);
+  REQUIRE(num_experts >= 1 && num_experts <= 256, "%s: num_experts must be in [1, 256]", fn);
+  REQUIRE(topk >= 1 && topk <= 16 && topk <= num_experts, "%s: topk must be in [1, min(16, E)]", fn);
+  REQUIRE(score_func == TTAMD_SCORE_SOFTMAX || score_func == TTAMD_SCORE_SIGMOID,
+          "%s: unknown score_func %d", fn, score_func);
+  REQUIRE(dim >= 64 && dim % 64 == 0 && dim <= (1 << 20), "%s: dim must be a positive multiple of 64", fn);
+  REQUIRE((int64_t)num_experts * dim * 2 < kI32Max && 128 * dim * 2 < kI32Max, "%s: router weight too large",
+          fn);
+  const int64_t M = num_tokens * topk;
+  REQUIRE(M <= (1 << 28), "%s: too many routed rows", fn);
+  REQUIRE(num_tokens == 0 || (x && w_router && top_scores && top_indices && sorted_indices),
+          "%s: null pointer argument", fn);
+  REQUIRE(w_router != nullptr, "%s: w_router is null", fn);
+  REQUIRE(aligned16(x) && aligned16(w_router), "%s: x and w_router must be 16-byte aligned", fn);
+  // the tile table is built from the offsets, the accumulator from the
+  // counts (on every scan path), so both buffers must be given with them
+  REQUIRE((gemm_plan == nullptr && tokens_per_expert == nullptr) || (counts && offsets),
+          "%s: gemm_plan and tokens_per_expert need the counts and offsets buffers", fn);
+  const size_t rbytes = align256(ttamd::router_workspace_bytes(num_tokens, num_experts, dim));
+  TRY(check_ws(fn, workspace, workspace_bytes, ::ttamd_router_route_workspace_bytes(num_tokens, num_experts, dim, topk)));
+  if (gemm_plan) {
+    REQUIRE(aligned16(gemm_plan), "%s: gemm_plan must be 16-byte aligned", fn);
+    REQUIRE(gemm_plan_bytes >= ttamd::gemm_plan_bytes(M, num_experts),
+            "%s: gemm_plan too small (%zu bytes, need %zu)", fn, gemm_plan_bytes,
+            ttamd::gemm_plan_bytes(M, num_experts));
+  }
+  hipStream_t s = (hipStream_t)stream;
+  int* hist = (int*)((char*)workspace + rbytes);
+  TRY(check_hip(ttamd::launch_router_hist(x, w_router, expert_bias, (int)num_tokens, num_experts, (int)dim, topk,
+                                          score_func, renorm, renorm_eps, route_scale, top_scores, top_indices,
+                                          nullptr, workspace, hist, s, groups),
+                fn));
+  return check_hip(ttamd::launch_route_from_hist(top_indices, true, (int)M, num_experts, top_scores, counts, offsets,
+                                                 sorted_indices, inverse, sorted_scores, hist, tokens_per_expert,
+                                                 gemm_plan, ttamd::gemm_fwd_tile_rows(), s),
+                   fn);
+}
+
 }  // namespace
 
 extern "C" {
@@ -121,30 +207,61 @@ size_t ttamd_router_workspace_bytes(int64_t num_tokens, int num_experts, int64_t
   return ttamd::router_workspace_bytes(num_tokens, num_experts, dim);
 }
 
-int ttamd_router_fused(const void* x, const void* w_router, const float* expert_bias,
-                       int64_t num_tokens, int num_experts, int64_t dim, int topk, int score_func,
-                       int renorm, float renorm_eps, float route_scale, float* top_scores,
-                       int64_t* top_indices, void* logits_out, void* workspace, size_t workspace_bytes,
-                       void* stream) {
-  const char* fn = "ttamd_router_fused";
+int ttamd_router_fused(const void* x, const void* w_router, const float* expert_bias, int64_t num_tokens,
+                       int num_experts, int64_t dim, int topk, int score_func, int renorm, float renorm_eps,
+                       float route_scale, float* top_scores, int64_t* top_indices, void* logits_out, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  return router_fused("ttamd_router_fused", nullptr, x, w_router, expert_bias, num_tokens, num_experts, dim, topk,
+                      score_func, renorm, renorm_eps, route_scale, top_scores, top_indices, logits_out, workspace,
+                      workspace_bytes, stream);
+}
+
+int ttamd_router_fused_grouped(const void* x, const void* w_router, const float* expert_bias, int64_t num_tokens,
+                               int num_experts, int64_t dim, int topk, int num_groups, int topk_groups,
+                               int group_score, int score_func, int renorm, float renorm_eps, float route_scale,
+                               float* top_scores, int64_t* top_indices, void* logits_out, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  const char* fn = "ttamd_router_fused_grouped";
+  TRY(check_groups(fn, num_experts, topk, num_groups, topk_groups, group_score));
+  const ttamd::RouterGroups g = {num_groups, topk_groups, group_score == TTAMD_GROUP_TOP2};
+  return router_fused(fn, &g, x, w_router, expert_bias, num_tokens, num_experts, dim, topk, score_func, renorm,
+                      renorm_eps, route_scale, top_scores, top_indices, logits_out, workspace, workspace_bytes,
+                      stream);
+}
+
+int ttamd_router_topk_grouped(const void* logits, int logits_are_bf16, const float* expert_bias, int64_t num_tokens,
+                              int num_experts, int topk, int num_groups, int topk_groups, int group_score,
+                              int score_func, int renorm, float renorm_eps, float route_scale, float* top_scores,
+                              int64_t* top_indices, void* stream) {
+  const char* fn = "ttamd_router_topk_grouped";
   REQUIRE(num_tokens >= 0 && num_tokens <= (1 << 24), "%s: num_tokens out of range", fn);
-  REQUIRE(num_experts >= 1 && num_experts <= 256, "%s: num_experts must be in [1, 256]", fn);
-  REQUIRE(topk >= 1 && topk <= 16 && topk <= num_experts, "%s: topk must be in [1, min(16, E)]",
-          fn);
-  REQUIRE(score_func == TTAMD_SCORE_SOFTMAX || score_func == TTAMD_SCORE_SIGMOID,
-          "%s: unknown score_func %d", fn, score_func);
-  REQUIRE(dim >= 64 && dim % 64 == 0 && dim <= (1 << 20), "%s: dim must be a positive multiple of 64",
-          fn);
-  REQUIRE((int64_t)num_experts * dim * 2 < kI32Max && 128 * dim * 2 < kI32Max,
-          "%s: router weight too large", fn);
+  REQUIRE(num_experts >= 1 && num_experts <= 1024, "%s: num_experts must be in [1, 1024]", fn);
+  TRY(check_groups(fn, num_experts, topk, num_groups, topk_groups, group_score));
+  REQUIRE(score_func == TTAMD_SCORE_SOFTMAX || score_func == TTAMD_SCORE_SIGMOID, "%s: unknown score_func %d", fn,
+          score_func);
   if (num_tokens == 0) return TTAMD_OK;
-  REQUIRE(x && w_router && top_scores && top_indices, "%s: null pointer argument", fn);
-  REQUIRE(aligned16(x) && aligned16(w_router), "%s: x and w_router must be 16-byte aligned", fn);
-  TRY(check_ws(fn, workspace, workspace_bytes, ttamd::router_workspace_bytes(num_tokens, num_experts, dim)));
-  return check_hip(ttamd::launch_router_fused(x, w_router, expert_bias, (int)num_tokens, num_experts,
-                                              (int)dim, topk, score_func, renorm, renorm_eps,
-                                              route_scale, top_scores, top_indices, logits_out, workspace,
-                                              (hipStream_t)stream),
+  REQUIRE(logits && top_scores && top_indices, "%s: null pointer argument", fn);
+  const ttamd::RouterGroups g = {num_groups, topk_groups, group_score == TTAMD_GROUP_TOP2};
+  return check_hip(ttamd::launch_router_topk_grouped(logits, logits_are_bf16 != 0, expert_bias, (int)num_tokens,
+                                                     num_experts, topk, g, score_func, renorm, renorm_eps,
+                                                     route_scale, top_scores, top_indices, (hipStream_t)stream),
+                   fn);
+}
+
+int ttamd_router_topk_backward(const float* grad_top_scores, const int64_t* top_indices, const void* logits,
+                               int logits_are_bf16, int64_t num_tokens, int num_experts, int topk, int score_func,
+                               int renorm, float renorm_eps, float route_scale, void* grad_logits, void* stream) {
+  const char* fn = "ttamd_router_topk_backward";
+  REQUIRE(num_tokens >= 0 && num_tokens <= (1 << 24), "%s: num_tokens out of range", fn);
+  REQUIRE(num_experts >= 1 && num_experts <= 1024, "%s: num_experts must be in [1, 1024]", fn);
+  REQUIRE(topk >= 1 && topk <= 16 && topk <= num_experts, "%s: topk must be in [1, min(16, E)]", fn);
+  REQUIRE(score_func == TTAMD_SCORE_SOFTMAX || score_func == TTAMD_SCORE_SIGMOID, "%s: unknown score_func %d", fn,
+          score_func);
+  if (num_tokens == 0) return TTAMD_OK;
+  REQUIRE(grad_top_scores && top_indices && logits && grad_logits, "%s: null pointer argument", fn);
+  return check_hip(ttamd::launch_router_topk_backward(grad_top_scores, top_indices, logits, logits_are_bf16 != 0,
+                                                      (int)num_tokens, num_experts, topk, score_func, renorm,
+                                                      renorm_eps, route_scale, grad_logits, (hipStream_t)stream),
                    fn);
 }
 
@@ -237,8 +354,6 @@ int ttamd_router_backward(const float* grad_top_scores, const int64_t* top_indic
                    fn);
 }
 
-static size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
-
 size_t ttamd_router_route_workspace_bytes(int64_t num_tokens, int num_experts, int64_t dim, int topk) {
   if (num_tokens < 0 || num_experts < 1 || dim < 64 || topk < 1) return 0;
   return align256(ttamd::router_workspace_bytes(num_tokens, num_experts, dim)) +
@@ -251,43 +366,26 @@ int ttamd_router_route(const void* x, const void* w_router, const float* expert_
                        int32_t* offsets, int32_t* sorted_indices, int32_t* inverse, float* sorted_scores,
                        float* tokens_per_expert, void* gemm_plan, size_t gemm_plan_bytes, void* workspace,
                        size_t workspace_bytes, void* stream) {
-  const char* fn = "ttamd_router_route";
-  REQUIRE(num_tokens >= 0 && num_tokens <= (1 << 24), "%s: num_tokens out of range", fn);
-  REQUIRE(num_experts >= 1 && num_experts <= 256, "%s: num_experts must be in [1, 256]", fn);
-  REQUIRE(topk >= 1 && topk <= 16 && topk <= num_experts, "%s: topk must be in [1, min(16, E)]", fn);
-  REQUIRE(score_func == TTAMD_SCORE_SOFTMAX || score_func == TTAMD_SCORE_SIGMOID,
-          "%s: unknown score_func %d", fn, score_func);
-  REQUIRE(dim >= 64 && dim % 64 == 0 && dim <= (1 << 20), "%s: dim must be a positive multiple of 64", fn);
-  REQUIRE((int64_t)num_experts * dim * 2 < kI32Max && 128 * dim * 2 < kI32Max, "%s: router weight too large",
-          fn);
-  const int64_t M = num_tokens * topk;
-  REQUIRE(M <= (1 << 28), "%s: too many routed rows", fn);
-  REQUIRE(num_tokens == 0 || (x && w_router && top_scores && top_indices && sorted_indices),
-          "%s: null pointer argument", fn);
-  REQUIRE(w_router != nullptr, "%s: w_router is null", fn);
-  REQUIRE(aligned16(x) && aligned16(w_router), "%s: x and w_router must be 16-byte aligned", fn);
-  // the tile table is built from the offsets, the accumulator from the
-  // counts (on every scan path), so both buffers must be given with them
-  REQUIRE((gemm_plan == nullptr && tokens_per_expert == nullptr) || (counts && offsets),
-          "%s: gemm_plan and tokens_per_expert need the counts and offsets buffers", fn);
-  const size_t rbytes = align256(ttamd::router_workspace_bytes(num_tokens, num_experts, dim));
-  TRY(check_ws(fn, workspace, workspace_bytes, ttamd_router_route_workspace_bytes(num_tokens, num_experts, dim, topk)));
-  if (gemm_plan) {
-    REQUIRE(aligned16(gemm_plan), "%s: gemm_plan must be 16-byte aligned", fn);
-    REQUIRE(gemm_plan_bytes >= ttamd::gemm_plan_bytes(M, num_experts),
-            "%s: gemm_plan too small (%zu bytes, need %zu)", fn, gemm_plan_bytes,
-            ttamd::gemm_plan_bytes(M, num_experts));
-  }
-  hipStream_t s = (hipStream_t)stream;
-  int* hist = (int*)((char*)workspace + rbytes);
-  TRY(check_hip(ttamd::launch_router_hist(x, w_router, expert_bias, (int)num_tokens, num_experts, (int)dim, topk,
-                                          score_func, renorm, renorm_eps, route_scale, top_scores, top_indices,
-                                          nullptr, workspace, hist, s),
-                fn));
-  return check_hip(ttamd::launch_route_from_hist(top_indices, true, (int)M, num_experts, top_scores, counts, offsets,
-                                                 sorted_indices, inverse, sorted_scores, hist, tokens_per_expert,
-                                                 gemm_plan, ttamd::gemm_fwd_tile_rows(), s),
-                   fn);
+  return router_route("ttamd_router_route", nullptr, x, w_router, expert_bias, num_tokens, num_experts, dim, topk,
+                      score_func, renorm, renorm_eps, route_scale, top_scores, top_indices, counts, offsets,
+                      sorted_indices, inverse, sorted_scores, tokens_per_expert, gemm_plan, gemm_plan_bytes,
+                      workspace, workspace_bytes, stream);
+}
+
+int ttamd_router_route_grouped(const void* x, const void* w_router, const float* expert_bias, int64_t num_tokens,
+                               int num_experts, int64_t dim, int topk, int num_groups, int topk_groups,
+                               int group_score, int score_func, int renorm, float renorm_eps, float route_scale,
+                               float* top_scores, int64_t* top_indices, int32_t* counts, int32_t* offsets,
+                               int32_t* sorted_indices, int32_t* inverse, float* sorted_scores,
+                               float* tokens_per_expert, void* gemm_plan, size_t gemm_plan_bytes, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  const char* fn = "ttamd_router_route_grouped";
+  TRY(check_groups(fn, num_experts, topk, num_groups, topk_groups, group_score));
+  const ttamd::RouterGroups g = {num_groups, topk_groups, group_score == TTAMD_GROUP_TOP2};
+  return router_route(fn, &g, x, w_router, expert_bias, num_tokens, num_experts, dim, topk, score_func, renorm,
+                      renorm_eps, route_scale, top_scores, top_indices, counts, offsets, sorted_indices, inverse,
+                      sorted_scores, tokens_per_expert, gemm_plan, gemm_plan_bytes, workspace, workspace_bytes,
+                      stream);
 }
 
 size_t ttamd_moe_experts_forward_workspace_bytes(int64_t num_tokens, int64_t dim, int64_t hidden,

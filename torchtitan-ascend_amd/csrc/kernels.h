@@ -54,19 +54,40 @@ hipError_t launch_router_topk(const float* logits, const float* bias, int T, int
                               int score_func, int renorm, float renorm_eps, float route_scale,
                               float* top_scores, int64_t* top_idx, hipStream_t stream);
 
+// Group-limited selection (router_group.hip): experts in `groups` equal runs,
+// `kept` of them eligible, a group's value the sum of its two largest
+// selection values (top2) or its largest.
+struct RouterGroups {
+  int groups, kept, top2;
+};
+
 // router.hip
 size_t router_workspace_bytes(int64_t T, int E, int64_t D);
 hipError_t launch_router_fused(const void* x, const void* w, const float* bias, int T, int E, int D, int K,
                                int score_func, int renorm, float renorm_eps, float route_scale,
                                float* top_scores, int64_t* top_idx, void* logits, void* ws,
-                               hipStream_t stream);
+                               hipStream_t stream, const RouterGroups* groups = nullptr);
 // The same router, also accumulating the route histogram of the picks into
 // `hist` ((E + 1) * route_num_chunks(T * K) ints, cleared by the gate GEMM
 // kernel first), ready for launch_route_from_hist.
 hipError_t launch_router_hist(const void* x, const void* w, const float* bias, int T, int E, int D, int K,
                               int score_func, int renorm, float renorm_eps, float route_scale,
                               float* top_scores, int64_t* top_idx, void* logits, void* ws, int* hist,
-                              hipStream_t stream);
+                              hipStream_t stream, const RouterGroups* groups = nullptr);
+
+// Group-limited selection (router_group.hip).
+hipError_t launch_router_topk_grouped(const void* logits, bool bf16, const float* bias, int T, int E, int K,
+                                      const RouterGroups& g, int score_func, int renorm, float renorm_eps,
+                                      float route_scale, float* top_scores, int64_t* top_idx, hipStream_t stream);
+// The same on the gate GEMM's partial logits [S][T][E] (E <= 256).
+hipError_t launch_group_topk_partials(const float* part, int S, const float* bias, int T, int E, int K,
+                                      const RouterGroups& g, int score_func, int renorm, float renorm_eps,
+                                      float route_scale, float* top_scores, int64_t* top_idx, void* logits, int* hist,
+                                      int nchunks, int chunk, hipStream_t stream);
+// d(top_scores) [T, K] -> d(logits) [T, E] in the logits' type.
+hipError_t launch_router_topk_backward(const float* grad, const int64_t* idx, const void* logits, bool bf16, int T,
+                                       int E, int K, int score_func, int renorm, float renorm_eps, float route_scale,
+                                       void* grad_logits, hipStream_t stream);
 
 // Router backward: d(top_scores) -> d(logits) -> dx (bf16 [T, D], nullable)
 // and dW_r ([E, D], fp32 or bf16, nullable).

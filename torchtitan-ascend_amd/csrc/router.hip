@@ -561,15 +561,15 @@ size_t router_workspace_bytes(int64_t T, int E, int64_t D) {
 hipError_t launch_router_fused(const void* x, const void* w, const float* bias, int T, int E, int D, int K,
                                int score_func, int renorm, float renorm_eps, float route_scale,
                                float* top_scores, int64_t* top_idx, void* logits, void* ws,
-                               hipStream_t stream) {
+                               hipStream_t stream, const RouterGroups* groups) {
   return launch_router_hist(x, w, bias, T, E, D, K, score_func, renorm, renorm_eps, route_scale, top_scores,
-                            top_idx, logits, ws, nullptr, stream);
+                            top_idx, logits, ws, nullptr, stream, groups);
 }
 
 hipError_t launch_router_hist(const void* x, const void* w, const float* bias, int T, int E, int D, int K,
                               int score_func, int renorm, float renorm_eps, float route_scale,
                               float* top_scores, int64_t* top_idx, void* logits, void* ws, int* hist,
-                              hipStream_t stream) {
+                              hipStream_t stream, const RouterGroups* groups) {
   if (T == 0) return hipSuccess;
   const int S = router_splits(T, D);
   RouterGemmArgs g;
@@ -590,6 +590,9 @@ hipError_t launch_router_hist(const void* x, const void* w, const float* bias, i
   else if (E <= 128) err = launch_gemm_eb<4>(g, S, stream);
   else err = launch_gemm_eb<8>(g, S, stream);
   if (err != hipSuccess) return err;
+  if (groups)
+    return launch_group_topk_partials(g.part, S, bias, T, E, K, *groups, score_func, renorm, renorm_eps, route_scale,
+                                      top_scores, top_idx, logits, hist, nchunks, route_chunk_labels(), stream);
 
   RouterTopkArgs k;
   k.part = g.part;

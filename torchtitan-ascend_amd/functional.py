@@ -46,15 +46,40 @@ def router(
     route_scale: float = 1.0,
     expert_bias: torch.Tensor | None = None,
     norm_eps: float = 1e-20,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """UPSTREAM TokenChoiceTopKRouter forward: (top_scores fp32 [T, K],
     selected_experts_indices int64 [T, K]).  x [..., D] and w_router [E, D]
     in any float dtype (bf16 inside the op, so their gradients come back in
     their own dtype); differentiable in x and w_router through ttamd::router's
-    registered backward, the expert ids carry no gradient."""
+    registered backward, the expert ids carry no gradient.  num_groups and
+    topk_groups limit a token's experts to its topk_groups best of num_groups
+    equal runs of experts (see ops.router_topk)."""
     xb = x.reshape(-1, x.shape[-1]).to(_BF16).contiguous()
-    scores, idx, _ = _T.router(xb, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps)
+    scores, idx, _ = _T.router(xb, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps,
+                               num_groups, topk_groups, group_score)
     return scores, idx
+
+
+def router_topk(
+    logits: torch.Tensor,
+    top_k: int,
+    score_func: str = "softmax",
+    route_norm: bool = False,
+    route_scale: float = 1.0,
+    expert_bias: torch.Tensor | None = None,
+    norm_eps: float = 1e-20,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The router's selection from given logits [T, E], differentiable in them
+    (models/qwen3_5/model.py:757-765): (top_scores fp32 [T, K],
+    selected_experts_indices int64 [T, K]); arguments as ops.router_topk."""
+    return _T.router_topk(logits, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups,
+                          topk_groups, group_score)
 
 
 def dispatch(x, scores_flat, sorted_indices, inverse, sorted_scores, top_k, score_before):

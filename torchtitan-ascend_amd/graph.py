@@ -47,6 +47,9 @@ class MoELayerGraph:
         expert_bias: torch.Tensor | None = None,
         swiglu_limit: float | None = None,
         warmup: int = 2,
+        num_groups: int | None = None,
+        topk_groups: int | None = None,
+        group_score: str = "top2",
     ):
         if x.dim() != 2 or x.dtype != _BF16:
             raise TypeError("x must be a bf16 [T, D] tensor")
@@ -55,6 +58,7 @@ class MoELayerGraph:
                 raise TypeError(f"{name} must be a contiguous bf16 tensor (read in place by the graph)")
         self._args = (w_router, w13, w2, top_k, score_func, route_norm, score_before_experts, route_scale,
                       expert_bias, swiglu_limit)
+        self._groups = (num_groups, topk_groups, group_score)
         self.static_x = x.detach().clone()
         # warm up on a side stream (first calls set kernel attributes), then capture
         side = torch.cuda.Stream(device=x.device)
@@ -69,7 +73,9 @@ class MoELayerGraph:
 
     def _step(self, x: torch.Tensor) -> torch.Tensor:
         w_router, w13, w2, top_k, func, norm, before, scale, bias, limit = self._args
-        _, _, r = ops.router_route(x, w_router, top_k, func, norm, scale, bias, with_inverse=False)
+        _, _, r = ops.router_route(x, w_router, top_k, func, norm, scale, bias, with_inverse=False,
+                                    num_groups=self._groups[0], topk_groups=self._groups[1],
+                                    group_score=self._groups[2])
         return ops.experts_forward(x, r, w13, w2, top_k, before, limit)
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:

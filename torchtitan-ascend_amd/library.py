@@ -13,6 +13,8 @@ no CPU or eager-torch fallback).
 Reference ops these stand for (torchtitanturbo/models/common/):
   * ttamd::router / router_backward   UPSTREAM TokenChoiceTopKRouter
                                       (closed form qwen3_5/model.py:752-766)
+  * ttamd::router_topk / router_topk_backward
+                                      its selection from given logits (:757-765)
   * ttamd::route                      histc + stable argsort of dispatch
                                       (npu_gmm.py:106-108)
   * ttamd::dispatch (+ backward)      dispatch gather / score-before
@@ -53,16 +55,21 @@ def _bf(w: Tensor) -> Tensor:
 # ---------------------------------------------------------------------------
 @torch.library.custom_op("ttamd::router", mutates_args=())
 def router(x: Tensor, w_router: Tensor, top_k: int, score_func: str, route_norm: bool, route_scale: float,
-           expert_bias: Optional[Tensor], norm_eps: float) -> tuple[Tensor, Tensor, Tensor]:
+           expert_bias: Optional[Tensor], norm_eps: float, num_groups: Optional[int] = None,
+           topk_groups: Optional[int] = None, group_score: str = "top2") -> tuple[Tensor, Tensor, Tensor]:
     """x bf16 [T, D], w_router [E, D] (bf16, or fp32 master weights used in
     bf16 as the gate Linear sees them) -> (top_scores fp32 [T, K],
-    selected_experts_indices int64 [T, K], logits bf16 [T, E])."""
+    selected_experts_indices int64 [T, K], logits bf16 [T, E]).  num_groups
+    and topk_groups limit the picks to groups of experts; the backward does
+    not depend on them."""
     return ops.router_fused(x, _bf(w_router), top_k, score_func, route_norm, route_scale, expert_bias, norm_eps,
-                            return_logits=True)
+                            return_logits=True, num_groups=num_groups, topk_groups=topk_groups,
+                            group_score=group_score)
 
 
 @router.register_fake
-def _(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps):
+def _(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups=None,
+      topk_groups=None, group_score="top2"):
     T, E = x.shape[0], w_router.shape[0]
     return (x.new_empty((T, top_k), dtype=_F32), x.new_empty((T, top_k), dtype=torch.int64),
             x.new_empty((T, E), dtype=_BF16))
@@ -84,8 +91,9 @@ def _(grad_scores, idx, logits, x, w_router, score_func, route_norm, route_scale
 
 
 def _router_setup(ctx, inputs, output):
-    x, w_router, _k, func, norm, scale, _bias, eps = inputs
+    x, w_router, _k, func, norm, scale, _bias, eps = inputs[:8]
     _, idx, logits = output
+    ctx.num_inputs = len(inputs)
     ctx.save_for_backward(x, w_router, idx, logits)
     ctx.cfg = (func, norm, scale, eps)
     # the logits are returned for the backward only: no zero gradient for them
@@ -93,15 +101,65 @@ def _router_setup(ctx, inputs, output):
 
 
 def _router_bwd(ctx, g_scores, _g_idx, _g_logits):
+    rest = (None,) * (ctx.num_inputs - 2)
     if g_scores is None:
-        return None, None, None, None, None, None, None, None
+        return None, None, *rest
     x, w_router, idx, logits = ctx.saved_tensors
     func, norm, scale, eps = ctx.cfg
     dx, dw = router_backward(g_scores.contiguous(), idx, logits, x, w_router, func, norm, scale, eps)
-    return dx, dw, None, None, None, None, None, None
+    return dx, dw, *rest
 
 
 router.register_autograd(_router_bwd, setup_context=_router_setup)
+
+
+@torch.library.custom_op("ttamd::router_topk", mutates_args=())
+def router_topk(logits: Tensor, top_k: int, score_func: str, route_norm: bool, route_scale: float,
+                expert_bias: Optional[Tensor], norm_eps: float, num_groups: Optional[int] = None,
+                topk_groups: Optional[int] = None, group_score: str = "top2") -> tuple[Tensor, Tensor]:
+    """(top_scores fp32 [T, K], selected_experts_indices int64 [T, K]) of given
+    logits [T, E] (fp32 or bf16)."""
+    return ops.router_topk(logits, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups,
+                           topk_groups, group_score)
+
+
+@router_topk.register_fake
+def _(logits, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups=None, topk_groups=None,
+      group_score="top2"):
+    T = logits.shape[0]
+    return logits.new_empty((T, top_k), dtype=_F32), logits.new_empty((T, top_k), dtype=torch.int64)
+
+
+@torch.library.custom_op("ttamd::router_topk_backward", mutates_args=())
+def router_topk_backward(grad_scores: Tensor, idx: Tensor, logits: Tensor, score_func: str, route_norm: bool,
+                         route_scale: float, norm_eps: float) -> Tensor:
+    """d(logits) [T, E] in the logits' type from d(top_scores) [T, K]."""
+    return ops.router_topk_backward(grad_scores, idx, logits, score_func, route_norm, route_scale,
+                                    norm_eps).to(logits.dtype)
+
+
+@router_topk_backward.register_fake
+def _(grad_scores, idx, logits, score_func, route_norm, route_scale, norm_eps):
+    return logits.new_empty(logits.shape)
+
+
+def _router_topk_setup(ctx, inputs, output):
+    logits, _k, func, norm, scale, _bias, eps = inputs[:7]
+    ctx.save_for_backward(logits, output[1])
+    ctx.cfg = (func, norm, scale, eps)
+    ctx.num_inputs = len(inputs)
+    ctx.set_materialize_grads(False)
+
+
+def _router_topk_bwd(ctx, g_scores, _g_idx):
+    rest = (None,) * (ctx.num_inputs - 1)
+    if g_scores is None:
+        return None, *rest
+    logits, idx = ctx.saved_tensors
+    return router_topk_backward(g_scores, idx, logits, *ctx.cfg), *rest
+
+
+router_topk.register_autograd(_router_topk_bwd, setup_context=_router_topk_setup)
 
 
 # ---------------------------------------------------------------------------

@@ -73,9 +73,35 @@ def _limit(swiglu_limit: float | None) -> float:
     return float(swiglu_limit)
 
 
+def _call(dev: torch.device, name: str, *args) -> None:
+    """_lib.call with `dev` as the current device: a kernel launches on the
+    device of its tensors whichever device is current."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        _lib.call(name, *args)
+        return
+    with torch.cuda.device(dev):
+        _lib.call(name, *args)
+
+
 # ---------------------------------------------------------------------------
 # Routing
 # ---------------------------------------------------------------------------
+_SCORE_FUNCS = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORES = {"top2": 0, "max": 1}
+
+
+def _groups(num_groups: int | None, topk_groups: int | None, group_score: str) -> tuple[int, int, int] | None:
+    """(num_groups, topk_groups, group score code) of a group-limited router,
+    None without groups."""
+    if num_groups is None and topk_groups is None:
+        return None
+    if num_groups is None or topk_groups is None:
+        raise ValueError("give num_groups and topk_groups together")
+    if group_score not in _GROUP_SCORES:
+        raise ValueError(f"group_score must be one of {sorted(_GROUP_SCORES)}")
+    return int(num_groups), int(topk_groups), _GROUP_SCORES[group_score]
+
+
 @dataclass
 class RouteResult:
     """Output of `route`: histogram, group offsets and the stable order."""
@@ -103,21 +129,32 @@ def router_topk(
     route_scale: float = 1.0,
     expert_bias: torch.Tensor | None = None,
     norm_eps: float = 1e-20,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Top-k selection of the router (upstream TokenChoiceTopKRouter; in-reference
     closed form torchtitanturbo/models/qwen3_5/model.py:757-765).
 
     Returns (top_scores fp32 [T, K], selected_experts_indices int64 [T, K]),
     sorted by descending score, ties broken towards the lower expert id.
+
+    num_groups and topk_groups limit the picks to the experts of the
+    topk_groups best of num_groups equal runs of experts (group_score: a
+    group's value is the sum of its two largest selection values, "top2", or
+    its largest, "max"); scores and selection are then 64-bit and bf16 logits
+    are read as they are (ttamd_router_topk_grouped).  No autograd here: see
+    functional.router_topk, router_topk_backward.
     """
     dev = _gpu("logits", logits)
     if logits.dim() != 2:
         raise ValueError("logits must be [T, E]")
-    logits = logits.float().contiguous()
+    groups = _groups(num_groups, topk_groups, group_score)
+    bf16 = groups is not None and logits.dtype == _BF16
+    logits = logits.contiguous() if bf16 else logits.float().contiguous()
     T, E = logits.shape
-    funcs = {"softmax": 0, "sigmoid": 1}
-    if score_func not in funcs:
-        raise ValueError(f"score_func must be one of {sorted(funcs)}")
+    if score_func not in _SCORE_FUNCS:
+        raise ValueError(f"score_func must be one of {sorted(_SCORE_FUNCS)}")
     if expert_bias is not None:
         _same_device(dev, expert_bias=expert_bias)
         expert_bias = expert_bias.float().contiguous()
@@ -125,11 +162,53 @@ def router_topk(
             raise ValueError("expert_bias must be [E]")
     scores = torch.empty(T, top_k, dtype=torch.float32, device=dev)
     idx = torch.empty(T, top_k, dtype=torch.int64, device=dev)
+    if groups is not None:
+        _call(
+            dev, "ttamd_router_topk_grouped", _p(logits), int(bf16), _p(expert_bias), T, E, top_k, *groups,
+            _SCORE_FUNCS[score_func], int(bool(route_norm)), float(norm_eps), float(route_scale), _p(scores),
+            _p(idx), _stream(dev),
+        )
+        return scores, idx
     _lib.call(
-        "ttamd_router_topk", _p(logits), _p(expert_bias), T, E, top_k, funcs[score_func],
+        "ttamd_router_topk", _p(logits), _p(expert_bias), T, E, top_k, _SCORE_FUNCS[score_func],
         int(bool(route_norm)), float(norm_eps), float(route_scale), _p(scores), _p(idx), _stream(dev),
     )
     return scores, idx
+
+
+def router_topk_backward(
+    grad_top_scores: torch.Tensor,
+    top_indices: torch.Tensor,
+    logits: torch.Tensor,
+    score_func: str = "softmax",
+    route_norm: bool = False,
+    route_scale: float = 1.0,
+    norm_eps: float = 1e-20,
+) -> torch.Tensor:
+    """d(logits) [T, E] (bf16 for bf16 logits, else fp32) of router_topk's
+    top_scores, with or without groups (ttamd_router_topk_backward): the
+    autograd of score, gather, renorm and scale; the selection has none."""
+    dev = _gpu("logits", logits)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [T, E]")
+    bf16 = logits.dtype == _BF16
+    logits = logits.contiguous() if bf16 else logits.float().contiguous()
+    T, E = logits.shape
+    if score_func not in _SCORE_FUNCS:
+        raise ValueError(f"score_func must be one of {sorted(_SCORE_FUNCS)}")
+    _same_device(dev, grad_top_scores=grad_top_scores, top_indices=top_indices)
+    K = top_indices.shape[-1]
+    if tuple(top_indices.shape) != (T, K) or tuple(grad_top_scores.shape) != (T, K):
+        raise ValueError(f"grad_top_scores and top_indices must be [{T}, K], got {tuple(grad_top_scores.shape)} and "
+                         f"{tuple(top_indices.shape)}")
+    grad = grad_top_scores.float().contiguous()
+    idx = top_indices.to(torch.int64).contiguous()
+    out = torch.empty_like(logits)
+    _call(
+        dev, "ttamd_router_topk_backward", _p(grad), _p(idx), _p(logits), int(bf16), T, E, K,
+        _SCORE_FUNCS[score_func], int(bool(route_norm)), float(norm_eps), float(route_scale), _p(out), _stream(dev),
+    )
+    return out
 
 
 def router_fused(
@@ -142,6 +221,9 @@ def router_fused(
     expert_bias: torch.Tensor | None = None,
     norm_eps: float = 1e-20,
     return_logits: bool = False,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
 ):
     """Gate GEMM + score + top-k in one kernel (upstream TokenChoiceTopKRouter;
     in-reference closed form torchtitanturbo/models/qwen3_5/model.py:752-766).
@@ -149,7 +231,8 @@ def router_fused(
     x bf16 [T, D] (any leading shape), w_router bf16 [E, D].  The logits are
     the bf16 F.linear output; selection as `router_topk` on them.  Returns
     (top_scores fp32 [T, K], selected_experts_indices int64 [T, K]) and, with
-    return_logits, the bf16 logits [T, E] as a third element.
+    return_logits, the bf16 logits [T, E] as a third element.  num_groups and
+    topk_groups limit the picks to groups of experts as in `router_topk`.
     """
     dev = _gpu("x", x)
     x = _want("x", x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), _BF16)
@@ -158,9 +241,9 @@ def router_fused(
     E, D2 = w_router.shape
     if D2 != D:
         raise ValueError(f"w_router must be [E, {D}], got {tuple(w_router.shape)}")
-    funcs = {"softmax": 0, "sigmoid": 1}
-    if score_func not in funcs:
-        raise ValueError(f"score_func must be one of {sorted(funcs)}")
+    if score_func not in _SCORE_FUNCS:
+        raise ValueError(f"score_func must be one of {sorted(_SCORE_FUNCS)}")
+    groups = _groups(num_groups, topk_groups, group_score)
     if expert_bias is not None:
         _same_device(dev, expert_bias=expert_bias)
         expert_bias = expert_bias.float().contiguous()
@@ -170,8 +253,9 @@ def router_fused(
     idx = torch.empty(T, top_k, dtype=torch.int64, device=dev)
     logits = torch.empty(T, E, dtype=_BF16, device=dev) if return_logits else None
     ws = _ws(_lib.load().ttamd_router_workspace_bytes(T, E, D), dev)
-    _lib.call(
-        "ttamd_router_fused", _p(x), _p(w_router), _p(expert_bias), T, E, D, top_k, funcs[score_func],
+    _call(
+        dev, "ttamd_router_fused" if groups is None else "ttamd_router_fused_grouped", _p(x), _p(w_router),
+        _p(expert_bias), T, E, D, top_k, *(groups or ()), _SCORE_FUNCS[score_func],
         int(bool(route_norm)), float(norm_eps), float(route_scale), _p(scores), _p(idx), _p(logits), _p(ws),
         ws.numel(), _stream(dev),
     )
@@ -233,6 +317,9 @@ def router_route(
     norm_eps: float = 1e-20,
     tokens_per_expert: torch.Tensor | None = None,
     with_inverse: bool = True,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
 ) -> tuple[torch.Tensor, torch.Tensor, RouteResult]:
     """Router forward + dispatch order in one C-ABI call (ttamd_router_route):
     the picks of `router_fused`, then the histogram and stable order of
@@ -240,7 +327,8 @@ def router_route(
     tokens_per_expert (fp32 [E], optional) is incremented by the counts, as
     upstream's router.tokens_per_expert buffer is.  Returns (top_scores
     fp32 [T, K], selected_experts_indices int64 [T, K], RouteResult with
-    sorted_scores = top_scores.view(-1)[sorted_indices])."""
+    sorted_scores = top_scores.view(-1)[sorted_indices]).  num_groups and
+    topk_groups limit the picks to groups of experts as in `router_topk`."""
     dev = _gpu("x", x)
     if torch.is_grad_enabled() and (x.requires_grad or w_router.requires_grad):
         raise RuntimeError(
@@ -253,9 +341,9 @@ def router_route(
     E, D2 = w_router.shape
     if D2 != D:
         raise ValueError(f"w_router must be [E, {D}], got {tuple(w_router.shape)}")
-    funcs = {"softmax": 0, "sigmoid": 1}
-    if score_func not in funcs:
-        raise ValueError(f"score_func must be one of {sorted(funcs)}")
+    if score_func not in _SCORE_FUNCS:
+        raise ValueError(f"score_func must be one of {sorted(_SCORE_FUNCS)}")
+    groups = _groups(num_groups, topk_groups, group_score)
     if expert_bias is not None:
         _same_device(dev, expert_bias=expert_bias)
         expert_bias = expert_bias.float().contiguous()
@@ -277,8 +365,9 @@ def router_route(
     sorted_scores = torch.empty(M, dtype=torch.float32, device=dev)
     plan = _ws(lib.ttamd_gemm_plan_bytes(M, E), dev)
     ws = _ws(lib.ttamd_router_route_workspace_bytes(T, E, D, top_k), dev)
-    _lib.call(
-        "ttamd_router_route", _p(x), _p(w_router), _p(expert_bias), T, E, D, top_k, funcs[score_func],
+    _call(
+        dev, "ttamd_router_route" if groups is None else "ttamd_router_route_grouped", _p(x), _p(w_router),
+        _p(expert_bias), T, E, D, top_k, *(groups or ()), _SCORE_FUNCS[score_func],
         int(bool(route_norm)), float(norm_eps), float(route_scale), _p(scores), _p(idx), _p(counts), _p(offsets),
         _p(sorted_idx), _p(inverse), _p(sorted_scores), _p(tokens_per_expert), _p(plan), plan.numel(), _p(ws),
         ws.numel(), _stream(dev),
