@@ -537,6 +537,84 @@ int ttamd_moe_experts_forward(const void* tokens, int64_t num_tokens,
                               void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * Norms before and after the block, with its gate, its residual scale and    *
+ * the combine.  The reference norms with npu_rms_norm and adds the residual  *
+ * in torch (upstream's TransformerBlock); these fuse the passes around the    *
+ * expert stage.                                                               *
+ * ------------------------------------------------------------------------ */
+
+/* What a gate of the block's output is given for. */
+enum {
+  TTAMD_GATE_NONE = 0,
+  TTAMD_GATE_TOKEN = 1,   /* [T]: one value per token */
+  TTAMD_GATE_CHANNEL = 2, /* [D]: one value per channel */
+  TTAMD_GATE_FULL = 3     /* [T, D] */
+};
+
+/* Operands that are fp32 instead of bf16 (ORed). */
+enum {
+  TTAMD_F32_STREAM = 1, /* residual and u (backward: du, dresidual) */
+  TTAMD_F32_POST = 2,   /* post_weight (backward: and its gradient) */
+  TTAMD_F32_GATE = 4,   /* gate (backward: and its gradient) */
+  TTAMD_F32_PRE = 8     /* pre_weight (backward: and its gradient) */
+};
+
+/*
+ * The end of one block and the norm of the next in one pass:
+ *   f[t] = sum_{k<topk} p(t,k) * rows[j(t,k)], j = inverse[t*topk + k]
+ *          (nullable -> t*topk + k; entries outside the rows are clamped to
+ *          them), p = probs[t*topk + k] (fp32, nullable -> 1); topk = 1
+ *          without both: the branch itself
+ *   p[t] = f * rsqrt(mean(f^2) + eps) * post_weight  (nullable -> p = f)
+ *   u[t] = residual + residual_scale * act(gate) * p (residual nullable -> 0;
+ *          act: sigmoid when gate_sigmoid, else the gate itself)
+ *   n[t] = u * rsqrt(mean(u^2) + eps) * pre_weight   (nullable: no n)
+ * rows bf16 [T * topk, D], or NULL: u = residual (a plain RMSNorm of it);
+ * n_out bf16 [T, D]; u_out (nullable) and residual bf16 [T, D], fp32 with
+ * TTAMD_F32_STREAM.  u_out may be the residual itself; no other output may
+ * overlap an input.  rstd_out (nullable) fp32 [2, T] receives the two
+ * reciprocal roots for the backward.  fp32 inside; u and n are each rounded
+ * once, n from the unrounded u.  Deterministic.
+ * D % 8 == 0, D <= 8192; 1 <= topk <= 64; T * topk <= 2^28; pointers to rows
+ * of D elements 16-byte aligned.
+ */
+int ttamd_residual_norm(const void* rows, const int32_t* inverse,
+                        const float* probs, int64_t num_tokens, int64_t dim,
+                        int topk, const void* residual,
+                        const void* post_weight, const void* gate,
+                        int gate_kind, int gate_sigmoid, float residual_scale,
+                        const void* pre_weight, float eps, int f32_mask,
+                        void* u_out, void* n_out, float* rstd_out,
+                        void* stream);
+
+/*
+ * Backward of ttamd_residual_norm with topk = 1 and no inverse or probs (for
+ * topk > 1: combine first, this, then ttamd_moe_token_unpermute_grad):
+ * from du (nullable -> 0) and dn (bf16, nullable -> 0; needs pre_weight) to
+ * the gradients asked for (each nullable).  branch (NULL where the forward
+ * had no rows) and the other inputs as in the forward, rstd the forward's
+ * rstd_out.  grad_branch bf16 [T, D]; grad_residual and du of the stream's
+ * type; grad_post, grad_gate, grad_pre of their inputs' types and shapes,
+ * accumulated in fp32 and rounded once.  Deterministic: the column sums are
+ * added in a fixed order.  workspace:
+ * ttamd_residual_norm_backward_workspace_bytes; contents need no
+ * initialisation.
+ */
+size_t ttamd_residual_norm_backward_workspace_bytes(int64_t num_tokens,
+                                                    int64_t dim);
+int ttamd_residual_norm_backward(const void* du, const void* dn,
+                                 const void* branch, int64_t num_tokens,
+                                 int64_t dim, const void* residual,
+                                 const void* post_weight, const void* gate,
+                                 int gate_kind, int gate_sigmoid,
+                                 float residual_scale, const void* pre_weight,
+                                 const float* rstd, int f32_mask,
+                                 void* grad_branch, void* grad_residual,
+                                 void* grad_post, void* grad_gate,
+                                 void* grad_pre, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
 /* out[t] = sum_{k<topk} in[t*topk + k] (fp32 accumulate, bf16 out). */
 int ttamd_moe_sum_topk(const void* in, int64_t num_tokens, int64_t hidden,
                        int topk, void* out, void* stream);

@@ -132,6 +132,17 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _i64, _i64, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _f32, _c_void_p,
          _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p, _sz, _c_void_p],
     ),
+    "ttamd_residual_norm": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _f32,
+         _c_void_p, _f32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "ttamd_residual_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "ttamd_residual_norm_backward": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _f32, _c_void_p,
+         _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p],
+    ),
     "ttamd_moe_sum_topk": (_i32, [_c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p]),
     "ttamd_shared_expert_add": (
         _i32,

@@ -88,6 +88,33 @@ int check_ws(const char* fn, const void* ws, size_t have, size_t need) {
     if (_rc != TTAMD_OK) return _rc; \
   } while (0)
 
+// Operands shared by ttamd_residual_norm and its backward.
+int norm_args(const char* fn, ttamd::NormArgs& a, const void* rows, int64_t T, int64_t D, int K, const void* residual,
+              const void* post, const void* gate, int gate_kind, int gate_sigmoid, float scale, const void* pre,
+              int f32_mask) {
+  TRY(check_hidden(fn, D));
+  REQUIRE(D <= 8192, "%s: dim must be at most 8192 (got %lld)", fn, (long long)D);
+  REQUIRE(K >= 1 && K <= 64, "%s: topk must be in [1, 64] (got %d)", fn, K);
+  REQUIRE(T >= 0 && T <= (1 << 28) && T * K <= (1 << 28), "%s: num_tokens out of range", fn);
+  REQUIRE(gate_kind >= TTAMD_GATE_NONE && gate_kind <= TTAMD_GATE_FULL, "%s: unknown gate_kind %d", fn, gate_kind);
+  REQUIRE((gate != nullptr) == (gate_kind != TTAMD_GATE_NONE) || T == 0, "%s: gate and gate_kind disagree", fn);
+  REQUIRE(f32_mask >= 0 && f32_mask < 16, "%s: unknown f32_mask %d", fn, f32_mask);
+  REQUIRE(rows || residual || T == 0, "%s: rows and residual are both null", fn);
+  REQUIRE(rows || (!post && !gate) || T == 0, "%s: post_weight and gate need rows", fn);
+  REQUIRE(aligned16(rows) && aligned16(residual) && aligned16(post) && aligned16(pre) &&
+              (gate_kind < TTAMD_GATE_CHANNEL || aligned16(gate)),
+          "%s: operands must be 16-byte aligned", fn);
+  a = {};
+  a.T = (int)T, a.D = (int)D, a.K = K;
+  a.rows = (const uint16_t*)rows;
+  a.residual = residual, a.post = post, a.gate = gate, a.pre = pre;
+  a.gate_kind = gate_kind, a.sigmoid = gate_sigmoid != 0;
+  a.stream32 = (f32_mask & TTAMD_F32_STREAM) != 0, a.post32 = (f32_mask & TTAMD_F32_POST) != 0;
+  a.gate32 = (f32_mask & TTAMD_F32_GATE) != 0, a.pre32 = (f32_mask & TTAMD_F32_PRE) != 0;
+  a.scale = scale;
+  return TTAMD_OK;
+}
+
 // Group-limited selection: equal groups, enough experts in the kept ones.
 int check_groups(const char* fn, int E, int K, int groups, int kept, int group_score) {
   REQUIRE(E >= 1 && groups >= 1 && groups <= 64 && E % groups == 0,
@@ -530,6 +557,57 @@ int ttamd_moe_dispatch_rows(const void* tokens, const int32_t* inverse, const fl
   return check_hip(ttamd::launch_dispatch_rows(tokens, inverse, scores, (int)num_tokens, topk, (int)hidden,
                                                out, (hipStream_t)stream),
                    fn);
+}
+
+int ttamd_residual_norm(const void* rows, const int32_t* inverse, const float* probs, int64_t num_tokens, int64_t dim,
+                        int topk, const void* residual, const void* post_weight, const void* gate, int gate_kind,
+                        int gate_sigmoid, float residual_scale, const void* pre_weight, float eps, int f32_mask,
+                        void* u_out, void* n_out, float* rstd_out, void* stream) {
+  const char* fn = "ttamd_residual_norm";
+  ttamd::NormArgs a;
+  TRY(norm_args(fn, a, rows, num_tokens, dim, topk, residual, post_weight, gate, gate_kind, gate_sigmoid,
+                residual_scale, pre_weight, f32_mask));
+  REQUIRE(eps >= 0.f, "%s: eps must be >= 0", fn);
+  REQUIRE(rows || (!inverse && !probs && topk == 1) || num_tokens == 0, "%s: inverse, probs and topk need rows", fn);
+  REQUIRE(aligned16(u_out) && aligned16(n_out), "%s: outputs must be 16-byte aligned", fn);
+  if (num_tokens == 0) return TTAMD_OK;
+  REQUIRE(u_out || n_out, "%s: no output asked for", fn);
+  REQUIRE((n_out != nullptr) == (pre_weight != nullptr), "%s: n_out and pre_weight go together", fn);
+  a.inverse = inverse, a.probs = probs, a.eps = eps;
+  a.u = u_out, a.n = n_out, a.rstd = rstd_out;
+  return check_hip(ttamd::launch_norm_forward(a, (hipStream_t)stream), fn);
+}
+
+size_t ttamd_residual_norm_backward_workspace_bytes(int64_t num_tokens, int64_t dim) {
+  if (num_tokens <= 0 || dim < 8) return 0;
+  return ttamd::norm_backward_workspace_bytes(num_tokens, dim);
+}
+
+int ttamd_residual_norm_backward(const void* du, const void* dn, const void* branch, int64_t num_tokens, int64_t dim,
+                                 const void* residual, const void* post_weight, const void* gate, int gate_kind,
+                                 int gate_sigmoid, float residual_scale, const void* pre_weight, const float* rstd,
+                                 int f32_mask, void* grad_branch, void* grad_residual, void* grad_post,
+                                 void* grad_gate, void* grad_pre, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  const char* fn = "ttamd_residual_norm_backward";
+  ttamd::NormBwdArgs b = {};
+  TRY(norm_args(fn, b.fwd, branch, num_tokens, dim, 1, residual, post_weight, gate, gate_kind, gate_sigmoid,
+                residual_scale, pre_weight, f32_mask));
+  REQUIRE(dn == nullptr || pre_weight, "%s: dn needs pre_weight", fn);
+  REQUIRE(((!grad_post || post_weight) && (!grad_pre || pre_weight) && (!grad_gate || gate) &&
+           (!grad_branch || branch)) || num_tokens == 0,
+          "%s: a gradient is asked for an operand that is not given", fn);
+  REQUIRE(aligned16(du) && aligned16(dn) && aligned16(grad_branch) && aligned16(grad_residual) &&
+              aligned16(grad_post) && aligned16(grad_pre) && (gate_kind < TTAMD_GATE_CHANNEL || aligned16(grad_gate)),
+          "%s: operands must be 16-byte aligned", fn);
+  if (num_tokens == 0) return TTAMD_OK;
+  REQUIRE(rstd, "%s: rstd is null", fn);
+  TRY(check_ws(fn, workspace, workspace_bytes, ttamd::norm_backward_workspace_bytes(num_tokens, dim)));
+  b.fwd.rstd = const_cast<float*>(rstd);
+  b.du = du, b.dn = dn;
+  b.dbranch = grad_branch, b.dresidual = grad_residual, b.dpost = grad_post, b.dgate = grad_gate, b.dpre = grad_pre;
+  b.part = (float*)workspace;
+  return check_hip(ttamd::launch_norm_backward(b, (hipStream_t)stream), fn);
 }
 
 int ttamd_moe_sum_topk(const void* in, int64_t num_tokens, int64_t hidden, int topk, void* out,

@@ -117,6 +117,31 @@ __device__ __forceinline__ float row16_sum(float v) {
   return v + dpp_f<kDppMirror>(v);
 }
 
+// v as the two 16- (32-) lane halves side by side: after the swap each lane
+// has its own half's value and its partner's, one in x and one in y.
+template <int DIST>
+__device__ __forceinline__ void swap_halves(uint32_t v, uint32_t& x, uint32_t& y) {
+  static_assert(DIST == 16 || DIST == 32, "half of a 32- or 64-lane run");
+  if constexpr (DIST == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    x = r[0], y = r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    x = r[0], y = r[1];
+  }
+}
+
+// Sum over the 64 lanes, in every lane, without LDS: the 16-lane rows, then
+// the two swaps.
+__device__ __forceinline__ float wave64_sum(float v) {
+  uint32_t x, y;
+  v = row16_sum(v);
+  swap_halves<16>(__float_as_uint(v), x, y);
+  v = __uint_as_float(x) + __uint_as_float(y);
+  swap_halves<32>(__float_as_uint(v), x, y);
+  return __uint_as_float(x) + __uint_as_float(y);
+}
+
 // Order-preserving unsigned key of a router selection value: a larger value
 // has a larger key, -inf the smallest of any number, NaN above +inf (the
 // largest key, whatever its sign and payload: torch.topk ranks NaN as the

@@ -97,6 +97,36 @@ hipError_t launch_router_backward(const float* grad, const int64_t* idx, const v
                                   float renorm_eps, float route_scale, void* dx, void* dw, bool dw_fp32,
                                   void* ws, hipStream_t stream);
 
+// block_norm.hip: f = K-way sum of branch rows; p = rmsnorm(f) * post;
+// u = residual + scale * act(gate) * p; n = rmsnorm(u) * pre.
+struct NormArgs {
+  int T, D, K;
+  const uint16_t* rows;   // bf16 [T * K, D], or null: u is the residual
+  const int* inverse;     // [T * K] row of slot t K + k, or null
+  const float* probs;     // [T * K], or null
+  const void* residual;   // [T, D] of the stream's type, or null
+  const void* post;       // [D], or null: p = f
+  const void* gate;       // [T], [D] or [T, D] by gate_kind
+  const void* pre;        // [D], or null: no n
+  int gate_kind;          // 0 none, 1 per token, 2 per channel, 3 per element
+  int sigmoid;            // act: sigmoid, else the gate itself
+  int stream32, post32, gate32, pre32;  // fp32 instead of bf16
+  float scale, eps;
+  void* u;                // [T, D] of the stream's type, or null
+  void* n;                // bf16 [T, D]
+  float* rstd;            // [2, T]: r_f, r_u; or null
+};
+hipError_t launch_norm_forward(const NormArgs& a, hipStream_t stream);
+struct NormBwdArgs {
+  NormArgs fwd;           // K = 1; rstd read; u, n unused
+  const void* du;         // [T, D] of the stream's type, or null: zero
+  const void* dn;         // bf16 [T, D], or null (no pre)
+  void *dbranch, *dresidual, *dpost, *dgate, *dpre;  // each nullable
+  float* part;
+};
+size_t norm_backward_workspace_bytes(int64_t T, int64_t D);
+hipError_t launch_norm_backward(const NormBwdArgs& a, hipStream_t stream);
+
 // gemm.hip
 int gemm_max_qtiles(int M, int E);
 size_t gemm_workspace_bytes(int64_t M, int E);

@@ -115,20 +115,8 @@ __device__ __forceinline__ double dpp_d(double v) {
   return as_f64((uint64_t)hi << 32 | lo);
 }
 
-// The two 16- (32-) lane halves side by side: each lane gets its own value
-// and its partner's, one in each result.
 template <int DIST>
-__device__ __forceinline__ void swap_halves(uint32_t v, uint32_t& x, uint32_t& y) {
-  if constexpr (DIST == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    x = r[0], y = r[1];
-  } else {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    x = r[0], y = r[1];
-  }
-}
-template <int DIST>
-__device__ __forceinline__ void swap_halves(double v, double& x, double& y) {
+__device__ __forceinline__ void swap_halves_d(double v, double& x, double& y) {
   const uint64_t b = as_u64(v);
   uint32_t xl, yl, xh, yh;
   swap_halves<DIST>((uint32_t)b, xl, yl);
@@ -137,9 +125,7 @@ __device__ __forceinline__ void swap_halves(double v, double& x, double& y) {
   y = as_f64((uint64_t)yh << 32 | yl);
 }
 
-// Reductions over the first `run` lanes' exchange steps (run a power of two,
-// uniform): every lane of an aligned run of lanes gets the run's result.
-// STEP(d) combines a lane with a partner in the other half of its 2d lanes.
+// Reductions over a token's LPT lanes; every lane gets the result.
 template <int LPT>
 __device__ __forceinline__ double all_max(double v) {
   v = __builtin_fmax(v, dpp_d<kDppXor1>(v));
@@ -148,9 +134,9 @@ __device__ __forceinline__ double all_max(double v) {
   v = __builtin_fmax(v, dpp_d<kDppMirror>(v));
   if constexpr (LPT == 64) {
     double x, y;
-    swap_halves<16>(v, x, y);
+    swap_halves_d<16>(v, x, y);
     v = __builtin_fmax(x, y);
-    swap_halves<32>(v, x, y);
+    swap_halves_d<32>(v, x, y);
     v = __builtin_fmax(x, y);
   }
   return v;
@@ -163,9 +149,9 @@ __device__ __forceinline__ double all_sum(double v) {
   v += dpp_d<kDppMirror>(v);
   if constexpr (LPT == 64) {
     double x, y;
-    swap_halves<16>(v, x, y);
+    swap_halves_d<16>(v, x, y);
     v = x + y;
-    swap_halves<32>(v, x, y);
+    swap_halves_d<32>(v, x, y);
     v = x + y;
   }
   return v;
@@ -181,6 +167,10 @@ __device__ __forceinline__ float all_maxf(float v) {
     v = fmaxf(__uint_as_float(x), __uint_as_float(y));
   }
   return v;
+}
+template <int LPT>
+__device__ __forceinline__ float all_sumf(float v) {
+  return LPT == 64 ? wave64_sum(v) : row16_sum(v);
 }
 template <int LPT>
 __device__ __forceinline__ int all_min(int v) {
@@ -203,6 +193,7 @@ __device__ __forceinline__ void merge2(double& a, double& b, double a2, double b
   b = __builtin_fmax(__builtin_fmin(a, a2), __builtin_fmax(b, b2));
   a = __builtin_fmax(a, a2);
 }
+// The two best of every aligned run of `run` lanes (a power of two, uniform).
 template <int LPT>
 __device__ __forceinline__ void run_top2(double& a, double& b, int run) {
   if (run > 1) merge2(a, b, dpp_d<kDppXor1>(a), dpp_d<kDppXor1>(b));
@@ -212,14 +203,14 @@ __device__ __forceinline__ void run_top2(double& a, double& b, int run) {
   if constexpr (LPT == 64) {
     double ax, ay, bx, by;
     if (run > 16) {
-      swap_halves<16>(a, ax, ay);
-      swap_halves<16>(b, bx, by);
+      swap_halves_d<16>(a, ax, ay);
+      swap_halves_d<16>(b, bx, by);
       a = ax, b = bx;
       merge2(a, b, ay, by);
     }
     if (run > 32) {
-      swap_halves<32>(a, ax, ay);
-      swap_halves<32>(b, bx, by);
+      swap_halves_d<32>(a, ax, ay);
+      swap_halves_d<32>(b, bx, by);
       a = ax, b = bx;
       merge2(a, b, ay, by);
     }
@@ -433,18 +424,6 @@ struct TopkBwdArgs {
   void* dz;            // [T, E] in z's type
 };
 
-__device__ __forceinline__ float row_sum(float v, bool wide) {
-  v = row16_sum(v);
-  if (wide) {
-    uint32_t x, y;
-    swap_halves<16>(__float_as_uint(v), x, y);
-    v = __uint_as_float(x) + __uint_as_float(y);
-    swap_halves<32>(__float_as_uint(v), x, y);
-    v = __uint_as_float(x) + __uint_as_float(y);
-  }
-  return v;
-}
-
 template <int LPT, int PL, bool BF16>
 __global__ __launch_bounds__(256) void topk_backward_kernel(const TopkBwdArgs a) {
   constexpr int TPB = 256 / LPT;
@@ -471,7 +450,7 @@ __global__ __launch_bounds__(256) void topk_backward_kernel(const TopkBwdArgs a)
       s[m] = gi + m * LPT < a.E ? expf(s[m] - mx) : 0.f;
       sum += s[m];
     }
-    const float inv = 1.f / row_sum(sum, LPT == 64);
+    const float inv = 1.f / all_sumf<LPT>(sum);
 #pragma unroll
     for (int m = 0; m < PL; ++m) s[m] *= inv;
   } else {
@@ -496,7 +475,7 @@ __global__ __launch_bounds__(256) void topk_backward_kernel(const TopkBwdArgs a)
       float v = 0.f;
 #pragma unroll
       for (int m = 0; m < PL; ++m) v = gi + m * LPT == ek ? s[m] : v;
-      v = row_sum(v, LPT == 64);  // one lane holds s[ek]
+      v = all_sumf<LPT>(v);  // one lane holds s[ek]
       S += v;
       gs += gk * v;
     }
@@ -514,7 +493,7 @@ __global__ __launch_bounds__(256) void topk_backward_kernel(const TopkBwdArgs a)
   if (a.score_func == 0) {
 #pragma unroll
     for (int m = 0; m < PL; ++m) dot += d[m] * s[m];
-    dot = row_sum(dot, LPT == 64);
+    dot = all_sumf<LPT>(dot);
   }
   if (!valid) return;
 #pragma unroll

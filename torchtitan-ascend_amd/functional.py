@@ -101,6 +101,33 @@ def combine(y, scores_flat, sorted_indices, inverse, top_k, score_after):
     return _T.combine(y, scores_flat, sorted_indices, inverse, top_k, score_after)
 
 
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+    """bf16 x * rsqrt(mean(x^2) + eps) * weight over the last dimension
+    (models/common/npu_rmsnorm.py:15-37), the norm in front of a block; x bf16
+    or fp32 [..., D], differentiable in x and weight."""
+    rows = x.reshape(-1, x.shape[-1])
+    return _T.rms_norm(rows, weight, eps, _needs_grad(x, weight))[0].view(x.shape)
+
+
+def residual_norm(
+    branch: torch.Tensor,
+    residual: torch.Tensor | None = None,
+    post_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    gate_func: str = "identity",
+    residual_scale: float = 1.0,
+    pre_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(u, n): u = residual + residual_scale * act(gate) * rmsnorm(branch) *
+    post_weight, n = rmsnorm(u) * pre_weight (None without pre_weight), rows
+    [T, D]; differentiable in every tensor.  Operands as ops.residual_norm."""
+    keep = _needs_grad(branch, residual, post_weight, gate, pre_weight)
+    u, n, _ = _T.residual_norm(branch.to(_BF16), residual, post_weight, gate, gate_func, residual_scale, pre_weight,
+                               eps, keep)
+    return u, (None if pre_weight is None else n)
+
+
 class HIPMoeTokenUnpermute:
     """Functional unpermute with backward; same contract as the reference's
     NPUMoeTokenUnpermute (torchtitanturbo/models/common/npu_permute.py:15-53):

@@ -20,6 +20,9 @@ Reference ops these stand for (torchtitanturbo/models/common/):
   * ttamd::dispatch (+ backward)      dispatch gather / score-before
   * ttamd::experts (+ backward)       _run_experts_grouped_mm, npu_gmm.py:21-40
   * ttamd::combine (+ backward)       combine / NPUMoeTokenUnpermute, npu_permute.py:15-53
+  * ttamd::residual_norm / rms_norm (+ backward)
+                                      npu_rms_norm (models/common/npu_rmsnorm.py:34) with the
+                                      block's gate and residual
   * ttamd::moe_experts_forward        the fused inference expert stage
   * ttamd::shared_expert_add          shared-expert tail, qwen3_5/model.py:796-809
   * ttamd::token_permute / token_unpermute (+ backward)
@@ -367,6 +370,105 @@ def _combine_bwd(ctx, dout):
 
 
 combine.register_autograd(_combine_bwd, setup_context=_combine_setup)
+
+
+# ---------------------------------------------------------------------------
+# Norms around the block (ops.residual_norm, ops.rms_norm)
+# ---------------------------------------------------------------------------
+@torch.library.custom_op("ttamd::residual_norm", mutates_args=())
+def residual_norm(branch: Tensor, residual: Optional[Tensor], post_weight: Optional[Tensor], gate: Optional[Tensor],
+                  gate_func: str, residual_scale: float, pre_weight: Optional[Tensor], eps: float,
+                  save_stats: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """(u, n, stats fp32 [2, T]); n is empty without pre_weight, stats unless
+    save_stats."""
+    u, n, *stats = ops.residual_norm(branch, residual, post_weight, gate, gate_func, residual_scale, pre_weight, eps,
+                                     save_stats)
+    return u, _empty(branch) if n is None else n, stats[0] if save_stats else branch.new_empty((0,), dtype=_F32)
+
+
+@residual_norm.register_fake
+def _(branch, residual, post_weight, gate, gate_func, residual_scale, pre_weight, eps, save_stats):
+    return (branch.new_empty(branch.shape, dtype=_BF16 if residual is None else residual.dtype),
+            branch.new_empty((0,) if pre_weight is None else branch.shape),
+            branch.new_empty((2, branch.shape[0]) if save_stats else (0,), dtype=_F32))
+
+
+@torch.library.custom_op("ttamd::rms_norm", mutates_args=())
+def rms_norm(x: Tensor, weight: Tensor, eps: float, save_stats: bool) -> tuple[Tensor, Tensor]:
+    """(bf16 x * rsqrt(mean(x^2) + eps) * weight, stats fp32 [2, T] or empty)."""
+    if save_stats:
+        return ops.rms_norm(x, weight, eps, True)
+    return ops.rms_norm(x, weight, eps), x.new_empty((0,), dtype=_F32)
+
+
+@rms_norm.register_fake
+def _(x, weight, eps, save_stats):
+    return (x.new_empty(x.shape, dtype=_BF16),
+            x.new_empty((2, x.shape[0]) if save_stats else (0,), dtype=_F32))
+
+
+@torch.library.custom_op("ttamd::residual_norm_backward", mutates_args=())
+def residual_norm_backward(grad_u: Optional[Tensor], grad_n: Optional[Tensor], branch: Optional[Tensor],
+                           stats: Tensor, residual: Optional[Tensor], post_weight: Optional[Tensor],
+                           gate: Optional[Tensor], gate_func: str, residual_scale: float,
+                           pre_weight: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """Gradients of (branch, residual, post_weight, gate, pre_weight), empty for
+    an operand that is None."""
+    g = ops.residual_norm_backward(grad_u, grad_n, branch, stats, residual, post_weight, gate, gate_func,
+                                   residual_scale, pre_weight)
+    return tuple(stats.new_empty((0,)) if t is None else t for t in g)
+
+
+@residual_norm_backward.register_fake
+def _(grad_u, grad_n, branch, stats, residual, post_weight, gate, gate_func, residual_scale, pre_weight):
+    return tuple(stats.new_empty((0,)) if t is None else t.new_empty(t.shape)
+                 for t in (branch, residual, post_weight, gate, pre_weight))
+
+
+def _residual_norm_setup(ctx, inputs, output):
+    branch, residual, post_weight, gate, func, scale, pre_weight, _eps, keep = inputs
+    ctx.save_for_backward(branch, residual, post_weight, gate, pre_weight, output[2])
+    ctx.cfg = (func, scale, keep)
+    ctx.set_materialize_grads(False)
+
+
+def _residual_norm_bwd(ctx, g_u, g_n, _g_stats):
+    branch, residual, post_weight, gate, pre_weight, stats = ctx.saved_tensors
+    func, scale, keep = ctx.cfg
+    if g_u is None and g_n is None:
+        return (None,) * 9
+    if not keep:
+        raise RuntimeError("ttamd::residual_norm ran without save_stats=True; its backward needs the stats")
+    db, dr, dp, dg, dw = residual_norm_backward(
+        None if g_u is None else g_u.contiguous(),
+        None if g_n is None or pre_weight is None else g_n.to(_BF16).contiguous(), branch, stats, residual,
+        post_weight, gate, func, scale, pre_weight)
+    return (db, None if residual is None else dr, None if post_weight is None else dp,
+            None if gate is None else dg, None, None, None if pre_weight is None else dw, None, None)
+
+
+residual_norm.register_autograd(_residual_norm_bwd, setup_context=_residual_norm_setup)
+
+
+def _rms_norm_setup(ctx, inputs, output):
+    x, weight, _eps, keep = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.keep = keep
+    ctx.set_materialize_grads(False)
+
+
+def _rms_norm_bwd(ctx, g_n, _g_stats):
+    if g_n is None:
+        return None, None, None, None
+    if not ctx.keep:
+        raise RuntimeError("ttamd::rms_norm ran without save_stats=True; its backward needs the stats")
+    x, weight, stats = ctx.saved_tensors
+    _, dx, _, _, dw = residual_norm_backward(None, g_n.to(_BF16).contiguous(), None, stats, x, None, None, "identity",
+                                             1.0, weight)
+    return dx, dw, None, None
+
+
+rms_norm.register_autograd(_rms_norm_bwd, setup_context=_rms_norm_setup)
 
 
 # ---------------------------------------------------------------------------

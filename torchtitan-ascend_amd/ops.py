@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -680,6 +681,209 @@ def sum_topk(y: torch.Tensor, top_k: int) -> torch.Tensor:
     out = torch.empty(M // top_k, D, dtype=_BF16, device=dev)
     _lib.call("ttamd_moe_sum_topk", _p(y), M // top_k, D, top_k, _p(out), _stream(dev))
     return out
+
+
+# ---------------------------------------------------------------------------
+# Norms around the block
+# ---------------------------------------------------------------------------
+_F32_STREAM, _F32_POST, _F32_GATE, _F32_PRE = 1, 2, 4, 8
+
+
+def _float_kind(name: str, t: torch.Tensor) -> bool:
+    """Whether t is fp32 (else bf16)."""
+    if t.dtype not in (_BF16, torch.float32):
+        raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
+    return t.dtype == torch.float32
+
+
+def _norm_operands(dev, T, D, residual, post_weight, gate, gate_func, pre_weight):
+    """Checked operands of a block norm: (residual, post_weight, gate,
+    gate kind, sigmoid, pre_weight, fp32 mask)."""
+    _same_device(dev, residual=residual, post_weight=post_weight, gate=gate, pre_weight=pre_weight)
+    mask = 0
+    if residual is not None:
+        if tuple(residual.shape) != (T, D):
+            raise ValueError(f"residual must be [{T}, {D}], got {tuple(residual.shape)}")
+        mask |= _F32_STREAM * _float_kind("residual", residual)
+        residual = residual.contiguous()
+    for name, w, bit in (("post_weight", post_weight, _F32_POST), ("pre_weight", pre_weight, _F32_PRE)):
+        if w is not None:
+            if tuple(w.shape) != (D,):
+                raise ValueError(f"{name} must be [{D}], got {tuple(w.shape)}")
+            mask |= bit * _float_kind(name, w)
+    post_weight = None if post_weight is None else post_weight.contiguous()
+    pre_weight = None if pre_weight is None else pre_weight.contiguous()
+    if gate_func not in ("identity", "sigmoid"):
+        raise ValueError(f"gate_func must be 'identity' or 'sigmoid', got {gate_func!r}")
+    kind = 0
+    if gate is not None:
+        kinds = {(T, 1): 1, (1, D): 2, (T, D): 3}
+        if T == 1:
+            kinds = {(1, 1): 1, (1, D): 2}
+        if tuple(gate.shape) not in kinds:
+            raise ValueError(f"gate must be [{T}, 1], [1, {D}] or [{T}, {D}], got {tuple(gate.shape)}")
+        kind = kinds[tuple(gate.shape)]
+        mask |= _F32_GATE * _float_kind("gate", gate)
+        gate = gate.contiguous()
+    return residual, post_weight, gate, kind, int(gate_func == "sigmoid"), pre_weight, mask
+
+
+def _residual_norm(dev, rows, T, D, top_k, inverse, probs, residual, post_weight, gate, gate_func, residual_scale,
+                   pre_weight, eps, save_stats, want_u=True):
+    residual, post_weight, gate, kind, sig, pre_weight, mask = _norm_operands(
+        dev, T, D, residual, post_weight, gate, gate_func, pre_weight)
+    u = torch.empty(T, D, dtype=residual.dtype if residual is not None else _BF16, device=dev) if want_u else None
+    n = torch.empty(T, D, dtype=_BF16, device=dev) if pre_weight is not None else None
+    stats = torch.empty(2, T, dtype=torch.float32, device=dev) if save_stats else None
+    _call(
+        dev, "ttamd_residual_norm", _p(rows), _p(inverse), _p(probs), T, D, top_k, _p(residual), _p(post_weight),
+        _p(gate), kind, sig, float(residual_scale), _p(pre_weight), float(eps), mask, _p(u), _p(n), _p(stats),
+        _stream(dev),
+    )
+    return u, n, stats
+
+
+def residual_norm(
+    branch: torch.Tensor,
+    residual: torch.Tensor | None = None,
+    post_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    gate_func: str = "identity",
+    residual_scale: float = 1.0,
+    pre_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    save_stats: bool = False,
+):
+    """The end of a block and the norm of the next in one pass
+    (ttamd_residual_norm):
+
+        u = residual + residual_scale * act(gate) * rmsnorm(branch) * post_weight
+        n = rmsnorm(u) * pre_weight
+
+    branch bf16 [T, D]; residual bf16 or fp32 [T, D] (None: 0); post_weight
+    [D] (None: the branch is not normed); gate [T, 1], [1, D] or [T, D] (None:
+    1; act is "identity" or "sigmoid"); pre_weight [D] (None: no n); weights
+    and gate bf16 or fp32.  Returns (u in the residual's type, n bf16 or
+    None), with save_stats also the fp32 [2, T] that residual_norm_backward
+    needs.  fp32 inside, u and n rounded once each."""
+    dev = _gpu("branch", branch)
+    if branch.dim() != 2:
+        raise ValueError(f"branch must be [T, D], got {tuple(branch.shape)}")
+    branch = _want("branch", branch, _BF16)
+    T, D = branch.shape
+    out = _residual_norm(dev, branch, T, D, 1, None, None, residual, post_weight, gate, gate_func, residual_scale,
+                         pre_weight, eps, save_stats)
+    return out if save_stats else out[:2]
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, save_stats: bool = False):
+    """bf16 x * rsqrt(mean(x^2) + eps) * weight of rows x [T, D] (bf16 or fp32);
+    with save_stats also the fp32 [2, T] for residual_norm_backward (branch
+    None, residual x)."""
+    dev = _gpu("x", x)
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, D], got {tuple(x.shape)}")
+    _, n, stats = _residual_norm(dev, None, *x.shape, 1, None, None, x, None, None, "identity", 1.0, weight, eps,
+                                 save_stats, want_u=False)
+    return (n, stats) if save_stats else n
+
+
+def combine_norm(
+    rows: torch.Tensor,
+    top_k: int,
+    inverse: torch.Tensor | None = None,
+    probs: torch.Tensor | None = None,
+    residual: torch.Tensor | None = None,
+    post_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    gate_func: str = "identity",
+    residual_scale: float = 1.0,
+    pre_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """`residual_norm` of the K-way combine in one pass: the branch of token t
+    is sum_k probs[t, k] * rows[inverse[t K + k]] in fp32 (inverse None: row
+    t K + k, the order experts_forward's w2 GEMM writes; probs None: 1), so
+    the combined [T, D] is never written.  rows bf16 [T * K, D].  Inference
+    only: for gradients use functional.combine, functional.residual_norm."""
+    dev = _gpu("rows", rows)
+    if rows.dim() != 2 or top_k < 1 or rows.shape[0] % top_k:
+        raise ValueError(f"rows must be [T * {top_k}, D], got {tuple(rows.shape)}")
+    rows = _want("rows", rows, _BF16)
+    M, D = rows.shape
+    T = M // top_k
+    _same_device(dev, inverse=inverse, probs=probs)
+    if inverse is not None:
+        inverse = _want("inverse", inverse.reshape(-1), torch.int32)
+        if inverse.numel() != M:
+            raise ValueError(f"inverse has {inverse.numel()} entries, expected {M}")
+    if probs is not None:
+        probs = _want("probs", probs.reshape(-1), torch.float32)
+        if probs.numel() != M:
+            raise ValueError(f"probs has {probs.numel()} entries, expected {M}")
+    return _residual_norm(dev, rows, T, D, top_k, inverse, probs, residual, post_weight, gate, gate_func,
+                          residual_scale, pre_weight, eps, False)[:2]
+
+
+class ResidualNormGrads(NamedTuple):
+    """Gradients of residual_norm's operands; None for one that was not given."""
+
+    branch: torch.Tensor | None
+    residual: torch.Tensor | None
+    post_weight: torch.Tensor | None
+    gate: torch.Tensor | None
+    pre_weight: torch.Tensor | None
+
+
+def residual_norm_backward(
+    grad_u: torch.Tensor | None,
+    grad_n: torch.Tensor | None,
+    branch: torch.Tensor | None,
+    stats: torch.Tensor,
+    residual: torch.Tensor | None = None,
+    post_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    gate_func: str = "identity",
+    residual_scale: float = 1.0,
+    pre_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+) -> ResidualNormGrads:
+    """Gradients of residual_norm (ttamd_residual_norm_backward) from those of
+    its two outputs (None: zero) and its stats; the other arguments as given
+    to the forward (eps lives in the stats).  With branch None: of rms_norm,
+    residual its x.  Each gradient has its operand's type and shape."""
+    del eps
+    ref = branch if branch is not None else residual
+    dev = _gpu("branch" if branch is not None else "residual", ref)
+    if ref.dim() != 2:
+        raise ValueError(f"rows must be [T, D], got {tuple(ref.shape)}")
+    T, D = ref.shape
+    if branch is not None:
+        branch = _want("branch", branch, _BF16)
+    residual, post_weight, gate, kind, sig, pre_weight, mask = _norm_operands(
+        dev, T, D, residual, post_weight, gate, gate_func, pre_weight)
+    _same_device(dev, grad_u=grad_u, grad_n=grad_n, stats=stats)
+    if grad_u is not None:
+        if tuple(grad_u.shape) != (T, D):
+            raise ValueError(f"grad_u must be [{T}, {D}], got {tuple(grad_u.shape)}")
+        grad_u = _want("grad_u", grad_u, residual.dtype if residual is not None else _BF16)
+    if grad_n is not None:
+        if tuple(grad_n.shape) != (T, D):
+            raise ValueError(f"grad_n must be [{T}, {D}], got {tuple(grad_n.shape)}")
+        grad_n = _want("grad_n", grad_n, _BF16)
+    stats = _want("stats", stats, torch.float32)
+    if tuple(stats.shape) != (2, T):
+        raise ValueError(f"stats must be [2, {T}], got {tuple(stats.shape)}")
+    make = torch.zeros_like if T == 0 else torch.empty_like
+    grads = ResidualNormGrads(*(None if t is None else make(t)
+                                for t in (branch, residual, post_weight, gate, pre_weight)))
+    ws = _ws(_lib.load().ttamd_residual_norm_backward_workspace_bytes(T, D), dev)
+    _call(
+        dev, "ttamd_residual_norm_backward", _p(grad_u), _p(grad_n), _p(branch), T, D, _p(residual), _p(post_weight),
+        _p(gate), kind, sig, float(residual_scale), _p(pre_weight), _p(stats), mask, *(_p(g) for g in grads), _p(ws),
+        ws.numel(), _stream(dev),
+    )
+    return grads
 
 
 def group_labels(counts_group: torch.Tensor, num_local_experts: int, num_rows: int) -> torch.Tensor:
