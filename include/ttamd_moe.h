@@ -693,6 +693,71 @@ int ttamd_grouped_mm_wgrad(const void* dy, const void* x, const int32_t* offs,
                            void* stream);
 
 /* ------------------------------------------------------------------------ *
+ * 8-bit activation checkpoints.  The reference keeps the expert path's       *
+ * activations in bf16 (autograd of npu_gmm.py:21-40) or recomputes them; a   *
+ * packed row takes 1 + 1/128 byte per value.                                 *
+ * ------------------------------------------------------------------------ */
+
+/*
+ * Pack bf16 rows [R, C] to e4m3 codes uint8 [R, C] and exponent bytes uint8
+ * [R, ceil(C / 128)]: per row and 128 columns the smallest e in [-118, 120]
+ * with max |v| <= 448 * 2^e over the finite values; code = e4m3fn(v * 2^-e),
+ * ties to even (with e = 120 at most 240: 256 * 2^120 is past bf16's range);
+ * exponent byte e + 127.  A NaN or an infinity becomes 0x7f (NaN).  C % 8 == 0; in and codes 16-byte aligned.
+ */
+int ttamd_pack_e4m3(const void* in, int64_t num_rows, int64_t cols,
+                    void* codes, void* exponents, void* stream);
+
+/*
+ * Restore packed rows: out[j] = code * 2^e of row src_index[j] / src_div
+ * (src_index nullable -> j; clamped into the num_src_rows rows), optionally
+ * times row_scale[j] in fp32; rounded to bf16 once (exact without a scale).
+ * out bf16 [num_rows, C].
+ */
+int ttamd_unpack_e4m3(const void* codes, const void* exponents,
+                      int64_t num_src_rows, int64_t cols,
+                      const int32_t* src_index, int src_div,
+                      const float* row_scale, int64_t num_rows, void* out,
+                      void* stream);
+
+/*
+ * ttamd_grouped_mm_dgrad_swiglu with the saved pre-activation packed: h is
+ * codes uint8 [M, 2H] with exponents uint8 [M, 2H / 128]; everything else as
+ * there.
+ */
+int ttamd_grouped_mm_dgrad_swiglu_packed(const void* dy, const void* w2,
+                                         const void* codes,
+                                         const void* exponents,
+                                         const int32_t* offs, int64_t num_rows,
+                                         int num_experts, int64_t dim,
+                                         int64_t hidden, float swiglu_limit,
+                                         void* dh, void* a_out,
+                                         void* workspace,
+                                         size_t workspace_bytes, void* stream);
+
+/*
+ * ttamd_grouped_mm_wgrad with x packed: x row m is packed row src_index[m] /
+ * src_div of num_src_rows (src_index nullable -> m; clamped), times
+ * row_scale[m] (nullable; rounded to bf16 once, as a dispatched row is).
+ * Without a scale each packed row is restored once and gathered by the GEMM's
+ * loads.  codes uint8 [num_src_rows, k], exponents [num_src_rows, k / 128].
+ * The workspace holds the restored bf16 rows (num_src_rows, with a scale
+ * num_rows of them), their ids and a GEMM workspace.
+ */
+size_t ttamd_grouped_mm_wgrad_packed_workspace_bytes(int64_t num_rows,
+                                                     int64_t num_src_rows,
+                                                     int num_experts,
+                                                     int64_t k, int scaled);
+int ttamd_grouped_mm_wgrad_packed(const void* dy, const void* codes,
+                                  const void* exponents, int64_t num_src_rows,
+                                  const int32_t* src_index, int src_div,
+                                  const float* row_scale, const int32_t* offs,
+                                  int64_t num_rows, int num_experts, int64_t n,
+                                  int64_t k, void* dw, int dw_is_fp32,
+                                  void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
+/* ------------------------------------------------------------------------ *
  * fp8 e4m3 experts with fp32 block scales.                                  *
  * The reference has no fp8 path; these follow the published recipe:         *
  * scale = absmax / 448 per block, code = e4m3fn(v /                         *

@@ -1,0 +1,312 @@
+"""8-bit activation checkpoints: packing and restoring against the definition in
+64 bits (exactly), and the backward products that read packed rows against
+the bf16 products on the restored rows (bit for bit: restored values are exact
+in bf16, and the kernels then do the same arithmetic) and against 64 bits."""
+from __future__ import annotations
+
+import importlib
+
+import numpy as np
+import pytest
+import torch
+
+from gpu_util import DEV, announce, rel_err_rows, to_np, zipf_counts
+
+BF16 = torch.bfloat16
+
+
+def define(x):
+    """(exponent bytes, values) of rows x (float64) by the definition: the block's power of two from a logarithm,
+    values on the grid of 3 places below their own power of two, at least 2^-6."""
+    x = np.asarray(x, np.float64)
+    R, C = x.shape
+    nb = (C + 127) // 128
+    pad = np.zeros((R, nb * 128))
+    pad[:, :C] = np.where(np.isfinite(x), np.abs(x), 0.0)
+    most = pad.reshape(R, nb, 128).max(2)
+    with np.errstate(divide="ignore"):
+        e = np.clip(np.ceil(np.log2(most / 448.0)), -118, 120)
+    s = np.exp2(e)[:, np.arange(C) // 128]
+    with np.errstate(invalid="ignore"):
+        v = x / s
+        step = np.exp2(np.floor(np.log2(np.maximum(np.abs(v), 2.0 ** -6))) - 3)
+        # at e = 120 codes end at 240: 256 * 2^120 = 2^128 is no bf16 number
+        r = np.round(v / step) * step
+        val = np.where(e[:, np.arange(C) // 128] == 120, np.clip(r, -240, 240), r) * s
+    return (e + 127).astype(np.int64), np.where(np.isfinite(x), val, np.nan)
+
+
+def rows(rng, R, C):
+    """bf16 rows whose columns span many binades."""
+    x = rng.standard_normal((R, C)) * np.exp2(rng.standard_normal((1, C)) * 4)
+    return torch.from_numpy(x).to(BF16).to(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(1, 8), (3, 128), (1003, 1544), (5, 136), (4096, 1536), (2, 8192), (257, 120),
+                                 (9000, 640), (1, 16384)])
+def test_pack_and_restore(ops, R, C):
+    rng = np.random.default_rng(R + C)
+    x = rows(rng, R, C)
+    announce(f"pack R={R} C={C}")
+    p = ops.pack_e4m3(x)
+    y = ops.unpack_e4m3(p)
+    torch.cuda.synchronize()
+    e, val = define(x.double().cpu().numpy())
+    np.testing.assert_array_equal(p.exponents.cpu().numpy(), e)
+    np.testing.assert_array_equal(y.double().cpu().numpy(), val)
+    assert p.codes.shape == (R, C) and p.exponents.shape == (R, (C + 127) // 128)
+    # packing restored rows gives the same values: the grid holds them
+    again = ops.unpack_e4m3(ops.pack_e4m3(y))
+    assert torch.equal(again, y)
+
+
+@pytest.mark.gpu
+def test_special_values(ops):
+    """Zeros of both signs, the ends of bf16's range, borders of the exponent
+    (448 * 2^e and the next bf16 value), ties, NaN and infinities beside
+    finite values, blocks of nothing else."""
+    x = np.zeros((12, 264), np.float64)
+    x[1, :] = -0.0
+    x[2, :3] = [3.3895e38, -3.3895e38, 1.0]
+    x[3, :3] = [9.2e-41, -1.2e-38, 2.0 ** -120]
+    x[4, :4] = [448.0, 450.0, 1.0, -0.3]
+    x[5, 0], x[5, 128], x[5, 256] = 448.0, 450.0, 1.75
+    x[6, :6] = [256.0, 17.0, 19.0, 0.0146484375, 0.0009765625, 0.00048828125]  # ties at 3 places, at 2^-9 and below
+    x[7, :4] = [np.nan, 1.0, np.inf, -np.inf]
+    x[7, 130] = 5.0
+    x[8, :128] = np.nan
+    x[9, :] = np.inf
+    x[10, 263] = -2.0 ** 100
+    x[11, 0] = 2.0 ** -112 * 1.875
+    t = torch.from_numpy(x).to(BF16).to(DEV)
+    p = ops.pack_e4m3(t)
+    y = ops.unpack_e4m3(p)
+    e, val = define(t.double().cpu().numpy())
+    np.testing.assert_array_equal(p.exponents.cpu().numpy(), e)
+    np.testing.assert_array_equal(y.double().cpu().numpy(), val)
+    assert not ops.unpack_e4m3(ops.pack_e4m3(t[:2])).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,C,K", [(1, 256, 8), (300, 136, 8), (1000, 2048, 1)])
+def test_unpack_gathered_and_scaled(ops, T, C, K):
+    rng = np.random.default_rng(T + C)
+    x = rows(rng, T, C)
+    p = ops.pack_e4m3(x)
+    y = ops.unpack_e4m3(p)
+    src = torch.from_numpy(rng.permutation(T * K).astype(np.int32)).to(DEV)
+    scale = torch.from_numpy(rng.random(T * K).astype(np.float32)).to(DEV)
+    announce(f"unpack gathered T={T} C={C} K={K}")
+    got = ops.unpack_e4m3(p, src, K)
+    assert torch.equal(got, y[src.long() // K])
+    got = ops.unpack_e4m3(p, src, K, scale)
+    assert torch.equal(got, (y.float()[src.long() // K] * scale[:, None]).to(BF16))
+    assert torch.equal(ops.unpack_e4m3(p, row_scale=scale[:T]), (y.float() * scale[:T, None]).to(BF16))
+    # an index past the rows is clamped to them
+    far = torch.tensor([0, T * K + 10 ** 6, -5], dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.unpack_e4m3(p, far, K), y[[0, T - 1, 0]])
+
+
+@pytest.mark.gpu
+def test_empty_strided_and_captured(ops):
+    assert ops.unpack_e4m3(ops.pack_e4m3(torch.empty(0, 64, dtype=BF16, device=DEV))).shape == (0, 64)
+    wide = torch.randn(50, 400, device=DEV).to(BF16)
+    assert torch.equal(ops.unpack_e4m3(ops.pack_e4m3(wide[:, 5:141])),
+                       ops.unpack_e4m3(ops.pack_e4m3(wide[:, 5:141].contiguous())))
+    x = torch.randn(500, 264, device=DEV).to(BF16)
+    ops.unpack_e4m3(ops.pack_e4m3(x))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.unpack_e4m3(ops.pack_e4m3(x))
+    for _ in range(3):
+        x.normal_()
+        g.replay()
+        want = ops.unpack_e4m3(ops.pack_e4m3(x))
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+def offsets(counts):
+    return torch.from_numpy(np.cumsum(counts).astype(np.int32)).to(DEV)
+
+
+GEMMS = [
+    # counts, D, H
+    ([5], 128, 128),
+    ([0, 1, 0, 63, 64, 65, 0], 192, 128),
+    ([321, 0, 640, 31], 256, 384),
+    ([0, 0, 0], 128, 128),
+    ([700, 900], 512, 256),
+    ([1] * 40, 256, 128),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,D,H", GEMMS)
+@pytest.mark.parametrize("limit", [None, 0.5])
+def test_dgrad_swiglu_packed(ops, counts, D, H, limit):
+    """Against the bf16 form on the restored h, bit for bit, and against 64
+    bits: one rounding to bf16 (2^-8 of the value) and fp32 sums of D products
+    (D 2^-24 of their sizes, far below) relative to the row's largest value,
+    for which 2^-7 leaves a factor of two."""
+    rng = np.random.default_rng(sum(counts) + D + H)
+    M, E = sum(counts) + 7, len(counts)  # seven rows behind the last expert
+    dy = torch.from_numpy(rng.standard_normal((M, D))).to(BF16).to(DEV)
+    w2 = torch.from_numpy(rng.standard_normal((E, D, H)) * 0.05).to(BF16).to(DEV)
+    h = ops.pack_e4m3(torch.from_numpy(rng.standard_normal((M, 2 * H))).to(BF16).to(DEV))
+    offs = offsets(counts)
+    announce(f"dgrad packed counts={counts} D={D} H={H} limit={limit}")
+    dh, a = ops.grouped_mm_dgrad_swiglu_packed(dy, w2, h, offs, limit, want_a=True)
+    hb = ops.unpack_e4m3(h)
+    dh0, a0 = ops.grouped_mm_dgrad_swiglu(dy, w2, hb, offs, limit, want_a=True)
+    torch.cuda.synchronize()
+    n = sum(counts)
+    assert torch.equal(dh[:n], dh0[:n]) and torch.equal(a[:n], a0[:n])
+    if n == 0:
+        return
+    hd = hb[:n].double().requires_grad_(True)
+    gate, up = hd[:, :H], hd[:, H:]
+    if limit is not None:
+        gate, up = gate.clamp(max=limit), up.clamp(-limit, limit)
+    act = torch.nn.functional.silu(gate) * up
+    e = np.repeat(np.arange(E), counts)
+    g = torch.cat([dy[i:i + 1].double() @ w2[e[i]].double() for i in range(n)])
+    (rdh,) = torch.autograd.grad(act, hd, g)
+    assert rel_err_rows(to_np(dh[:n]), rdh.cpu().numpy()) < 2.0 ** -7
+    assert rel_err_rows(to_np(a[:n]), act.detach().cpu().numpy()) < 2.0 ** -7
+    # without a
+    dh1, none = ops.grouped_mm_dgrad_swiglu_packed(dy, w2, h, offs, limit)
+    assert none is None and torch.equal(dh1[:n], dh[:n])
+
+
+@pytest.mark.gpu
+def test_dgrad_rows_behind_the_last_expert_stay(ops):
+    """Through the C ABI into given buffers: rows at and past offs[E - 1] are not written."""
+    import ctypes
+
+    L = importlib.import_module("torchtitan-ascend_amd._lib")
+    rng = np.random.default_rng(3)
+    M, D, H, n = 90, 128, 128, 70
+    dy = torch.from_numpy(rng.standard_normal((M, D))).to(BF16).to(DEV)
+    w2 = torch.from_numpy(rng.standard_normal((2, D, H)) * 0.05).to(BF16).to(DEV)
+    h = ops.pack_e4m3(torch.from_numpy(rng.standard_normal((M, 2 * H))).to(BF16).to(DEV))
+    offs = offsets([30, 40])
+    dh = torch.full((M, 2 * H), 7.0, dtype=BF16, device=DEV)
+    a = torch.full((M, H), 7.0, dtype=BF16, device=DEV)
+    ws = torch.empty(L.load().ttamd_gemm_workspace_bytes(M, 2), dtype=torch.uint8, device=DEV)
+    p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    L.call("ttamd_grouped_mm_dgrad_swiglu_packed", p(dy), p(w2), p(h.codes), p(h.exponents), p(offs), M, 2, D, H,
+           float("nan"), p(dh), p(a), p(ws), ws.numel(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert bool((dh[n:] == 7).all()) and bool((a[n:] == 7).all()) and not bool((dh[:n] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,E,N,D,skew", [
+    (1, 1, 1, 128, 128, 0.0), (37, 8, 16, 256, 128, 1.0), (500, 2, 3, 384, 640, 0.5), (640, 8, 20, 256, 512, 1.2),
+    (3000, 1, 4, 128, 256, 0.0), (50, 4, 64, 128, 384, 0.0),
+])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_wgrad_packed(ops, T, K, E, N, D, skew, dtype):
+    """Against the bf16 form on the restored, gathered rows: bit for bit, with
+    and without a row scale; and the fp32 gradient against 64 bits: fp32 sums
+    of the expert's rows, each term's rounding 2^-24 of its size and at most
+    rows + 16 of them."""
+    rng = np.random.default_rng(T + K + E)
+    M = T * K
+    counts = zipf_counts(M, E, skew, max(1, E - E // 4), rng)
+    x = ops.pack_e4m3(torch.from_numpy(rng.standard_normal((T, D))).to(BF16).to(DEV))
+    dy = torch.from_numpy(rng.standard_normal((M, N))).to(BF16).to(DEV)
+    src = torch.from_numpy(rng.permutation(M).astype(np.int32)).to(DEV)
+    scale = torch.from_numpy(rng.random(M).astype(np.float32)).to(DEV)
+    offs = offsets(counts)
+    announce(f"wgrad packed T={T} K={K} E={E} N={N} D={D} {dtype}")
+    routed = ops.unpack_e4m3(x, src, K)
+    got = ops.grouped_mm_wgrad_packed(dy, x, offs, E, dtype, src, K)
+    want = ops.grouped_mm_wgrad(dy, routed, offs, E, dtype)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    got = ops.grouped_mm_wgrad_packed(dy, x, offs, E, dtype, src, K, scale)
+    assert torch.equal(got, ops.grouped_mm_wgrad(dy, ops.unpack_e4m3(x, src, K, scale), offs, E, dtype))
+    if K == 1:
+        got = ops.grouped_mm_wgrad_packed(dy, x, offs, E, dtype)
+        assert torch.equal(got, ops.grouped_mm_wgrad(dy, ops.unpack_e4m3(x), offs, E, dtype))
+    if dtype == torch.float32:
+        ends = np.cumsum(counts)
+        for e in range(E):
+            a, b = int(ends[e] - counts[e]), int(ends[e])
+            ref = dy[a:b].double().t() @ routed[a:b].double()
+            size = dy[a:b].double().abs().t() @ routed[a:b].double().abs()
+            assert bool(((want[e].double() - ref).abs() <= size * (b - a + 16) * 2.0 ** -24).all())
+
+
+@pytest.mark.gpu
+def test_wgrad_packed_large_gathered(ops):
+    """Full rounds, a split tail and experts that end inside a stage."""
+    rng = np.random.default_rng(9)
+    T, K, E, N, D = 1024, 8, 24, 768, 1024
+    M = T * K
+    counts = zipf_counts(M, E, 0.8, 20, rng)
+    x = ops.pack_e4m3(torch.from_numpy(rng.standard_normal((T, D))).to(BF16).to(DEV))
+    dy = torch.from_numpy(rng.standard_normal((M, N))).to(BF16).to(DEV)
+    src = torch.from_numpy(rng.permutation(M).astype(np.int32)).to(DEV)
+    announce("wgrad packed large")
+    got = ops.grouped_mm_wgrad_packed(dy, x, offsets(counts), E, torch.float32, src, K)
+    want = ops.grouped_mm_wgrad(dy, ops.unpack_e4m3(x, src, K), offsets(counts), E, torch.float32)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------------------
+# Refusals (CPU: nothing is launched)
+# ---------------------------------------------------------------------------
+def _err(name, *args):
+    L = importlib.import_module("torchtitan-ascend_amd._lib").load()
+    assert getattr(L, name)(*args) == 1
+    return L.ttamd_last_error().decode()
+
+
+def test_refusals():
+    import ctypes
+
+    p, odd, nan = ctypes.c_void_p(256), ctypes.c_void_p(260), float("nan")
+    assert "multiple of 8" in _err("ttamd_pack_e4m3", p, 4, 12, p, p, None)
+    assert "aligned" in _err("ttamd_pack_e4m3", odd, 4, 64, p, p, None)
+    assert "aligned" in _err("ttamd_pack_e4m3", p, 4, 64, odd, p, None)
+    assert "null" in _err("ttamd_pack_e4m3", p, 4, 64, p, None, None)
+    assert "out of range" in _err("ttamd_pack_e4m3", p, -1, 64, p, p, None)
+    assert "too many" in _err("ttamd_pack_e4m3", p, 1 << 28, 64, p, p, None)
+    assert "too few packed rows" in _err("ttamd_unpack_e4m3", p, p, 3, 64, None, 1, None, 4, p, None)
+    assert "too few packed rows" in _err("ttamd_unpack_e4m3", p, p, 0, 64, p, 1, None, 4, p, None)
+    assert "src_div" in _err("ttamd_unpack_e4m3", p, p, 4, 64, p, 0, None, 4, p, None)
+    assert "null" in _err("ttamd_unpack_e4m3", p, None, 4, 64, None, 1, None, 4, p, None)
+    L = importlib.import_module("torchtitan-ascend_amd._lib").load()
+    ws = L.ttamd_gemm_workspace_bytes(64, 2)
+    dgrad = "ttamd_grouped_mm_dgrad_swiglu_packed"
+    assert "hidden" in _err(dgrad, p, p, p, p, p, 64, 2, 128, 64, nan, p, p, p, ws, None)
+    assert "swiglu_limit" in _err(dgrad, p, p, p, p, p, 64, 2, 128, 128, -1.0, p, p, p, ws, None)
+    assert "exponents" in _err(dgrad, p, p, p, None, p, 64, 2, 128, 128, nan, p, p, p, ws, None)
+    assert "workspace" in _err(dgrad, p, p, p, p, p, 64, 2, 128, 128, nan, p, p, p, ws - 1, None)
+    wgrad = "ttamd_grouped_mm_wgrad_packed"
+    need = L.ttamd_grouped_mm_wgrad_packed_workspace_bytes(64, 16, 2, 128, 0)
+    assert need >= 16 * 128 * 2 + 64 * 4 + ws
+    assert L.ttamd_grouped_mm_wgrad_packed_workspace_bytes(64, 16, 2, 128, 1) >= 64 * 128 * 2 + ws
+    assert "workspace" in _err(wgrad, p, p, p, 16, p, 4, None, p, 64, 2, 128, 128, p, 1, p, need - 1, None)
+    assert "multiple of 128" in _err(wgrad, p, p, p, 16, p, 4, None, p, 64, 2, 64, 128, p, 1, p, need, None)
+    assert "too few packed rows" in _err(wgrad, p, p, p, 16, None, 1, None, p, 64, 2, 128, 128, p, 1, p, need, None)
+    assert "src_div" in _err(wgrad, p, p, p, 16, p, 0, None, p, 64, 2, 128, 128, p, 1, p, need, None)
+
+
+def test_python_refusals(ops):
+    x = torch.zeros(4, 64, dtype=BF16)
+    u8 = torch.zeros(4, 64, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        ops.pack_e4m3(x)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        ops.unpack_e4m3(ops.PackedRows(u8, u8[:, :1]))
+    with pytest.raises(ValueError, match="do not match"):
+        ops._packed("x", ops.PackedRows(u8, u8), u8.device)
+    with pytest.raises(TypeError, match="codes"):
+        ops._packed("x", ops.PackedRows(x, u8[:, :1]), u8.device)

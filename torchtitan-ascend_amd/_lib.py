@@ -161,6 +161,21 @@ SIGNATURES: dict[str, tuple] = {
         _i32,
         [_c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i64, _i64, _c_void_p, _i32, _c_void_p, _sz, _c_void_p],
     ),
+    "ttamd_pack_e4m3": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p]),
+    "ttamd_unpack_e4m3": (
+        _i32, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i32, _c_void_p, _i64, _c_void_p, _c_void_p]
+    ),
+    "ttamd_grouped_mm_dgrad_swiglu_packed": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i64, _i64, _f32, _c_void_p, _c_void_p,
+         _c_void_p, _sz, _c_void_p],
+    ),
+    "ttamd_grouped_mm_wgrad_packed_workspace_bytes": (_sz, [_i64, _i64, _i32, _i64, _i32]),
+    "ttamd_grouped_mm_wgrad_packed": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i32, _c_void_p, _c_void_p, _i64, _i32, _i64, _i64,
+         _c_void_p, _i32, _c_void_p, _sz, _c_void_p],
+    ),
     "ttamd_quantize_fp8_rows": (
         _i32, [_c_void_p, _c_void_p, _i32, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p]
     ),

@@ -942,6 +942,98 @@ int check_fp8_gemm(const char* fn, const void* xq, const float* sx, const void* 
 
 }  // namespace
 
+// ---------------------------------------------------------------------------
+// 8-bit activation checkpoints
+// ---------------------------------------------------------------------------
+int ttamd_pack_e4m3(const void* in, int64_t num_rows, int64_t cols, void* codes, void* exponents, void* stream) {
+  const char* fn = "ttamd_pack_e4m3";
+  TRY(check_hidden(fn, cols));
+  REQUIRE(num_rows >= 0 && num_rows <= (1 << 28) && cols <= (1 << 20), "%s: num_rows or cols out of range", fn);
+  TRY(check_rows(fn, "in", in, num_rows, cols));
+  TRY(check_bytes(fn, "codes", codes, num_rows * cols));
+  if (num_rows == 0) return TTAMD_OK;
+  REQUIRE(exponents, "%s: exponents is null", fn);
+  return check_hip(ttamd::launch_pack_rows(in, num_rows, (int)cols, codes, exponents, (hipStream_t)stream), fn);
+}
+
+int ttamd_unpack_e4m3(const void* codes, const void* exponents, int64_t num_src_rows, int64_t cols,
+                      const int32_t* src_index, int src_div, const float* row_scale, int64_t num_rows, void* out,
+                      void* stream) {
+  const char* fn = "ttamd_unpack_e4m3";
+  TRY(check_hidden(fn, cols));
+  REQUIRE(num_rows >= 0 && num_rows <= (1 << 28) && cols <= (1 << 20), "%s: num_rows or cols out of range", fn);
+  REQUIRE(num_src_rows >= 0 && num_src_rows <= (1 << 28), "%s: num_src_rows out of range", fn);
+  REQUIRE(src_div >= 1, "%s: src_div must be >= 1", fn);
+  REQUIRE(src_index ? num_src_rows >= 1 || num_rows == 0 : num_src_rows >= num_rows,
+          "%s: too few packed rows (%lld for %lld)", fn, (long long)num_src_rows, (long long)num_rows);
+  TRY(check_rows(fn, "out", out, num_rows, cols));
+  TRY(check_bytes(fn, "codes", codes, num_src_rows * cols));
+  if (num_rows == 0) return TTAMD_OK;
+  REQUIRE(exponents, "%s: exponents is null", fn);
+  return check_hip(ttamd::launch_unpack_rows(codes, exponents, (int)num_src_rows, src_index, src_div, row_scale,
+                                             num_rows, (int)cols, out, nullptr, nullptr, 0, (hipStream_t)stream),
+                   fn);
+}
+
+int ttamd_grouped_mm_dgrad_swiglu_packed(const void* dy, const void* w2, const void* codes, const void* exponents,
+                                         const int32_t* offs, int64_t num_rows, int num_experts, int64_t dim,
+                                         int64_t hidden, float swiglu_limit, void* dh, void* a_out, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
+  const char* fn = "ttamd_grouped_mm_dgrad_swiglu_packed";
+  TRY(check_gemm_common(fn, offs, num_rows, num_experts));
+  TRY(check_dim(fn, "dim", dim, 64));
+  TRY(check_dim(fn, "hidden", hidden, 128));
+  REQUIRE(std::isnan(swiglu_limit) || swiglu_limit >= 0.f, "%s: swiglu_limit must be NaN (no clamp) or >= 0", fn);
+  REQUIRE(w2 && aligned16(w2), "%s: w2 must be non-null and 16-byte aligned", fn);
+  TRY(check_rows(fn, "dy", dy, num_rows, dim));
+  TRY(check_rows(fn, "dh", dh, num_rows, 2 * hidden));
+  TRY(check_bytes(fn, "codes", codes, num_rows * 2 * hidden));
+  if (a_out) TRY(check_rows(fn, "a_out", a_out, num_rows, hidden));
+  TRY(check_ws(fn, workspace, workspace_bytes, ttamd::gemm_workspace_bytes(num_rows, num_experts)));
+  if (num_rows == 0) return TTAMD_OK;
+  REQUIRE(exponents, "%s: exponents is null", fn);
+  return check_hip(ttamd::launch_grouped_mm_dgrad_swiglu_packed(dy, w2, codes, exponents, offs, (int)num_rows,
+                                                                num_experts, (int)dim, (int)hidden, swiglu_limit, dh,
+                                                                a_out, workspace, (hipStream_t)stream),
+                   fn);
+}
+
+size_t ttamd_grouped_mm_wgrad_packed_workspace_bytes(int64_t num_rows, int64_t num_src_rows, int num_experts,
+                                                     int64_t k, int scaled) {
+  if (num_rows < 0 || num_src_rows < 0 || num_experts < 1 || k < 1) return 0;
+  return ttamd::wgrad_packed_workspace_bytes(scaled ? num_rows : num_src_rows, num_rows, num_experts, k);
+}
+
+int ttamd_grouped_mm_wgrad_packed(const void* dy, const void* codes, const void* exponents, int64_t num_src_rows,
+                                  const int32_t* src_index, int src_div, const float* row_scale, const int32_t* offs,
+                                  int64_t num_rows, int num_experts, int64_t n, int64_t k, void* dw, int dw_is_fp32,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "ttamd_grouped_mm_wgrad_packed";
+  TRY(check_gemm_common(fn, offs, num_rows, num_experts));
+  TRY(check_dim(fn, "n", n, 128));
+  TRY(check_dim(fn, "k", k, 128));
+  REQUIRE(num_src_rows >= 0 && num_src_rows <= (1 << 28), "%s: num_src_rows out of range", fn);
+  REQUIRE(src_div >= 1, "%s: src_div must be >= 1", fn);
+  REQUIRE(src_index ? num_src_rows >= 1 || num_rows == 0 : num_src_rows >= num_rows,
+          "%s: too few packed rows (%lld for %lld)", fn, (long long)num_src_rows, (long long)num_rows);
+  TRY(check_rows(fn, "dy", dy, num_rows, n));
+  TRY(check_bytes(fn, "codes", codes, num_src_rows * k));
+  REQUIRE(exponents || num_rows == 0, "%s: exponents is null", fn);
+  REQUIRE(dw && aligned16(dw), "%s: dw must be non-null and 16-byte aligned", fn);
+  REQUIRE((int64_t)num_experts * n * k <= (int64_t)1 << 40, "%s: dw too large", fn);
+  REQUIRE((int64_t)num_experts * (n / 128) * (k / 128) <= kI32Max, "%s: too many tiles", fn);
+  const int64_t rows = row_scale ? num_rows : num_src_rows;
+  REQUIRE(num_rows * n * 2 <= (int64_t)0xffffffffLL && rows * k * 2 <= (int64_t)0xffffffffLL &&
+              num_rows * k <= (int64_t)1 << 33,
+          "%s: dy and the restored rows must each stay below 4 GiB", fn);
+  TRY(check_ws(fn, workspace, workspace_bytes,
+               ttamd::wgrad_packed_workspace_bytes(rows, num_rows, num_experts, k)));
+  return check_hip(ttamd::launch_grouped_mm_wgrad_packed(dy, codes, exponents, (int)num_src_rows, src_index, src_div,
+                                                         row_scale, offs, (int)num_rows, num_experts, (int)n, (int)k,
+                                                         dw, dw_is_fp32 != 0, workspace, (hipStream_t)stream),
+                   fn);
+}
+
 int ttamd_quantize_fp8_rows(const void* in, const int32_t* src_index, int src_div, const float* row_scale,
                             int64_t num_in_rows, int64_t num_rows, int64_t k, void* q_out, float* scale_t,
                             void* stream) {

@@ -66,6 +66,16 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
   return v;
 }
 
+// Four e4m3 codes (low byte first) times a scale.
+__device__ __forceinline__ void unpack_e4m3x4(uint32_t codes, float scale, float* f) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+  f[0] = lo[0] * scale;
+  f[1] = lo[1] * scale;
+  f[2] = hi[0] * scale;
+  f[3] = hi[1] * scale;
+}
+
 // Streaming (non-temporal) 16-byte load and store, for data a kernel reads
 // or writes exactly once.
 __device__ __forceinline__ uint4 load_stream(const uint4* p) {

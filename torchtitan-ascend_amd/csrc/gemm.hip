@@ -465,11 +465,44 @@ hipError_t launch_grouped_mm_dgrad_swiglu(const void* dy, const void* w2, const 
   return dgrad(EPI_SWIGLU_BWD, g, offs, E, M, ws, split_part_in(ws, M, E), stream);
 }
 
+hipError_t launch_grouped_mm_dgrad_swiglu_packed(const void* dy, const void* w2, const void* codes, const void* exps,
+                                                 const int* offs, int M, int E, int D, int H, float limit, void* dh,
+                                                 void* a_out, void* ws, hipStream_t stream) {
+  DgradGemm g = {};
+  g.dy = dy; g.w = w2; g.n_red = D; g.n_out = H; g.out = dh; g.h = codes; g.h_exps = exps; g.limit = limit;
+  g.a_out = a_out;
+  return dgrad(EPI_SWIGLU_BWD_PACKED, g, offs, E, M, ws, split_part_in(ws, M, E), stream);
+}
+
+// bf16 rows of the tokens (gathered inside the GEMM's loads) or, with a row
+// scale, of the routed rows; then row ids; then the GEMM's workspace.
+size_t wgrad_packed_workspace_bytes(int64_t rows, int64_t M, int E, int64_t K) {
+  return al256((size_t)rows * K * 2) + al256((size_t)M * 4) + gemm_workspace_bytes(M, E);
+}
+
+hipError_t launch_grouped_mm_wgrad_packed(const void* dy, const void* codes, const void* exps, int n_src,
+                                          const int* src_index, int src_div, const float* row_scale, const int* offs,
+                                          int M, int E, int N, int K, void* dw, bool fp32, void* ws,
+                                          hipStream_t stream) {
+  // A token's row is unpacked once, however many experts read it; only a
+  // scale per routed row needs the routed rows themselves.
+  const bool gather = src_index != nullptr && row_scale == nullptr;
+  const int rows = gather ? n_src : M;
+  char* x = (char*)ws;
+  int* ids = (int*)(x + al256((size_t)rows * K * 2));
+  void* gws = (char*)ids + al256((size_t)M * 4);
+  hipError_t err = launch_unpack_rows(codes, exps, n_src, gather ? nullptr : src_index, src_div, row_scale, rows, K, x,
+                                      gather ? src_index : nullptr, gather ? ids : nullptr, gather ? M : 0, stream);
+  if (err != hipSuccess) return err;
+  return launch_grouped_mm_wgrad(dy, x, offs, M, E, N, K, dw, fp32, gws, stream, gather ? ids : nullptr);
+}
+
 hipError_t launch_grouped_mm_wgrad(const void* dy, const void* x, const int* offs, int M, int E,
-                                   int N, int K, void* dw, bool fp32, void* ws, hipStream_t stream) {
+                                   int N, int K, void* dw, bool fp32, void* ws, hipStream_t stream,
+                                   const int* x_rows) {
   WgradDmaArgs a = {};
   a.dy = (const bf16_t*)dy; a.lddy = N;
-  a.x = (const bf16_t*)x; a.ldx = K;
+  a.x = (const bf16_t*)x; a.ldx = K; a.x_rows = x_rows;
   a.offs = offs; a.E = E; a.M = M; a.N = N; a.K = K;
   a.n_tiles = (N + 255) / 256; a.k_tiles = (K + 255) / 256;
   a.dw = dw; a.dw_fp32 = fp32 ? 1 : 0;

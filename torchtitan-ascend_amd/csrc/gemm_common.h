@@ -13,6 +13,7 @@ enum Epi {
   EPI_SWIGLU = 1,      // gate/up pairs -> silu(clamp(gate)) * clamp(up)
   EPI_SCATTER = 2,     // out[dest[q]][p] = scale[q] * acc
   EPI_SWIGLU_BWD = 3,  // dh from dA = acc and the saved pre-activation h
+  EPI_SWIGLU_BWD_PACKED = 4,  // the same, h as e4m3 codes and exponents (checkpoint.hip)
 };
 
 // 1 / (1 + exp(-x)) with the hardware reciprocal (1 ulp) in place of an
@@ -235,6 +236,8 @@ struct FwdArgs {
   int64_t ldh;
   // EPI_SWIGLU_BWD
   const bf16_t* h_in;  // saved pre-activation [M][2H]
+  const uint8_t* h_codes;  // EPI_SWIGLU_BWD_PACKED: e4m3 codes [M][2H]
+  const uint8_t* h_exps;   // ... exponent bytes [M][2H / 128]
   bf16_t* a_out;       // recomputed activation [M][H] (nullable)
   // EPI_SCATTER
   const float* row_scale;
@@ -263,6 +266,7 @@ struct DgradGemm {
   void* out;  // EPI_STORE: [M][n_out]; EPI_SWIGLU_BWD: dh [M][2 n_out]
   // EPI_SWIGLU_BWD
   const void* h;  // [M][2 n_out]
+  const void* h_exps;  // EPI_SWIGLU_BWD_PACKED: h is e4m3 codes, these their exponent bytes
   float limit;
   void* a_out;
 };
@@ -274,6 +278,7 @@ struct WgradDmaArgs {
   int64_t lddy;
   const bf16_t* x;  // [M][K]
   int64_t ldx;
+  const int* x_rows;  // nullable, [M]: reduction row m reads x row x_rows[m] (in range: the caller's)
   const int* offs;  // inclusive, [E]
   int E, M, N, K;
   int n_tiles, k_tiles;  // per expert, 256-wide

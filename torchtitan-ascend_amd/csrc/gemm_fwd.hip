@@ -664,10 +664,26 @@ __global__ __launch_bounds__(FTHREADS, 1) void gg_fwd_kernel(const FwdArgs a) {
       return u32x4_t{x[0], x[1], y[0], y[1]};
     };
     const int pcol = 16 * (eg4 & 1) + 8 * (eg4 >> 1);  // the lane's columns in a block pair
-    // EPI_SWIGLU_BWD: saved pre-activation of token block jj
+    // EPI_SWIGLU_BWD: saved pre-activation of token block jj (packed: four
+    // e4m3 codes in .x; the wave's 64 columns lie in one 128-column block, so
+    // a row has one exponent for its gate and one for its up columns there,
+    // in .y of the first block)
+    constexpr bool SWIGLU_BWD = EPI == EPI_SWIGLU_BWD || EPI == EPI_SWIGLU_BWD_PACKED;
     auto load_h = [&](int jj, uint2 (&dst)[NPB][2]) {
+      const int qrow = min(row0 + 32 * jj + 16 * wq + er16, row1 - 1);
+      if constexpr (EPI == EPI_SWIGLU_BWD_PACKED) {
+        const uint8_t* erow = a.h_exps + (int64_t)qrow * (a.ldh >> 7) + (min(pt * TP + arow0, a.n_p - 64) >> 7);
+        dst[0][0].y = erow[0];
+        dst[0][1].y = erow[a.hidden >> 7];
+#pragma unroll
+        for (int pb = 0; pb < NPB; ++pb) {
+          const int col = min(pt * TP + arow(pb), a.n_p - 16) + 4 * eg4;
+          const uint8_t* hrow = a.h_codes + (int64_t)qrow * a.ldh + col;
+          dst[pb][0].x = *(const uint32_t*)hrow;
+          dst[pb][1].x = *(const uint32_t*)(hrow + a.hidden);
+        }
+      }
       if constexpr (EPI == EPI_SWIGLU_BWD) {
-        const int qrow = min(row0 + 32 * jj + 16 * wq + er16, row1 - 1);
 #pragma unroll
         for (int pb = 0; pb < NPB; ++pb) {
           const int col = min(pt * TP + arow(pb), a.n_p - 16) + 4 * eg4;
@@ -680,7 +696,7 @@ __global__ __launch_bounds__(FTHREADS, 1) void gg_fwd_kernel(const FwdArgs a) {
     // EPI_SWIGLU_BWD: the h values of token block j are loaded one block
     // ahead, into the other half of hbuf (double buffer).
     uint2 hbuf[2][NPB][2];
-    if constexpr (EPI == EPI_SWIGLU_BWD) load_h(0, hbuf[0]);
+    if constexpr (SWIGLU_BWD) load_h(0, hbuf[0]);
 #pragma unroll
     for (int j = 0; j < NJV; ++j) {
       const int trow = 32 * j + 16 * wq + er16;
@@ -735,7 +751,7 @@ __global__ __launch_bounds__(FTHREADS, 1) void gg_fwd_kernel(const FwdArgs a) {
           else
             swiglu_rows(std::false_type{});
         }
-      } else if constexpr (EPI == EPI_SWIGLU_BWD) {
+      } else if constexpr (SWIGLU_BWD) {
         // acc = dA = g for output columns p of the activation; with the saved
         // bf16 pre-activation h = [gate | up]: dgate, dup (clamp masks from
         // the bf16 h, as the reference's autograd sees them).
@@ -754,10 +770,18 @@ __global__ __launch_bounds__(FTHREADS, 1) void gg_fwd_kernel(const FwdArgs a) {
             const int pb = pp + b2;
             const uint2 hg = hv[pb][0];
             const uint2 hu = hv[pb][1];
-            const float gate[4] = {bf16_to_f32(hg.x & 0xffff), bf16_to_f32(hg.x >> 16), bf16_to_f32(hg.y & 0xffff),
-                                   bf16_to_f32(hg.y >> 16)};
-            const float up[4] = {bf16_to_f32(hu.x & 0xffff), bf16_to_f32(hu.x >> 16), bf16_to_f32(hu.y & 0xffff),
-                                 bf16_to_f32(hu.y >> 16)};
+            float gate[4], up[4];
+            if constexpr (EPI == EPI_SWIGLU_BWD_PACKED) {
+              // code * 2^e, exact in fp32; a byte e + 127 is 2^e's exponent field
+              const float sg = __uint_as_float(hv[0][0].y << 23), su = __uint_as_float(hv[0][1].y << 23);
+              unpack_e4m3x4(hg.x, sg, gate);
+              unpack_e4m3x4(hu.x, su, up);
+            } else {
+              gate[0] = bf16_to_f32(hg.x & 0xffff), gate[1] = bf16_to_f32(hg.x >> 16);
+              gate[2] = bf16_to_f32(hg.y & 0xffff), gate[3] = bf16_to_f32(hg.y >> 16);
+              up[0] = bf16_to_f32(hu.x & 0xffff), up[1] = bf16_to_f32(hu.x >> 16);
+              up[2] = bf16_to_f32(hu.y & 0xffff), up[3] = bf16_to_f32(hu.y >> 16);
+            }
             float dg[4], du[4], av[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -966,13 +990,18 @@ hipError_t launch_dgrad_gemm(int epi, const DgradGemm& g, hipStream_t stream) {
   a.split_cnt = g.split_cnt;
   a.split_max = split_max();
   a.out = (bf16_t*)g.out;
-  if (epi == EPI_SWIGLU_BWD) {
+  if (epi == EPI_SWIGLU_BWD || epi == EPI_SWIGLU_BWD_PACKED) {
     a.ldo = 2 * (int64_t)g.n_out;
     a.hidden = g.n_out;
     a.limit = g.limit;
-    a.h_in = (const bf16_t*)g.h;
     a.ldh = 2 * (int64_t)g.n_out;
     a.a_out = (bf16_t*)g.a_out;
+    if (epi == EPI_SWIGLU_BWD_PACKED) {
+      a.h_codes = (const uint8_t*)g.h;
+      a.h_exps = (const uint8_t*)g.h_exps;
+      return launch_fwd<EPI_SWIGLU_BWD_PACKED, true>(a, stream);
+    }
+    a.h_in = (const bf16_t*)g.h;
     return launch_fwd<EPI_SWIGLU_BWD, true>(a, stream);
   }
   a.ldo = g.n_out;

@@ -76,6 +76,7 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4_t lds_short4_t;
 typedef __attribute__((address_space(1))) int gint_t;
 typedef __attribute__((address_space(1))) floatx4_t gfloatx4_t;
+typedef const __attribute__((address_space(4))) int cint_t;  // read only while the kernel runs: scalar loads
 
 // Chunk permutation of a row (as gemm_fwd.hip's reduction-major weights).
 __device__ __forceinline__ int ptswz(int m) { return 2 * ((m & 3) | ((m >> 2) & 4)); }
@@ -89,6 +90,11 @@ __device__ __forceinline__ void static_for(F&& f) {
   }
 }
 
+// GATHER: reduction row m is x row x_rows[m] (a token that several experts
+// read).  A wave moves two rows per x instruction, so a stage's row ids are
+// eight scalar loads, made when the cursor reaches the stage, one stage ahead
+// of the instructions that use them.
+template <bool GATHER>
 __global__ __launch_bounds__(THREADS, 1) void gg_wgrad_dma_kernel(const WgradDmaArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -177,8 +183,21 @@ __global__ __launch_bounds__(THREADS, 1) void gg_wgrad_dma_kernel(const WgradDma
   };
   const int m_max = max(a.M - 1, 0);
   auto row_of = [&](int i) { return min(max(min(d_mstage + d_row + 2 * WAVES * i, d_last), 0), m_max); };
+  // GATHER: x rows of the cursor's stage, instruction i rows 2 i and 2 i + 1
+  int g_row[2 * DMA_OP];
+  auto gather_rows = [&]() {
+    if constexpr (GATHER) {
+      const int m0 = c_t.m0 + TK * c_ks + 2 * w, last = max(min(c_t.m1 - 1, m_max), 0);
+#pragma unroll
+      for (int i = 0; i < 2 * DMA_OP; ++i) {
+        const int m = min(max(m0 + 2 * WAVES * (i >> 1) + (i & 1), 0), last);
+        g_row[i] = a.M > 0 ? ((cint_t*)a.x_rows)[__builtin_amdgcn_readfirstlane(m)] : 0;
+      }
+    }
+  };
   auto issue_x = [&](int i) {
-    const uint32_t voff = (uint32_t)row_of(i) * (uint32_t)(a.ldx * 2) + (((d_chunk ^ (8 * (i & 1))) & d_xmask) << 4);
+    const int row = GATHER ? ((l >> 5) ? g_row[2 * i + 1] : g_row[2 * i]) : row_of(i);
+    const uint32_t voff = (uint32_t)row * (uint32_t)(a.ldx * 2) + (((d_chunk ^ (8 * (i & 1))) & d_xmask) << 4);
     dma16(voff, d_xb, d_st + i * (WAVES * 1024));
   };
   auto issue_y = [&](int i) {
@@ -194,6 +213,7 @@ __global__ __launch_bounds__(THREADS, 1) void gg_wgrad_dma_kernel(const WgradDma
       c_ks = 0;
       c_t = tile_of(c_r);
     }
+    gather_rows();
   };
 
   // ---- fragments: transposed reads (see gemm_fwd.hip, PT) ---------------------
@@ -245,6 +265,7 @@ __global__ __launch_bounds__(THREADS, 1) void gg_wgrad_dma_kernel(const WgradDma
   };
 
   // ---- prologue --------------------------------------------------------------
+  gather_rows();
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
     issue_prep(st);
@@ -486,11 +507,15 @@ hipError_t launch_split_cnt_zero(int* split_cnt, int n, hipStream_t stream) {
 
 hipError_t launch_wgrad_dma(const WgradDmaArgs& a, hipStream_t stream) {
   // set once per process (thread-safe static initialisation)
-  static const hipError_t attr_err =
-      hipFuncSetAttribute((const void*)gg_wgrad_dma_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_TOTAL);
+  static const hipError_t attr_err = hipFuncSetAttribute((const void*)gg_wgrad_dma_kernel<false>,
+                                                         hipFuncAttributeMaxDynamicSharedMemorySize, LDS_TOTAL);
+  static const hipError_t attr_err_g = hipFuncSetAttribute((const void*)gg_wgrad_dma_kernel<true>,
+                                                           hipFuncAttributeMaxDynamicSharedMemorySize, LDS_TOTAL);
   if (attr_err != hipSuccess) return attr_err;
+  if (attr_err_g != hipSuccess) return attr_err_g;
   const int grid = (num_cus() + 7) & ~7;
-  return launch_k(false, gg_wgrad_dma_kernel, dim3(grid), dim3(THREADS), LDS_TOTAL, stream, a);
+  if (a.x_rows) return launch_k(false, gg_wgrad_dma_kernel<true>, dim3(grid), dim3(THREADS), LDS_TOTAL, stream, a);
+  return launch_k(false, gg_wgrad_dma_kernel<false>, dim3(grid), dim3(THREADS), LDS_TOTAL, stream, a);
 }
 
 }  // namespace ttamd

@@ -177,8 +177,28 @@ hipError_t launch_grouped_mm_dgrad_swiglu(const void* dy, const void* w2, const 
                                           hipStream_t stream);
 // ws: NULL (no tail split) or gemm_workspace_bytes(M, E) bytes (the
 // leftover tiles' partial sums and arrival counters).
+// x_rows (nullable, [M]): reduction row m reads x row x_rows[m].
 hipError_t launch_grouped_mm_wgrad(const void* dy, const void* x, const int* offs, int M, int E,
-                                   int N, int K, void* dw, bool fp32, void* ws, hipStream_t stream);
+                                   int N, int K, void* dw, bool fp32, void* ws, hipStream_t stream,
+                                   const int* x_rows = nullptr);
+
+// 8-bit activation checkpoints (checkpoint.hip): e4m3 codes [R, C], exponent
+// bytes [R, ceil(C / 128)].
+hipError_t launch_pack_rows(const void* in, int64_t R, int C, void* codes, void* exps, hipStream_t stream);
+// out row j = row src_index[j] / src_div of n_src (nullable -> j), times
+// row_scale[j] (nullable).  ids_out[j] (nullable) = the clamped row of
+// ids_index[j], j < n_ids.
+hipError_t launch_unpack_rows(const void* codes, const void* exps, int n_src, const int* src_index, int src_div,
+                              const float* row_scale, int64_t R, int C, void* out, const int* ids_index, int* ids_out,
+                              int n_ids, hipStream_t stream);
+hipError_t launch_grouped_mm_dgrad_swiglu_packed(const void* dy, const void* w2, const void* codes, const void* exps,
+                                                 const int* offs, int M, int E, int D, int H, float limit, void* dh,
+                                                 void* a_out, void* ws, hipStream_t stream);
+size_t wgrad_packed_workspace_bytes(int64_t rows, int64_t M, int E, int64_t K);
+hipError_t launch_grouped_mm_wgrad_packed(const void* dy, const void* codes, const void* exps, int n_src,
+                                          const int* src_index, int src_div, const float* row_scale, const int* offs,
+                                          int M, int E, int N, int K, void* dw, bool fp32, void* ws,
+                                          hipStream_t stream);
 
 // fp8 e4m3 path (quant.hip, gemm_fp8.hip via gemm.hip)
 hipError_t launch_quantize_rows(const void* in, const int* src_index, int src_div, const float* row_mul,

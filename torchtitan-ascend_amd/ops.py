@@ -1120,6 +1120,134 @@ def grouped_mm_wgrad(
 
 
 # ---------------------------------------------------------------------------
+# 8-bit activation checkpoints
+# ---------------------------------------------------------------------------
+@dataclass
+class PackedRows:
+    """bf16 rows [R, C] as e4m3 codes with one power-of-two scale per row and
+    128 columns: value = code * 2^(exponent - 127), exact in bf16."""
+
+    codes: torch.Tensor  # uint8 [R, C]
+    exponents: torch.Tensor  # uint8 [R, ceil(C / 128)]
+
+
+def _packed(name: str, p: PackedRows, dev: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    codes = _want(f"{name}.codes", p.codes, torch.uint8)
+    exps = _want(f"{name}.exponents", p.exponents, torch.uint8)
+    _same_device(dev, **{f"{name}.codes": codes, f"{name}.exponents": exps})
+    if codes.dim() != 2 or tuple(exps.shape) != (codes.shape[0], (codes.shape[1] + 127) // 128):
+        raise ValueError(f"{name}: codes {tuple(codes.shape)} and exponents {tuple(exps.shape)} do not match")
+    return codes, exps
+
+
+def pack_e4m3(x: torch.Tensor) -> PackedRows:
+    """8-bit checkpoint of bf16 rows x [R, C] (ttamd_pack_e4m3): 1 + 1/128 byte
+    per value, a relative error of at most 2^-4 for values down to 2^-15 of
+    their block's largest.  NaN and infinities come back as NaN."""
+    dev = _gpu("x", x)
+    if x.dim() != 2:
+        raise ValueError(f"x must be [R, C], got {tuple(x.shape)}")
+    x = _want("x", x, _BF16)
+    R, C = x.shape
+    codes = torch.empty(R, C, dtype=torch.uint8, device=dev)
+    exps = torch.empty(R, (C + 127) // 128, dtype=torch.uint8, device=dev)
+    _call(dev, "ttamd_pack_e4m3", _p(x), R, C, _p(codes), _p(exps), _stream(dev))
+    return PackedRows(codes, exps)
+
+
+def unpack_e4m3(
+    packed: PackedRows,
+    src_index: torch.Tensor | None = None,
+    src_div: int = 1,
+    row_scale: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """bf16 rows of a checkpoint (ttamd_unpack_e4m3): row j is packed row
+    src_index[j] // src_div (None: j), times row_scale[j] in fp32, rounded
+    once; exact without a scale."""
+    dev = _gpu("packed.codes", packed.codes)
+    codes, exps = _packed("packed", packed, dev)
+    R, C = codes.shape
+    _same_device(dev, src_index=src_index, row_scale=row_scale)
+    if src_index is not None:
+        src_index = _want("src_index", src_index.reshape(-1), torch.int32)
+    rows = R if src_index is None else src_index.numel()
+    if row_scale is not None:
+        row_scale = _want("row_scale", row_scale.reshape(-1), torch.float32)
+        if row_scale.numel() != rows:
+            raise ValueError(f"row_scale has {row_scale.numel()} entries, expected {rows}")
+    out = torch.empty(rows, C, dtype=_BF16, device=dev)
+    _call(dev, "ttamd_unpack_e4m3", _p(codes), _p(exps), R, C, _p(src_index), int(src_div), _p(row_scale), rows,
+          _p(out), _stream(dev))
+    return out
+
+
+def grouped_mm_dgrad_swiglu_packed(
+    dy: torch.Tensor, w2: torch.Tensor, h: PackedRows, offs: torch.Tensor,
+    swiglu_limit: float | None = None, want_a: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """grouped_mm_dgrad_swiglu from a packed pre-activation h [M, 2H]: the GEMM's
+    epilogue rebuilds gate and up from their codes.  Returns (dh [M, 2H],
+    a [M, H] or None)."""
+    dev = _gpu("dy", dy)
+    dy = _want("dy", dy, _BF16)
+    w2 = _want("w2", w2, _BF16)
+    codes, exps = _packed("h", h, dev)
+    _same_device(dev, w2=w2)
+    offs = _offs(offs, dev)
+    M, D = dy.shape
+    E, D2, H = w2.shape
+    if D2 != D or tuple(codes.shape) != (M, 2 * H) or offs.numel() != E:
+        raise ValueError(f"dy {tuple(dy.shape)}, w2 {tuple(w2.shape)}, h {tuple(codes.shape)} and offs "
+                         f"[{offs.numel()}] disagree")
+    dh = torch.empty(M, 2 * H, dtype=_BF16, device=dev)
+    a = torch.empty(M, H, dtype=_BF16, device=dev) if want_a else None
+    ws = _gemm_ws(M, E, dev)
+    _call(
+        dev, "ttamd_grouped_mm_dgrad_swiglu_packed", _p(dy), _p(w2), _p(codes), _p(exps), _p(offs), M, E, D, H,
+        _limit(swiglu_limit), _p(dh), _p(a), _p(ws), ws.numel(), _stream(dev),
+    )
+    return dh, a
+
+
+def grouped_mm_wgrad_packed(
+    dy: torch.Tensor, x: PackedRows, offs: torch.Tensor, num_experts: int,
+    out_dtype: torch.dtype = torch.float32, src_index: torch.Tensor | None = None, src_div: int = 1,
+    row_scale: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """grouped_mm_wgrad with x packed: x row m is packed row src_index[m] //
+    src_div (None: m), times row_scale[m] rounded once (None: 1).  Without a
+    scale each packed row is restored once, however many experts read it."""
+    dev = _gpu("dy", dy)
+    dy = _want("dy", dy, _BF16)
+    codes, exps = _packed("x", x, dev)
+    offs = _offs(offs, dev)
+    M, N = dy.shape
+    R, K = codes.shape
+    _same_device(dev, src_index=src_index, row_scale=row_scale)
+    if src_index is not None:
+        src_index = _want("src_index", src_index.reshape(-1), torch.int32)
+    if (R if src_index is None else src_index.numel()) != M:
+        raise ValueError(f"x gives {R if src_index is None else src_index.numel()} rows for {M} rows of dy")
+    if offs.numel() != num_experts:
+        raise ValueError(f"offs has {offs.numel()} entries for {num_experts} experts")
+    if row_scale is not None:
+        row_scale = _want("row_scale", row_scale.reshape(-1), torch.float32)
+        if row_scale.numel() != M:
+            raise ValueError(f"row_scale has {row_scale.numel()} entries, expected {M}")
+    if out_dtype not in (torch.float32, _BF16):
+        raise TypeError("wgrad output must be float32 or bfloat16")
+    dw = torch.empty(num_experts, N, K, dtype=out_dtype, device=dev)
+    ws = _ws(_lib.load().ttamd_grouped_mm_wgrad_packed_workspace_bytes(M, R, num_experts, K,
+                                                                       int(row_scale is not None)), dev)
+    _call(
+        dev, "ttamd_grouped_mm_wgrad_packed", _p(dy), _p(codes), _p(exps), R, _p(src_index), int(src_div),
+        _p(row_scale), _p(offs), M, num_experts, N, K, _p(dw), int(out_dtype == torch.float32), _p(ws), ws.numel(),
+        _stream(dev),
+    )
+    return dw
+
+
+# ---------------------------------------------------------------------------
 # fp8 e4m3 experts (block scales, absmax / 448)
 # ---------------------------------------------------------------------------
 _U8 = torch.uint8
