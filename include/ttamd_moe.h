@@ -185,8 +185,8 @@ enum { TTAMD_GROUP_TOP2 = 0, TTAMD_GROUP_MAX = 1 };
  *   the topk experts of the kept groups with the largest v, descending (ties
  *   to the lower id; NaN before every number, -inf after every finite value:
  *   an expert masked with a -inf bias is picked only when the kept groups
- *   hold too few others).  Values within 2^-42 of each other count as equal;
- *   logits below -700 count as -700.
+ *   hold too few others).  Values are compared by their sign, exponent and
+ *   first 42 places; a score below exp(-700) counts as that.
  *   top_scores fp32 [T, topk] = s of the picks; renorm: divided by (their sum
  *   + renorm_eps); times route_scale.  top_indices int64 [T, topk].
  * Requires T <= 2^24, E <= 1024, num_groups <= 64 dividing E, 1 <= topk <=

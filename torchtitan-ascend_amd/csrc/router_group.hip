@@ -35,7 +35,6 @@
 namespace ttamd {
 namespace {
 
-constexpr int kGroupWaveTokens = 2048;
 constexpr int kIdBits = 10;
 constexpr uint64_t kIdMask = (1u << kIdBits) - 1;
 // Order of values that are not finite numbers: NaN first, then +inf, the
@@ -48,27 +47,55 @@ constexpr uint32_t kDeadHi = 0xffefffffu;
 __device__ __forceinline__ double as_f64(uint64_t b) { return __builtin_bit_cast(double, b); }
 __device__ __forceinline__ uint64_t as_u64(double d) { return __builtin_bit_cast(uint64_t, d); }
 
-// exp(x) for -745 <= x <= 700 (clamped; NaN stays NaN).
+// p r + c with the constant in a scalar register pair (left to itself the
+// compiler copies every constant of a Horner chain into vector registers
+// first, three instructions a step instead of one).
+__device__ __forceinline__ double fma_s(double p, double r, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(p), "v"(r), "s"(c));
+  return d;
+}
+
+// The larger and the smaller of two numbers (no NaN comes here; the builtins
+// first canonicalise each operand, one more instruction apiece).
+__device__ __forceinline__ double max_d(double a, double b) {
+  double d;
+  asm("v_max_f64 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
+  return d;
+}
+__device__ __forceinline__ double min_d(double a, double b) {
+  double d;
+  asm("v_min_f64 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
+  return d;
+}
+
+// exp(x), x clamped to [-700, 700] (a NaN becomes -700: the callers look for
+// it themselves).
 __device__ __forceinline__ double exp_f64(double x) {
-  x = x < -745.0 ? -745.0 : (x > 700.0 ? 700.0 : x);
-  const double n = x == x ? __builtin_rint(x * 1.4426950408889634) : 0.0;  // defined as an int below
+  x = min_d(max_d(x, -700.0), 700.0);
+  // n = round(x / ln 2) by adding 1.5 * 2^52: n is then also the sum's low word
+  const double magic = 6755399441055744.0;
+  const double shifted = __builtin_fma(x, 1.4426950408889634, magic);
+  const double n = shifted - magic;
   // ln 2 in two parts: floor(2^32 ln 2) / 2^32, whose product with n is exact,
   // and the rest
   double r = __builtin_fma(-n, 2977044471.0 / 4294967296.0, x);
   r = __builtin_fma(-n, 1.9082149292705877e-10, r);
-  double p = 1.0 / 39916800.0;
-  p = __builtin_fma(p, r, 1.0 / 3628800.0);
-  p = __builtin_fma(p, r, 1.0 / 362880.0);
-  p = __builtin_fma(p, r, 1.0 / 40320.0);
-  p = __builtin_fma(p, r, 1.0 / 5040.0);
-  p = __builtin_fma(p, r, 1.0 / 720.0);
-  p = __builtin_fma(p, r, 1.0 / 120.0);
-  p = __builtin_fma(p, r, 1.0 / 24.0);
-  p = __builtin_fma(p, r, 1.0 / 6.0);
+  double p = fma_s(1.0 / 39916800.0, r, 1.0 / 3628800.0);
+  p = fma_s(p, r, 1.0 / 362880.0);
+  p = fma_s(p, r, 1.0 / 40320.0);
+  p = fma_s(p, r, 1.0 / 5040.0);
+  p = fma_s(p, r, 1.0 / 720.0);
+  p = fma_s(p, r, 1.0 / 120.0);
+  p = fma_s(p, r, 1.0 / 24.0);
+  p = fma_s(p, r, 1.0 / 6.0);
   p = __builtin_fma(p, r, 0.5);
   p = __builtin_fma(p, r, 1.0);
   p = __builtin_fma(p, r, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)n);
+  // times 2^n: |n| <= 1010 and 0.7 < p < 1.5, so the exponent field takes it
+  const uint64_t b = as_u64(p);
+  const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)as_u64(shifted) << 20);
+  return as_f64((uint64_t)hi << 32 | (uint32_t)b);
 }
 
 // 1 / d for 1 <= d <= 1.1e304, or NaN.
@@ -80,12 +107,18 @@ __device__ __forceinline__ double rcp_f64(double d) {
 
 __device__ __forceinline__ double sigmoid_f64(double z) { return rcp_f64(1.0 + exp_f64(-z)); }
 
+// Scores of single logits, NaN included.
+__device__ __forceinline__ double score_of(float z, bool softmax, float mx, double inv) {
+  const double s = softmax ? exp_f64((double)z - (double)mx) * inv : sigmoid_f64((double)z);
+  return z == z ? s : __builtin_nan("");
+}
+
 // A selection value in the kernel's total order.
 __device__ __forceinline__ double ordered(double v) {
   if (v != v) return as_f64(kNanKey);
   if (v == __builtin_inf()) return as_f64(kPosKey);
   if (v == -__builtin_inf()) return as_f64(kNegKey);
-  return v + 0.0;  // -0 becomes +0
+  return v;
 }
 
 // a >= b, both ordered(): the group's value as the sum of the two.
@@ -100,8 +133,10 @@ __device__ __forceinline__ double group_sum(double a, double b) {
 // The value with its expert's id in the low bits: of equal values the lower
 // id is the larger key, on either side of zero.
 __device__ __forceinline__ double with_id(double v, int e) {
-  const uint64_t b = as_u64(v) & ~kIdMask;
-  return as_f64(b | ((b >> 63) ? (uint64_t)e : kIdMask - (uint64_t)e));
+  const uint64_t b = as_u64(v);
+  const uint32_t hi = (uint32_t)(b >> 32);
+  const uint32_t id = (uint32_t)e ^ (~(uint32_t)((int32_t)hi >> 31) & (uint32_t)kIdMask);  // kIdMask - e above zero
+  return as_f64((uint64_t)hi << 32 | (((uint32_t)b & ~(uint32_t)kIdMask) | id));
 }
 __device__ __forceinline__ int id_of(double key) {
   const uint64_t b = as_u64(key);
@@ -128,16 +163,16 @@ __device__ __forceinline__ void swap_halves_d(double v, double& x, double& y) {
 // Reductions over a token's LPT lanes; every lane gets the result.
 template <int LPT>
 __device__ __forceinline__ double all_max(double v) {
-  v = __builtin_fmax(v, dpp_d<kDppXor1>(v));
-  v = __builtin_fmax(v, dpp_d<kDppXor2>(v));
-  v = __builtin_fmax(v, dpp_d<kDppHalfMirror>(v));
-  v = __builtin_fmax(v, dpp_d<kDppMirror>(v));
+  v = max_d(v, dpp_d<kDppXor1>(v));
+  v = max_d(v, dpp_d<kDppXor2>(v));
+  v = max_d(v, dpp_d<kDppHalfMirror>(v));
+  v = max_d(v, dpp_d<kDppMirror>(v));
   if constexpr (LPT == 64) {
     double x, y;
     swap_halves_d<16>(v, x, y);
-    v = __builtin_fmax(x, y);
+    v = max_d(x, y);
     swap_halves_d<32>(v, x, y);
-    v = __builtin_fmax(x, y);
+    v = max_d(x, y);
   }
   return v;
 }
@@ -157,6 +192,10 @@ __device__ __forceinline__ double all_sum(double v) {
   return v;
 }
 template <int LPT>
+__device__ __forceinline__ float all_sumf(float v) {
+  return LPT == 64 ? wave64_sum(v) : row16_sum(v);
+}
+template <int LPT>
 __device__ __forceinline__ float all_maxf(float v) {
   v = row16_max(v);
   if constexpr (LPT == 64) {
@@ -168,30 +207,76 @@ __device__ __forceinline__ float all_maxf(float v) {
   }
   return v;
 }
-template <int LPT>
-__device__ __forceinline__ float all_sumf(float v) {
-  return LPT == 64 ? wave64_sum(v) : row16_sum(v);
+// ---- sorted lists of N keys per lane (descending; N a power of two) ----------
+__device__ __forceinline__ void order2(double& hi, double& lo) {
+  const double a = max_d(hi, lo), b = min_d(hi, lo);
+  hi = a, lo = b;
 }
-template <int LPT>
-__device__ __forceinline__ int all_min(int v) {
-  v = min(v, dpp_i<kDppXor1>(v));
-  v = min(v, dpp_i<kDppXor2>(v));
-  v = min(v, dpp_i<kDppHalfMirror>(v));
-  v = min(v, dpp_i<kDppMirror>(v));
+// A list in any order (odd-even merge sort).
+template <int N>
+__device__ __forceinline__ void sort_list(double (&v)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j <= N - 1 - k; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k && i < N - j - k; ++i)
+          if ((i + j) / (2 * p) == (i + j + k) / (2 * p)) order2(v[i + j], v[i + j + k]);
+}
+// The N largest of two sorted lists: the larger of a's i-th and b's i-th from
+// the end form a bitonic sequence that holds them.
+template <int N>
+__device__ __forceinline__ void merge_lists(double (&a)[N], const double (&b)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = max_d(a[i], b[N - 1 - i]);
+#pragma unroll
+  for (int k = N / 2; k >= 1; k /= 2)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & k) == 0) order2(a[i], a[i + k]);
+}
+template <int CTRL, int N>
+__device__ __forceinline__ void merge_dpp(double (&a)[N]) {
+  double b[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) b[i] = dpp_d<CTRL>(a[i]);
+  merge_lists(a, b);
+}
+template <int DIST, int N>
+__device__ __forceinline__ void merge_swap(double (&a)[N]) {
+  double x[N], y[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) swap_halves_d<DIST>(a[i], x[i], y[i]);
+  merge_lists(x, y);
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = x[i];
+}
+// The token's N largest keys, sorted, in every lane.
+template <int LPT, int N>
+__device__ __forceinline__ void merge_lanes(double (&a)[N]) {
+  merge_dpp<kDppXor1>(a);
+  merge_dpp<kDppXor2>(a);
+  merge_dpp<kDppHalfMirror>(a);
+  merge_dpp<kDppMirror>(a);
   if constexpr (LPT == 64) {
-    uint32_t x, y;
-    swap_halves<16>((uint32_t)v, x, y);
-    v = min((int)x, (int)y);
-    swap_halves<32>((uint32_t)v, x, y);
-    v = min((int)x, (int)y);
+    merge_swap<16>(a);
+    merge_swap<32>(a);
   }
-  return v;
+}
+
+// How many of the 16 lanes of this lane's row hold a key above v.
+template <int R>
+__device__ __forceinline__ void count_above(double key, double v, int& n) {
+  n += dpp_d<0x120 + R>(key) > v ? 1 : 0;  // row rotated by R
+  if constexpr (R > 1) count_above<R - 1>(key, v, n);
 }
 
 // Merge the two best (a >= b) of two halves of a run.
 __device__ __forceinline__ void merge2(double& a, double& b, double a2, double b2) {
-  b = __builtin_fmax(__builtin_fmin(a, a2), __builtin_fmax(b, b2));
-  a = __builtin_fmax(a, a2);
+  b = max_d(min_d(a, a2), max_d(b, b2));
+  a = max_d(a, a2);
 }
 // The two best of every aligned run of `run` lanes (a power of two, uniform).
 template <int LPT>
@@ -249,7 +334,7 @@ __device__ __forceinline__ float logit_at(const GroupTopkArgs& a, int64_t t, int
   return round_bf16(z);
 }
 
-template <int LPT, int PL, int SRC>
+template <int LPT, int PL, int KL, int SRC>
 __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) {
   constexpr int TPB = 256 / LPT;
   const int gi = threadIdx.x & (LPT - 1);
@@ -261,31 +346,41 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
   const int n_live = group < a.G ? min(max(a.EG - in0, 0), a.per_lane) : 0;
   const int e0 = group * a.EG + in0;
 
+  // Loads are unconditional, at indices clamped into the row (no branch
+  // around each): whole 16-byte (bf16: 8-byte) loads where every lane's run of
+  // experts is a multiple of 4.
   float z[PL];
-  // whole 16-byte loads where every lane's run of experts is a multiple of 4
-  const bool quads = SRC != SRC_BF16 && PL % 4 == 0 && a.aligned && (a.EG & 3) == 0 && (a.per_lane & 3) == 0;
+  const bool quads = PL % 4 == 0 && a.aligned && (a.EG & 3) == 0 && (a.per_lane & 3) == 0;
   if (quads) {
     if constexpr (PL % 4 == 0) {
-      const float* row = (const float*)a.z + t * a.E + e0;
 #pragma unroll
       for (int m = 0; m < PL; m += 4) {
-        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (m < n_live) {
-          q = *(const float4*)(row + m);
+        const int64_t at = t * a.E + min(e0 + m, a.E - 4);
+        if constexpr (SRC == SRC_BF16) {
+          const uint2 q = *(const uint2*)((const bf16_t*)a.z + at);
+          z[m] = bf16_to_f32(q.x & 0xffff), z[m + 1] = bf16_to_f32(q.x >> 16);
+          z[m + 2] = bf16_to_f32(q.y & 0xffff), z[m + 3] = bf16_to_f32(q.y >> 16);
+        } else {
+          float4 q = *(const float4*)((const float*)a.z + at);
           if constexpr (SRC == SRC_PARTIALS) {
             for (int s = 1; s < a.S; ++s) {
-              const float4 p = *(const float4*)(row + (int64_t)s * a.T * a.E + m);
+              const float4 p = *(const float4*)((const float*)a.z + at + (int64_t)s * a.T * a.E);
               q.x += p.x, q.y += p.y, q.z += p.z, q.w += p.w;
             }
             q.x = round_bf16(q.x), q.y = round_bf16(q.y), q.z = round_bf16(q.z), q.w = round_bf16(q.w);
           }
+          z[m] = q.x, z[m + 1] = q.y, z[m + 2] = q.z, z[m + 3] = q.w;
         }
-        z[m] = q.x, z[m + 1] = q.y, z[m + 2] = q.z, z[m + 3] = q.w;
       }
     }
   } else {
 #pragma unroll
-    for (int m = 0; m < PL; ++m) z[m] = m < n_live ? logit_at<SRC>(a, t, e0 + m) : 0.f;
+    for (int m = 0; m < PL; ++m) z[m] = logit_at<SRC>(a, t, min(e0 + m, a.E - 1));
+  }
+  float bias[PL];
+  if (a.bias) {
+#pragma unroll
+    for (int m = 0; m < PL; ++m) bias[m] = a.bias[min(e0 + m, a.E - 1)];
   }
   if constexpr (SRC == SRC_PARTIALS) {
     if (a.logits && valid) {
@@ -297,17 +392,22 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
 
   // scores, then selection values
   double v[PL];
-  float mx = 0.f;
+  float mx = 0.f, nan = 0.f;  // nan: NaN when a logit is (or softmax has no finite maximum)
   double inv = 1.0;
+#pragma unroll
+  for (int m = 0; m < PL; ++m) nan += z[m] == z[m] ? 0.f : z[m];
   if (a.score_func == 0) {
     mx = -INFINITY;
 #pragma unroll
-    for (int m = 0; m < PL; ++m) mx = fmaxf(mx, m < n_live ? z[m] : -INFINITY);
+    for (int m = 0; m < PL; ++m) mx = fmaxf(mx, z[m]);  // (a clamped index repeats a logit of the row)
     mx = all_maxf<LPT>(mx);
+    if (!__builtin_isfinite(mx)) nan = __builtin_nanf("");  // inf - inf
+    nan = all_sumf<LPT>(nan);                               // one NaN makes the whole row NaN
     double sum = 0.0;
 #pragma unroll
     for (int m = 0; m < PL; ++m) {
-      v[m] = m < n_live ? exp_f64((double)z[m] - (double)mx) : 0.0;
+      const double x = exp_f64((double)z[m] - (double)mx);
+      v[m] = m < n_live ? x : 0.0;
       sum += v[m];
     }
     inv = rcp_f64(all_sum<LPT>(sum));
@@ -317,55 +417,96 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
 #pragma unroll
     for (int m = 0; m < PL; ++m) v[m] = sigmoid_f64((double)z[m]);
   }
+  float odd = nan;
+  if (a.bias) {
 #pragma unroll
-  for (int m = 0; m < PL; ++m) {
-    if (a.bias) v[m] += m < n_live ? (double)a.bias[e0 + m] : 0.0;
-    v[m] = ordered(v[m]);
+    for (int m = 0; m < PL; ++m) {
+      v[m] += (double)bias[m];
+      odd = fmaf(bias[m], 0.f, odd);
+    }
+  }
+  // NaN and infinities take the general order; numbers are in it already
+  if (__builtin_amdgcn_ballot_w64(odd != odd)) {
+#pragma unroll
+    for (int m = 0; m < PL; ++m) {
+      const bool bad = a.score_func == 0 ? nan != nan : z[m] != z[m];
+      v[m] = ordered(bad ? __builtin_nan("") : v[m]);
+    }
   }
 
+  // slots without an expert: the high word alone makes them the least
+  auto kill = [](double d) { return as_f64((uint64_t)kDeadHi << 32 | (uint32_t)as_u64(d)); };
+  if (a.per_lane < PL || a.EG != a.per_lane << a.log_run || a.G << a.log_run != LPT) {  // uniform
+#pragma unroll
+    for (int m = 0; m < PL; ++m) v[m] = m < n_live ? v[m] : kill(v[m]);
+  }
   const double dead = as_f64((uint64_t)kDeadHi << 32);
   bool keep = n_live > 0;
   if (a.kept < a.G) {  // uniform
     double b1 = dead, b2 = dead;
 #pragma unroll
     for (int m = 0; m < PL; ++m) {
-      const double x = m < n_live ? v[m] : dead;
-      b2 = __builtin_fmax(b2, __builtin_fmin(b1, x));
-      b1 = __builtin_fmax(b1, x);
+      b2 = max_d(b2, min_d(b1, v[m]));
+      b1 = max_d(b1, v[m]);
     }
     run_top2<LPT>(b1, b2, 1 << a.log_run);
     double value = (a.top2 && a.EG > 1) ? group_sum(b1, b2) : b1;
-    if (group >= a.G) value = dead;
+    value = group < a.G ? with_id(value, group) : dead;
     bool in = false;
-    for (int r = 0; r < a.kept; ++r) {
-      const double best = all_max<LPT>(value);
-      const int win = all_min<LPT>(value == best ? group : LPT);
-      if (group == win) {
-        in = true;
-        value = dead;
+    if (LPT == 16 || a.log_run >= 2) {  // uniform
+      // a group is kept if fewer than `kept` groups are above it, counted over
+      // a row's 16 lanes (LPT 64: every fourth lane's value, which meets every
+      // group equally often)
+      double key = value;
+      int shift = a.log_run;
+      if constexpr (LPT == 64) {
+        const uint64_t b = as_u64(value);
+        const int from = 16 * (gi & 15);  // byte address of lane 4 (gi % 16)
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)b);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(b >> 32));
+        key = as_f64((uint64_t)hi << 32 | lo);
+        shift = a.log_run - 2;
+      }
+      int above = key > value ? 1 : 0;
+      count_above<15>(key, value, above);
+      in = above < (a.kept << shift);
+    } else {
+      for (int r = 0; r < a.kept; ++r) {
+        const double best = all_max<LPT>(value);
+        if (value == best) {
+          in = true;
+          value = dead;
+        }
       }
     }
     keep = keep && in;
   }
 #pragma unroll
-  for (int m = 0; m < PL; ++m) v[m] = (keep && m < n_live) ? with_id(v[m], e0 + m) : dead;
-
-  int my_i = 0;
-  for (int k = 0; k < a.K; ++k) {
-    double best = v[0];
-#pragma unroll
-    for (int m = 1; m < PL; ++m) best = __builtin_fmax(best, v[m]);
-    best = all_max<LPT>(best);
-    // K picks fit the kept groups, so a live key is left in every round; the
-    // clamp only keeps the index in range regardless
-    if (gi == k) my_i = min(id_of(best), a.E - 1);
-#pragma unroll
-    for (int m = 0; m < PL; ++m) {
-      const uint64_t b = as_u64(v[m]);
-      const uint32_t hi = v[m] == best ? kDeadHi : (uint32_t)(b >> 32);
-      v[m] = as_f64((uint64_t)hi << 32 | (uint32_t)b);
-    }
+  for (int m = 0; m < PL; ++m) {
+    const double key = with_id(v[m], e0 + m);
+    v[m] = keep ? key : kill(key);
   }
+
+  // the lane's KL best, then the token's
+  double top[KL];
+#pragma unroll
+  for (int i = 0; i < KL; ++i) top[i] = i < PL ? v[i] : dead;
+  sort_list(top);
+#pragma unroll
+  for (int c = KL; c < PL; c += KL) {
+    double more[KL];
+#pragma unroll
+    for (int i = 0; i < KL; ++i) more[i] = c + i < PL ? v[c + i] : dead;
+    sort_list(more);
+    merge_lists(top, more);
+  }
+  merge_lanes<LPT>(top);
+  double mine = top[0];
+#pragma unroll
+  for (int i = 1; i < KL; ++i) mine = gi == i ? top[i] : mine;
+  // K picks fit the kept groups, so no dead key is among the first K; the
+  // clamp only keeps the index in range regardless
+  const int my_i = min(id_of(mine), a.E - 1);
 
   const bool out = gi < a.K;
   if constexpr (SRC == SRC_PARTIALS) {
@@ -391,8 +532,8 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
   // instead of every expert's score kept through the selection)
   double w = 0.0;
   if (out) {
-    const double zi = (double)logit_at<SRC>(a, t, my_i);
-    w = a.score_func == 0 ? exp_f64(zi - (double)mx) * inv : sigmoid_f64(zi);
+    w = score_of(logit_at<SRC>(a, t, my_i), a.score_func == 0, mx, inv);
+    if (a.score_func == 0 && nan != nan) w = __builtin_nan("");
   }
   if (a.renorm) {
     const double total = all_sum<LPT>(w) + (double)a.eps;
@@ -410,9 +551,12 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
 //   g_k = route_scale * grad[k];  S = sum_k s[idx_k] + eps
 //   ds_k = renorm ? g_k / S - (sum_j g_j s[idx_j]) / S^2 : g_k
 //   softmax: dz = s * (ds - sum_k ds_k s[idx_k]);  sigmoid: dz = ds s (1 - s)
-// 32-bit arithmetic (every step is smooth).  LPT lanes per token, lane i the
-// experts i, i + LPT, ...: coalesced.  An index outside [0, E) matches no
-// expert; one that occurs twice adds twice.  One pass over the logits.
+// The differences cancel (a renormalised weight near 1, a softmax score near
+// 1), so scores and sums are 64-bit as in the forward, and dz is rounded once.
+// Lane k holds pick k; only softmax needs a score per expert.  LPT lanes per
+// token, each a run of 4 experts of every 4 LPT: whole 16-byte (bf16: 8-byte)
+// stores where E % 4 == 0.  An index outside [0, E) contributes nothing; one
+// that occurs twice adds twice.
 // ---------------------------------------------------------------------------
 struct TopkBwdArgs {
   const float* grad;   // [T, K]
@@ -422,6 +566,7 @@ struct TopkBwdArgs {
   int score_func, renorm;
   float eps, route_scale;
   void* dz;            // [T, E] in z's type
+  int aligned;         // dz starts at a multiple of 16 bytes
 };
 
 template <int LPT, int PL, bool BF16>
@@ -431,80 +576,94 @@ __global__ __launch_bounds__(256) void topk_backward_kernel(const TopkBwdArgs a)
   const int64_t t_own = (int64_t)blockIdx.x * TPB + threadIdx.x / LPT;
   const bool valid = t_own < a.T;
   const int64_t t = valid ? t_own : a.T - 1;
-  float s[PL], d[PL];
-  float mx = -INFINITY;
-#pragma unroll
-  for (int m = 0; m < PL; ++m) {
-    const int e = gi + m * LPT;
-    s[m] = -INFINITY;
-    if (e < a.E)
-      s[m] = BF16 ? bf16_to_f32(((const bf16_t*)a.z)[t * a.E + e]) : ((const float*)a.z)[t * a.E + e];
-    mx = fmaxf(mx, s[m]);
-    d[m] = 0.f;
+  auto eid = [&](int m) { return 4 * gi + (m & 3) + 4 * LPT * (m >> 2); };
+  auto logit = [&](int e) {
+    return BF16 ? bf16_to_f32(((const bf16_t*)a.z)[t * a.E + e]) : ((const float*)a.z)[t * a.E + e];
+  };
+  // this lane's pick
+  int my_e = -1;
+  double g = 0.0;
+  if (gi < a.K) {
+    const int64_t e = a.idx[t * a.K + gi];
+    if (e >= 0 && e < a.E) {
+      my_e = (int)e;
+      g = (double)a.grad[t * a.K + gi] * (double)a.route_scale;
+    }
   }
+  const float my_z = logit(max(my_e, 0));
+
+  double s[PL];  // softmax: the scores
+  double w;      // the pick's score
   if (a.score_func == 0) {
-    mx = all_maxf<LPT>(mx);
-    float sum = 0.f;
+    float z[PL], mx = -INFINITY;
 #pragma unroll
     for (int m = 0; m < PL; ++m) {
-      s[m] = gi + m * LPT < a.E ? expf(s[m] - mx) : 0.f;
+      z[m] = logit(min(eid(m), a.E - 1));
+      mx = fmaxf(mx, z[m]);  // (a repeated last one changes no maximum)
+    }
+    mx = all_maxf<LPT>(mx);
+    double sum = 0.0;
+#pragma unroll
+    for (int m = 0; m < PL; ++m) {
+      const double x = score_of(z[m], true, mx, 1.0);
+      s[m] = eid(m) < a.E ? x : 0.0;
       sum += s[m];
     }
-    const float inv = 1.f / all_sumf<LPT>(sum);
+    const double inv = __builtin_isfinite(mx) ? rcp_f64(all_sum<LPT>(sum)) : __builtin_nan("");
 #pragma unroll
     for (int m = 0; m < PL; ++m) s[m] *= inv;
+    w = score_of(my_z, true, mx, inv);
   } else {
-#pragma unroll
-    for (int m = 0; m < PL; ++m) s[m] = 1.f / (1.f + expf(-s[m]));
+    w = score_of(my_z, false, 0.f, 1.0);
   }
-  // the lanes' picks: lane k holds pick k (K <= 16 <= LPT)
-  int64_t my = -1;
-  float g = 0.f;
-  if (gi < a.K) {
-    my = a.idx[t * a.K + gi];
-    g = a.grad[t * a.K + gi] * a.route_scale;
-  }
-  const int my_e = (my >= 0 && my < a.E) ? (int)my : -1;
-  // lanes of this token in the wave
-  const int base = lane_id() & ~(LPT - 1);
-  float S = 0.f, gs = 0.f;
+  if (my_e < 0) w = 0.0;
+  double d = g;
   if (a.renorm) {
-    for (int k = 0; k < a.K; ++k) {
-      const int ek = __shfl(my_e, base + k, kWave);
-      const float gk = __shfl(g, base + k, kWave);
-      float v = 0.f;
-#pragma unroll
-      for (int m = 0; m < PL; ++m) v = gi + m * LPT == ek ? s[m] : v;
-      v = all_sumf<LPT>(v);  // one lane holds s[ek]
-      S += v;
-      gs += gk * v;
-    }
-    S += a.eps;
+    const double S = all_sum<LPT>(w) + (double)a.eps, gs = all_sum<LPT>(g * w);
+    d = (g - gs / S) / S;
   }
-  const float sub = a.renorm ? gs / (S * S) : 0.f;
+  if (my_e < 0) d = 0.0;
+  double dot = 0.0;
+  if (a.score_func == 0) dot = all_sum<LPT>(d * w);
+  else d *= w * (1.0 - w);
+
+  // the picks' terms to the lanes of their experts, in pick order
+  double acc[PL];
+#pragma unroll
+  for (int m = 0; m < PL; ++m) acc[m] = 0.0;
+  const int base = lane_id() & ~(LPT - 1);  // lanes of this token in the wave
   for (int k = 0; k < a.K; ++k) {
     const int ek = __shfl(my_e, base + k, kWave);
-    const float gk = __shfl(g, base + k, kWave);
-    const float dk = a.renorm ? gk / S - sub : gk;
+    const double dk = __shfl(d, base + k, kWave);
 #pragma unroll
-    for (int m = 0; m < PL; ++m) d[m] += gi + m * LPT == ek ? dk : 0.f;
-  }
-  float dot = 0.f;
-  if (a.score_func == 0) {
-#pragma unroll
-    for (int m = 0; m < PL; ++m) dot += d[m] * s[m];
-    dot = all_sumf<LPT>(dot);
+    for (int m = 0; m < PL; ++m) acc[m] += eid(m) == ek ? dk : 0.0;
   }
   if (!valid) return;
+  const bool quads = (a.E & 3) == 0 && a.aligned;
 #pragma unroll
-  for (int m = 0; m < PL; ++m) {
-    const int e = gi + m * LPT;
-    if (e >= a.E) continue;
-    const float r = a.score_func == 0 ? s[m] * (d[m] - dot) : d[m] * s[m] * (1.f - s[m]);
-    if constexpr (BF16)
-      ((bf16_t*)a.dz)[t * a.E + e] = (bf16_t)f32_to_bf16(r);
-    else
-      ((float*)a.dz)[t * a.E + e] = r;
+  for (int m = 0; m < PL; m += 4) {
+    float r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (float)(a.score_func == 0 ? s[m + i] * (acc[m + i] - dot) : acc[m + i]);
+    const int64_t at = t * a.E + eid(m);
+    if (quads) {
+      if (eid(m) < a.E) {
+        if constexpr (BF16)
+          *(uint2*)((bf16_t*)a.dz + at) = make_uint2(pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]));
+        else
+          *(float4*)((float*)a.dz + at) = make_float4(r[0], r[1], r[2], r[3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (eid(m + i) < a.E) {
+          if constexpr (BF16)
+            ((bf16_t*)a.dz)[at + i] = (bf16_t)f32_to_bf16(r[i]);
+          else
+            ((float*)a.dz)[at + i] = r[i];
+        }
+      }
+    }
   }
 }
 
@@ -514,13 +673,17 @@ int log2_ceil(int v) {
   return n;
 }
 
-template <int LPT, int PL>
-hipError_t go_group(int src, const GroupTopkArgs& a, hipStream_t stream) {
+template <int LPT, int PL, int KL>
+hipError_t go_source(int src, const GroupTopkArgs& a, hipStream_t stream) {
   constexpr int TPB = 256 / LPT;
   const dim3 grid((unsigned)((a.T + TPB - 1) / TPB));
-  if (src == SRC_F32) return launch_k(false, group_topk_kernel<LPT, PL, SRC_F32>, grid, dim3(256), 0, stream, a);
-  if (src == SRC_BF16) return launch_k(false, group_topk_kernel<LPT, PL, SRC_BF16>, grid, dim3(256), 0, stream, a);
-  return launch_k(false, group_topk_kernel<LPT, PL, SRC_PARTIALS>, grid, dim3(256), 0, stream, a);
+  if (src == SRC_F32) return launch_k(false, group_topk_kernel<LPT, PL, KL, SRC_F32>, grid, dim3(256), 0, stream, a);
+  if (src == SRC_BF16) return launch_k(false, group_topk_kernel<LPT, PL, KL, SRC_BF16>, grid, dim3(256), 0, stream, a);
+  return launch_k(false, group_topk_kernel<LPT, PL, KL, SRC_PARTIALS>, grid, dim3(256), 0, stream, a);
+}
+template <int LPT, int PL>
+hipError_t go_group(int src, const GroupTopkArgs& a, hipStream_t stream) {
+  return a.K <= 8 ? go_source<LPT, PL, 8>(src, a, stream) : go_source<LPT, PL, 16>(src, a, stream);
 }
 
 // Experts per lane with LPT lanes per token: every group an equal
@@ -533,21 +696,22 @@ int experts_per_lane(int lpt, int G, int EG, int* log_run) {
 }
 
 hipError_t launch_group_topk(int src, GroupTopkArgs a, hipStream_t stream) {
-  // A wave per token while there are few tokens (its chain of rounds is
-  // short), four tokens per wave where issue slots count.
+  // 16 lanes per token while they hold at most 4 experts each, and wherever
+  // issue slots count; a wave per token in between, whose lists are shorter
+  // to build.  Measured (us, 16 lanes / 64): E = 256, 8 groups, 1024 tokens
+  // 6.4 / 4.4, 2048 6.5 / 5.6, 4096 6.7 / 8.0, 16384 14.6 / 23.1; E = 160,
+  // 1024 5.6 / 4.5, 2048 5.7 / 5.9; E = 64, 32 tokens 3.6 / 4.2.
   int lr16 = 0, lr64 = 0;
   const int p16 = experts_per_lane(16, a.G, a.EG, &lr16), p64 = experts_per_lane(64, a.G, a.EG, &lr64);
-  const bool narrow = p16 > 0 && p16 <= 16 && a.T > kGroupWaveTokens;
+  const bool narrow = p16 > 0 && p16 <= 16 && (p16 <= 4 || a.T > 160 * p16);
   a.log_run = narrow ? lr16 : lr64;
   a.per_lane = narrow ? p16 : p64;
   if (narrow) {
-    if (p16 <= 2) return go_group<16, 2>(src, a, stream);
     if (p16 <= 4) return go_group<16, 4>(src, a, stream);
     if (p16 <= 8) return go_group<16, 8>(src, a, stream);
     if (p16 <= 12) return go_group<16, 12>(src, a, stream);
     return go_group<16, 16>(src, a, stream);
   }
-  if (p64 <= 2) return go_group<64, 2>(src, a, stream);
   if (p64 <= 4) return go_group<64, 4>(src, a, stream);
   if (p64 <= 8) return go_group<64, 8>(src, a, stream);
   if (p64 <= 16) return go_group<64, 16>(src, a, stream);
@@ -595,6 +759,7 @@ hipError_t launch_router_topk_backward(const float* grad, const int64_t* idx, co
   a.grad = grad, a.idx = idx, a.z = logits, a.T = T, a.E = E, a.K = K;
   a.score_func = score_func, a.renorm = renorm, a.eps = renorm_eps, a.route_scale = route_scale;
   a.dz = grad_logits;
+  a.aligned = ((uintptr_t)grad_logits & 15) == 0;
   auto go = [&](auto lpt, auto pl) {
     constexpr int LPT = decltype(lpt)::value, PL = decltype(pl)::value;
     const dim3 grid((unsigned)((T + 256 / LPT - 1) / (256 / LPT)));
