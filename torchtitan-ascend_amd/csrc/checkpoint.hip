@@ -108,8 +108,9 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const uint4* __restrict_
   }
 }
 
-// One row per wave pass: 8 columns per lane and step.  The first n_ids
-// threads of the grid also resolve the routed rows' ids.
+// 8 columns per lane and step.  With n_ids > 0 the grid also resolves the
+// routed rows' ids, and pads them by 64 for the GEMM that reads them a stage
+// at a time.
 template <bool SCALE>
 __global__ __launch_bounds__(256) void unpack_rows_kernel(const uint2* __restrict__ codes,
                                                           const uint8_t* __restrict__ exps, int n_src,
@@ -119,7 +120,10 @@ __global__ __launch_bounds__(256) void unpack_rows_kernel(const uint2* __restric
                                                           const int* __restrict__ ids_index, int* __restrict__ ids_out,
                                                           int n_ids) {
   const uint32_t threads = gridDim.x * 256, t0 = blockIdx.x * 256 + threadIdx.x;
-  for (uint32_t i = t0; i < (uint32_t)n_ids; i += threads) ids_out[i] = min(max(ids_index[i] / src_div, 0), n_src - 1);
+  if (n_ids > 0) {
+    for (uint32_t i = t0; i < (uint32_t)n_ids + 64; i += threads)
+      ids_out[i] = i < (uint32_t)n_ids ? min(max(ids_index[i] / src_div, 0), n_src - 1) : 0;
+  }
   for (uint32_t i0 = t0; i0 < total; i0 += kUnroll * threads) {
     uint2 q[kUnroll];
     int e[kUnroll];

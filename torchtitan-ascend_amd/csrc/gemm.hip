@@ -477,7 +477,7 @@ hipError_t launch_grouped_mm_dgrad_swiglu_packed(const void* dy, const void* w2,
 // bf16 rows of the tokens (gathered inside the GEMM's loads) or, with a row
 // scale, of the routed rows; then row ids; then the GEMM's workspace.
 size_t wgrad_packed_workspace_bytes(int64_t rows, int64_t M, int E, int64_t K) {
-  return al256((size_t)rows * K * 2) + al256((size_t)M * 4) + gemm_workspace_bytes(M, E);
+  return al256((size_t)rows * K * 2) + al256((size_t)(M + 64) * 4) + gemm_workspace_bytes(M, E);
 }
 
 hipError_t launch_grouped_mm_wgrad_packed(const void* dy, const void* codes, const void* exps, int n_src,
@@ -486,11 +486,11 @@ hipError_t launch_grouped_mm_wgrad_packed(const void* dy, const void* codes, con
                                           hipStream_t stream) {
   // A token's row is unpacked once, however many experts read it; only a
   // scale per routed row needs the routed rows themselves.
-  const bool gather = src_index != nullptr && row_scale == nullptr;
+  const bool gather = src_index != nullptr && row_scale == nullptr && M > 0;
   const int rows = gather ? n_src : M;
   char* x = (char*)ws;
   int* ids = (int*)(x + al256((size_t)rows * K * 2));
-  void* gws = (char*)ids + al256((size_t)M * 4);
+  void* gws = (char*)ids + al256((size_t)(M + 64) * 4);
   hipError_t err = launch_unpack_rows(codes, exps, n_src, gather ? nullptr : src_index, src_div, row_scale, rows, K, x,
                                       gather ? src_index : nullptr, gather ? ids : nullptr, gather ? M : 0, stream);
   if (err != hipSuccess) return err;

@@ -278,7 +278,7 @@ struct WgradDmaArgs {
   int64_t lddy;
   const bf16_t* x;  // [M][K]
   int64_t ldx;
-  const int* x_rows;  // nullable, [M]: reduction row m reads x row x_rows[m] (in range: the caller's)
+  const int* x_rows;  // nullable, [M + 64]: reduction row m reads x row x_rows[m]; all in range, M > 0
   const int* offs;  // inclusive, [E]
   int E, M, N, K;
   int n_tiles, k_tiles;  // per expert, 256-wide

@@ -76,7 +76,10 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4_t lds_short4_t;
 typedef __attribute__((address_space(1))) int gint_t;
 typedef __attribute__((address_space(1))) floatx4_t gfloatx4_t;
-typedef const __attribute__((address_space(4))) int cint_t;  // read only while the kernel runs: scalar loads
+// read only while the kernel runs: scalar loads
+typedef __attribute__((address_space(4))) int cint_t;
+typedef int int2u_t __attribute__((ext_vector_type(2), aligned(4)));
+typedef __attribute__((address_space(4))) int2u_t cint2_t;
 
 // Chunk permutation of a row (as gemm_fwd.hip's reduction-major weights).
 __device__ __forceinline__ int ptswz(int m) { return 2 * ((m & 3) | ((m >> 2) & 4)); }
@@ -92,8 +95,8 @@ __device__ __forceinline__ void static_for(F&& f) {
 
 // GATHER: reduction row m is x row x_rows[m] (a token that several experts
 // read).  A wave moves two rows per x instruction, so a stage's row ids are
-// eight scalar loads, made when the cursor reaches the stage, one stage ahead
-// of the instructions that use them.
+// scalar loads, made when the cursor reaches the stage, one stage ahead of the
+// instructions that use them.
 template <bool GATHER>
 __global__ __launch_bounds__(THREADS, 1) void gg_wgrad_dma_kernel(const WgradDmaArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -183,20 +186,20 @@ __global__ __launch_bounds__(THREADS, 1) void gg_wgrad_dma_kernel(const WgradDma
   };
   const int m_max = max(a.M - 1, 0);
   auto row_of = [&](int i) { return min(max(min(d_mstage + d_row + 2 * WAVES * i, d_last), 0), m_max); };
-  // GATHER: x rows of the cursor's stage, instruction i rows 2 i and 2 i + 1
-  int g_row[2 * DMA_OP];
+  // GATHER: x rows of the cursor's stage, instruction i rows g_row[i][0..1].
+  // Rows past the expert's (another's, or the padding of the id array) are as
+  // readable as its own and masked like the clamped ones of the other form, so
+  // a stage's ids are four loads at fixed distances.
+  int2u_t g_row[DMA_OP];
   auto gather_rows = [&]() {
     if constexpr (GATHER) {
-      const int m0 = c_t.m0 + TK * c_ks + 2 * w, last = max(min(c_t.m1 - 1, m_max), 0);
+      const cint_t* ids = (const cint_t*)a.x_rows + __builtin_amdgcn_readfirstlane(c_t.m0 + TK * c_ks + 2 * w);
 #pragma unroll
-      for (int i = 0; i < 2 * DMA_OP; ++i) {
-        const int m = min(max(m0 + 2 * WAVES * (i >> 1) + (i & 1), 0), last);
-        g_row[i] = a.M > 0 ? ((cint_t*)a.x_rows)[__builtin_amdgcn_readfirstlane(m)] : 0;
-      }
+      for (int i = 0; i < DMA_OP; ++i) g_row[i] = *(const cint2_t*)(ids + 2 * WAVES * i);
     }
   };
   auto issue_x = [&](int i) {
-    const int row = GATHER ? ((l >> 5) ? g_row[2 * i + 1] : g_row[2 * i]) : row_of(i);
+    const int row = GATHER ? ((l >> 5) ? g_row[i][1] : g_row[i][0]) : row_of(i);
     const uint32_t voff = (uint32_t)row * (uint32_t)(a.ldx * 2) + (((d_chunk ^ (8 * (i & 1))) & d_xmask) << 4);
     dma16(voff, d_xb, d_st + i * (WAVES * 1024));
   };

@@ -177,7 +177,8 @@ hipError_t launch_grouped_mm_dgrad_swiglu(const void* dy, const void* w2, const 
                                           hipStream_t stream);
 // ws: NULL (no tail split) or gemm_workspace_bytes(M, E) bytes (the
 // leftover tiles' partial sums and arrival counters).
-// x_rows (nullable, [M]): reduction row m reads x row x_rows[m].
+// x_rows (nullable, [M + 64], every entry a row of x): reduction row m reads x
+// row x_rows[m].
 hipError_t launch_grouped_mm_wgrad(const void* dy, const void* x, const int* offs, int M, int E,
                                    int N, int K, void* dw, bool fp32, void* ws, hipStream_t stream,
                                    const int* x_rows = nullptr);
@@ -187,7 +188,7 @@ hipError_t launch_grouped_mm_wgrad(const void* dy, const void* x, const int* off
 hipError_t launch_pack_rows(const void* in, int64_t R, int C, void* codes, void* exps, hipStream_t stream);
 // out row j = row src_index[j] / src_div of n_src (nullable -> j), times
 // row_scale[j] (nullable).  ids_out[j] (nullable) = the clamped row of
-// ids_index[j], j < n_ids.
+// ids_index[j], j < n_ids, and row 0 in the 64 entries after them.
 hipError_t launch_unpack_rows(const void* codes, const void* exps, int n_src, const int* src_index, int src_div,
                               const float* row_scale, int64_t R, int C, void* out, const int* ids_index, int* ids_out,
                               int n_ids, hipStream_t stream);

@@ -77,7 +77,7 @@ def _limit(swiglu_limit: float | None) -> float:
 def _call(dev: torch.device, name: str, *args) -> None:
     """_lib.call with `dev` as the current device: a kernel launches on the
     device of its tensors whichever device is current."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
+    if dev.index is None or dev.index == torch._C._cuda_getDevice():  # (a tensor of dev exists: HIP is initialised)
         _lib.call(name, *args)
         return
     with torch.cuda.device(dev):
@@ -689,42 +689,41 @@ def sum_topk(y: torch.Tensor, top_k: int) -> torch.Tensor:
 _F32_STREAM, _F32_POST, _F32_GATE, _F32_PRE = 1, 2, 4, 8
 
 
-def _float_kind(name: str, t: torch.Tensor) -> bool:
-    """Whether t is fp32 (else bf16)."""
-    if t.dtype not in (_BF16, torch.float32):
-        raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
-    return t.dtype == torch.float32
+def _float_operand(name: str, t: torch.Tensor, dev: torch.device, shape: tuple) -> tuple[torch.Tensor, bool]:
+    """(t contiguous, whether it is fp32) of a bf16 or fp32 operand of the given shape."""
+    if t.device != dev:
+        raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    dt = t.dtype
+    if dt is not _BF16 and dt is not torch.float32:
+        raise TypeError(f"{name} must be bfloat16 or float32, got {dt}")
+    return t.contiguous(), dt is torch.float32
 
 
 def _norm_operands(dev, T, D, residual, post_weight, gate, gate_func, pre_weight):
     """Checked operands of a block norm: (residual, post_weight, gate,
     gate kind, sigmoid, pre_weight, fp32 mask)."""
-    _same_device(dev, residual=residual, post_weight=post_weight, gate=gate, pre_weight=pre_weight)
-    mask = 0
+    mask = kind = 0
     if residual is not None:
-        if tuple(residual.shape) != (T, D):
-            raise ValueError(f"residual must be [{T}, {D}], got {tuple(residual.shape)}")
-        mask |= _F32_STREAM * _float_kind("residual", residual)
-        residual = residual.contiguous()
-    for name, w, bit in (("post_weight", post_weight, _F32_POST), ("pre_weight", pre_weight, _F32_PRE)):
-        if w is not None:
-            if tuple(w.shape) != (D,):
-                raise ValueError(f"{name} must be [{D}], got {tuple(w.shape)}")
-            mask |= bit * _float_kind(name, w)
-    post_weight = None if post_weight is None else post_weight.contiguous()
-    pre_weight = None if pre_weight is None else pre_weight.contiguous()
-    if gate_func not in ("identity", "sigmoid"):
+        residual, wide = _float_operand("residual", residual, dev, (T, D))
+        mask = _F32_STREAM if wide else 0
+    if post_weight is not None:
+        post_weight, wide = _float_operand("post_weight", post_weight, dev, (D,))
+        mask |= _F32_POST if wide else 0
+    if pre_weight is not None:
+        pre_weight, wide = _float_operand("pre_weight", pre_weight, dev, (D,))
+        mask |= _F32_PRE if wide else 0
+    if gate_func != "identity" and gate_func != "sigmoid":
         raise ValueError(f"gate_func must be 'identity' or 'sigmoid', got {gate_func!r}")
-    kind = 0
     if gate is not None:
-        kinds = {(T, 1): 1, (1, D): 2, (T, D): 3}
-        if T == 1:
-            kinds = {(1, 1): 1, (1, D): 2}
-        if tuple(gate.shape) not in kinds:
-            raise ValueError(f"gate must be [{T}, 1], [1, {D}] or [{T}, {D}], got {tuple(gate.shape)}")
-        kind = kinds[tuple(gate.shape)]
-        mask |= _F32_GATE * _float_kind("gate", gate)
-        gate = gate.contiguous()
+        # one token's [1, D] gate is per channel and per element alike
+        shape = tuple(gate.shape)
+        kind = 1 if shape == (T, 1) else 2 if shape == (1, D) else 3 if shape == (T, D) else 0
+        if kind == 0:
+            raise ValueError(f"gate must be [{T}, 1], [1, {D}] or [{T}, {D}], got {shape}")
+        gate, wide = _float_operand("gate", gate, dev, shape)
+        mask |= _F32_GATE if wide else 0
     return residual, post_weight, gate, kind, int(gate_func == "sigmoid"), pre_weight, mask
 
 
@@ -737,8 +736,7 @@ def _residual_norm(dev, rows, T, D, top_k, inverse, probs, residual, post_weight
     stats = torch.empty(2, T, dtype=torch.float32, device=dev) if save_stats else None
     _call(
         dev, "ttamd_residual_norm", _p(rows), _p(inverse), _p(probs), T, D, top_k, _p(residual), _p(post_weight),
-        _p(gate), kind, sig, float(residual_scale), _p(pre_weight), float(eps), mask, _p(u), _p(n), _p(stats),
-        _stream(dev),
+        _p(gate), kind, sig, residual_scale, _p(pre_weight), eps, mask, _p(u), _p(n), _p(stats), _stream(dev),
     )
     return u, n, stats
 
@@ -812,7 +810,8 @@ def combine_norm(
     rows = _want("rows", rows, _BF16)
     M, D = rows.shape
     T = M // top_k
-    _same_device(dev, inverse=inverse, probs=probs)
+    if inverse is not None or probs is not None:
+        _same_device(dev, inverse=inverse, probs=probs)
     if inverse is not None:
         inverse = _want("inverse", inverse.reshape(-1), torch.int32)
         if inverse.numel() != M:
