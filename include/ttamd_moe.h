@@ -537,6 +537,25 @@ int ttamd_moe_experts_forward(const void* tokens, int64_t num_tokens,
                               void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/*
+ * ttamd_moe_experts_forward without the K-way sum at its end: out bf16
+ * [T * topk, D], row t * topk + k the (weighted) output of token t's k-th
+ * expert, for a combine that does more (ttamd_residual_norm).  Everything else
+ * as there.
+ */
+size_t ttamd_moe_experts_rows_workspace_bytes(int64_t num_tokens, int64_t dim,
+                                              int64_t hidden, int num_experts,
+                                              int topk,
+                                              int score_before_experts);
+int ttamd_moe_experts_rows(const void* tokens, int64_t num_tokens, int64_t dim,
+                           int64_t hidden, int num_experts, int topk,
+                           const int32_t* sorted_indices, const int32_t* offs,
+                           const float* sorted_scores, int score_before_experts,
+                           float swiglu_limit, const void* w13, const void* w2,
+                           void* out, void* gemm_plan, size_t gemm_plan_bytes,
+                           void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 /* ------------------------------------------------------------------------ *
  * Norms before and after the block, with its gate, its residual scale and    *
  * the combine.  The reference norms with npu_rms_norm and adds the residual  *

@@ -10,7 +10,7 @@ The directory name is not a Python identifier; import it with
 `importlib.import_module("torchtitan-ascend_amd")`.  Importing it has no
 side effects: nothing is patched, nothing is loaded until an op runs.
 """
-from .functional import HIPMoeTokenUnpermute, moe_experts_forward, run_experts_grouped_mm
+from .functional import HIPMoeTokenUnpermute, moe_block, moe_experts_forward, run_experts_grouped_mm
 from .grouped_experts import HipGroupedExperts, HipGroupedExpertsConverter
 from .protocol import HAVE_TORCHTITAN
 from . import state_dict
@@ -24,6 +24,7 @@ __all__ = [
     "HipGroupedExpertsConverter",
     "HipTokenDispatcher",
     "HipTokenDispatcherConverter",
+    "moe_block",
     "moe_experts_forward",
     "run_experts_grouped_mm",
     "state_dict",

@@ -132,6 +132,12 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _i64, _i64, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _f32, _c_void_p,
          _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p, _sz, _c_void_p],
     ),
+    "ttamd_moe_experts_rows_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32, _i32]),
+    "ttamd_moe_experts_rows": (
+        _i32,
+        [_c_void_p, _i64, _i64, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _f32, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p, _sz, _c_void_p],
+    ),
     "ttamd_residual_norm": (
         _i32,
         [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _f32,

@@ -201,6 +201,47 @@ int router_route(const char* fn, const ttamd::RouterGroups* groups, const void* 
                    fn);
 }
 
+// The expert stage, with or without the K-way sum at its end.
+int experts_stage(const char* fn, bool rows, const void* tokens, int64_t num_tokens, int64_t dim, int64_t hidden,
+                  int num_experts, int topk, const int32_t* sorted_indices, const int32_t* offs,
+                  const float* sorted_scores, int score_before_experts, float swiglu_limit,
+                  const void* w13, const void* w2, void* out, void* gemm_plan,
+                  size_t gemm_plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  REQUIRE(topk >= 1 && topk <= 64, "%s: topk must be in [1, 64]", fn);
+  REQUIRE(num_tokens >= 0 && num_tokens * topk <= (1 << 28), "%s: num_tokens out of range", fn);
+  const int64_t M = num_tokens * topk;
+  TRY(check_gemm_common(fn, offs, M, num_experts));
+  TRY(check_dim(fn, "dim", dim, 128));
+  TRY(check_dim(fn, "hidden", hidden, 64));
+  REQUIRE(std::isnan(swiglu_limit) || swiglu_limit >= 0.f, "%s: swiglu_limit must be NaN (no clamp) or >= 0",
+          fn);
+  REQUIRE(w13 && aligned16(w13) && w2 && aligned16(w2), "%s: w13 and w2 must be non-null and 16-byte aligned",
+          fn);
+  REQUIRE(num_tokens * dim * 2 <= (int64_t)0xffffffffLL, "%s: tokens must stay below 4 GiB", fn);
+  TRY(check_rows(fn, "tokens", tokens, num_tokens, dim));
+  TRY(check_rows(fn, "out", out, rows ? M : num_tokens, dim));
+  REQUIRE(M * (dim / 8) <= (int64_t(1) << 30) && M * (hidden / 8) <= (int64_t(1) << 30),
+          "%s: too many routed elements (%lld rows)", fn, (long long)M);
+  if (M > 0) REQUIRE(sorted_indices != nullptr, "%s: sorted_indices is null", fn);
+  REQUIRE(score_before_experts == 0 || sorted_scores != nullptr || M == 0,
+          "%s: score_before_experts needs sorted_scores", fn);
+  if (gemm_plan) {
+    REQUIRE(aligned16(gemm_plan), "%s: gemm_plan must be 16-byte aligned", fn);
+    REQUIRE(gemm_plan_bytes >= ttamd::gemm_plan_bytes(M, num_experts),
+            "%s: gemm_plan too small (%zu bytes, need %zu)", fn, gemm_plan_bytes,
+            ttamd::gemm_plan_bytes(M, num_experts));
+  }
+  TRY(check_ws(fn, workspace, workspace_bytes,
+               ttamd::moe_experts_forward_workspace_bytes(num_tokens, dim, hidden, num_experts, topk,
+                                                          score_before_experts != 0 || dim < 128, rows)));
+  if (M == 0) return TTAMD_OK;
+  return check_hip(ttamd::launch_moe_experts_forward(tokens, (int)num_tokens, (int)dim, (int)hidden, num_experts,
+                                                     topk, sorted_indices, offs, sorted_scores,
+                                                     score_before_experts != 0, swiglu_limit, w13, w2, out,
+                                                     gemm_plan, workspace, (hipStream_t)stream, rows),
+                   fn);
+}
+
 }  // namespace
 
 extern "C" {
@@ -427,40 +468,26 @@ int ttamd_moe_experts_forward(const void* tokens, int64_t num_tokens, int64_t di
                               const float* sorted_scores, int score_before_experts, float swiglu_limit,
                               const void* w13, const void* w2, void* out, void* gemm_plan,
                               size_t gemm_plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* fn = "ttamd_moe_experts_forward";
-  REQUIRE(topk >= 1 && topk <= 64, "%s: topk must be in [1, 64]", fn);
-  REQUIRE(num_tokens >= 0 && num_tokens * topk <= (1 << 28), "%s: num_tokens out of range", fn);
-  const int64_t M = num_tokens * topk;
-  TRY(check_gemm_common(fn, offs, M, num_experts));
-  TRY(check_dim(fn, "dim", dim, 128));
-  TRY(check_dim(fn, "hidden", hidden, 64));
-  REQUIRE(std::isnan(swiglu_limit) || swiglu_limit >= 0.f, "%s: swiglu_limit must be NaN (no clamp) or >= 0",
-          fn);
-  REQUIRE(w13 && aligned16(w13) && w2 && aligned16(w2), "%s: w13 and w2 must be non-null and 16-byte aligned",
-          fn);
-  REQUIRE(num_tokens * dim * 2 <= (int64_t)0xffffffffLL, "%s: tokens must stay below 4 GiB", fn);
-  TRY(check_rows(fn, "tokens", tokens, num_tokens, dim));
-  TRY(check_rows(fn, "out", out, num_tokens, dim));
-  REQUIRE(M * (dim / 8) <= (int64_t(1) << 30) && M * (hidden / 8) <= (int64_t(1) << 30),
-          "%s: too many routed elements (%lld rows)", fn, (long long)M);
-  if (M > 0) REQUIRE(sorted_indices != nullptr, "%s: sorted_indices is null", fn);
-  REQUIRE(score_before_experts == 0 || sorted_scores != nullptr || M == 0,
-          "%s: score_before_experts needs sorted_scores", fn);
-  if (gemm_plan) {
-    REQUIRE(aligned16(gemm_plan), "%s: gemm_plan must be 16-byte aligned", fn);
-    REQUIRE(gemm_plan_bytes >= ttamd::gemm_plan_bytes(M, num_experts),
-            "%s: gemm_plan too small (%zu bytes, need %zu)", fn, gemm_plan_bytes,
-            ttamd::gemm_plan_bytes(M, num_experts));
-  }
-  TRY(check_ws(fn, workspace, workspace_bytes,
-               ttamd_moe_experts_forward_workspace_bytes(num_tokens, dim, hidden, num_experts, topk,
-                                                         score_before_experts)));
-  if (M == 0) return TTAMD_OK;
-  return check_hip(ttamd::launch_moe_experts_forward(tokens, (int)num_tokens, (int)dim, (int)hidden, num_experts,
-                                                     topk, sorted_indices, offs, sorted_scores,
-                                                     score_before_experts != 0, swiglu_limit, w13, w2, out,
-                                                     gemm_plan, workspace, (hipStream_t)stream),
-                   fn);
+  return experts_stage("ttamd_moe_experts_forward", false, tokens, num_tokens, dim, hidden, num_experts, topk, sorted_indices, offs,
+                       sorted_scores, score_before_experts, swiglu_limit, w13, w2, out, gemm_plan, gemm_plan_bytes,
+                       workspace, workspace_bytes, stream);
+}
+
+size_t ttamd_moe_experts_rows_workspace_bytes(int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts,
+                                              int topk, int score_before_experts) {
+  if (num_tokens < 0 || dim < 1 || hidden < 1 || num_experts < 1 || topk < 1) return 0;
+  return ttamd::moe_experts_forward_workspace_bytes(num_tokens, dim, hidden, num_experts, topk,
+                                                    score_before_experts != 0 || dim < 128, true);
+}
+
+int ttamd_moe_experts_rows(const void* tokens, int64_t num_tokens, int64_t dim, int64_t hidden,
+                           int num_experts, int topk, const int32_t* sorted_indices, const int32_t* offs,
+                           const float* sorted_scores, int score_before_experts, float swiglu_limit,
+                           const void* w13, const void* w2, void* out, void* gemm_plan,
+                           size_t gemm_plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  return experts_stage("ttamd_moe_experts_rows", true, tokens, num_tokens, dim, hidden, num_experts, topk, sorted_indices, offs,
+                       sorted_scores, score_before_experts, swiglu_limit, w13, w2, out, gemm_plan, gemm_plan_bytes,
+                       workspace, workspace_bytes, stream);
 }
 
 int ttamd_moe_gather_rows(const void* in, const int32_t* src_index, const float* row_scale,

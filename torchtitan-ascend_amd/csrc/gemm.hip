@@ -283,20 +283,21 @@ hipError_t launch_grouped_mm_unpermute(const void* act, const void* w2, const in
 }
 
 // ---- the expert stage of the MoE layer forward in one call ---------------------
-size_t moe_experts_forward_workspace_bytes(int64_t T, int64_t D, int64_t H, int E, int K, bool permute_first) {
+size_t moe_experts_forward_workspace_bytes(int64_t T, int64_t D, int64_t H, int E, int K, bool permute_first,
+                                           bool rows) {
   const int64_t M = T * K;
   auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
   size_t n = al(gemm_workspace_bytes(M, E));                 // tile plan
   n += al((size_t)M * H * 2);                                // a = swiglu(x w13^T)
   if (permute_first) n += al((size_t)M * D * 2);             // routed rows
-  if (K > 1) n += al((size_t)M * D * 2);                     // y in flat-slot order
+  if (K > 1 && !rows) n += al((size_t)M * D * 2);            // y in flat-slot order
   return n;
 }
 
 hipError_t launch_moe_experts_forward(const void* tokens, int T, int D, int H, int E, int K,
                                       const int* sorted_idx, const int* offs, const float* sorted_scores,
                                       bool score_before, float limit, const void* w13, const void* w2,
-                                      void* out, void* plan, void* ws, hipStream_t stream) {
+                                      void* out, void* plan, void* ws, hipStream_t stream, bool rows) {
   const int M = T * K;
   const bool permute_first = score_before || D < 128;
   auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -310,7 +311,7 @@ hipError_t launch_moe_experts_forward(const void* tokens, int T, int D, int H, i
     routed = p;
     p += al((size_t)M * D * 2);
   }
-  void* y = (K > 1) ? (void*)p : out;
+  void* y = (K > 1 && !rows) ? (void*)p : out;
   hipError_t err;
   // one tile table for both GEMMs
   void* tp = plan;
@@ -339,7 +340,7 @@ hipError_t launch_moe_experts_forward(const void* tokens, int T, int D, int H, i
   g2.dest = sorted_idx;
   g2.n_dest = (K > 1) ? M : T;
   if ((err = fwd(EPI_SCATTER, g2, offs, E, M, tp, part, stream, true)) != hipSuccess) return err;
-  if (K > 1) return launch_combine(y, nullptr, nullptr, T, K, D, out, stream);
+  if (K > 1 && !rows) return launch_combine(y, nullptr, nullptr, T, K, D, out, stream);
   return hipSuccess;
 }
 

@@ -160,12 +160,14 @@ hipError_t launch_shared_expert_add(const void* x, int T, int D, int H, const vo
                                    void* ws, hipStream_t stream);
 // The expert stage of the inference forward: (gather [+ score] ->) w13 +
 // SwiGLU -> w2 + score + scatter (-> K-way sum), both GEMMs on one tile
-// table (`plan`, or one built into the workspace when plan is null).
-size_t moe_experts_forward_workspace_bytes(int64_t T, int64_t D, int64_t H, int E, int K, bool permute_first);
+// table (`plan`, or one built into the workspace when plan is null).  rows:
+// `out` takes the weighted rows in flat-slot order, without the K-way sum.
+size_t moe_experts_forward_workspace_bytes(int64_t T, int64_t D, int64_t H, int E, int K, bool permute_first,
+                                           bool rows = false);
 hipError_t launch_moe_experts_forward(const void* tokens, int T, int D, int H, int E, int K,
                                       const int* sorted_idx, const int* offs, const float* sorted_scores,
                                       bool score_before, float limit, const void* w13, const void* w2,
-                                      void* out, void* plan, void* ws, hipStream_t stream);
+                                      void* out, void* plan, void* ws, hipStream_t stream, bool rows = false);
 hipError_t launch_grouped_mm_dgrad(const void* dy, const void* w, const int* offs, int M, int E,
                                    int N, int K, void* dx, void* ws, hipStream_t stream);
 // The same without the tail split: plan is gemm_plan_bytes(M, E) bytes.

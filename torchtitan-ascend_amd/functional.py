@@ -14,7 +14,9 @@ on its own:
   combine   (upstream combine, npu_gmm.py:110)
       out[t] = sum_k (score[t,k] if score after experts else 1) * y[pos(t,k)]
 
-plus the reference's own NPUMoeTokenUnpermute (npu_permute.py:15-53).
+plus the reference's own NPUMoeTokenUnpermute (npu_permute.py:15-53), the
+norms around the block (models/common/npu_rmsnorm.py:15-37) and `moe_block`,
+the whole of them.
 `moe_experts_forward` chains them; without autograd it takes the fused
 inference op (one C-ABI call for the whole expert stage).
 """
@@ -205,8 +207,16 @@ def moe_experts_forward(
     score_before_experts: bool,
     swiglu_limit: float | None = None,
     stage_events: dict | None = None,
+    checkpoint: str | None = None,
 ) -> torch.Tensor:
     """dispatch -> experts -> combine for one GPU; x [T, D], scores/indices [T, K] -> [T, D].
+
+    ``checkpoint="e4m3"`` keeps the activations that the backward needs in 8
+    bits (x, the pre-activation and the experts' outputs, packed by
+    ops.pack_e4m3): about a third of the bf16 ones' memory (a quarter with
+    many choices per token).  The output is the same; the weights' and the
+    scores' gradients are those at the stored values, within e4m3's 2^-4 of
+    each activation.
 
     With autograd off (or nothing requiring grad) the expert stage is one
     op (ttamd::moe_experts_forward: both grouped GEMMs on one tile table,
@@ -266,10 +276,70 @@ def moe_experts_forward(
             out = ops.sum_topk(ybuf, K)
             mark("sum_topk", True)
         return out.to(x.dtype)
+    if checkpoint is not None:
+        if checkpoint != "e4m3":
+            raise ValueError(f"checkpoint must be 'e4m3' or None, got {checkpoint!r}")
+        keep_y = not score_before_experts and scores_flat.requires_grad
+        out = _T.experts_packed(xb, scores_flat, sorted_idx, inverse, sorted_scores, offs, w13, w2, K,
+                                score_before_experts, swiglu_limit, keep_y)[0]
+        return out.to(x.dtype)
     routed = dispatch(xb, scores_flat, sorted_idx, inverse, sorted_scores, K, score_before_experts)
     y = experts(routed, w13, w2, offs, swiglu_limit)
     out = combine(y, scores_flat, sorted_idx, inverse, K, not score_before_experts)
     return out.to(x.dtype)
+
+
+def moe_block(
+    x: torch.Tensor,
+    w_router: torch.Tensor,
+    w13: torch.Tensor,
+    w2: torch.Tensor,
+    top_k: int,
+    pre_weight: torch.Tensor | None = None,
+    post_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    gate_func: str = "identity",
+    residual_scale: float = 1.0,
+    next_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    score_func: str = "softmax",
+    route_norm: bool = False,
+    route_scale: float = 1.0,
+    expert_bias: torch.Tensor | None = None,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
+    score_before_experts: bool = False,
+    swiglu_limit: float | None = None,
+    checkpoint: str | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """One MoE block of a transformer on one GPU: x [T, D] (the residual stream,
+    bf16 or fp32) to (u, n),
+
+        h = rmsnorm(x) * pre_weight             (None: x itself)
+        f = experts of h's routing, combined    (router, moe_experts_forward)
+        u = x + residual_scale * act(gate) * rmsnorm(f) * post_weight
+        n = rmsnorm(u) * next_weight            (None without next_weight)
+
+    in the places of upstream's TransformerBlock ffn_norm, moe and residual sum
+    and the next block's first norm.  With autograd every piece carries its
+    registered backward; without, the norms after the block run inside the
+    combine (ops.combine_norm).  Routing arguments as `router`, checkpoint as
+    `moe_experts_forward`, norm arguments as `residual_norm`; D % 128 == 0."""
+    groups = dict(num_groups=num_groups, topk_groups=topk_groups, group_score=group_score)
+    how = dict(post_weight=post_weight, gate=gate, gate_func=gate_func, residual_scale=residual_scale,
+               pre_weight=next_weight, eps=eps)
+    if not _needs_grad(x, w_router, w13, w2, pre_weight, post_weight, gate, next_weight):
+        u, n = _T.moe_block_forward(x, w_router, w13, w2, top_k, pre_weight, post_weight, gate, gate_func,
+                                    residual_scale, next_weight, eps, score_func, route_norm, route_scale,
+                                    expert_bias, num_groups, topk_groups, group_score, score_before_experts,
+                                    swiglu_limit)
+        return u, (None if next_weight is None else n)
+    h = x.to(_BF16) if pre_weight is None else rms_norm(x, pre_weight, eps)
+    scores, idx = router(h, w_router, top_k, score_func, route_norm, route_scale, expert_bias, **groups)
+    f = moe_experts_forward(h, scores, idx, w13, w2, w13.shape[0], score_before_experts, swiglu_limit,
+                            checkpoint=checkpoint)
+    return residual_norm(f, x, **how)
 
 
 def moe_experts_forward_fp8(

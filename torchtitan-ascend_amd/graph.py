@@ -19,6 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
+from .functional import moe_block
 
 _BF16 = torch.bfloat16
 
@@ -31,6 +32,10 @@ class MoELayerGraph:
     on the current stream and returns the graph's output buffer: the next
     call overwrites it, so clone it to keep it.  Weights are read where they
     are at capture time (update them in place, not by rebinding).
+
+    With ``residual``, or any of the norm weights or a gate, the graph holds
+    the block around the layer (functional.moe_block: norm, layer, norm, gate,
+    residual sum, next norm; the gate is read in place too) and returns (u, n).
     """
 
     def __init__(
@@ -50,6 +55,14 @@ class MoELayerGraph:
         num_groups: int | None = None,
         topk_groups: int | None = None,
         group_score: str = "top2",
+        pre_weight: torch.Tensor | None = None,
+        post_weight: torch.Tensor | None = None,
+        gate: torch.Tensor | None = None,
+        gate_func: str = "identity",
+        residual_scale: float = 1.0,
+        next_weight: torch.Tensor | None = None,
+        eps: float = 1e-6,
+        residual: bool = False,
     ):
         if x.dim() != 2 or x.dtype != _BF16:
             raise TypeError("x must be a bf16 [T, D] tensor")
@@ -58,7 +71,11 @@ class MoELayerGraph:
                 raise TypeError(f"{name} must be a contiguous bf16 tensor (read in place by the graph)")
         self._args = (w_router, w13, w2, top_k, score_func, route_norm, score_before_experts, route_scale,
                       expert_bias, swiglu_limit)
-        self._groups = (num_groups, topk_groups, group_score)
+        self._groups = dict(num_groups=num_groups, topk_groups=topk_groups, group_score=group_score)
+        self._block = None
+        if residual or any(t is not None for t in (pre_weight, post_weight, gate, next_weight)):
+            self._block = dict(pre_weight=pre_weight, post_weight=post_weight, gate=gate, gate_func=gate_func,
+                               residual_scale=residual_scale, next_weight=next_weight, eps=eps)
         self.static_x = x.detach().clone()
         # warm up on a side stream (first calls set kernel attributes), then capture
         side = torch.cuda.Stream(device=x.device)
@@ -71,21 +88,24 @@ class MoELayerGraph:
         with torch.no_grad(), torch.cuda.graph(self.graph):
             self.static_out = self._step(self.static_x)
 
-    def _step(self, x: torch.Tensor) -> torch.Tensor:
+    def _step(self, x: torch.Tensor):
         w_router, w13, w2, top_k, func, norm, before, scale, bias, limit = self._args
+        if self._block is not None:
+            return moe_block(x, w_router, w13, w2, top_k, score_func=func, route_norm=norm, route_scale=scale,
+                             expert_bias=bias, score_before_experts=before, swiglu_limit=limit, **self._block,
+                             **self._groups)
         _, _, r = ops.router_route(x, w_router, top_k, func, norm, scale, bias, with_inverse=False,
-                                    num_groups=self._groups[0], topk_groups=self._groups[1],
-                                    group_score=self._groups[2])
+                                    **self._groups)
         return ops.experts_forward(x, r, w13, w2, top_k, before, limit)
 
-    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+    def __call__(self, x: torch.Tensor):
         if x.shape != self.static_x.shape:
             raise ValueError(f"captured for x {tuple(self.static_x.shape)}, got {tuple(x.shape)}")
         self.static_x.copy_(x)
         self.graph.replay()
         return self.static_out
 
-    def replay(self) -> torch.Tensor:
+    def replay(self):
         """Replay on the input already in ``static_x``."""
         self.graph.replay()
         return self.static_out

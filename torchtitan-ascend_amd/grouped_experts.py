@@ -61,11 +61,17 @@ class HipGroupedExperts(Module):
         num_experts: int
         token_dispatcher: Any
         swiglu_limit: float | None = None
+        # "e4m3": the training forward keeps its activations in 8 bits
+        # (functional.moe_experts_forward); None: in bf16
+        activation_checkpoint: str | None = None
 
     def __init__(self, config: "HipGroupedExperts.Config"):
         super().__init__()
+        if config.activation_checkpoint not in (None, "e4m3"):
+            raise ValueError(f"activation_checkpoint must be 'e4m3' or None, got {config.activation_checkpoint!r}")
         self.num_experts = config.num_experts
         self.swiglu_limit = config.swiglu_limit
+        self.activation_checkpoint = config.activation_checkpoint
         E, D, H = config.num_experts, config.dim, config.hidden_dim
         self.w13 = nn.Parameter(torch.empty(E, 2 * H, D))
         self.w2 = nn.Parameter(torch.empty(E, D, H))
@@ -100,7 +106,7 @@ class HipGroupedExperts(Module):
             w13, w2 = self._weights()
             return moe_experts_forward(
                 x, top_scores, selected_experts_indices, w13, w2, self.num_experts,
-                disp.score_before_experts, self.swiglu_limit,
+                disp.score_before_experts, self.swiglu_limit, checkpoint=self.activation_checkpoint,
             )
         routed_input, num_tokens_local, metadata = disp.dispatch(x, top_scores, selected_experts_indices)
         routed_output = self._experts_forward(routed_input, num_tokens_local)
@@ -121,10 +127,12 @@ class HipGroupedExpertsConverter(ModelConfigConverter):
     @dataclass(kw_only=True, slots=True)
     class Config(ModelConfigConverter.Config):
         swiglu_limit: float | None = None
+        activation_checkpoint: str | None = None
 
     def __init__(self, config: "HipGroupedExpertsConverter.Config"):
         self.config = config
         self.swiglu_limit = config.swiglu_limit
+        self.activation_checkpoint = config.activation_checkpoint
 
     def convert(self, model_config) -> None:
         count = 0
@@ -135,6 +143,7 @@ class HipGroupedExpertsConverter(ModelConfigConverter):
                 num_experts=cfg.num_experts,
                 token_dispatcher=cfg.token_dispatcher,
                 swiglu_limit=self.swiglu_limit,
+                activation_checkpoint=self.activation_checkpoint,
             )
             for extra in ("param_init", "sharding_config"):
                 if hasattr(cfg, extra):

@@ -19,11 +19,14 @@ Reference ops these stand for (torchtitanturbo/models/common/):
                                       (npu_gmm.py:106-108)
   * ttamd::dispatch (+ backward)      dispatch gather / score-before
   * ttamd::experts (+ backward)       _run_experts_grouped_mm, npu_gmm.py:21-40
+  * ttamd::experts_packed (+ backward)
+                                      the three above with 8-bit activation checkpoints
   * ttamd::combine (+ backward)       combine / NPUMoeTokenUnpermute, npu_permute.py:15-53
   * ttamd::residual_norm / rms_norm (+ backward)
                                       npu_rms_norm (models/common/npu_rmsnorm.py:34) with the
                                       block's gate and residual
   * ttamd::moe_experts_forward        the fused inference expert stage
+  * ttamd::moe_block_forward          the inference block: norms, router, experts, residual
   * ttamd::shared_expert_add          shared-expert tail, qwen3_5/model.py:796-809
   * ttamd::token_permute / token_unpermute (+ backward)
                                       npu_moe_token_permute / unpermute, npu_permute.py:74-88
@@ -373,6 +376,114 @@ combine.register_autograd(_combine_bwd, setup_context=_combine_setup)
 
 
 # ---------------------------------------------------------------------------
+# The expert stage with 8-bit activation checkpoints: dispatch -> experts ->
+# combine keeping x, the pre-activation and (for the routing scores' gradient)
+# the experts' outputs packed, in place of the routed rows, h, a and y in bf16
+# ---------------------------------------------------------------------------
+@torch.library.custom_op("ttamd::experts_packed", mutates_args=())
+def experts_packed(x: Tensor, scores_flat: Tensor, sorted_indices: Tensor, inverse: Tensor, sorted_scores: Tensor,
+                   offs: Tensor, w13: Tensor, w2: Tensor, top_k: int, score_before: bool,
+                   swiglu_limit: Optional[float], keep_y: bool
+                   ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(out [T, D], codes and exponents of x [T, D], of h [M, 2H] and of y
+    [M, D] (empty unless keep_y))."""
+    w13b, w2b = _bf(w13), _bf(w2)
+    if score_before or x.shape[1] < 128:
+        routed = dispatch(x, scores_flat, sorted_indices, inverse, sorted_scores, top_k, score_before)
+        a, h = ops.grouped_mm_swiglu(routed, w13b, offs, swiglu_limit, save_h=True)
+        del routed
+    else:
+        a, h = ops.grouped_mm_swiglu_gather(x, sorted_indices, top_k, w13b, offs, swiglu_limit, save_h=True)
+    hp = ops.pack_e4m3(h)
+    del h
+    y = ops.grouped_mm_unpermute(a, w2b, offs)
+    del a
+    out = ops.combine(y, inverse, None if score_before else scores_flat, top_k)
+    xp = ops.pack_e4m3(x)
+    e = lambda: x.new_empty((0,), dtype=torch.uint8)  # noqa: E731
+    yp = ops.pack_e4m3(y) if keep_y else ops.PackedRows(e(), e())
+    return out, xp.codes, xp.exponents, hp.codes, hp.exponents, yp.codes, yp.exponents
+
+
+def _packed_shapes(like, rows, cols):
+    return (like.new_empty((rows, cols), dtype=torch.uint8), like.new_empty((rows, (cols + 127) // 128),
+                                                                            dtype=torch.uint8))
+
+
+@experts_packed.register_fake
+def _(x, scores_flat, sorted_indices, inverse, sorted_scores, offs, w13, w2, top_k, score_before, swiglu_limit, keep_y):
+    (T, D), M, H2 = x.shape, sorted_indices.numel(), w13.shape[1]
+    empty = lambda: x.new_empty((0,), dtype=torch.uint8)  # noqa: E731
+    y = _packed_shapes(x, M, D) if keep_y else (empty(), empty())
+    return (x.new_empty((T, D), dtype=_BF16), *_packed_shapes(x, T, D), *_packed_shapes(x, M, H2), *y)
+
+
+@torch.library.custom_op("ttamd::experts_packed_backward", mutates_args=())
+def experts_packed_backward(dout: Tensor, x_codes: Tensor, x_exps: Tensor, h_codes: Tensor, h_exps: Tensor,
+                            y_codes: Tensor, y_exps: Tensor, scores_flat: Tensor, sorted_indices: Tensor,
+                            inverse: Tensor, sorted_scores: Tensor, offs: Tensor, w13: Tensor, w2: Tensor, top_k: int,
+                            score_before: bool, swiglu_limit: Optional[float], need_dx: bool, need_ds: bool,
+                            need_dw13: bool, need_dw2: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(dx [T, D], d scores_flat [M], dw13, dw2) at the stored activations; a
+    gradient not asked for is empty."""
+    w13b, w2b = _bf(w13), _bf(w2)
+    E = w13.shape[0]
+    xp, hp = ops.PackedRows(x_codes, x_exps), ops.PackedRows(h_codes, h_exps)
+    dx, ds, dw13, dw2 = _empty(dout), _empty(scores_flat), _empty(w13), _empty(w2)
+    keep_y = need_ds and not score_before
+    y = ops.unpack_e4m3(ops.PackedRows(y_codes, y_exps)) if keep_y else None
+    dy, dsy = ops.token_unpermute_grad(dout.to(_BF16).contiguous(), sorted_indices,
+                                       None if score_before else scores_flat, y, top_k, need_probs_grad=keep_y)
+    del y
+    if keep_y:
+        ds = dsy
+    dh, a = ops.grouped_mm_dgrad_swiglu_packed(dy, w2b, hp, offs, swiglu_limit, want_a=need_dw2)
+    if need_dw2:
+        dw2 = ops.grouped_mm_wgrad(dy, a, offs, E, _F32 if w2.dtype != _BF16 else _BF16).to(w2.dtype)
+    del dy, a
+    if need_dw13:
+        dw13 = ops.grouped_mm_wgrad_packed(dh, xp, offs, E, _F32 if w13.dtype != _BF16 else _BF16, sorted_indices,
+                                           top_k, sorted_scores if score_before else None).to(w13.dtype)
+    if need_dx or (need_ds and score_before):
+        d_routed = ops.grouped_mm_dgrad(dh, w13b, offs)
+        if need_dx:
+            dx = ops.combine(d_routed, inverse, scores_flat if score_before else None, top_k)
+        if need_ds and score_before:
+            ds = ops.rowdot_scatter(d_routed, ops.unpack_e4m3(xp), sorted_indices, top_k)
+    return dx, ds, dw13, dw2
+
+
+@experts_packed_backward.register_fake
+def _(dout, x_codes, x_exps, h_codes, h_exps, y_codes, y_exps, scores_flat, sorted_indices, inverse, sorted_scores, offs,
+      w13, w2, top_k, score_before, swiglu_limit, need_dx, need_ds, need_dw13, need_dw2):
+    return (dout.new_empty(x_codes.shape if need_dx else (0,), dtype=_BF16),
+            scores_flat.new_empty(scores_flat.shape if need_ds else (0,)),
+            w13.new_empty(w13.shape if need_dw13 else (0,)), w2.new_empty(w2.shape if need_dw2 else (0,)))
+
+
+def _experts_packed_setup(ctx, inputs, output):
+    _x, scores_flat, sorted_indices, inverse, sorted_scores, offs, w13, w2, top_k, before, limit, keep_y = inputs
+    ctx.save_for_backward(*output[1:], scores_flat, sorted_indices, inverse, sorted_scores, offs, w13, w2)
+    ctx.cfg = (top_k, before, limit)
+    ctx.keep_y = keep_y
+    ctx.set_materialize_grads(False)
+
+
+def _experts_packed_bwd(ctx, dout, *_codes):
+    if dout is None:
+        return (None,) * 12
+    need = ctx.needs_input_grad
+    if need[1] and not ctx.cfg[1] and not ctx.keep_y:
+        raise RuntimeError("ttamd::experts_packed ran without keep_y=True; the scores' gradient needs the outputs")
+    dx, ds, dw13, dw2 = experts_packed_backward(dout, *ctx.saved_tensors, *ctx.cfg, need[0], need[1], need[6], need[7])
+    return (dx if need[0] else None, ds if need[1] else None, None, None, None, None, dw13 if need[6] else None,
+            dw2 if need[7] else None, None, None, None, None)
+
+
+experts_packed.register_autograd(_experts_packed_bwd, setup_context=_experts_packed_setup)
+
+
+# ---------------------------------------------------------------------------
 # Norms around the block (ops.residual_norm, ops.rms_norm)
 # ---------------------------------------------------------------------------
 @torch.library.custom_op("ttamd::residual_norm", mutates_args=())
@@ -486,6 +597,32 @@ def moe_experts_forward(x: Tensor, sorted_indices: Tensor, offsets: Tensor, sort
 @moe_experts_forward.register_fake
 def _(x, sorted_indices, offsets, sorted_scores, w13, w2, top_k, score_before, swiglu_limit):
     return x.new_empty(x.shape, dtype=_BF16)
+
+
+@torch.library.custom_op("ttamd::moe_block_forward", mutates_args=())
+def moe_block_forward(x: Tensor, w_router: Tensor, w13: Tensor, w2: Tensor, top_k: int, pre_weight: Optional[Tensor],
+                      post_weight: Optional[Tensor], gate: Optional[Tensor], gate_func: str, residual_scale: float,
+                      next_weight: Optional[Tensor], eps: float, score_func: str, route_norm: bool,
+                      route_scale: float, expert_bias: Optional[Tensor], num_groups: Optional[int],
+                      topk_groups: Optional[int], group_score: str, score_before: bool,
+                      swiglu_limit: Optional[float]) -> tuple[Tensor, Tensor]:
+    """norm -> router + route -> experts -> combine with norm, gate, residual and
+    the next norm: (u [T, D], n [T, D] or empty)."""
+    h = x.to(_BF16).contiguous() if pre_weight is None else ops.rms_norm(x, pre_weight, eps)
+    _, _, r = ops.router_route(h, _bf(w_router), top_k, score_func, route_norm, route_scale, expert_bias,
+                               with_inverse=False, num_groups=num_groups, topk_groups=topk_groups,
+                               group_score=group_score)
+    rows = ops.experts_forward(h, r, _bf(w13), _bf(w2), top_k, score_before, swiglu_limit, sum_rows=False)
+    u, n = ops.combine_norm(rows, top_k, residual=x, post_weight=post_weight, gate=gate, gate_func=gate_func,
+                            residual_scale=residual_scale, pre_weight=next_weight, eps=eps)
+    return u, _empty(rows) if n is None else n
+
+
+@moe_block_forward.register_fake
+def _(x, w_router, w13, w2, top_k, pre_weight, post_weight, gate, gate_func, residual_scale, next_weight, eps,
+      score_func, route_norm, route_scale, expert_bias, num_groups, topk_groups, group_score, score_before,
+      swiglu_limit):
+    return x.new_empty(x.shape), x.new_empty((0,) if next_weight is None else x.shape, dtype=_BF16)
 
 
 @torch.library.custom_op("ttamd::shared_expert_add", mutates_args=())

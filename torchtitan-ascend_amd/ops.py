@@ -384,12 +384,15 @@ def experts_forward(
     top_k: int,
     score_before_experts: bool,
     swiglu_limit: float | None = None,
+    sum_rows: bool = True,
 ) -> torch.Tensor:
     """The expert stage of the inference forward in one C-ABI call
     (ttamd_moe_experts_forward): dispatch -> w13 + SwiGLU -> w2 + score ->
     combine (npu_gmm.py:100-110 with :21-40) on the routing `r` (from
     `route` or `router_route`; r.sorted_scores must be set).  Both grouped
-    GEMMs use r.plan when present.  x bf16 [T, D] -> out bf16 [T, D]."""
+    GEMMs use r.plan when present.  x bf16 [T, D] -> out bf16 [T, D]; without
+    sum_rows the weighted rows [T * K, D] in token order, before the K-way sum
+    (ttamd_moe_experts_rows), for `combine_norm`."""
     dev = _gpu("x", x)
     x = _want("x", x, _BF16)
     w13 = _want("w13", w13, _BF16)
@@ -405,11 +408,12 @@ def experts_forward(
         raise ValueError("routing does not match T * top_k rows")
     lib = _lib.load()
     offsets = r.offsets.contiguous()  # inclusive offsets: its int32 entries from the second on
-    out = torch.empty(T, D, dtype=_BF16, device=dev)
-    ws = _ws(lib.ttamd_moe_experts_forward_workspace_bytes(T, D, H, E, top_k, int(bool(score_before_experts))), dev)
+    out = torch.empty(T if sum_rows else T * top_k, D, dtype=_BF16, device=dev)
+    need = lib.ttamd_moe_experts_forward_workspace_bytes if sum_rows else lib.ttamd_moe_experts_rows_workspace_bytes
+    ws = _ws(need(T, D, H, E, top_k, int(bool(score_before_experts))), dev)
     plan = r.plan
-    _lib.call(
-        "ttamd_moe_experts_forward", _p(x), T, D, H, E, top_k, _p(r.sorted_indices), _p(offsets) + 4,
+    _call(
+        dev, "ttamd_moe_experts_forward" if sum_rows else "ttamd_moe_experts_rows", _p(x), T, D, H, E, top_k, _p(r.sorted_indices), _p(offsets) + 4,
         _p(r.sorted_scores), int(bool(score_before_experts)), _limit(swiglu_limit), _p(w13), _p(w2), _p(out),
         _p(plan), 0 if plan is None else plan.numel(), _p(ws), ws.numel(), _stream(dev),
     )
