@@ -70,7 +70,6 @@ __device__ __forceinline__ void store8(void* p, int64_t i, bool f32, const float
 __device__ __forceinline__ float load1(const void* p, int64_t i, bool f32) {
   return f32 ? ((const float*)p)[i] : bf16_to_f32(((const bf16_t*)p)[i]);
 }
-__device__ __forceinline__ float sigmoid_of(float g) { return 1.f / (1.f + expf(-g)); }
 __device__ __forceinline__ Raw8 no_raw() {
   Raw8 r;
   r.a = r.b = make_uint4(0u, 0u, 0u, 0u);
@@ -122,18 +121,6 @@ __global__ __launch_bounds__(1024) void norm_forward_kernel(const NormArgs a) {
   float wu[8], wn[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) wu[j] = 1.f, wn[j] = 0.f;
-  if (on) {
-    if (a.post) load8(a.post, col, a.post32, wu);
-    if (a.pre) load8(a.pre, col, a.pre32, wn);
-    if constexpr (GATE == GATE_CHANNEL) {
-      float g[8];
-      load8(a.gate, col, a.gate32, g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) wu[j] *= a.sigmoid ? sigmoid_of(g[j]) : g[j];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) wu[j] *= a.scale;
   const float inv_d = 1.f / (float)D;
   const int last_row = a.T * a.K - 1;
 
@@ -176,6 +163,18 @@ __global__ __launch_bounds__(1024) void norm_forward_kernel(const NormArgs a) {
     fetch(t);
     fetch_ids(min(t + step, a.T - 1));
   }
+  if (on) {
+    if (a.post) load8(a.post, col, a.post32, wu);
+    if (a.pre) load8(a.pre, col, a.pre32, wn);
+    if constexpr (GATE == GATE_CHANNEL) {
+      float g[8];
+      load8(a.gate, col, a.gate32, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) wu[j] *= a.sigmoid ? sigmoid_f(g[j]) : g[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) wu[j] *= a.scale;
   for (; t < a.T; t += step) {
     float x[8], r[8];  // x: f, then u
     if constexpr (COMBINE) {
@@ -218,11 +217,11 @@ __global__ __launch_bounds__(1024) void norm_forward_kernel(const NormArgs a) {
     if constexpr (GATE == GATE_FULL) {
       if (a.sigmoid) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = sigmoid_of(g[j]);
+        for (int j = 0; j < 8; ++j) g[j] = sigmoid_f(g[j]);
       }
     }
     if constexpr (GATE == GATE_TOKEN) {
-      if (a.sigmoid) g[0] = sigmoid_of(g[0]);
+      if (a.sigmoid) g[0] = sigmoid_f(g[0]);
     }
     float rf = 1.f;
     if (a.post) {
@@ -288,20 +287,7 @@ __global__ __launch_bounds__(MAX_THREADS) void norm_backward_kernel(const NormBw
   float s_f[8], s_n[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) wu[j] = 1.f, wn[j] = 0.f, s_f[j] = 0.f, s_n[j] = 0.f;
-  if (on) {
-    if (f.post) load8(f.post, col, f.post32, wu);
-    if (f.pre) load8(f.pre, col, f.pre32, wn);
-    if constexpr (GATE == GATE_CHANNEL) {
-      float g[8];
-      load8(f.gate, col, f.gate32, g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) wu[j] *= f.sigmoid ? sigmoid_of(g[j]) : g[j];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) wu[j] *= f.scale;
   const float inv_d = 1.f / (float)D;
-
   Raw8 q_f = no_raw(), q_r = no_raw(), q_u = no_raw(), q_n = no_raw(), q_g = no_raw();
   float q_rf = 1.f, q_ru = 1.f, q_t = 1.f;
   auto fetch = [&](int t) {
@@ -316,7 +302,19 @@ __global__ __launch_bounds__(MAX_THREADS) void norm_backward_kernel(const NormBw
     if constexpr (GATE == GATE_FULL) q_g = fetch8(f.gate, at, f.gate32);
   };
   int t = blockIdx.x;
-  if (t < f.T) fetch(t);
+  if (t < f.T) fetch(t);  // in flight before the weights are waited for
+  if (on) {
+    if (f.post) load8(f.post, col, f.post32, wu);
+    if (f.pre) load8(f.pre, col, f.pre32, wn);
+    if constexpr (GATE == GATE_CHANNEL) {
+      float g[8];
+      load8(f.gate, col, f.gate32, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) wu[j] *= f.sigmoid ? sigmoid_f(g[j]) : g[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) wu[j] *= f.scale;
   for (; t < f.T; t += gridDim.x) {
     const int64_t at = (int64_t)t * D + col;
     float x[8], u[8], g[8], dn[8], act[GATE == GATE_FULL ? 8 : 1];  // g: du, then dU
@@ -330,7 +328,7 @@ __global__ __launch_bounds__(MAX_THREADS) void norm_backward_kernel(const NormBw
     if constexpr (GATE == GATE_TOKEN) act[0] = q_t;
     if (GATE >= GATE_TOKEN && GATE != GATE_CHANNEL && f.sigmoid) {
 #pragma unroll
-      for (int j = 0; j < (GATE == GATE_FULL ? 8 : 1); ++j) act[j] = sigmoid_of(act[j]);
+      for (int j = 0; j < (GATE == GATE_FULL ? 8 : 1); ++j) act[j] = sigmoid_f(act[j]);
     }
     auto gate = [&](int j) { return act[GATE == GATE_FULL ? j : 0]; };
     if (t + (int)gridDim.x < f.T) fetch(t + gridDim.x);
@@ -388,9 +386,10 @@ __global__ __launch_bounds__(MAX_THREADS) void norm_backward_kernel(const NormBw
 }
 
 // The n partial rows of each column added in a fixed order: 64 runs of rows
-// side by side, 8 loads of each in flight, then the runs; and the factors that
-// turn S into dw_post and the channel gate's gradient.  A workgroup takes 16
-// columns; blockIdx.y: 0 S, 1 dw_pre.
+// side by side, 8 loads of each in flight, then the runs pairwise (16 in a
+// wave's lanes, then the four waves); and the factors that turn S into dw_post
+// and the channel gate's gradient.  A workgroup takes 16 columns; blockIdx.y:
+// 0 S, 1 dw_pre.
 __device__ __forceinline__ void store4(void* out, int c, bool f32, const float4& s) {
   if (f32)
     *(float4*)((float*)out + c) = s;
@@ -398,7 +397,7 @@ __device__ __forceinline__ void store4(void* out, int c, bool f32, const float4&
     *(uint2*)((bf16_t*)out + c) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
 }
 __global__ __launch_bounds__(256) void column_sum_kernel(const NormBwdArgs a, int n) {
-  __shared__ float4 sh[64][4];
+  __shared__ float4 sh[4][4];
   const NormArgs& f = a.fwd;
   const bool channel = a.dgate && f.gate_kind == GATE_CHANNEL;
   if (blockIdx.y == 0 ? !(a.dpost || channel) : !a.dpre) return;
@@ -413,10 +412,16 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const NormBwdArgs a, in
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
   }
-  sh[ry][cx] = s;
+#pragma unroll
+  for (int d = 4; d < 64; d *= 2) {
+    s.x += __shfl_xor(s.x, d, kWave), s.y += __shfl_xor(s.y, d, kWave);
+    s.z += __shfl_xor(s.z, d, kWave), s.w += __shfl_xor(s.w, d, kWave);
+  }
+  if ((threadIdx.x & 63) < 4) sh[threadIdx.x >> 6][cx] = s;
   __syncthreads();
   if (ry != 0 || c >= f.D) return;
-  for (int r = 1; r < 64; ++r) {
+#pragma unroll
+  for (int r = 1; r < 4; ++r) {
     const float4 v = sh[r][cx];
     s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
   }
@@ -429,7 +434,7 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const NormBwdArgs a, in
     if (f.gate_kind == GATE_CHANNEL) {
       act = load1(f.gate, c + j, f.gate32);
       if (f.sigmoid) {
-        act = sigmoid_of(act);
+        act = sigmoid_f(act);
         dact = act * (1.f - act);
       }
     }
