@@ -77,8 +77,10 @@ def _limit(swiglu_limit: float | None) -> float:
 def _call(dev: torch.device, name: str, *args) -> None:
     """_lib.call with `dev` as the current device: a kernel launches on the
     device of its tensors whichever device is current."""
-    if dev.index is None or dev.index == torch._C._cuda_getDevice():  # (a tensor of dev exists: HIP is initialised)
-        _lib.call(name, *args)
+    if dev.index == torch._C._cuda_getDevice():  # (a tensor of dev exists: HIP is initialised)
+        rc = getattr(_lib._lib or _lib.load(), name)(*args)
+        if rc:
+            _lib.check(rc)
         return
     with torch.cuda.device(dev):
         _lib.call(name, *args)
