@@ -243,6 +243,36 @@ def test_wgrad_packed(ops, T, K, E, N, D, skew, dtype):
 
 
 @pytest.mark.gpu
+def test_wgrad_packed_without_rows(ops):
+    """No rows at all, and no rows of any expert: exact zeros."""
+    x = ops.pack_e4m3(torch.randn(16, 128, device=DEV).to(BF16))
+    none = torch.zeros(3, dtype=torch.int32, device=DEV)
+    src = torch.zeros(0, dtype=torch.int32, device=DEV)
+    announce("wgrad packed without rows")
+    for dtype in (torch.float32, BF16):
+        dw = ops.grouped_mm_wgrad_packed(torch.empty(0, 128, dtype=BF16, device=DEV), x, none, 3, dtype, src, 8)
+        assert dw.shape == (3, 128, 128) and not dw.any()
+        dy = torch.randn(16, 128, device=DEV).to(BF16)
+        src16 = torch.arange(16, dtype=torch.int32, device=DEV)
+        dw = ops.grouped_mm_wgrad_packed(dy, x, none, 3, dtype, src16, 1)
+        assert not dw.any()
+
+
+@pytest.mark.gpu
+def test_wgrad_packed_same_token_everywhere(ops):
+    """Every routed row the same token, and indices out of range (clamped)."""
+    rng = np.random.default_rng(12)
+    x = ops.pack_e4m3(torch.from_numpy(rng.standard_normal((5, 256))).to(BF16).to(DEV))
+    dy = torch.from_numpy(rng.standard_normal((200, 128))).to(BF16).to(DEV)
+    offs = offsets([90, 0, 110])
+    for v, row in ((3, 3), (10 ** 6, 4), (-9, 0)):
+        src = torch.full((200,), v, dtype=torch.int32, device=DEV)
+        got = ops.grouped_mm_wgrad_packed(dy, x, offs, 3, torch.float32, src, 1)
+        want = ops.grouped_mm_wgrad(dy, ops.unpack_e4m3(x)[row].expand(200, 256).contiguous(), offs, 3, torch.float32)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_wgrad_packed_large_gathered(ops):
     """Full rounds, a split tail and experts that end inside a stage."""
     rng = np.random.default_rng(9)

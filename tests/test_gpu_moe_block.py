@@ -360,6 +360,78 @@ def test_opcheck(ops, name):
     torch.library.opcheck(op, args)
 
 
+@pytest.mark.gpu
+def test_calls_on_two_streams(ops):
+    """The same operators on two streams at once, with nothing between them:
+    each gives what it gives alone."""
+    rng = np.random.default_rng(31)
+    c = [inputs(rng, 700, 512, 256, 16) for _ in range(2)]
+    kw = dict(score_func="sigmoid", route_norm=True, num_groups=4, topk_groups=2)
+    idx = [routing_idx(ops, v, 4, kw) for v in c]
+    sc = torch.rand(700, 4, device=DEV)
+
+    def work(v, i):
+        with torch.no_grad():
+            u, n = call(v, 4, **kw)
+        leaves = [v["x"].clone().requires_grad_(True), v["w13"].clone().requires_grad_(True)]
+        out = F().moe_experts_forward(leaves[0], sc, i, leaves[1], v["w2"], 16, False, checkpoint="e4m3")
+        out.backward(u)
+        return u, n, out.detach(), leaves[0].grad, leaves[1].grad
+
+    announce("two streams")
+    alone = [work(v, i) for v, i in zip(c, idx)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in c]
+    for _ in range(3):
+        both = []
+        for s, v, i in zip(streams, c, idx):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                both.append(work(v, i))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, both):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y)
+
+
+def routing_idx(ops, c, K, kw):
+    h = ops.rms_norm(c["x"], c["pre_weight"], EPS)
+    return ops.router_fused(h, c["w_router"], K, kw["score_func"], kw["route_norm"],
+                            num_groups=kw["num_groups"], topk_groups=kw["topk_groups"])[1]
+
+
+@pytest.mark.gpu
+def test_repeatable(ops):
+    """The same call gives the same bits: no sum depends on an arrival order."""
+    rng = np.random.default_rng(32)
+    c = inputs(rng, 3000, 512, 256, 16, "channel")
+    kw = dict(score_func="softmax", num_groups=4, topk_groups=3, checkpoint="e4m3")
+
+    def step():
+        names = [k for k in c if k != "expert_bias"]
+        leaves = {k: c[k].clone().requires_grad_(True) for k in names}
+        u, n = call({**c, **leaves}, 4, **kw)
+        torch.autograd.backward([u, n], [c["x"], c["x"]])
+        return [u, n] + [leaves[k].grad for k in names]
+
+    announce("repeatable")
+    first = step()
+    for _ in range(3):
+        for a, b in zip(first, step()):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_block_without_tokens(ops):
+    rng = np.random.default_rng(33)
+    c = inputs(rng, 4, 128, 128, 8)
+    c["x"], c["gate"] = c["x"][:0], c["gate"][:0]
+    announce("block without tokens")
+    with torch.no_grad():
+        u, n = call(c, 2, score_func="sigmoid", num_groups=4, topk_groups=2)
+    assert u.shape == (0, 128) and n.shape == (0, 128)
+
+
 def test_module_refuses_an_unknown_checkpoint(pkg):
     P = importlib.import_module("torchtitan-ascend_amd.protocol")
     mc = P.ModelConfig()

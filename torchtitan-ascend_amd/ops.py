@@ -1147,7 +1147,7 @@ def _packed(name: str, p: PackedRows, dev: torch.device) -> tuple[torch.Tensor, 
 
 def pack_e4m3(x: torch.Tensor) -> PackedRows:
     """8-bit checkpoint of bf16 rows x [R, C] (ttamd_pack_e4m3): 1 + 1/128 byte
-    per value, a relative error of at most 2^-4 for values down to 2^-15 of
+    per value, a relative error of at most 2^-4 for values down to 2^-13 of
     their block's largest.  NaN and infinities come back as NaN."""
     dev = _gpu("x", x)
     if x.dim() != 2:
