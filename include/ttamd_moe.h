@@ -115,7 +115,8 @@ int ttamd_router_fused(const void* x, const void* w_router,
  *   grad_w_router [E, D] = dlogits^T . x              (nullable; fp32 when
  *                                                      grad_w_is_fp32, else bf16)
  * s is recomputed from logits (bf16 [T, E], the forward's logits_out).
- * expert_bias only steers the selection and has no gradient here.
+ * expert_bias only steers the selection and has no gradient here.  Without
+ * tokens grad_w_router is zeros.
  * D % 128 == 0; other limits as ttamd_router_fused.  workspace:
  * ttamd_router_backward_workspace_bytes.
  */
@@ -616,7 +617,7 @@ int ttamd_residual_norm(const void* rows, const int32_t* inverse,
  * rstd_out.  grad_branch bf16 [T, D]; grad_residual and du of the stream's
  * type; grad_post, grad_gate, grad_pre of their inputs' types and shapes,
  * accumulated in fp32 and rounded once.  Deterministic: the column sums are
- * added in a fixed order.  workspace:
+ * added in a fixed order (zeros when num_tokens is 0).  workspace:
  * ttamd_residual_norm_backward_workspace_bytes; contents need no
  * initialisation.
  */
@@ -722,7 +723,8 @@ int ttamd_grouped_mm_wgrad(const void* dy, const void* x, const int32_t* offs,
  * [R, ceil(C / 128)]: per row and 128 columns the smallest e in [-118, 120]
  * with max |v| <= 448 * 2^e over the finite values; code = e4m3fn(v * 2^-e),
  * ties to even (with e = 120 at most 240: 256 * 2^120 is past bf16's range);
- * exponent byte e + 127.  A NaN or an infinity becomes 0x7f (NaN).  C % 8 == 0; in and codes 16-byte aligned.
+ * exponent byte e + 127.  A NaN or an infinity becomes 0x7f (NaN).
+ * C % 8 == 0; in and codes 16-byte aligned.
  */
 int ttamd_pack_e4m3(const void* in, int64_t num_rows, int64_t cols,
                     void* codes, void* exponents, void* stream);

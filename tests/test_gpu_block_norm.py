@@ -401,6 +401,77 @@ def _forward(rows=256, inverse=None, probs=None, T=4, D=64, K=1, residual=256, p
     return L.load().ttamd_last_error().decode()
 
 
+@pytest.mark.gpu
+def test_output_in_place_of_the_residual(ops):
+    """u_out may be the residual itself (the C entry point)."""
+    from importlib import import_module
+
+    lib = import_module("torchtitan-ascend_amd._lib")
+    rng = np.random.default_rng(41)
+    for stream in ("bf16", "fp32"):
+        c = case(rng, 5000, 520, stream=stream)
+        want, _ = ops.residual_norm(c["branch"], c["residual"], c["post_weight"], pre_weight=c["pre_weight"], eps=EPS)
+        res = c["residual"].clone()
+        n = torch.empty_like(c["branch"])
+        announce(f"u over the {stream} residual")
+        p = lambda t: t.data_ptr()  # noqa: E731
+        lib.call("ttamd_residual_norm", p(c["branch"]), None, None, 5000, 520, 1, p(res), p(c["post_weight"]), None, 0, 0,
+                 1.0, p(c["pre_weight"]), EPS, 1 if stream == "fp32" else 0, p(res), p(n), None,
+                 torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(res, want)
+
+
+@pytest.mark.gpu
+def test_backward_without_rows(ops):
+    """No tokens: the weights' and the channel gate's gradients are zeros."""
+    rng = np.random.default_rng(42)
+    c = case(rng, 3, 264, gate="channel")
+    stats = torch.empty(2, 0, device=DEV)
+    announce("backward without rows")
+    for _ in range(3):
+        torch.full((1 << 16,), float("nan"), device=DEV)  # what the allocator hands out next
+        g = ops.residual_norm_backward(c["branch"][:0], c["branch"][:0], c["branch"][:0], stats, c["residual"][:0],
+                                       c["post_weight"], c["gate"], "sigmoid", 0.5, c["pre_weight"])
+        assert g.branch.shape == (0, 264) and g.residual.shape == (0, 264)
+        for t, like in ((g.post_weight, c["post_weight"]), (g.gate, c["gate"]), (g.pre_weight, c["pre_weight"])):
+            assert t.shape == like.shape and not t.any()
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits(ops):
+    """More than 2^31 elements: the last rows are those of a small call."""
+    T, D, few = 300_000, 8192, 257
+    g = torch.Generator(device=DEV).manual_seed(5)
+    mk = lambda *s: torch.randn(*s, device=DEV, generator=g, dtype=torch.bfloat16)  # noqa: E731
+    branch, residual, w1, w2 = mk(T, D), mk(T, D), mk(D), mk(D)
+    announce("rows past 32 bits")
+    u, n, st = ops.residual_norm(branch, residual, w1, pre_weight=w2, eps=EPS, save_stats=True)
+    tail = slice(T - few, T)
+    us, ns, sts = ops.residual_norm(branch[tail], residual[tail], w1, pre_weight=w2, eps=EPS, save_stats=True)
+    assert torch.equal(u[tail], us) and torch.equal(n[tail], ns) and torch.equal(st[:, tail], sts)
+    got = ops.residual_norm_backward(u, n, branch, st, residual, w1, pre_weight=w2)
+    few_grads = ops.residual_norm_backward(us, ns, branch[tail], sts.contiguous(), residual[tail], w1, pre_weight=w2)
+    assert torch.equal(got.branch[tail], few_grads.branch) and torch.equal(got.residual[tail], few_grads.residual)
+    del u, n, got
+    K = 4
+    idx = (T - 1 - torch.arange(few * K, device=DEV, dtype=torch.int32)) % T
+    every = torch.arange(T, device=DEV, dtype=torch.int32)
+    every[: few * K] = idx  # the first tokens read the last rows
+    u, _ = ops.combine_norm(branch, K, inverse=every, post_weight=w1, eps=EPS)
+    want, _ = ops.combine_norm(branch[idx.long()], K, post_weight=w1, eps=EPS)
+    assert torch.equal(u[:few], want)
+
+
+@pytest.mark.gpu
+def test_combine_norm_has_no_backward(ops):
+    rows = torch.zeros(8, 64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.combine_norm(rows, 2)
+    with torch.no_grad():
+        assert not ops.combine_norm(rows, 2)[0].any()
+
+
 def test_forward_refusals():
     assert "multiple of 8" in _forward(D=60)
     assert "multiple of 8" in _forward(D=0)

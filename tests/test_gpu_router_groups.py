@@ -318,6 +318,39 @@ def _topk(E=64, K=4, G=8, kept=2, value=0, T=4, func=1):
     return _lib.load().ttamd_last_error().decode()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_router_backward_without_tokens(ops, dtype):
+    """No tokens: the gate weight's gradient is zeros, whatever memory it gets."""
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    announce("router backward without tokens")
+    for _ in range(3):
+        torch.full((8, 256), float("nan"), dtype=dtype, device=DEV)  # what the allocator hands out next
+        dx, dw = ops.router_backward(torch.zeros(0, 2, device=DEV), torch.zeros(0, 2, dtype=torch.int64, device=DEV),
+                                     bf(0, 8), bf(0, 256), bf(8, 256), dw_dtype=dtype)
+        assert dx.shape == (0, 256) and dw.shape == (8, 256) and not dw.any()
+
+
+@pytest.mark.gpu
+def test_grouped_topk_past_32_bits(ops):
+    """More than 2^31 logits: the last tokens are those of a small call."""
+    T, E, K, few = 9_000_001, 256, 8, 500
+    z = torch.empty(T, E, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    z[: T - few].fill_(0.25)
+    z[T - few:] = torch.randn(few, E, device=DEV, generator=g)
+    announce("grouped top-k past 32 bits")
+    for func in ("sigmoid", "softmax"):
+        how = dict(score_func=func, route_norm=True, num_groups=8, topk_groups=4)
+        s, i = ops.router_topk(z, K, **how)
+        ss, si = ops.router_topk(z[T - few:], K, **how)
+        assert torch.equal(i[T - few:], si) and torch.equal(s[T - few:], ss)
+        assert torch.equal(i[: T - few], i[:1].expand(T - few, K))
+        d = ops.router_topk_backward(s, i, z, func, True)
+        assert torch.equal(d[T - few:], ops.router_topk_backward(ss, si, z[T - few:], func, True))
+        del s, i, d
+
+
 def test_grouped_topk_refusals():
     assert "divide num_experts" in _topk(G=7)
     assert "num_groups" in _topk(E=128, G=128)

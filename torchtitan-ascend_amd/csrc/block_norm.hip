@@ -521,9 +521,10 @@ size_t norm_backward_workspace_bytes(int64_t T, int64_t D) {
 
 hipError_t launch_norm_backward(const NormBwdArgs& b, hipStream_t stream) {
   const NormArgs& a = b.fwd;
-  if (a.T == 0) return hipSuccess;
-  const int groups = even_groups(a.T, backward_most(a.T, a.D));
-  const hipError_t err = a.stream32 ? go_backward<true>(b, groups, stream) : go_backward<false>(b, groups, stream);
+  // (no rows: no partial sums either, and the column sums are zeros)
+  const int groups = a.T == 0 ? 0 : even_groups(a.T, backward_most(a.T, a.D));
+  hipError_t err = hipSuccess;
+  if (a.T > 0) err = a.stream32 ? go_backward<true>(b, groups, stream) : go_backward<false>(b, groups, stream);
   if (err != hipSuccess || !(b.dpost || b.dpre || (b.dgate && a.gate_kind == GATE_CHANNEL))) return err;
   return launch_k(false, column_sum_kernel, dim3((a.D + 15) / 16, 2), dim3(256), 0, stream, b, groups);
 }

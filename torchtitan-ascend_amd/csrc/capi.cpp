@@ -128,11 +128,10 @@ int check_groups(const char* fn, int E, int K, int groups, int kept, int group_s
 }
 
 // The gate GEMM + selection of the plain and the grouped entry point.
-int router_fused(const char* fn, const ttamd::RouterGroups* groups, const void* x, const void* w_router, const float* expert_bias,
-                       int64_t num_tokens, int num_experts, int64_t dim, int topk, int score_func,
-                       int renorm, float renorm_eps, float route_scale, float* top_scores,
-                       int64_t* top_indices, void* logits_out, void* workspace, size_t workspace_bytes,
-                       void* stream) {
+int router_fused(const char* fn, const ttamd::RouterGroups* groups, const void* x, const void* w_router,
+                 const float* expert_bias, int64_t num_tokens, int num_experts, int64_t dim, int topk, int score_func,
+                 int renorm, float renorm_eps, float route_scale, float* top_scores, int64_t* top_indices,
+                 void* logits_out, void* workspace, size_t workspace_bytes, void* stream) {
   REQUIRE(num_tokens >= 0 && num_tokens <= (1 << 24), "%s: num_tokens out of range", fn);
   REQUIRE(num_experts >= 1 && num_experts <= 256, "%s: num_experts must be in [1, 256]", fn);
   REQUIRE(topk >= 1 && topk <= 16 && topk <= num_experts, "%s: topk must be in [1, min(16, E)]",
@@ -157,12 +156,12 @@ int router_fused(const char* fn, const ttamd::RouterGroups* groups, const void* 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // The same followed by the dispatch order.
-int router_route(const char* fn, const ttamd::RouterGroups* groups, const void* x, const void* w_router, const float* expert_bias, int64_t num_tokens,
-                       int num_experts, int64_t dim, int topk, int score_func, int renorm, float renorm_eps,
-                       float route_scale, float* top_scores, int64_t* top_indices, int32_t* counts,
-                       int32_t* offsets, int32_t* sorted_indices, int32_t* inverse, float* sorted_scores,
-                       float* tokens_per_expert, void* gemm_plan, size_t gemm_plan_bytes, void* workspace,
-                       size_t workspace_bytes, void* stream) {
+int router_route(const char* fn, const ttamd::RouterGroups* groups, const void* x, const void* w_router,
+                 const float* expert_bias, int64_t num_tokens, int num_experts, int64_t dim, int topk, int score_func,
+                 int renorm, float renorm_eps, float route_scale, float* top_scores, int64_t* top_indices,
+                 int32_t* counts, int32_t* offsets, int32_t* sorted_indices, int32_t* inverse, float* sorted_scores,
+                 float* tokens_per_expert, void* gemm_plan, size_t gemm_plan_bytes, void* workspace,
+                 size_t workspace_bytes, void* stream) {
   REQUIRE(num_tokens >= 0 && num_tokens <= (1 << 24), "%s: num_tokens out of range", fn);
   REQUIRE(num_experts >= 1 && num_experts <= 256, "%s: num_experts must be in [1, 256]", fn);
   REQUIRE(topk >= 1 && topk <= 16 && topk <= num_experts, "%s: topk must be in [1, min(16, E)]", fn);
@@ -182,7 +181,8 @@ int router_route(const char* fn, const ttamd::RouterGroups* groups, const void* 
   REQUIRE((gemm_plan == nullptr && tokens_per_expert == nullptr) || (counts && offsets),
           "%s: gemm_plan and tokens_per_expert need the counts and offsets buffers", fn);
   const size_t rbytes = align256(ttamd::router_workspace_bytes(num_tokens, num_experts, dim));
-  TRY(check_ws(fn, workspace, workspace_bytes, ::ttamd_router_route_workspace_bytes(num_tokens, num_experts, dim, topk)));
+  TRY(check_ws(fn, workspace, workspace_bytes,
+               ::ttamd_router_route_workspace_bytes(num_tokens, num_experts, dim, topk)));
   if (gemm_plan) {
     REQUIRE(aligned16(gemm_plan), "%s: gemm_plan must be 16-byte aligned", fn);
     REQUIRE(gemm_plan_bytes >= ttamd::gemm_plan_bytes(M, num_experts),
@@ -406,15 +406,15 @@ int ttamd_router_backward(const float* grad_top_scores, const int64_t* top_indic
   REQUIRE(score_func == TTAMD_SCORE_SOFTMAX || score_func == TTAMD_SCORE_SIGMOID,
           "%s: unknown score_func %d", fn, score_func);
   REQUIRE(dim >= 128 && dim % 128 == 0 && dim <= (1 << 20), "%s: dim must be a positive multiple of 128", fn);
-  if (num_tokens == 0) return TTAMD_OK;
-  REQUIRE(grad_top_scores && top_indices && logits && w_router, "%s: null pointer argument", fn);
-  REQUIRE(grad_w_router == nullptr || x != nullptr, "%s: the weight gradient needs x", fn);
+  REQUIRE(num_tokens == 0 || (grad_top_scores && top_indices && logits && w_router), "%s: null pointer argument", fn);
+  REQUIRE(grad_w_router == nullptr || x != nullptr || num_tokens == 0, "%s: the weight gradient needs x", fn);
   REQUIRE(aligned16(w_router), "%s: w_router must be 16-byte aligned", fn);
   if (x) TRY(check_rows(fn, "x", x, num_tokens, dim));
   if (grad_x) TRY(check_rows(fn, "grad_x", grad_x, num_tokens, dim));
   if (grad_w_router) REQUIRE(aligned16(grad_w_router), "%s: grad_w_router must be 16-byte aligned", fn);
   REQUIRE(num_tokens * dim * 2 <= (int64_t)0xffffffffLL, "%s: x must stay below 4 GiB", fn);
-  TRY(check_ws(fn, workspace, workspace_bytes, ttamd::router_backward_workspace_bytes(num_tokens, num_experts, dim)));
+  if (num_tokens > 0)
+    TRY(check_ws(fn, workspace, workspace_bytes, ttamd::router_backward_workspace_bytes(num_tokens, num_experts, dim)));
   return check_hip(ttamd::launch_router_backward(grad_top_scores, top_indices, logits, x, w_router, (int)num_tokens,
                                                  num_experts, (int)dim, topk, score_func, renorm, renorm_eps,
                                                  route_scale, grad_x, grad_w_router, grad_w_is_fp32 != 0, workspace,
@@ -468,8 +468,8 @@ int ttamd_moe_experts_forward(const void* tokens, int64_t num_tokens, int64_t di
                               const float* sorted_scores, int score_before_experts, float swiglu_limit,
                               const void* w13, const void* w2, void* out, void* gemm_plan,
                               size_t gemm_plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
-  return experts_stage("ttamd_moe_experts_forward", false, tokens, num_tokens, dim, hidden, num_experts, topk, sorted_indices, offs,
-                       sorted_scores, score_before_experts, swiglu_limit, w13, w2, out, gemm_plan, gemm_plan_bytes,
+  return experts_stage("ttamd_moe_experts_forward", false, tokens, num_tokens, dim, hidden, num_experts, topk,
+                       sorted_indices, offs, sorted_scores, score_before_experts, swiglu_limit, w13, w2, out, gemm_plan, gemm_plan_bytes,
                        workspace, workspace_bytes, stream);
 }
 
@@ -485,8 +485,8 @@ int ttamd_moe_experts_rows(const void* tokens, int64_t num_tokens, int64_t dim, 
                            const float* sorted_scores, int score_before_experts, float swiglu_limit,
                            const void* w13, const void* w2, void* out, void* gemm_plan,
                            size_t gemm_plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
-  return experts_stage("ttamd_moe_experts_rows", true, tokens, num_tokens, dim, hidden, num_experts, topk, sorted_indices, offs,
-                       sorted_scores, score_before_experts, swiglu_limit, w13, w2, out, gemm_plan, gemm_plan_bytes,
+  return experts_stage("ttamd_moe_experts_rows", true, tokens, num_tokens, dim, hidden, num_experts, topk,
+                       sorted_indices, offs, sorted_scores, score_before_experts, swiglu_limit, w13, w2, out, gemm_plan, gemm_plan_bytes,
                        workspace, workspace_bytes, stream);
 }
 
@@ -621,15 +621,17 @@ int ttamd_residual_norm_backward(const void* du, const void* dn, const void* bra
   TRY(norm_args(fn, b.fwd, branch, num_tokens, dim, 1, residual, post_weight, gate, gate_kind, gate_sigmoid,
                 residual_scale, pre_weight, f32_mask));
   REQUIRE(dn == nullptr || pre_weight, "%s: dn needs pre_weight", fn);
-  REQUIRE(((!grad_post || post_weight) && (!grad_pre || pre_weight) && (!grad_gate || gate) &&
-           (!grad_branch || branch)) || num_tokens == 0,
+  REQUIRE((!grad_post || post_weight) && (!grad_pre || pre_weight) &&
+              (!grad_gate || gate || (num_tokens == 0 && gate_kind != TTAMD_GATE_CHANNEL)) &&
+              (!grad_branch || branch || num_tokens == 0),
           "%s: a gradient is asked for an operand that is not given", fn);
   REQUIRE(aligned16(du) && aligned16(dn) && aligned16(grad_branch) && aligned16(grad_residual) &&
               aligned16(grad_post) && aligned16(grad_pre) && (gate_kind < TTAMD_GATE_CHANNEL || aligned16(grad_gate)),
           "%s: operands must be 16-byte aligned", fn);
-  if (num_tokens == 0) return TTAMD_OK;
-  REQUIRE(rstd, "%s: rstd is null", fn);
-  TRY(check_ws(fn, workspace, workspace_bytes, ttamd::norm_backward_workspace_bytes(num_tokens, dim)));
+  if (num_tokens > 0) {
+    REQUIRE(rstd, "%s: rstd is null", fn);
+    TRY(check_ws(fn, workspace, workspace_bytes, ttamd::norm_backward_workspace_bytes(num_tokens, dim)));
+  }
   b.fwd.rstd = const_cast<float*>(rstd);
   b.du = du, b.dn = dn;
   b.dbranch = grad_branch, b.dresidual = grad_residual, b.dpost = grad_post, b.dgate = grad_gate, b.dpre = grad_pre;

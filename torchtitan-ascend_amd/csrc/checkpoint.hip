@@ -167,11 +167,9 @@ hipError_t launch_pack_rows(const void* in, int64_t R, int C, void* codes, void*
   const dim3 grid((unsigned)std::min<int64_t>(groups, 32 * num_cus()));
   if (C % 128 == 0)
     return launch_k(false, pack_rows_kernel<true>, grid, dim3(256), 0, stream, (const uint4*)in, (uint32_t)nblocks, nb,
-                    C / 8,
-                    (uint2*)codes, (uint8_t*)exps);
+                    C / 8, (uint2*)codes, (uint8_t*)exps);
   return launch_k(false, pack_rows_kernel<false>, grid, dim3(256), 0, stream, (const uint4*)in, (uint32_t)nblocks, nb,
-                    C / 8,
-                  (uint2*)codes, (uint8_t*)exps);
+                  C / 8, (uint2*)codes, (uint8_t*)exps);
 }
 
 hipError_t launch_unpack_rows(const void* codes, const void* exps, int n_src, const int* src_index, int src_div,
@@ -186,11 +184,9 @@ hipError_t launch_unpack_rows(const void* codes, const void* exps, int n_src, co
   if (row_scale)
     return launch_k(false, unpack_rows_kernel<true>, grid, dim3(256), 0, stream, (const uint2*)codes,
                     (const uint8_t*)exps, n_src, src_index, src_div, row_scale, (uint32_t)total, C / 8, nb,
-                    (uint4*)out,
-                    ids_index, ids_out, n_ids);
+                    (uint4*)out, ids_index, ids_out, n_ids);
   return launch_k(false, unpack_rows_kernel<false>, grid, dim3(256), 0, stream, (const uint2*)codes,
-                  (const uint8_t*)exps, n_src, src_index, src_div, row_scale, (uint32_t)total, C / 8, nb,
-                    (uint4*)out,
+                  (const uint8_t*)exps, n_src, src_index, src_div, row_scale, (uint32_t)total, C / 8, nb, (uint4*)out,
                   ids_index, ids_out, n_ids);
 }
 

@@ -540,6 +540,12 @@ int router_splits(int T, int D) {
   return (stages + per - 1) / per;  // no empty slice
 }
 
+// The weight gradient of no tokens.
+__global__ __launch_bounds__(256) void zero_kernel(uint4* __restrict__ p, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 }  // namespace
 
 // The most partial logits that any call of at most T tokens and D columns
@@ -656,7 +662,11 @@ hipError_t launch_router_backward(const float* grad, const int64_t* idx, const v
                                   const void* w, int T, int E, int D, int K, int score_func, int renorm,
                                   float renorm_eps, float route_scale, void* dx, void* dw, bool dw_fp32,
                                   void* ws, hipStream_t stream) {
-  if (T == 0) return hipSuccess;
+  if (T == 0) {
+    if (!dw) return hipSuccess;
+    const int n = E * (D / 8) * (dw_fp32 ? 2 : 1);
+    return launch_k(false, zero_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, (uint4*)dw, n);
+  }
   const int P = router_pad_e(E);
   const int G = router_dw_groups(T, E, D);
   const int NR = router_dw_rows(E);

@@ -415,8 +415,8 @@ def experts_forward(
     ws = _ws(need(T, D, H, E, top_k, int(bool(score_before_experts))), dev)
     plan = r.plan
     _call(
-        dev, "ttamd_moe_experts_forward" if sum_rows else "ttamd_moe_experts_rows", _p(x), T, D, H, E, top_k, _p(r.sorted_indices), _p(offsets) + 4,
-        _p(r.sorted_scores), int(bool(score_before_experts)), _limit(swiglu_limit), _p(w13), _p(w2), _p(out),
+        dev, "ttamd_moe_experts_forward" if sum_rows else "ttamd_moe_experts_rows", _p(x), T, D, H, E, top_k,
+        _p(r.sorted_indices), _p(offsets) + 4, _p(r.sorted_scores), int(bool(score_before_experts)), _limit(swiglu_limit), _p(w13), _p(w2), _p(out),
         _p(plan), 0 if plan is None else plan.numel(), _p(ws), ws.numel(), _stream(dev),
     )
     return out
@@ -811,6 +811,9 @@ def combine_norm(
     the combined [T, D] is never written.  rows bf16 [T * K, D].  Inference
     only: for gradients use functional.combine, functional.residual_norm."""
     dev = _gpu("rows", rows)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
+                                       (rows, probs, residual, post_weight, gate, pre_weight)):
+        raise RuntimeError("combine_norm has no backward: use functional.combine and functional.residual_norm")
     if rows.dim() != 2 or top_k < 1 or rows.shape[0] % top_k:
         raise ValueError(f"rows must be [T * {top_k}, D], got {tuple(rows.shape)}")
     rows = _want("rows", rows, _BF16)
@@ -879,8 +882,7 @@ def residual_norm_backward(
     stats = _want("stats", stats, torch.float32)
     if tuple(stats.shape) != (2, T):
         raise ValueError(f"stats must be [2, {T}], got {tuple(stats.shape)}")
-    make = torch.zeros_like if T == 0 else torch.empty_like
-    grads = ResidualNormGrads(*(None if t is None else make(t)
+    grads = ResidualNormGrads(*(None if t is None else torch.empty_like(t)
                                 for t in (branch, residual, post_weight, gate, pre_weight)))
     ws = _ws(_lib.load().ttamd_residual_norm_backward_workspace_bytes(T, D), dev)
     _call(
