@@ -298,6 +298,47 @@ def _err(name, *args):
     return L.ttamd_last_error().decode()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [2048, 2056])
+def test_pack_past_32_bits(ops, C):
+    """More than 2^31 values: the last rows are those of a small call."""
+    R, few = 1_050_001, 300
+    g = torch.Generator(device=DEV).manual_seed(7)
+    x = torch.randn(R, C, device=DEV, generator=g, dtype=BF16)
+    announce(f"pack past 32 bits, {C} columns")
+    p, q = ops.pack_e4m3(x), ops.pack_e4m3(x[R - few:])
+    assert torch.equal(p.codes[R - few:], q.codes) and torch.equal(p.exponents[R - few:], q.exponents)
+    del x
+    small = ops.unpack_e4m3(q)
+    assert torch.equal(ops.unpack_e4m3(p)[R - few:], small)
+    src = torch.arange(R - 1, R - 1 - few, -1, dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.unpack_e4m3(p, src), small.flip(0))
+
+
+@pytest.mark.gpu
+def test_dgrad_packed_past_32_bits(ops):
+    """More than 2^31 codes: as from the same h in bf16."""
+    D, H, last = 128, 2048, 300
+    counts = [540_000, 0, last]
+    M = sum(counts)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    dy = torch.zeros(M, D, dtype=BF16, device=DEV)
+    dy[M - last:] = torch.randn(last, D, device=DEV, generator=g)
+    w2 = torch.randn(3, D, H, device=DEV, generator=g).to(BF16)
+    h = torch.randn(last, 2 * H, device=DEV, generator=g).to(BF16)
+    tail = ops.pack_e4m3(h)
+    codes = torch.zeros(M, 2 * H, dtype=torch.uint8, device=DEV)
+    exps = torch.full((M, 2 * H // 128), 127, dtype=torch.uint8, device=DEV)
+    codes[M - last:], exps[M - last:] = tail.codes, tail.exponents
+    announce("packed dgrad past 32 bits")
+    dh, a = ops.grouped_mm_dgrad_swiglu_packed(dy, w2, ops.PackedRows(codes, exps), offsets(counts), want_a=True)
+    hb = torch.zeros(M, 2 * H, dtype=BF16, device=DEV)
+    hb[M - last:] = ops.unpack_e4m3(tail)
+    want, a_want = ops.grouped_mm_dgrad_swiglu(dy, w2, hb, offsets(counts), want_a=True)
+    assert want[M - last:].any()
+    assert torch.equal(dh, want) and torch.equal(a, a_want)
+
+
 def test_refusals():
     import ctypes
 

@@ -432,6 +432,48 @@ def test_block_without_tokens(ops):
     assert u.shape == (0, 128) and n.shape == (0, 128)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_block_gradients_without_tokens(ops, checkpoint):
+    """No tokens: empty outputs and exact zeros for every weight."""
+    rng = np.random.default_rng(34)
+    c = inputs(rng, 4, 128, 128, 8, "channel")
+    c["x"] = c["x"][:0]
+    names = [k for k in c if k != "expert_bias"]
+    leaves = {k: c[k].clone().requires_grad_(True) for k in names}
+    announce(f"block gradients without tokens, checkpoint {checkpoint}")
+    u, n = call({**c, **leaves}, 2, score_func="sigmoid", num_groups=4, topk_groups=2, checkpoint=checkpoint)
+    (u.float().sum() + n.float().sum()).backward()
+    for k in names:
+        g = leaves[k].grad
+        assert g is not None and g.shape == c[k].shape and not g.any(), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("before", [False, True])
+def test_gradients_of_some_inputs_are_those_of_all(ops, before):
+    """Whatever is asked for beside it, an input's gradient has the same bits;
+    the upstream gradient is a broadcast one."""
+    rng = np.random.default_rng(35)
+    c = inputs(rng, 300, 256, 128, 8)
+    sc = torch.rand(300, 4, device=DEV)
+    idx = torch.rand(300, 8, device=DEV).argsort(1)[:, :4]
+    names = ("x", "scores", "w13", "w2")
+
+    def grads(wanted):
+        t = dict(x=c["x"].clone(), scores=sc.clone(), w13=c["w13"].clone(), w2=c["w2"].clone())
+        for k in wanted:
+            t[k].requires_grad_(True)
+        F().moe_experts_forward(t["x"], t["scores"], idx, t["w13"], t["w2"], 8, before,
+                                checkpoint="e4m3").sum().backward()
+        return {k: t[k].grad for k in wanted}
+
+    announce("gradients of some inputs")
+    every = grads(names)
+    for k in names:
+        assert torch.equal(grads((k,))[k], every[k]), k
+
+
 def test_module_refuses_an_unknown_checkpoint(pkg):
     P = importlib.import_module("torchtitan-ascend_amd.protocol")
     mc = P.ModelConfig()
@@ -441,6 +483,24 @@ def test_module_refuses_an_unknown_checkpoint(pkg):
     pkg.HipGroupedExpertsConverter(pkg.HipGroupedExpertsConverter.Config(activation_checkpoint="int8")).convert(mc)
     with pytest.raises(ValueError, match="activation_checkpoint"):
         mc.moe.build()
+
+
+def test_module_refuses_a_checkpoint_with_another_dispatcher(pkg):
+    P = importlib.import_module("torchtitan-ascend_amd.protocol")
+    mc = P.ModelConfig()
+    mc.moe = P.GroupedExperts.Config(
+        dim=128, hidden_dim=128, num_experts=4,
+        token_dispatcher=P.AllToAllTokenDispatcher.Config(num_experts=4, top_k=1, score_before_experts=False))
+    pkg.HipGroupedExpertsConverter(pkg.HipGroupedExpertsConverter.Config(activation_checkpoint="e4m3")).convert(mc)
+    m = mc.moe.build()
+    with pytest.raises(NotImplementedError, match="HipTokenDispatcher"):
+        m(torch.zeros(1, 2, 128), torch.zeros(1, 2, 1), torch.zeros(1, 2, 1, dtype=torch.int64))
+
+
+def test_unknown_checkpoint_refused_without_autograd():
+    with torch.no_grad(), pytest.raises(ValueError, match="checkpoint"):
+        F().moe_experts_forward(torch.zeros(2, 128), torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int64),
+                                torch.zeros(4, 256, 128), torch.zeros(4, 128, 128), 4, False, checkpoint="int8")
 
 
 def test_experts_rows_refusals():

@@ -228,6 +228,8 @@ def moe_experts_forward(
     """
     T, D = x.shape
     K = top_scores.shape[-1]
+    if checkpoint not in (None, "e4m3"):
+        raise ValueError(f"checkpoint must be 'e4m3' or None, got {checkpoint!r}")
     training = _needs_grad(x, top_scores, w13, w2)
     ev = stage_events if (stage_events is not None and not training) else None
 
@@ -277,8 +279,6 @@ def moe_experts_forward(
             mark("sum_topk", True)
         return out.to(x.dtype)
     if checkpoint is not None:
-        if checkpoint != "e4m3":
-            raise ValueError(f"checkpoint must be 'e4m3' or None, got {checkpoint!r}")
         keep_y = not score_before_experts and scores_flat.requires_grad
         out = _T.experts_packed(xb, scores_flat, sorted_idx, inverse, sorted_scores, offs, w13, w2, K,
                                 score_before_experts, swiglu_limit, keep_y)[0]

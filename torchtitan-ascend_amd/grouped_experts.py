@@ -62,7 +62,8 @@ class HipGroupedExperts(Module):
         token_dispatcher: Any
         swiglu_limit: float | None = None
         # "e4m3": the training forward keeps its activations in 8 bits
-        # (functional.moe_experts_forward); None: in bf16
+        # (functional.moe_experts_forward, so with a local HipTokenDispatcher
+        # only); None: in bf16
         activation_checkpoint: str | None = None
 
     def __init__(self, config: "HipGroupedExperts.Config"):
@@ -108,6 +109,10 @@ class HipGroupedExperts(Module):
                 x, top_scores, selected_experts_indices, w13, w2, self.num_experts,
                 disp.score_before_experts, self.swiglu_limit, checkpoint=self.activation_checkpoint,
             )
+        if self.activation_checkpoint is not None and torch.is_grad_enabled():
+            # the packed stage holds dispatch and combine itself
+            raise NotImplementedError(
+                f"activation_checkpoint={self.activation_checkpoint!r} needs the single-GPU HipTokenDispatcher")
         routed_input, num_tokens_local, metadata = disp.dispatch(x, top_scores, selected_experts_indices)
         routed_output = self._experts_forward(routed_input, num_tokens_local)
         return disp.combine(routed_output, metadata, x)
