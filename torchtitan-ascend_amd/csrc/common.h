@@ -66,14 +66,13 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
   return v;
 }
 
-// Four e4m3 codes (low byte first) times a scale.
+// Four e4m3 codes (low byte first) times a power of two, in the conversion
+// itself.
 __device__ __forceinline__ void unpack_e4m3x4(uint32_t codes, float scale, float* f) {
-  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
-  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
-  f[0] = lo[0] * scale;
-  f[1] = lo[1] * scale;
-  f[2] = hi[0] * scale;
-  f[3] = hi[1] * scale;
+  const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, scale, false);
+  const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, scale, true);
+  f[0] = lo[0], f[1] = lo[1];
+  f[2] = hi[0], f[3] = hi[1];
 }
 
 // Streaming (non-temporal) 16-byte load and store, for data a kernel reads

@@ -237,7 +237,7 @@ struct FwdArgs {
   // EPI_SWIGLU_BWD
   const bf16_t* h_in;  // saved pre-activation [M][2H]
   const uint8_t* h_codes;  // EPI_SWIGLU_BWD_PACKED: e4m3 codes [M][2H]
-  const uint8_t* h_exps;   // ... exponent bytes [M][2H / 128]
+  const uint8_t* h_exps;   // ... exponent bytes [M][2H / 128] (read together: keep them adjacent)
   bf16_t* a_out;       // recomputed activation [M][H] (nullable)
   // EPI_SCATTER
   const float* row_scale;

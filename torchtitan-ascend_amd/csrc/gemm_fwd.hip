@@ -111,6 +111,8 @@ static_assert(kSplitPartBytes == (size_t)WAVES * NJ * NPB * 4 * 64 * 4, "partial
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4_t lds_short4_t;
 typedef __attribute__((address_space(1))) int gint_t;
+typedef const __attribute__((address_space(1))) uint8_t gbyte_t;
+typedef const __attribute__((address_space(1))) uint32_t gword_t;
 typedef __attribute__((address_space(1))) floatx4_t gfloatx4_t;
 
 // Chunk permutation of the 512-byte reduction-major weight rows (PT): the 16
@@ -666,21 +668,35 @@ __global__ __launch_bounds__(FTHREADS, 1) void gg_fwd_kernel(const FwdArgs a) {
     const int pcol = 16 * (eg4 & 1) + 8 * (eg4 >> 1);  // the lane's columns in a block pair
     // EPI_SWIGLU_BWD: saved pre-activation of token block jj (packed: four
     // e4m3 codes in .x; the wave's 64 columns lie in one 128-column block, so
-    // a row has one exponent for its gate and one for its up columns there,
-    // in .y of the first block)
+    // a row has one exponent for its gate and one for its up columns there:
+    // in .y of the first block the even lane groups hold the gate's, the odd
+    // ones the up's)
     constexpr bool SWIGLU_BWD = EPI == EPI_SWIGLU_BWD || EPI == EPI_SWIGLU_BWD_PACKED;
+    // Packed: offsets from the tile's first row, in 32 bits beside uniform
+    // bases (the lane has no registers for 64-bit ones beside the
+    // accumulators; opaque, or the compiler adds the bases' distance per
+    // lane).  The pointers are re-read here rather than held through the k loop.
+    uint64_t h_gate = 0, h_up = 0, h_exp = 0;
+    if constexpr (EPI == EPI_SWIGLU_BWD_PACKED) {
+      const int4 hp = sload_int4((const int4*)((const char*)__builtin_amdgcn_kernarg_segment_ptr() +
+                                               offsetof(FwdArgs, h_codes)));
+      h_gate = ((uint64_t)(uint32_t)hp.y << 32 | (uint32_t)hp.x) + (uint64_t)((int64_t)row0 * a.ldh);
+      h_up = h_gate + (uint64_t)a.hidden;
+      h_exp = ((uint64_t)(uint32_t)hp.w << 32 | (uint32_t)hp.z) + (uint64_t)((int64_t)row0 * (a.ldh >> 7));
+      asm volatile("" : "+s"(h_gate), "+s"(h_up), "+s"(h_exp));
+    }
     auto load_h = [&](int jj, uint2 (&dst)[NPB][2]) {
       const int qrow = min(row0 + 32 * jj + 16 * wq + er16, row1 - 1);
       if constexpr (EPI == EPI_SWIGLU_BWD_PACKED) {
-        const uint8_t* erow = a.h_exps + (int64_t)qrow * (a.ldh >> 7) + (min(pt * TP + arow0, a.n_p - 64) >> 7);
-        dst[0][0].y = erow[0];
-        dst[0][1].y = erow[a.hidden >> 7];
+        const uint32_t lrow = (uint32_t)max(qrow - row0, 0), ldh = (uint32_t)a.ldh;
+        const int col = min(pt * TP + arow0, a.n_p - 64);  // the wave's 64 columns are valid or not together
+        const uint32_t eoff = lrow * (ldh >> 7) + (uint32_t)(col >> 7);
+        dst[0][0].y = ((gbyte_t*)h_exp)[eoff + (uint32_t)((a.hidden >> 7) & -(eg4 & 1))];
+        const uint32_t off = lrow * ldh + (uint32_t)(col + 4 * eg4);
 #pragma unroll
         for (int pb = 0; pb < NPB; ++pb) {
-          const int col = min(pt * TP + arow(pb), a.n_p - 16) + 4 * eg4;
-          const uint8_t* hrow = a.h_codes + (int64_t)qrow * a.ldh + col;
-          dst[pb][0].x = *(const uint32_t*)hrow;
-          dst[pb][1].x = *(const uint32_t*)(hrow + a.hidden);
+          dst[pb][0].x = *(gword_t*)((gbyte_t*)h_gate + off + 16 * pb);
+          dst[pb][1].x = *(gword_t*)((gbyte_t*)h_up + off + 16 * pb);
         }
       }
       if constexpr (EPI == EPI_SWIGLU_BWD) {
@@ -772,8 +788,11 @@ __global__ __launch_bounds__(FTHREADS, 1) void gg_fwd_kernel(const FwdArgs a) {
             const uint2 hu = hv[pb][1];
             float gate[4], up[4];
             if constexpr (EPI == EPI_SWIGLU_BWD_PACKED) {
-              // code * 2^e, exact in fp32; a byte e + 127 is 2^e's exponent field
-              const float sg = __uint_as_float(hv[0][0].y << 23), su = __uint_as_float(hv[0][1].y << 23);
+              // code * 2^e, exact in fp32; a byte e + 127 is 2^e's exponent
+              // field (gate's to every lane, then up's)
+              uint32_t ex, ey;
+              swap_halves<16>(hv[0][0].y, ex, ey);
+              const float sg = __uint_as_float(ex << 23), su = __uint_as_float(ey << 23);
               unpack_e4m3x4(hg.x, sg, gate);
               unpack_e4m3x4(hu.x, su, up);
             } else {
