@@ -19,7 +19,8 @@
 // Memory-bound: 2 bytes in, 1 + 1/128 out (back: the reverse).  16 lanes share
 // a block, 8 columns (16 bytes) each; the maximum is an integer maximum of the
 // bf16 bits (ordered as the values are), the exponent comes from its bits, and
-// v_cvt_pk_fp8_f32 rounds.
+// v_cvt_pk_fp8_f32 rounds.  Measured (65536 rows of 1536): pack 54 us, unpack
+// 48 us, 5.6 and 6.3 TB/s; 1003 rows of 1544 4.2 and 3.4 us, a launch each.
 #include <algorithm>
 
 #include "common.h"

@@ -670,7 +670,9 @@ __global__ __launch_bounds__(FTHREADS, 1) void gg_fwd_kernel(const FwdArgs a) {
     // e4m3 codes in .x; the wave's 64 columns lie in one 128-column block, so
     // a row has one exponent for its gate and one for its up columns there:
     // in .y of the first block the even lane groups hold the gate's, the odd
-    // ones the up's)
+    // ones the up's).  The main loop hides the packed form as it does the
+    // other: 32 experts, 32768 rows, w2 of 7168 x 2048, 915 us from codes, 923
+    // from bf16, with a_out 940 and 950.
     constexpr bool SWIGLU_BWD = EPI == EPI_SWIGLU_BWD || EPI == EPI_SWIGLU_BWD_PACKED;
     // Packed: offsets from the tile's first row, in 32 bits beside uniform
     // bases (the lane has no registers for 64-bit ones beside the

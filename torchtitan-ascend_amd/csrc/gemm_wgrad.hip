@@ -96,7 +96,9 @@ __device__ __forceinline__ void static_for(F&& f) {
 // GATHER: reduction row m is x row x_rows[m] (a token that several experts
 // read).  A wave moves two rows per x instruction, so a stage's row ids are
 // scalar loads, made when the cursor reaches the stage, one stage ahead of the
-// instructions that use them.
+// instructions that use them.  128 experts, 8192 tokens to 8 each, 1536 x 2048:
+// 576 us with fp32 gradients, as on routed rows (bf16: 467; with one vector
+// load of an id per lane and instruction 490); unpacking the tokens takes 12.
 template <bool GATHER>
 __global__ __launch_bounds__(THREADS, 1) void gg_wgrad_dma_kernel(const WgradDmaArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];

@@ -26,8 +26,8 @@
 // experts: 17.8 -> 15.6 us, one token 4.8 -> 4.1).
 //
 // What bounds it: few tokens, the latency of one launch (4 us); many tokens,
-// VALU issue (1300 instructions per wave of four tokens at E = 256, K = 8: 9 of
-// 14.5 us at 16384 tokens), not the logits' bytes (3.4 us).
+// VALU issue (1240 instructions per wave of four tokens at E = 256, K = 8: 9 of
+// 14.0 us at 16384 tokens), not the logits' bytes (3.4 us).
 #include <type_traits>
 
 #include "common.h"
@@ -559,6 +559,9 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
 // token, each a run of 4 experts of every 4 LPT: whole 16-byte (bf16: 8-byte)
 // stores where E % 4 == 0.  An index outside [0, E) contributes nothing; one
 // that occurs twice adds twice.
+// Bound by the launch up to a few thousand tokens (softmax, 256 experts: 32
+// tokens 6.3 us, 4096 7.2), then by VALU issue (16384 17.2; sigmoid, without
+// the scores of the other experts, 11.3; the bytes alone 6.9).
 // ---------------------------------------------------------------------------
 struct TopkBwdArgs {
   const float* grad;   // [T, K]
@@ -701,7 +704,7 @@ hipError_t launch_group_topk(int src, GroupTopkArgs a, hipStream_t stream) {
   // 16 lanes per token while they hold at most 4 experts each, and wherever
   // issue slots count; a wave per token in between, whose lists are shorter
   // to build.  Measured (us, 16 lanes / 64): E = 256, 8 groups, 1024 tokens
-  // 6.4 / 4.4, 2048 6.5 / 5.6, 4096 6.7 / 8.0, 16384 14.6 / 23.1; E = 160,
+  // 6.4 / 4.4, 2048 6.5 / 5.6, 4096 6.6 / 8.0, 16384 14.0 / 23.1; E = 160,
   // 1024 5.6 / 4.5, 2048 5.7 / 5.9; E = 64, 32 tokens 3.6 / 4.2.
   int lr16 = 0, lr64 = 0;
   const int p16 = experts_per_lane(16, a.G, a.EG, &lr16), p64 = experts_per_lane(64, a.G, a.EG, &lr64);

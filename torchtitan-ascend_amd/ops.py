@@ -172,8 +172,8 @@ def router_topk(
             _p(idx), _stream(dev),
         )
         return scores, idx
-    _lib.call(
-        "ttamd_router_topk", _p(logits), _p(expert_bias), T, E, top_k, _SCORE_FUNCS[score_func],
+    _call(
+        dev, "ttamd_router_topk", _p(logits), _p(expert_bias), T, E, top_k, _SCORE_FUNCS[score_func],
         int(bool(route_norm)), float(norm_eps), float(route_scale), _p(scores), _p(idx), _stream(dev),
     )
     return scores, idx
