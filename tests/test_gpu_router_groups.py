@@ -139,6 +139,26 @@ def test_grouped_topk_special_values(ops, func, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("func", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("T", [7, 2061])
+def test_grouped_topk_huge_logits(ops, func, T):
+    """Logits whose differences or sizes leave exp's range (their scores are
+    equal then: the lower ids win), up to fp32's largest."""
+    rng = np.random.default_rng(51)
+    E, K, G, kept = 64, 6, 8, 3
+    for size in (3e3, 1e10, 1e30, 3.4e38):
+        z = (rng.uniform(-1.0, 1.0, (T, E)) * size).astype(np.float32)
+        z[:, ::5] = np.float32(0.999 * size)
+        announce(f"grouped topk huge logits {func} T={T} {size}")
+        s, i = ops.router_topk(torch.from_numpy(z).to(DEV), K, func, True, 1.0, None, EPS, num_groups=G,
+                               topk_groups=kept)
+        torch.cuda.synchronize()
+        _, ws, wi = plain(z, K, func, True, 1.0, None, G, kept, "top2")
+        np.testing.assert_array_equal(i.cpu().numpy(), wi)
+        np.testing.assert_allclose(s.cpu().numpy(), ws, rtol=2.0 ** -23, atol=1e-38)
+
+
+@pytest.mark.gpu
 def test_grouped_topk_unaligned_and_strided(ops):
     """Logits that start off a 16-byte border, and a column slice."""
     rng = np.random.default_rng(6)

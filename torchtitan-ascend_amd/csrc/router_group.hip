@@ -23,11 +23,12 @@
 // sorts its K best with a sorting network; lists then merge pairwise across
 // the token's lanes (16 lanes: 4 merges, in the VALU's own lane exchanges), in
 // place of K dependent rounds of a maximum over all lanes (16384 tokens of 256
-// experts: 17.8 -> 15.6 us, one token 4.8 -> 4.1).
+// experts: 17.8 -> 15.6 us, one token 4.8 -> 4.1).  A lane's first two are also
+// its share of its group's value.
 //
 // What bounds it: few tokens, the latency of one launch (4 us); many tokens,
-// VALU issue (1240 instructions per wave of four tokens at E = 256, K = 8: 9 of
-// 14.0 us at 16384 tokens), not the logits' bytes (3.4 us).
+// VALU issue (1140 instructions per wave of four tokens at E = 256, K = 8: 8 of
+// 13.6 us at 16384 tokens), not the logits' bytes (3.4 us).
 #include <type_traits>
 
 #include "common.h"
@@ -71,10 +72,15 @@ __device__ __forceinline__ double min_d(double a, double b) {
   return d;
 }
 
-// exp(x), x clamped to [-700, 700] (a NaN becomes -700: the callers look for
-// it themselves).
+// The largest size of three numbers; NaN if one is.
+__device__ __forceinline__ float most3(float a, float b, float c) {
+  float d;
+  asm("v_maximum3_f32 %0, |%1|, |%2|, |%3|" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
+// exp(x), |x| <= 700.
 __device__ __forceinline__ double exp_f64(double x) {
-  x = min_d(max_d(x, -700.0), 700.0);
   // n = round(x / ln 2) by adding 1.5 * 2^52: n is then also the sum's low word
   const double magic = 6755399441055744.0;
   const double shifted = __builtin_fma(x, 1.4426950408889634, magic);
@@ -107,11 +113,17 @@ __device__ __forceinline__ double rcp_f64(double d) {
   return __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
 }
 
-__device__ __forceinline__ double sigmoid_f64(double z) { return rcp_f64(1.0 + exp_f64(-z)); }
-
-// Scores of single logits, NaN included.
+// Scores of single logits.  Exponents past 700 count as 700, a NaN as the
+// least: the callers look for it themselves.
+__device__ __forceinline__ double sigmoid_f64(float z) {
+  return rcp_f64(1.0 + exp_f64(-(double)__builtin_amdgcn_fmed3f(z, -700.f, 700.f)));
+}
+__device__ __forceinline__ double exp_below(float z, float mx) {  // exp(z - mx), mx the row's maximum
+  return exp_f64(max_d((double)z - (double)mx, -700.0));
+}
+// The same, NaN included.
 __device__ __forceinline__ double score_of(float z, bool softmax, float mx, double inv) {
-  const double s = softmax ? exp_f64((double)z - (double)mx) * inv : sigmoid_f64((double)z);
+  const double s = softmax ? exp_below(z, mx) * inv : sigmoid_f64(z);
   return z == z ? s : __builtin_nan("");
 }
 
@@ -396,19 +408,32 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
   double v[PL];
   float mx = 0.f, nan = 0.f;  // nan: NaN when a logit is (or softmax has no finite maximum)
   double inv = 1.0;
+  // is any logit or bias of the wave's tokens NaN or infinite?
+  float size = 0.f;
 #pragma unroll
-  for (int m = 0; m < PL; ++m) nan += z[m] == z[m] ? 0.f : z[m];
+  for (int m = 0; m < PL; m += 2) size = most3(z[m], z[m + 1], size);
+  if (a.bias) {
+#pragma unroll
+    for (int m = 0; m < PL; m += 2) size = most3(bias[m], bias[m + 1], size);
+  }
+  const bool special = __builtin_amdgcn_ballot_w64(!(size < INFINITY)) != 0;
+  if (special) {
+#pragma unroll
+    for (int m = 0; m < PL; ++m) nan += z[m] == z[m] ? 0.f : z[m];
+  }
   if (a.score_func == 0) {
     mx = -INFINITY;
 #pragma unroll
     for (int m = 0; m < PL; ++m) mx = fmaxf(mx, z[m]);  // (a clamped index repeats a logit of the row)
     mx = all_maxf<LPT>(mx);
-    if (!__builtin_isfinite(mx)) nan = __builtin_nanf("");  // inf - inf
-    nan = all_sumf<LPT>(nan);                               // one NaN makes the whole row NaN
+    if (special) {
+      if (!__builtin_isfinite(mx)) nan = __builtin_nanf("");  // inf - inf
+      nan = all_sumf<LPT>(nan);                               // one NaN makes the whole row NaN
+    }
     double sum = 0.0;
 #pragma unroll
     for (int m = 0; m < PL; ++m) {
-      const double x = exp_f64((double)z[m] - (double)mx);
+      const double x = exp_below(z[m], mx);
       v[m] = m < n_live ? x : 0.0;
       sum += v[m];
     }
@@ -417,18 +442,14 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
     for (int m = 0; m < PL; ++m) v[m] *= inv;
   } else {
 #pragma unroll
-    for (int m = 0; m < PL; ++m) v[m] = sigmoid_f64((double)z[m]);
+    for (int m = 0; m < PL; ++m) v[m] = sigmoid_f64(z[m]);
   }
-  float odd = nan;
   if (a.bias) {
 #pragma unroll
-    for (int m = 0; m < PL; ++m) {
-      v[m] += (double)bias[m];
-      odd = fmaf(bias[m], 0.f, odd);
-    }
+    for (int m = 0; m < PL; ++m) v[m] += (double)bias[m];
   }
   // NaN and infinities take the general order; numbers are in it already
-  if (__builtin_amdgcn_ballot_w64(odd != odd)) {
+  if (special) {
 #pragma unroll
     for (int m = 0; m < PL; ++m) {
       const bool bad = a.score_func == 0 ? nan != nan : z[m] != z[m];
@@ -436,21 +457,33 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
     }
   }
 
-  // slots without an expert: the high word alone makes them the least
+  // keys; slots without an expert: the high word alone makes them the least
   auto kill = [](double d) { return as_f64((uint64_t)kDeadHi << 32 | (uint32_t)as_u64(d)); };
+#pragma unroll
+  for (int m = 0; m < PL; ++m) v[m] = with_id(v[m], e0 + m);
   if (a.per_lane < PL || a.EG != a.per_lane << a.log_run || a.G << a.log_run != LPT) {  // uniform
 #pragma unroll
     for (int m = 0; m < PL; ++m) v[m] = m < n_live ? v[m] : kill(v[m]);
   }
   const double dead = as_f64((uint64_t)kDeadHi << 32);
-  bool keep = n_live > 0;
-  if (a.kept < a.G) {  // uniform
-    double b1 = dead, b2 = dead;
+
+  // the lane's KL best
+  double top[KL];
 #pragma unroll
-    for (int m = 0; m < PL; ++m) {
-      b2 = max_d(b2, min_d(b1, v[m]));
-      b1 = max_d(b1, v[m]);
-    }
+  for (int i = 0; i < KL; ++i) top[i] = i < PL ? v[i] : dead;
+  sort_list(top);
+#pragma unroll
+  for (int c = KL; c < PL; c += KL) {
+    double more[KL];
+#pragma unroll
+    for (int i = 0; i < KL; ++i) more[i] = c + i < PL ? v[c + i] : dead;
+    sort_list(more);
+    merge_lists(top, more);
+  }
+
+  if (a.kept < a.G) {  // uniform
+    // (without the ids: groups of equal values are equal)
+    double b1 = as_f64(as_u64(top[0]) & ~kIdMask), b2 = as_f64(as_u64(top[1]) & ~kIdMask);
     run_top2<LPT>(b1, b2, 1 << a.log_run);
     double value = (a.top2 && a.EG > 1) ? group_sum(b1, b2) : b1;
     value = group < a.G ? with_id(value, group) : dead;
@@ -481,27 +514,10 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
         }
       }
     }
-    keep = keep && in;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) top[i] = in ? top[i] : kill(top[i]);
   }
-#pragma unroll
-  for (int m = 0; m < PL; ++m) {
-    const double key = with_id(v[m], e0 + m);
-    v[m] = keep ? key : kill(key);
-  }
-
-  // the lane's KL best, then the token's
-  double top[KL];
-#pragma unroll
-  for (int i = 0; i < KL; ++i) top[i] = i < PL ? v[i] : dead;
-  sort_list(top);
-#pragma unroll
-  for (int c = KL; c < PL; c += KL) {
-    double more[KL];
-#pragma unroll
-    for (int i = 0; i < KL; ++i) more[i] = c + i < PL ? v[c + i] : dead;
-    sort_list(more);
-    merge_lists(top, more);
-  }
+  // the token's
   merge_lanes<LPT>(top);
   double mine = top[0];
 #pragma unroll
@@ -704,7 +720,7 @@ hipError_t launch_group_topk(int src, GroupTopkArgs a, hipStream_t stream) {
   // 16 lanes per token while they hold at most 4 experts each, and wherever
   // issue slots count; a wave per token in between, whose lists are shorter
   // to build.  Measured (us, 16 lanes / 64): E = 256, 8 groups, 1024 tokens
-  // 6.4 / 4.4, 2048 6.5 / 5.6, 4096 6.6 / 8.0, 16384 14.0 / 23.1; E = 160,
+  // 6.4 / 4.4, 2048 6.5 / 5.6, 4096 6.6 / 8.0, 16384 13.6 / 23.1; E = 160,
   // 1024 5.6 / 4.5, 2048 5.7 / 5.9; E = 64, 32 tokens 3.6 / 4.2.
   int lr16 = 0, lr64 = 0;
   const int p16 = experts_per_lane(16, a.G, a.EG, &lr16), p64 = experts_per_lane(64, a.G, a.EG, &lr64);
