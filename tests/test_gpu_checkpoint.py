@@ -316,6 +316,25 @@ def test_pack_past_32_bits(ops, C):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("counts", [[238] * 12, [700], [3000, 0, 1, 129, 5], [64, 65, 128], [31], [4000, 1, 4000]])
+@pytest.mark.parametrize("D,H", [(1024, 384), (64, 128), (1408, 512)])
+def test_dgrad_packed_few_tiles(ops, counts, D, H):
+    """Few tiles (shorter ones than the bf16 form's): the same bits, since a
+    reduction of fewer than 24 stages of 64 is never cut and its order does not
+    depend on the tiles."""
+    rng = np.random.default_rng(len(counts) + D)
+    M, E = sum(counts) + 3, len(counts)
+    dy = torch.from_numpy(rng.standard_normal((M, D))).to(BF16).to(DEV)
+    w2 = torch.from_numpy(rng.standard_normal((E, D, H)) * 0.05).to(BF16).to(DEV)
+    h = ops.pack_e4m3(torch.from_numpy(rng.standard_normal((M, 2 * H))).to(BF16).to(DEV))
+    announce(f"dgrad packed few tiles counts={counts} D={D} H={H}")
+    n = sum(counts)
+    dh, a = ops.grouped_mm_dgrad_swiglu_packed(dy, w2, h, offsets(counts), None, want_a=True)
+    dh0, a0 = ops.grouped_mm_dgrad_swiglu(dy, w2, ops.unpack_e4m3(h), offsets(counts), None, want_a=True)
+    assert torch.equal(dh[:n], dh0[:n]) and torch.equal(a[:n], a0[:n])
+
+
+@pytest.mark.gpu
 def test_dgrad_packed_past_32_bits(ops):
     """More than 2^31 codes: as from the same h in bf16."""
     D, H, last = 128, 2048, 300
