@@ -545,3 +545,16 @@ def test_python_refusals(ops):
     assert ops._norm_operands(dev, 4, 64, **{**base, "gate": x})[3] == 3
     assert ops._norm_operands(dev, 1, 64, **{**base, "gate": x[:1]})[3] == 2
     assert ops._norm_operands(dev, 1, 64, **{**base, "gate": x[:1, :1]})[3] == 1
+
+
+def test_backward_refuses_a_missing_channel_gate_without_tokens():
+    """post_weight's gradient is written without tokens too, and a channel gate
+    is a factor of it: without the gate nothing is launched."""
+    import ctypes
+
+    L = importlib.import_module("torchtitan-ascend_amd._lib").load()
+    p = ctypes.c_void_p(256)
+    rc = L.ttamd_residual_norm_backward(None, None, p, 0, 64, None, p, None, 2, 0, 1.0, None, p, 0, p, None, p, None,
+                                        None, None, 0, None)
+    assert rc == 1
+    assert "gate" in L.ttamd_last_error().decode()

@@ -625,6 +625,8 @@ int ttamd_residual_norm_backward(const void* du, const void* dn, const void* bra
               (!grad_gate || gate || (num_tokens == 0 && gate_kind != TTAMD_GATE_CHANNEL)) &&
               (!grad_branch || branch || num_tokens == 0),
           "%s: a gradient is asked for an operand that is not given", fn);
+  // (the column sums are launched without tokens too, and a channel gate is read there)
+  REQUIRE(gate || gate_kind != TTAMD_GATE_CHANNEL || !grad_post, "%s: gate and gate_kind disagree", fn);
   REQUIRE(aligned16(du) && aligned16(dn) && aligned16(grad_branch) && aligned16(grad_residual) &&
               aligned16(grad_post) && aligned16(grad_pre) && (gate_kind < TTAMD_GATE_CHANNEL || aligned16(grad_gate)),
           "%s: operands must be 16-byte aligned", fn);
