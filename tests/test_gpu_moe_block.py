@@ -515,3 +515,44 @@ def test_experts_rows_refusals():
     assert "ttamd_moe_experts_rows: dim" in L.ttamd_last_error().decode()
     assert L.ttamd_moe_experts_rows(*args(128, need - 1)) == 1
     assert "workspace" in L.ttamd_last_error().decode()
+
+
+def _experts(E, D=128, H=128, device="cpu"):
+    bf = lambda *n: torch.zeros(*n, dtype=BF16, device=device)  # noqa: E731
+    return bf(E, 2 * H, D), bf(E, D, H)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("E", [4, 16])
+def test_block_refuses_a_gate_of_other_experts(grad, E):
+    """A router of 8 experts before 4 or 16: the offsets and the tile table that
+    it makes are not those the expert stage reads."""
+    w13, w2 = _experts(E)
+    x = torch.zeros(2, 128, dtype=BF16, requires_grad=grad)
+    with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="experts"):
+        F().moe_block(x, torch.zeros(8, 128, dtype=BF16), w13, w2, 2)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_expert_stage_refuses_another_number_of_experts(grad, checkpoint):
+    w13, w2 = _experts(4)
+    x = torch.zeros(2, 128, dtype=BF16, requires_grad=grad)
+    with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="experts"):
+        F().moe_experts_forward(x, torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int64), w13, w2, 8, False,
+                                checkpoint=checkpoint)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sum_rows", [True, False])
+def test_experts_forward_refuses_a_routing_of_other_experts(ops, sum_rows):
+    """Refused on the host, with a tile plan and without."""
+    x = torch.zeros(6, 128, dtype=BF16, device=DEV)
+    idx = torch.arange(6, device=DEV).view(6, 1)
+    w13, w2 = _experts(8, device=DEV)
+    for E in (4, 16):
+        announce(f"experts_forward on a routing of {E} experts")
+        for r in (ops.route(idx % E, E, torch.ones(6, 1, device=DEV)),
+                  ops.router_route(x, torch.zeros(E, 128, dtype=BF16, device=DEV), 1)[2]):
+            with pytest.raises(ValueError, match="experts"):
+                ops.experts_forward(x, r, w13, w2, 1, False, sum_rows=sum_rows)

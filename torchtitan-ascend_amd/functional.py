@@ -230,6 +230,8 @@ def moe_experts_forward(
     K = top_scores.shape[-1]
     if checkpoint not in (None, "e4m3"):
         raise ValueError(f"checkpoint must be 'e4m3' or None, got {checkpoint!r}")
+    if w13.shape[0] != num_experts:
+        raise ValueError(f"w13 holds {w13.shape[0]} experts, num_experts is {num_experts}")
     training = _needs_grad(x, top_scores, w13, w2)
     ev = stage_events if (stage_events is not None and not training) else None
 
@@ -326,6 +328,8 @@ def moe_block(
     registered backward; without, the norms after the block run inside the
     combine (ops.combine_norm).  Routing arguments as `router`, checkpoint as
     `moe_experts_forward`, norm arguments as `residual_norm`; D % 128 == 0."""
+    if w_router.shape[0] != w13.shape[0]:
+        raise ValueError(f"w_router chooses among {w_router.shape[0]} experts, w13 holds {w13.shape[0]}")
     groups = dict(num_groups=num_groups, topk_groups=topk_groups, group_score=group_score)
     how = dict(post_weight=post_weight, gate=gate, gate_func=gate_func, residual_scale=residual_scale,
                pre_weight=next_weight, eps=eps)

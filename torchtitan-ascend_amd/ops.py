@@ -408,6 +408,8 @@ def experts_forward(
         raise ValueError("experts_forward needs the routing scores (route(..., scores))")
     if r.sorted_indices.numel() != T * top_k:
         raise ValueError("routing does not match T * top_k rows")
+    if r.offsets.numel() != E + 1:
+        raise ValueError(f"the routing is over {r.offsets.numel() - 1} experts, w13 holds {E}")
     lib = _lib.load()
     offsets = r.offsets.contiguous()  # inclusive offsets: its int32 entries from the second on
     out = torch.empty(T if sum_rows else T * top_k, D, dtype=_BF16, device=dev)
