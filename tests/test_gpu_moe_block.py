@@ -556,3 +556,12 @@ def test_experts_forward_refuses_a_routing_of_other_experts(ops, sum_rows):
                   ops.router_route(x, torch.zeros(E, 128, dtype=BF16, device=DEV), 1)[2]):
             with pytest.raises(ValueError, match="experts"):
                 ops.experts_forward(x, r, w13, w2, 1, False, sum_rows=sum_rows)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_block_refuses_an_unknown_checkpoint(grad):
+    """With autograd and without, where nothing is kept."""
+    w13, w2 = _experts(4)
+    x = torch.zeros(2, 128, dtype=BF16, requires_grad=grad)
+    with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="checkpoint"):
+        F().moe_block(x, torch.zeros(4, 128, dtype=BF16), w13, w2, 2, checkpoint="int8")

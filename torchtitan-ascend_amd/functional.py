@@ -197,6 +197,11 @@ def shared_expert_combine(
     return routed_out + y
 
 
+def _check_checkpoint(checkpoint: str | None) -> None:
+    if checkpoint not in (None, "e4m3"):
+        raise ValueError(f"checkpoint must be 'e4m3' or None, got {checkpoint!r}")
+
+
 def moe_experts_forward(
     x: torch.Tensor,
     top_scores: torch.Tensor,
@@ -228,8 +233,7 @@ def moe_experts_forward(
     """
     T, D = x.shape
     K = top_scores.shape[-1]
-    if checkpoint not in (None, "e4m3"):
-        raise ValueError(f"checkpoint must be 'e4m3' or None, got {checkpoint!r}")
+    _check_checkpoint(checkpoint)
     if w13.shape[0] != num_experts:
         raise ValueError(f"w13 holds {w13.shape[0]} experts, num_experts is {num_experts}")
     training = _needs_grad(x, top_scores, w13, w2)
@@ -328,6 +332,7 @@ def moe_block(
     registered backward; without, the norms after the block run inside the
     combine (ops.combine_norm).  Routing arguments as `router`, checkpoint as
     `moe_experts_forward`, norm arguments as `residual_norm`; D % 128 == 0."""
+    _check_checkpoint(checkpoint)
     if w_router.shape[0] != w13.shape[0]:
         raise ValueError(f"w_router chooses among {w_router.shape[0]} experts, w13 holds {w13.shape[0]}")
     groups = dict(num_groups=num_groups, topk_groups=topk_groups, group_score=group_score)
