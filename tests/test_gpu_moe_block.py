@@ -565,3 +565,38 @@ def test_block_refuses_an_unknown_checkpoint(grad):
     x = torch.zeros(2, 128, dtype=BF16, requires_grad=grad)
     with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="checkpoint"):
         F().moe_block(x, torch.zeros(4, 128, dtype=BF16), w13, w2, 2, checkpoint="int8")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block", [True, False])
+def test_graph_of_an_fp32_stream(block):
+    """What moe_block takes, the graph of it takes: an fp32 residual stream,
+    with norms and without; every replay equals the eager block."""
+    MoELayerGraph = importlib.import_module("torchtitan-ascend_amd.graph").MoELayerGraph
+    rng = np.random.default_rng(36)
+    T, D, K = 70, 256, 4
+    c = inputs(rng, T, D, 128, 8, "channel", torch.float32)
+    names = ("pre_weight", "post_weight", "next_weight", "gate") if block else ()
+    how = dict(gate_func="sigmoid" if block else "identity", residual_scale=0.5, eps=EPS, score_func="sigmoid",
+               route_norm=True, expert_bias=c["expert_bias"], **{k: c[k] for k in names})
+    announce(f"graph of an fp32 stream block={block}")
+    g = MoELayerGraph(c["x"], c["w_router"], c["w13"], c["w2"], K, residual=True, **how)
+    with torch.no_grad():
+        for i in range(4):
+            x = torch.from_numpy(rng.standard_normal((T, D)).astype(np.float32)).to(DEV)
+            u, n = g(x)
+            eu, en = F().moe_block(x, c["w_router"], c["w13"], c["w2"], K, **how)
+            torch.cuda.synchronize()
+            assert u.dtype == torch.float32 and torch.equal(u, eu), f"replay {i}"
+            assert (n is None and en is None) if not block else torch.equal(n, en)
+
+
+def test_graph_refuses_an_fp32_layer():
+    """The layer without the block around it takes bf16 tokens."""
+    MoELayerGraph = importlib.import_module("torchtitan-ascend_amd.graph").MoELayerGraph
+    w13, w2 = _experts(4)
+    with pytest.raises(TypeError, match="bf16"):
+        MoELayerGraph(torch.zeros(2, 128), torch.zeros(4, 128, dtype=BF16), w13, w2, 2)
+    with pytest.raises(TypeError, match="fp32"):
+        MoELayerGraph(torch.zeros(2, 128, dtype=torch.float16), torch.zeros(4, 128, dtype=BF16), w13, w2, 2,
+                      residual=True)

@@ -35,7 +35,8 @@ class MoELayerGraph:
 
     With ``residual``, or any of the norm weights or a gate, the graph holds
     the block around the layer (functional.moe_block: norm, layer, norm, gate,
-    residual sum, next norm; the gate is read in place too) and returns (u, n).
+    residual sum, next norm; the gate is read in place too) and returns (u, n);
+    x, the residual stream, is then bf16 or fp32.
     """
 
     def __init__(
@@ -64,8 +65,9 @@ class MoELayerGraph:
         eps: float = 1e-6,
         residual: bool = False,
     ):
-        if x.dim() != 2 or x.dtype != _BF16:
-            raise TypeError("x must be a bf16 [T, D] tensor")
+        block = residual or any(t is not None for t in (pre_weight, post_weight, gate, next_weight))
+        if x.dim() != 2 or x.dtype != _BF16 and not (block and x.dtype == torch.float32):
+            raise TypeError("x must be a bf16 [T, D] tensor, or an fp32 one with the block around the layer")
         for name, t in (("w_router", w_router), ("w13", w13), ("w2", w2)):
             if t.dtype != _BF16 or not t.is_contiguous():
                 raise TypeError(f"{name} must be a contiguous bf16 tensor (read in place by the graph)")
@@ -73,7 +75,7 @@ class MoELayerGraph:
                       expert_bias, swiglu_limit)
         self._groups = dict(num_groups=num_groups, topk_groups=topk_groups, group_score=group_score)
         self._block = None
-        if residual or any(t is not None for t in (pre_weight, post_weight, gate, next_weight)):
+        if block:
             self._block = dict(pre_weight=pre_weight, post_weight=post_weight, gate=gate, gate_func=gate_func,
                                residual_scale=residual_scale, next_weight=next_weight, eps=eps)
         self.static_x = x.detach().clone()
