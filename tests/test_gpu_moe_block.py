@@ -600,3 +600,13 @@ def test_graph_refuses_an_fp32_layer():
     with pytest.raises(TypeError, match="fp32"):
         MoELayerGraph(torch.zeros(2, 128, dtype=torch.float16), torch.zeros(4, 128, dtype=BF16), w13, w2, 2,
                       residual=True)
+
+
+@pytest.mark.parametrize("only", [dict(residual_scale=0.5), dict(gate_func="sigmoid")])
+def test_graph_refuses_block_arguments_without_a_block(only):
+    """A scale or an activation of the gate would have nothing to act on: the
+    graph would hold the bare layer and leave it out."""
+    MoELayerGraph = importlib.import_module("torchtitan-ascend_amd.graph").MoELayerGraph
+    w13, w2 = _experts(4)
+    with pytest.raises(ValueError, match="residual"):
+        MoELayerGraph(torch.zeros(2, 128, dtype=BF16), torch.zeros(4, 128, dtype=BF16), w13, w2, 2, **only)

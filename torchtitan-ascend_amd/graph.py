@@ -68,6 +68,8 @@ class MoELayerGraph:
         block = residual or any(t is not None for t in (pre_weight, post_weight, gate, next_weight))
         if x.dim() != 2 or x.dtype != _BF16 and not (block and x.dtype == torch.float32):
             raise TypeError("x must be a bf16 [T, D] tensor, or an fp32 one with the block around the layer")
+        if not block and (residual_scale != 1.0 or gate_func != "identity"):
+            raise ValueError("residual_scale and gate_func need the block: residual=True, a norm weight or a gate")
         for name, t in (("w_router", w_router), ("w13", w13), ("w2", w2)):
             if t.dtype != _BF16 or not t.is_contiguous():
                 raise TypeError(f"{name} must be a contiguous bf16 tensor (read in place by the graph)")
