@@ -237,7 +237,7 @@ struct FwdArgs {
   // EPI_SWIGLU_BWD
   const bf16_t* h_in;  // saved pre-activation [M][2H]
   const uint8_t* h_codes;  // EPI_SWIGLU_BWD_PACKED: e4m3 codes [M][2H]
-  const uint8_t* h_exps;   // ... exponent bytes [M][2H / 128] (read together: keep them adjacent)
+  const uint8_t* h_exps;   // ... exponent bytes [M][2H / 128]
   bf16_t* a_out;       // recomputed activation [M][H] (nullable)
   // EPI_SCATTER
   const float* row_scale;
@@ -251,6 +251,10 @@ struct FwdArgs {
 static_assert(offsetof(FwdArgs, split_cnt) == offsetof(FwdArgs, part) + sizeof(float*) &&
                   offsetof(FwdArgs, part) % 8 == 0,
               "FwdArgs: split_cnt must directly follow part");
+// The packed SwiGLU-backward epilogue reads h_codes and h_exps the same way.
+static_assert(offsetof(FwdArgs, h_exps) == offsetof(FwdArgs, h_codes) + sizeof(uint8_t*) &&
+                  offsetof(FwdArgs, h_codes) % 8 == 0,
+              "FwdArgs: h_exps must directly follow h_codes");
 
 // Grouped dgrad through the forward kernel's reduction-major weight mode:
 // out[m, k] = sum_n dy[m, n] w[e(m), n, k], w [E, n_red, n_out].
