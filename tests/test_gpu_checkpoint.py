@@ -400,3 +400,32 @@ def test_python_refusals(ops):
         ops._packed("x", ops.PackedRows(u8, u8), u8.device)
     with pytest.raises(TypeError, match="codes"):
         ops._packed("x", ops.PackedRows(x, u8[:, :1]), u8.device)
+
+
+@pytest.mark.gpu
+def test_dgrad_packed_few_tiles_split(ops):
+    """A skewed load whose low token tiles are cut along a reduction of 32
+    stages (72 tiles of 128 rows, three pieces each; an even load of as many
+    experts has 100 tall ones, uncut): against 64 bits by the bound of
+    test_dgrad_swiglu_packed, and the same bits every time."""
+    D, H, E = 2048, 256, 100
+    counts = np.zeros(E, np.int64)
+    counts[[7, 50, 99]] = 3001, 2999, 3000
+    M = int(counts.sum())
+    gen = torch.Generator(device=DEV).manual_seed(22)
+    dy = torch.randn(M, D, device=DEV, generator=gen).to(BF16)
+    w2 = (torch.randn(E, D, H, device=DEV, generator=gen) * 0.05).to(BF16)
+    h = ops.pack_e4m3(torch.randn(M, 2 * H, device=DEV, generator=gen).to(BF16))
+    announce("dgrad packed few tiles, split")
+    dh, a = ops.grouped_mm_dgrad_swiglu_packed(dy, w2, h, offsets(counts), None, want_a=True)
+    torch.cuda.synchronize()
+    hd = ops.unpack_e4m3(h).double().requires_grad_(True)
+    act = torch.nn.functional.silu(hd[:, :H]) * hd[:, H:]
+    ends = np.cumsum(counts)
+    g = torch.cat([dy[ends[e] - counts[e]:ends[e]].double() @ w2[e].double() for e in (7, 50, 99)])
+    (rdh,) = torch.autograd.grad(act, hd, g)
+    assert rel_err_rows(to_np(dh), rdh.cpu().numpy()) < 2.0 ** -7
+    assert rel_err_rows(to_np(a), act.detach().cpu().numpy()) < 2.0 ** -7
+    for _ in range(3):
+        dh1, a1 = ops.grouped_mm_dgrad_swiglu_packed(dy, w2, h, offsets(counts), None, want_a=True)
+        assert torch.equal(dh1, dh) and torch.equal(a1, a)

@@ -417,7 +417,10 @@ hipError_t launch_grouped_mm_fp8_unpermute(const void* aq, const float* sa, cons
 
 // Whether the packed dgrad takes token tiles of 64 or 128 rows (the plan's
 // small table): where the full ones would leave most of the chip idle, are not
-// split, and are high enough to be cut.  A row's sum is the same either way.
+// split, and are high enough to be cut.  A row's sum is the same either way
+// where the reduction has fewer than 24 stages (split_pieces never cuts those);
+// a longer one the kernel may cut in either form, by the tiles that the load
+// really makes, and its sums then differ in order.
 // Measured, us, 320-row tiles against these: 12 experts of 1024 x 384, 238 rows
 // each 51 -> 39; one of 1408 x 1024, 300 rows 66 -> 33, 700 rows 58 -> 36; 16 of
 // 1408 x 512, 256 rows 61 -> 46; 4 of 1024 x 256, 1000 rows 50 -> 39.  With one
