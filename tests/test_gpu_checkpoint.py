@@ -429,3 +429,34 @@ def test_dgrad_packed_few_tiles_split(ops):
     for _ in range(3):
         dh1, a1 = ops.grouped_mm_dgrad_swiglu_packed(dy, w2, h, offsets(counts), None, want_a=True)
         assert torch.equal(dh1, dh) and torch.equal(a1, a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_wgrad_packed_ignores_the_next_experts_special_tokens(ops, dtype):
+    """A stage of 64 rows that an expert fills in part also loads the next
+    experts' tokens, and behind the last row token 0: NaN and infinities there
+    (NaN once packed) stay out of the gradients of experts that do not read
+    them, and an expert without rows gets exact zeros."""
+    rng = np.random.default_rng(21)
+    counts, D, N = [30, 40, 0, 65], 256, 128
+    M = sum(counts)
+    x = rng.standard_normal((M, D))
+    x[0, 5], x[0, 77], x[1, 9] = np.nan, np.inf, -np.inf
+    src = np.roll(np.arange(M), -2)  # finite tokens ...
+    src[[30, 70]] = 0, 1             # ... but the first ones of experts 1 and 3
+    src[-2:] = 2, 3                  # (where tokens 0 and 1 were)
+    assert src[M - 1] > 1 and (np.delete(src, [30, 70]) > 1).all()
+    p = ops.pack_e4m3(torch.from_numpy(x).to(BF16).to(DEV))
+    dy = torch.from_numpy(rng.standard_normal((M, N))).to(BF16).to(DEV)
+    ids = torch.from_numpy(src.astype(np.int32)).to(DEV)
+    announce(f"wgrad packed beside special tokens {dtype}")
+    got = ops.grouped_mm_wgrad_packed(dy, p, offsets(counts), 4, dtype, ids, 1)
+    want = ops.grouped_mm_wgrad(dy, ops.unpack_e4m3(p, ids, 1), offsets(counts), 4, dtype)
+    torch.cuda.synchronize()
+    assert bool(((got == want) | (got.isnan() & want.isnan())).all())
+    nan = torch.zeros(4, N, D, dtype=torch.bool, device=DEV)
+    nan[1, :, [5, 77]] = True
+    nan[3, :, 9] = True
+    assert torch.equal(got.isnan(), nan) and not bool(got.isinf().any())
+    assert not got[2].any()
