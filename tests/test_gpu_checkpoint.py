@@ -460,3 +460,44 @@ def test_wgrad_packed_ignores_the_next_experts_special_tokens(ops, dtype):
     nan[3, :, 9] = True
     assert torch.equal(got.isnan(), nan) and not bool(got.isinf().any())
     assert not got[2].any()
+
+
+@pytest.mark.gpu
+def test_every_code_and_exponent(ops):
+    """Each of the 256 codes at each exponent that packing makes: exact, down to
+    the least code's 2^-9 * 2^-118 = 2^-127, which bf16 and fp32 hold below
+    their normal numbers.  (At e = 120 codes end at 240.)"""
+    code = np.arange(256)
+    mant, expo = code & 7, (code >> 3) & 15
+    value = np.where(expo == 0, mant * 2.0 ** -9, (8 + mant) * np.exp2(expo - 10.0))
+    value = np.where((code & 127) == 127, np.nan, value) * np.where(code & 128, -1.0, 1.0)
+    bytes_ = np.arange(127 - 118, 127 + 120 + 1)
+    want = value[None, :] * np.exp2(bytes_[:, None] - 127.0)
+    want[-1, np.abs(value) > 240] = 0.0
+    codes = np.tile(code.astype(np.uint8), (len(bytes_), 1))
+    codes[-1, np.abs(value) > 240] = 0
+    p = ops.PackedRows(torch.from_numpy(codes).to(DEV),
+                       torch.from_numpy(np.repeat(bytes_[:, None].astype(np.uint8), 2, axis=1)).to(DEV))
+    announce("every code and exponent")
+    y = ops.unpack_e4m3(p).cpu().double().numpy()
+    np.testing.assert_array_equal(y, want)
+    # with a scale of one: the same values
+    one = torch.ones(len(bytes_), device=DEV)
+    np.testing.assert_array_equal(ops.unpack_e4m3(p, row_scale=one).cpu().double().numpy(), want)
+
+
+@pytest.mark.gpu
+def test_least_values(ops):
+    """Blocks at the lowest exponent: values on, between and below the grid's
+    step of 2^-127, both signs (1/2, 3/2 and 5/2 steps are ties)."""
+    steps = np.array([0.0, 0.25, 0.5, 0.75, 1.0, 1.25, 1.5, 1.75, 2.0, 2.5, 3.0, 4.0, 5.5, 7.0, 8.0, 9.0, 17.0])
+    x = np.concatenate([steps, -steps]) * 2.0 ** -127
+    x = np.pad(x, (0, 8 - len(x) % 8))
+    x = np.stack([x, np.roll(x, 5)])
+    t = torch.from_numpy(x).to(BF16)
+    np.testing.assert_array_equal(t.double().numpy(), x)  # bf16 holds them
+    announce("least values")
+    p = ops.pack_e4m3(t.to(DEV))
+    e, val = define(x)
+    np.testing.assert_array_equal(p.exponents.cpu().numpy(), e)
+    np.testing.assert_array_equal(ops.unpack_e4m3(p).cpu().double().numpy(), val)

@@ -13,8 +13,9 @@
 // four significant bits, bf16 eight, so a restored row goes to the matrix
 // cores, or an epilogue rebuilds it, without a second rounding.  It costs at
 // most half a binade of range, none of the code's relative precision.  Blocks
-// below 448 * 2^-118 lose range at the bottom instead of leaving fp32's
-// normal numbers.
+// below 448 * 2^-118 lose range at the bottom: their least code is 2^-127, a
+// subnormal number of bf16 and fp32 (kept by every step here), where the scale
+// of a lower exponent would lead out of bf16.
 //
 // Memory-bound: 2 bytes in, 1 + 1/128 out (back: the reverse).  16 lanes share
 // a block, 8 columns (16 bytes) each; the maximum is an integer maximum of the

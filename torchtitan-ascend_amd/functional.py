@@ -220,8 +220,9 @@ def moe_experts_forward(
     bits (x, the pre-activation and the experts' outputs, packed by
     ops.pack_e4m3): about a third of the bf16 ones' memory (a quarter with
     many choices per token).  The output is the same; the weights' and the
-    scores' gradients are those at the stored values, within e4m3's 2^-4 of
-    each activation.
+    scores' gradients are those at the stored values: within 2^-4 of an
+    activation of at least 2^-13 of the largest in its row's 128 columns, a
+    smaller one within 2^-17 of that largest (so the least become 0).
 
     With autograd off (or nothing requiring grad) the expert stage is one
     op (ttamd::moe_experts_forward: both grouped GEMMs on one tile table,

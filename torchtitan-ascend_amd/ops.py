@@ -1152,7 +1152,8 @@ def _packed(name: str, p: PackedRows, dev: torch.device) -> tuple[torch.Tensor, 
 def pack_e4m3(x: torch.Tensor) -> PackedRows:
     """8-bit checkpoint of bf16 rows x [R, C] (ttamd_pack_e4m3): 1 + 1/128 byte
     per value, a relative error of at most 2^-4 for values down to 2^-13 of
-    their block's largest.  NaN and infinities come back as NaN."""
+    their block's largest, below that an error of at most 2^-17 of it (blocks
+    of nothing above 2^-110: of 2^-128).  NaN and infinities come back as NaN."""
     dev = _gpu("x", x)
     if x.dim() != 2:
         raise ValueError(f"x must be [R, C], got {tuple(x.shape)}")
