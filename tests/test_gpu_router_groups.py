@@ -404,3 +404,54 @@ def test_grouped_ops_need_a_gpu(ops):
         ops.router_topk(z, 4, num_groups=8, topk_groups=2)
     with pytest.raises(RuntimeError, match="HIP device"):
         ops.router_topk_backward(torch.zeros(4, 4), torch.zeros(4, 4, dtype=torch.int64), z)
+
+
+# ---------------------------------------------------------------------------
+# The 64-bit arithmetic's own bounds
+# ---------------------------------------------------------------------------
+def grad_bound(p, idx, ref, g, func, norm, scale, bf16):
+    """What topk_backward_kernel may be off by.  Its scores are within 2^-43 of
+    themselves (exponential and sum 2^-45.6 each, reciprocal 2^-45) and
+    everything else is 64-bit, so an element is within a few such steps (16:
+    2^-39) of the sum of its terms' sizes, before any cancels; then one
+    rounding to fp32, or two to bf16, and half a step of the smallest numbers."""
+    w = np.take_along_axis(p, idx, 1)
+    d = np.abs(np.asarray(g, np.float64)) * scale
+    if norm:
+        S = w.sum(1, keepdims=True) + EPS
+        d = d / S + (d * w).sum(1, keepdims=True) / (S * S)
+    a = np.zeros_like(p)
+    for k in range(idx.shape[1]):
+        np.add.at(a, (np.arange(len(p)), idx[:, k]), d[:, k])
+    size = p * (a + (d * w).sum(1, keepdims=True)) if func == "softmax" else p * a
+    step = 2.0 ** -8 + 2.0 ** -23 if bf16 else 2.0 ** -24
+    return np.abs(ref) * step + size * 2.0 ** -39 + (2.0 ** -133 if bf16 else 2.0 ** -149)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,K,G,kept,value", [(4099, 160, 6, 8, 3, "max"), (33, 256, 8, 8, 4, "top2"),
+                                                (70, 64, 1, 64, 1, "top2"), (9, 1023, 16, 33, 5, "top2"),
+                                                (50, 48, 2, 4, 2, "top2")])
+@pytest.mark.parametrize("func,norm", [("sigmoid", True), ("sigmoid", False), ("softmax", False), ("softmax", True)])
+@pytest.mark.parametrize("peak", [0.0, 10.0, 20.0])
+def test_topk_backward_is_64_bit(ops, T, E, K, G, kept, value, func, norm, peak):
+    """Ordinary rows and peaked ones (a logit 10 or 20 above the rest), where a
+    renormalised weight or a softmax score is close to 1 and the differences
+    of the formulas cancel."""
+    rng = np.random.default_rng(T + 5 * E + int(peak))
+    z = rng.standard_normal((T, E)).astype(np.float32) * 1.5
+    z[np.arange(T), rng.integers(0, E, T)] += np.float32(peak)
+    for bf16 in (False, True):
+        zt = torch.from_numpy(z).to(DEV)
+        zt = zt.to(torch.bfloat16) if bf16 else zt
+        g = rng.standard_normal((T, K)).astype(np.float32)
+        announce(f"64-bit topk backward T={T} E={E} K={K} {func} norm={norm} peak={peak} bf16={bf16}")
+        _, i = ops.router_topk(zt, K, func, norm, 2.5, num_groups=G, topk_groups=kept, group_score=value)
+        dz = ops.router_topk_backward(torch.from_numpy(g).to(DEV), i, zt, func, norm, 2.5, EPS)
+        torch.cuda.synchronize()
+        p, _, _ = plain(to_np(zt), K, func, norm, 2.5, None, G, kept, value)
+        idx = i.cpu().numpy()
+        ref = plain_grad(p, idx, g, func, norm, 2.5)
+        tol = grad_bound(p, idx, ref, g, func, norm, 2.5, bf16)
+        got = dz.cpu().double().numpy()
+        assert (np.abs(got - ref) <= tol).all(), float((np.abs(got - ref) / tol).max())
