@@ -455,3 +455,39 @@ def test_topk_backward_is_64_bit(ops, T, E, K, G, kept, value, func, norm, peak)
         tol = grad_bound(p, idx, ref, g, func, norm, 2.5, bf16)
         got = dz.cpu().double().numpy()
         assert (np.abs(got - ref) <= tol).all(), float((np.abs(got - ref) / tol).max())
+
+
+def truncated(v):
+    """The first 42 places of the values."""
+    return (np.asarray(v, np.float64).view(np.uint64) & ~np.uint64(1023)).view(np.float64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [7, 2061])
+@pytest.mark.parametrize("G,kept,value", [(1, 1, "max"), (4, 4, "top2"), (4, 2, "max"), (4, 2, "top2")])
+def test_saturated_sigmoids_compare_42_places(ops, T, G, kept, value):
+    """Sigmoid scores so close to 1 that 64 bits still tell them apart and 42
+    places do not (logits of 30 and 36): equal values, so the lower id (group)
+    wins.  None of these logits' scores is within the kernel's 2^-45 of a
+    border of the 42 places."""
+    rng = np.random.default_rng(T + G)
+    E, K = 32, 6
+    pool = np.array([28.0, 28.5, 29.0, 29.5, 30.0, 30.5, 31.0, 32.0, 33.0, 35.0, 36.0, 38.0, 40.0])
+    z = rng.choice(pool, (T, E)).astype(np.float32)
+    announce(f"saturated sigmoids T={T} G={G} kept={kept} {value}")
+    s, i = ops.router_topk(torch.from_numpy(z).to(DEV), K, "sigmoid", False, 1.0, num_groups=G, topk_groups=kept,
+                           group_score=value)
+    torch.cuda.synchronize()
+    score = 1.0 / (1.0 + np.exp(-z.astype(np.float64)))
+    v = truncated(score)
+    best = -np.sort(-v.reshape(T, G, E // G), axis=2)
+    gv = truncated(best[:, :, 0] + best[:, :, 1]) if value == "top2" else best[:, :, 0]
+    keep = np.argsort(-gv, axis=1, kind="stable")[:, :kept]
+    in_kept = np.zeros((T, G), bool)
+    np.put_along_axis(in_kept, keep, True, 1)
+    v = np.where(np.repeat(in_kept, E // G, axis=1), v, -1.0)
+    want = np.argsort(-v, axis=1, kind="stable")[:, :K]
+    np.testing.assert_array_equal(i.cpu().numpy(), want)
+    np.testing.assert_allclose(s.cpu().numpy(), np.take_along_axis(score, want, 1), rtol=2.0 ** -23)
+    # what the documentation says of it: the definition's own 64-bit order differs here
+    assert (np.argsort(-np.where(v < 0, -1.0, score), axis=1, kind="stable")[:, :K] != want).any()

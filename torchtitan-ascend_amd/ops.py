@@ -145,8 +145,10 @@ def router_topk(
     num_groups and topk_groups limit the picks to the experts of the
     topk_groups best of num_groups equal runs of experts (group_score: a
     group's value is the sum of its two largest selection values, "top2", or
-    its largest, "max"); scores and selection are then 64-bit and bf16 logits
-    are read as they are (ttamd_router_topk_grouped).  No autograd here: see
+    its largest, "max"); bf16 logits are then read as they are, scores are
+    64-bit, and the selection compares the first 42 places of 64-bit values:
+    ones that agree in those (the sigmoid scores of logits 30 and 36) are
+    ties (ttamd_router_topk_grouped).  No autograd here: see
     functional.router_topk, router_topk_backward.
     """
     dev = _gpu("logits", logits)
