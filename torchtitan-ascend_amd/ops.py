@@ -303,8 +303,8 @@ def router_backward(
     dx = torch.empty(T, D, dtype=_BF16, device=dev) if need_dx else None
     dw = torch.empty(E, D, dtype=dw_dtype, device=dev) if need_dw else None
     ws = _ws(_lib.load().ttamd_router_backward_workspace_bytes(T, E, D), dev)
-    _lib.call(
-        "ttamd_router_backward", _p(g), _p(idx), _p(logits), _p(x), _p(w_router), T, E, D, K, funcs[score_func],
+    _call(
+        dev, "ttamd_router_backward", _p(g), _p(idx), _p(logits), _p(x), _p(w_router), T, E, D, K, funcs[score_func],
         int(bool(route_norm)), float(norm_eps), float(route_scale), _p(dx), _p(dw), int(dw_dtype == torch.float32),
         _p(ws), ws.numel(), _stream(dev),
     )
@@ -458,8 +458,8 @@ def route(
     lib = _lib.load()
     wsb = lib.ttamd_route_workspace_bytes(M, num_experts)
     ws = _ws(wsb, dev)
-    _lib.call(
-        "ttamd_moe_route", _p(labels), int(labels.dtype == torch.int64), M, num_experts, _p(sc),
+    _call(
+        dev, "ttamd_moe_route", _p(labels), int(labels.dtype == torch.int64), M, num_experts, _p(sc),
         _p(counts), _p(offsets), _p(sorted_idx), _p(inverse), _p(sorted_scores), _p(ws), ws.numel(),
         _stream(dev),
     )
@@ -479,8 +479,8 @@ def gather_rows(
     out = torch.empty(rows, D, dtype=_BF16, device=dev)
     if row_scale is not None:
         row_scale = _want("row_scale", row_scale, torch.float32)
-    _lib.call(
-        "ttamd_moe_gather_rows", _p(x), _p(src_index), _p(row_scale), x.numel() // D, rows, D, top_k,
+    _call(
+        dev, "ttamd_moe_gather_rows", _p(x), _p(src_index), _p(row_scale), x.numel() // D, rows, D, top_k,
         _p(out), _stream(dev),
     )
     return out
@@ -514,7 +514,7 @@ def dispatch_rows(
     if scores_flat is not None:
         scores_flat = _want("scores_flat", scores_flat, torch.float32)
     out = torch.empty(T * top_k, D, dtype=_BF16, device=dev)
-    _lib.call("ttamd_moe_dispatch_rows", _p(x), _p(inverse), _p(scores_flat), T, D, top_k, _p(out), _stream(dev))
+    _call(dev, "ttamd_moe_dispatch_rows", _p(x), _p(inverse), _p(scores_flat), T, D, top_k, _p(out), _stream(dev))
     return out
 
 
@@ -540,7 +540,7 @@ def gather_rows_exact(x: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
     out = torch.empty(rows, W, dtype=_BF16, device=dev)
     if W % 8:
         raise ValueError(f"row width of {x.shape[1]} {x.dtype} elements is not a multiple of 16 bytes")
-    _lib.call("ttamd_moe_gather_rows", _p(xv), _p(index), None, xv.shape[0], rows, W, 1, _p(out), _stream(dev))
+    _call(dev, "ttamd_moe_gather_rows", _p(xv), _p(index), None, xv.shape[0], rows, W, 1, _p(out), _stream(dev))
     return out.view(x.dtype)
 
 
@@ -556,7 +556,7 @@ def scatter_rows_exact(x: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
     if W % 8:
         raise ValueError(f"row width of {x.shape[1]} {x.dtype} elements is not a multiple of 16 bytes")
     out = torch.empty(T, W, dtype=_BF16, device=dev)
-    _lib.call("ttamd_moe_dispatch_rows", _p(xv), _p(index), None, T, W, 1, _p(out), _stream(dev))
+    _call(dev, "ttamd_moe_dispatch_rows", _p(xv), _p(index), None, T, W, 1, _p(out), _stream(dev))
     return out.view(x.dtype)
 
 
@@ -586,8 +586,8 @@ def token_permute(
     counts = torch.empty(num_experts, dtype=torch.int32, device=dev)
     lib = _lib.load()
     ws = _ws(lib.ttamd_route_workspace_bytes(M, num_experts), dev)
-    _lib.call(
-        "ttamd_moe_token_permute", _p(tokens), _p(labels), int(labels.dtype == torch.int64), T, D, topk,
+    _call(
+        dev, "ttamd_moe_token_permute", _p(tokens), _p(labels), int(labels.dtype == torch.int64), T, D, topk,
         num_experts, _p(permuted), _p(sorted_idx), _p(counts), _p(ws), ws.numel(), _stream(dev),
     )
     if return_counts:
@@ -616,8 +616,8 @@ def token_unpermute(
     out = torch.empty(T, D, dtype=_BF16, device=dev)
     lib = _lib.load()
     ws = _ws(lib.ttamd_unpermute_workspace_bytes(T, top_k), dev)
-    _lib.call(
-        "ttamd_moe_token_unpermute", _p(permuted), _p(sorted_indices), _p(probs), T, D, top_k, _p(out),
+    _call(
+        dev, "ttamd_moe_token_unpermute", _p(permuted), _p(sorted_indices), _p(probs), T, D, top_k, _p(out),
         _p(ws), ws.numel(), _stream(dev),
     )
     return out
@@ -647,8 +647,8 @@ def token_unpermute_grad(
         permuted = _want("permuted", permuted, _BF16)
         gp = torch.empty(M, dtype=torch.float32, device=dev)
     g = torch.empty(M, D, dtype=_BF16, device=dev)
-    _lib.call(
-        "ttamd_moe_token_unpermute_grad", _p(grad_out), _p(sorted_indices), _p(probs),
+    _call(
+        dev, "ttamd_moe_token_unpermute_grad", _p(grad_out), _p(sorted_indices), _p(probs),
         _p(permuted if need_probs_grad else None), T, D, top_k, _p(g), _p(gp), _stream(dev),
     )
     return g, gp
@@ -666,7 +666,7 @@ def combine(
     if probs is not None:
         probs = probs.reshape(-1).float().contiguous()
     out = torch.empty(T, D, dtype=_BF16, device=dev)
-    _lib.call("ttamd_moe_combine", _p(permuted), _p(inverse), _p(probs), T, D, top_k, _p(out), _stream(dev))
+    _call(dev, "ttamd_moe_combine", _p(permuted), _p(inverse), _p(probs), T, D, top_k, _p(out), _stream(dev))
     return out
 
 
@@ -677,8 +677,8 @@ def rowdot_scatter(a: torch.Tensor, b: torch.Tensor, index: torch.Tensor, div: i
     b = _want("b", b, _BF16)
     index = _want("index", index, torch.int32)
     out = torch.empty(a.shape[0], dtype=torch.float32, device=dev)
-    _lib.call(
-        "ttamd_moe_rowdot", _p(a), _p(b), _p(index), div, 1, a.shape[0], b.shape[0], a.shape[1], _p(out),
+    _call(
+        dev, "ttamd_moe_rowdot", _p(a), _p(b), _p(index), div, 1, a.shape[0], b.shape[0], a.shape[1], _p(out),
         _stream(dev),
     )
     return out
@@ -689,7 +689,7 @@ def sum_topk(y: torch.Tensor, top_k: int) -> torch.Tensor:
     y = _want("y", y, _BF16)
     M, D = y.shape
     out = torch.empty(M // top_k, D, dtype=_BF16, device=dev)
-    _lib.call("ttamd_moe_sum_topk", _p(y), M // top_k, D, top_k, _p(out), _stream(dev))
+    _call(dev, "ttamd_moe_sum_topk", _p(y), M // top_k, D, top_k, _p(out), _stream(dev))
     return out
 
 
@@ -903,7 +903,7 @@ def group_labels(counts_group: torch.Tensor, num_local_experts: int, num_rows: i
     dev = _gpu("counts_group", counts_group)
     cg = counts_group.reshape(-1).to(torch.int32).contiguous()
     out = torch.empty(num_rows, dtype=torch.int32, device=dev)
-    _lib.call("ttamd_moe_group_labels", _p(cg), cg.numel(), num_local_experts, num_rows, _p(out), _stream(dev))
+    _call(dev, "ttamd_moe_group_labels", _p(cg), cg.numel(), num_local_experts, num_rows, _p(out), _stream(dev))
     return out
 
 
@@ -982,7 +982,7 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offs: torch.Tensor) -> torch.Te
         raise ValueError(f"x has K={K}, w has K={K2}")
     out = torch.empty(M, N, dtype=_BF16, device=dev)
     ws = _gemm_ws(M, E, dev)
-    _lib.call("ttamd_grouped_mm", _p(x), _p(w), _p(offs), M, E, N, K, _p(out), _p(ws), ws.numel(), _stream(dev))
+    _call(dev, "ttamd_grouped_mm", _p(x), _p(w), _p(offs), M, E, N, K, _p(out), _p(ws), ws.numel(), _stream(dev))
     return out
 
 
@@ -1002,8 +1002,8 @@ def grouped_mm_swiglu(
     a = torch.empty(M, H, dtype=_BF16, device=dev)
     h = torch.empty(M, 2 * H, dtype=_BF16, device=dev) if save_h else None
     ws = _gemm_ws(M, E, dev)
-    _lib.call(
-        "ttamd_grouped_mm_swiglu", _p(x), _p(w13), _p(offs), M, E, H, D, _limit(swiglu_limit), _p(a), _p(h),
+    _call(
+        dev, "ttamd_grouped_mm_swiglu", _p(x), _p(w13), _p(offs), M, E, H, D, _limit(swiglu_limit), _p(a), _p(h),
         _p(ws), ws.numel(), _stream(dev),
     )
     return a, h
@@ -1029,8 +1029,8 @@ def grouped_mm_swiglu_gather(
     a = torch.empty(M, H, dtype=_BF16, device=dev)
     h = torch.empty(M, 2 * H, dtype=_BF16, device=dev) if save_h else None
     ws = _gemm_ws(M, E, dev)
-    _lib.call(
-        "ttamd_grouped_mm_swiglu_gather", _p(tokens), T, _p(src_index), int(src_div), _p(w13), _p(offs), M, E, H,
+    _call(
+        dev, "ttamd_grouped_mm_swiglu_gather", _p(tokens), T, _p(src_index), int(src_div), _p(w13), _p(offs), M, E, H,
         D, _limit(swiglu_limit), _p(a), _p(h), _p(ws), ws.numel(), _stream(dev),
     )
     return a, h
@@ -1060,8 +1060,8 @@ def grouped_mm_unpermute(
     nd = M if num_dest_rows is None else int(num_dest_rows)
     out = torch.empty(nd, D, dtype=_BF16, device=dev)
     ws = _gemm_ws(M, E, dev)
-    _lib.call(
-        "ttamd_grouped_mm_unpermute", _p(a), _p(w2), _p(offs), M, E, D, H, _p(row_scale), _p(dest), nd, _p(out),
+    _call(
+        dev, "ttamd_grouped_mm_unpermute", _p(a), _p(w2), _p(offs), M, E, D, H, _p(row_scale), _p(dest), nd, _p(out),
         _p(ws), ws.numel(), _stream(dev),
     )
     return out
@@ -1079,7 +1079,7 @@ def grouped_mm_dgrad(dy: torch.Tensor, w: torch.Tensor, offs: torch.Tensor) -> t
         raise ValueError("dy and w disagree on N")
     dx = torch.empty(M, K, dtype=_BF16, device=dev)
     ws = _gemm_ws(M, E, dev)
-    _lib.call("ttamd_grouped_mm_dgrad", _p(dy), _p(w), _p(offs), M, E, N, K, _p(dx), _p(ws), ws.numel(), _stream(dev))
+    _call(dev, "ttamd_grouped_mm_dgrad", _p(dy), _p(w), _p(offs), M, E, N, K, _p(dx), _p(ws), ws.numel(), _stream(dev))
     return dx
 
 
@@ -1100,8 +1100,8 @@ def grouped_mm_dgrad_swiglu(
     dh = torch.empty(M, 2 * H, dtype=_BF16, device=dev)
     a = torch.empty(M, H, dtype=_BF16, device=dev) if want_a else None
     ws = _gemm_ws(M, E, dev)
-    _lib.call(
-        "ttamd_grouped_mm_dgrad_swiglu", _p(dy), _p(w2), _p(h), _p(offs), M, E, D, H, _limit(swiglu_limit),
+    _call(
+        dev, "ttamd_grouped_mm_dgrad_swiglu", _p(dy), _p(w2), _p(h), _p(offs), M, E, D, H, _limit(swiglu_limit),
         _p(dh), _p(a), _p(ws), ws.numel(), _stream(dev),
     )
     return dh, a
@@ -1123,8 +1123,8 @@ def grouped_mm_wgrad(
         raise TypeError("wgrad output must be float32 or bfloat16")
     dw = torch.empty(num_experts, N, K, dtype=out_dtype, device=dev)
     ws = _gemm_ws(M, num_experts, dev)  # tail split of the leftover output tiles
-    _lib.call(
-        "ttamd_grouped_mm_wgrad", _p(dy), _p(x), _p(offs), M, num_experts, N, K, _p(dw),
+    _call(
+        dev, "ttamd_grouped_mm_wgrad", _p(dy), _p(x), _p(offs), M, num_experts, N, K, _p(dw),
         int(out_dtype == torch.float32), _p(ws), ws.numel(), _stream(dev),
     )
     return dw
@@ -1293,8 +1293,8 @@ def shared_expert_add(
         gate_logits = _want("gate_logits", gate_logits.reshape(T), torch.float32)
     a = torch.empty(T, H, dtype=_BF16, device=dev)
     ws = _gemm_ws(T, 1, dev)
-    _lib.call(
-        "ttamd_shared_expert_add", _p(x), T, D, H, _p(w13_shared), _p(w2_shared), _p(gate_logits),
+    _call(
+        dev, "ttamd_shared_expert_add", _p(x), T, D, H, _p(w13_shared), _p(w2_shared), _p(gate_logits),
         _limit(swiglu_limit), _p(a), _p(out),
         _p(ws), ws.numel(), _stream(dev),
     )
@@ -1323,8 +1323,8 @@ def quantize_fp8_rows(
         row_scale = _want("row_scale", row_scale, torch.float32)
     q = torch.empty(R, K, dtype=_U8, device=dev)
     s = torch.empty(K // 128 if K % 128 == 0 else 0, R, dtype=torch.float32, device=dev)
-    _lib.call(
-        "ttamd_quantize_fp8_rows", _p(x), _p(src_index), int(src_div), _p(row_scale), n_in, R, K, _p(q), _p(s),
+    _call(
+        dev, "ttamd_quantize_fp8_rows", _p(x), _p(src_index), int(src_div), _p(row_scale), n_in, R, K, _p(q), _p(s),
         _stream(dev),
     )
     return q, s
@@ -1338,7 +1338,7 @@ def quantize_fp8_blocks(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     E, N, K = w.shape
     q = torch.empty(E, N, K, dtype=_U8, device=dev)
     s = torch.empty(E, N // 128, K // 128, dtype=torch.float32, device=dev)
-    _lib.call("ttamd_quantize_fp8_blocks", _p(w), E, N, K, _p(q), _p(s), _stream(dev))
+    _call(dev, "ttamd_quantize_fp8_blocks", _p(w), E, N, K, _p(q), _p(s), _stream(dev))
     return q, s
 
 
@@ -1364,8 +1364,8 @@ def grouped_mm_fp8(xq: torch.Tensor, sx_t: torch.Tensor, wq: torch.Tensor, sw: t
     offs = _offs(offs, dev)
     out = torch.empty(M, N, dtype=_BF16, device=dev)
     ws = _gemm_ws(M, E, dev)
-    _lib.call(
-        "ttamd_grouped_mm_fp8", _p(xq), _p(sx_t), _p(wq), _p(sw), _p(offs), M, E, N, K, _p(out), _p(ws),
+    _call(
+        dev, "ttamd_grouped_mm_fp8", _p(xq), _p(sx_t), _p(wq), _p(sw), _p(offs), M, E, N, K, _p(out), _p(ws),
         ws.numel(), _stream(dev),
     )
     return out
@@ -1383,8 +1383,8 @@ def grouped_mm_fp8_swiglu(
     a = torch.empty(M, H, dtype=_BF16, device=dev)
     h = torch.empty(M, 2 * H, dtype=_BF16, device=dev) if save_h else None
     ws = _gemm_ws(M, E, dev)
-    _lib.call(
-        "ttamd_grouped_mm_fp8_swiglu", _p(xq), _p(sx_t), _p(w13q), _p(s13), _p(offs), M, E, H, D,
+    _call(
+        dev, "ttamd_grouped_mm_fp8_swiglu", _p(xq), _p(sx_t), _p(w13q), _p(s13), _p(offs), M, E, H, D,
         _limit(swiglu_limit), _p(a), _p(h), _p(ws), ws.numel(), _stream(dev),
     )
     return a, h
@@ -1405,8 +1405,8 @@ def grouped_mm_fp8_unpermute(
     nd = M if num_dest_rows is None else int(num_dest_rows)
     out = torch.empty(nd, D, dtype=_BF16, device=dev)
     ws = _gemm_ws(M, E, dev)
-    _lib.call(
-        "ttamd_grouped_mm_fp8_unpermute", _p(aq), _p(sa_t), _p(w2q), _p(s2), _p(offs), M, E, D, H, _p(row_scale),
+    _call(
+        dev, "ttamd_grouped_mm_fp8_unpermute", _p(aq), _p(sa_t), _p(w2q), _p(s2), _p(offs), M, E, D, H, _p(row_scale),
         _p(dest), nd, _p(out), _p(ws), ws.numel(), _stream(dev),
     )
     return out
