@@ -129,3 +129,35 @@ def test_calls_run_on_their_tensors_device(recorder, ops, name, index):
         calls(ops, torch.device("cuda", index))[name]()
     assert recorder.calls and all(dev == index for _, dev in recorder.calls), recorder.calls
     assert recorder.current == 0
+
+
+def test_graph_is_captured_on_its_tensors_device(recorder, ops, monkeypatch):
+    """MoELayerGraph of tensors on another device than the current one: warm-up,
+    capture and the calls in them."""
+    graph = importlib.import_module("torchtitan-ascend_amd.graph")
+    captured = []
+
+    class Stream:
+        def __init__(self, device=None):
+            self.device = device
+
+        def wait_stream(self, other):
+            pass
+
+    @contextlib.contextmanager
+    def capture(_graph, stream=None):
+        # (torch's default capture stream belongs to the first device it was used on)
+        captured.append((recorder.current, stream.device.index))
+        yield
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: Stream(dev))
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: None)
+    monkeypatch.setattr(torch.cuda, "graph", capture)
+    with FakeTensorMode():
+        t = lambda *s: torch.empty(*s, dtype=BF16, device="cuda:1")  # noqa: E731
+        graph.MoELayerGraph(t(T, D), t(E, D), t(E, 2 * H, D), t(E, D, H), K)
+    assert captured == [(1, 1)]
+    assert recorder.calls and all(dev == 1 for _, dev in recorder.calls)
+    assert recorder.current == 0

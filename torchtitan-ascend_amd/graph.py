@@ -89,7 +89,7 @@ class MoELayerGraph:
                 self._step(self.static_x)
         torch.cuda.current_stream(x.device).wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.no_grad(), torch.cuda.graph(self.graph):
+        with torch.no_grad(), torch.cuda.device(x.device), torch.cuda.graph(self.graph, stream=side):
             self.static_out = self._step(self.static_x)
 
     def _step(self, x: torch.Tensor):
