@@ -469,8 +469,8 @@ int ttamd_moe_experts_forward(const void* tokens, int64_t num_tokens, int64_t di
                               const void* w13, const void* w2, void* out, void* gemm_plan,
                               size_t gemm_plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   return experts_stage("ttamd_moe_experts_forward", false, tokens, num_tokens, dim, hidden, num_experts, topk,
-                       sorted_indices, offs, sorted_scores, score_before_experts, swiglu_limit, w13, w2, out, gemm_plan, gemm_plan_bytes,
-                       workspace, workspace_bytes, stream);
+                       sorted_indices, offs, sorted_scores, score_before_experts, swiglu_limit, w13, w2, out,
+                       gemm_plan, gemm_plan_bytes, workspace, workspace_bytes, stream);
 }
 
 size_t ttamd_moe_experts_rows_workspace_bytes(int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts,
@@ -486,8 +486,8 @@ int ttamd_moe_experts_rows(const void* tokens, int64_t num_tokens, int64_t dim, 
                            const void* w13, const void* w2, void* out, void* gemm_plan,
                            size_t gemm_plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   return experts_stage("ttamd_moe_experts_rows", true, tokens, num_tokens, dim, hidden, num_experts, topk,
-                       sorted_indices, offs, sorted_scores, score_before_experts, swiglu_limit, w13, w2, out, gemm_plan, gemm_plan_bytes,
-                       workspace, workspace_bytes, stream);
+                       sorted_indices, offs, sorted_scores, score_before_experts, swiglu_limit, w13, w2, out,
+                       gemm_plan, gemm_plan_bytes, workspace, workspace_bytes, stream);
 }
 
 int ttamd_moe_gather_rows(const void* in, const int32_t* src_index, const float* row_scale,

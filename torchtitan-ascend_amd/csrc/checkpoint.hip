@@ -49,8 +49,9 @@ __device__ __forceinline__ int exponent_byte(int bits) {
 // Block `blk` of the tensor (row-major over [R, nb]): 128 columns of a row.
 // EXACT: C % 128 == 0, blocks follow one another in memory.
 template <bool EXACT>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const uint4* __restrict__ in, uint32_t nblocks, uint32_t nb, uint32_t cv,
-                                                        uint2* __restrict__ codes, uint8_t* __restrict__ exps) {
+__global__ __launch_bounds__(256) void pack_rows_kernel(const uint4* __restrict__ in, uint32_t nblocks, uint32_t nb,
+                                                        uint32_t cv, uint2* __restrict__ codes,
+                                                        uint8_t* __restrict__ exps) {
   const uint32_t l16 = threadIdx.x & 15;
   const uint32_t stride = gridDim.x * 16;  // indices stay below 2^31: the caller's
   for (uint32_t b0 = blockIdx.x * 16 + (threadIdx.x >> 4); b0 < nblocks; b0 += kUnroll * stride) {

@@ -23,12 +23,14 @@
 // sorts its K best with a sorting network; lists then merge pairwise across
 // the token's lanes (16 lanes: 4 merges, in the VALU's own lane exchanges), in
 // place of K dependent rounds of a maximum over all lanes (16384 tokens of 256
-// experts: 17.8 -> 15.6 us, one token 4.8 -> 4.1).  A lane's first two are also
+// experts: 19.0 -> 15.6 us, one token 5.4 -> 3.8).  A lane's first two are also
 // its share of its group's value.
 //
 // What bounds it: few tokens, the latency of one launch (4 us); many tokens,
 // VALU issue (1140 instructions per wave of four tokens at E = 256, K = 8: 8 of
-// 13.6 us at 16384 tokens), not the logits' bytes (3.4 us).
+// 13.6 us at 16384 tokens), not the logits' bytes (3.4 us).  The bias is 4 of
+// the 13.6: a load per expert and lane, 88 instructions.  On the gate GEMM's
+// partials, with the histogram, 22 us.
 #include <type_traits>
 
 #include "common.h"
@@ -576,8 +578,9 @@ __global__ __launch_bounds__(256) void group_topk_kernel(const GroupTopkArgs a) 
 // stores where E % 4 == 0.  An index outside [0, E) contributes nothing; one
 // that occurs twice adds twice.
 // Bound by the launch up to a few thousand tokens (softmax, 256 experts: 32
-// tokens 6.3 us, 4096 7.2), then by VALU issue (16384 17.2; sigmoid, without
-// the scores of the other experts, 11.3; the bytes alone 6.9).
+// tokens 6.4 us, 4096 7.1), then by VALU issue (16384 16.1 us, of which 1489
+// instructions per wave take 10; sigmoid, without the scores of the other
+// experts, 11.0 and 6; the bytes alone 6.9).
 // ---------------------------------------------------------------------------
 struct TopkBwdArgs {
   const float* grad;   // [T, K]

@@ -222,7 +222,10 @@ def moe_experts_forward(
     many choices per token).  The output is the same; the weights' and the
     scores' gradients are those at the stored values: within 2^-4 of an
     activation of at least 2^-13 of the largest in its row's 128 columns, a
-    smaller one within 2^-17 of that largest (so the least become 0).
+    smaller one within 2^-17 of that largest (so the least become 0).  A step
+    takes longer: 8192 tokens to 8 of 128 experts of 1536 x 2048, 2.40 -> 2.59 ms
+    and 107 -> 35 KB kept per token; with fp32 weights, whose bf16 copies
+    (1.2 GB here) are made again instead of kept, 3.13 -> 3.97 ms.
 
     With autograd off (or nothing requiring grad) the expert stage is one
     op (ttamd::moe_experts_forward: both grouped GEMMs on one tile table,

@@ -420,8 +420,9 @@ def experts_forward(
     plan = r.plan
     _call(
         dev, "ttamd_moe_experts_forward" if sum_rows else "ttamd_moe_experts_rows", _p(x), T, D, H, E, top_k,
-        _p(r.sorted_indices), _p(offsets) + 4, _p(r.sorted_scores), int(bool(score_before_experts)), _limit(swiglu_limit), _p(w13), _p(w2), _p(out),
-        _p(plan), 0 if plan is None else plan.numel(), _p(ws), ws.numel(), _stream(dev),
+        _p(r.sorted_indices), _p(offsets) + 4, _p(r.sorted_scores), int(bool(score_before_experts)),
+        _limit(swiglu_limit), _p(w13), _p(w2), _p(out), _p(plan), 0 if plan is None else plan.numel(), _p(ws),
+        ws.numel(), _stream(dev),
     )
     return out
 
