@@ -741,6 +741,123 @@ int ttamd_unpack_e4m3(const void* codes, const void* exponents,
                       const float* row_scale, int64_t num_rows, void* out,
                       void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * 4-bit weights and the MoE layer for a few tokens (serving).  The           *
+ * reference has neither: its expert weights are bf16 or fp32                 *
+ * (npu_gmm.py:63-64) and every batch takes the grouped GEMMs (:100-110).     *
+ * ------------------------------------------------------------------------ */
+
+/*
+ * 4-bit weights [E, N, K]: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign
+ * bit) with one power-of-two scale per row and 32 columns; value = code * 2^e,
+ * exact in bf16.  e is the smallest integer in [-126, 125] with max |v| <= 6 *
+ * 2^e, codes are nearest, ties to the even code (with e = 125 at most 6); the
+ * exponent byte is e + 127, or 255 where one of the 32 is a NaN or infinite, and
+ * the 32 are then NaN.
+ *
+ * Layout: tiles of 16 rows x 128 columns, NB = ceil(N / 16) by C = ceil(K / 128).
+ *   codes      uint8 [E, NB, C, 64, 16]: place l holds row l % 16, columns
+ *              32 (l / 16) .. + 31 of the tile; byte b columns 2 b (low half) and
+ *              2 b + 1
+ *   exponents  uint8 [E, NB, ceil(C / 4), 64, 4]: place l of four tiles along K
+ * Places outside [N, K] hold zeros.  K % 32 == 0; w bf16 or fp32 (w_is_fp32 = 1);
+ * codes, exponents and w 16-byte aligned.
+ */
+int ttamd_pack_e2m1(const void* w, int w_is_fp32, int64_t num_matrices,
+                    int64_t n, int64_t k, void* codes, void* exponents,
+                    void* stream);
+/* out bf16 [E, N, K] = the values of packed weights. */
+int ttamd_unpack_e2m1(const void* codes, const void* exponents,
+                      int64_t num_matrices, int64_t n, int64_t k, void* out,
+                      void* stream);
+
+/*
+ * Products of rows with 4-bit weights: out[m, :] = x[m, :] w[e]^T (+ bias), x bf16
+ * [M, K], out bf16 [M, N], sums in fp32, rounded once.  offs int32 [E] as in
+ * ttamd_grouped_mm (rows at or past offs[E-1] are not written), or NULL with
+ * num_experts = 1: all rows.  bias [N] (bias_is_fp32: fp32, else bf16) or NULL;
+ * only without offs.  Meant for few rows: every 64 rows of an expert stream its
+ * weights again.  K % 32 == 0.
+ */
+int ttamd_grouped_mm_e2m1(const void* x, const void* codes,
+                          const void* exponents, const int32_t* offs,
+                          const void* bias, int bias_is_fp32, int64_t num_rows,
+                          int num_experts, int64_t n, int64_t k, void* out,
+                          void* stream);
+
+/*
+ * Router of a few tokens (at most 64): logits bf16 [T, E] = x w_router^T with sums
+ * in 64 bits, then the selection of ttamd_router_topk_grouped on them (groups = 1
+ * and kept = 1: no groups).  w_gate (nullable, bf16 [dim]): gate_out fp32 [T] =
+ * sigmoid(bf16(x w_gate^T)), the factor of a shared expert
+ * (models/qwen3_5/model.py:796-800).  topk <= 16, E <= 1024, dim % 8 == 0.
+ * workspace: ttamd_router_decode_workspace_bytes(T, E).
+ */
+size_t ttamd_router_decode_workspace_bytes(int64_t num_tokens, int num_experts);
+int ttamd_router_decode(const void* x, const void* w_router,
+                        const float* expert_bias, const void* w_gate,
+                        int64_t num_tokens, int num_experts, int64_t dim,
+                        int topk, int num_groups, int topk_groups,
+                        int group_score, int score_func, int renormalize,
+                        float renorm_eps, float route_scale, float* top_scores,
+                        int64_t* top_indices, float* gate_out, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * The expert stage for a few tokens (at most 64) in two kernels: dispatch ->
+ * w13 + SwiGLU -> w2 + score -> combine (npu_gmm.py:100-110 with :21-40) on given
+ * picks; out bf16 [T, D].
+ *   a[s] = bf16(silu(min(g, L)) clamp(u, -L, L)), (g, u) = w13[e_s] x[t]
+ *   out[t] = sum_k score[t, k] w2[e] a[t K + k] (+ gate[t] shared(x[t]))
+ * with the score on g and u instead when score_before (npu_gmm.py dispatches
+ * score * x).  All else is fp32, added over k in order, rounded once.
+ *   indices: int64 or int32 [T, K]; one outside [0, E) adds nothing, a repeated
+ *   one counts each time.  w13 [E, 2H, D] and w2 [E, D, H] in bf16 (exponents
+ *   NULL), or all weights as 4-bit codes with their exponents.
+ *   shared_hidden > 0: a shared expert w13_shared [2 Hs, D], w2_shared [D, Hs] of
+ *   the same type, times shared_gate fp32 [T] (nullable).
+ * topk <= 16, E <= 1024; D, H and Hs multiples of 32; swiglu_limit NaN: none.
+ * workspace: ttamd_experts_decode_workspace_bytes (contents need no
+ * initialisation; one call at a time).
+ */
+size_t ttamd_experts_decode_workspace_bytes(int64_t num_tokens, int64_t dim,
+                                            int64_t hidden, int topk,
+                                            int64_t shared_hidden);
+int ttamd_experts_decode(const void* x, int64_t num_tokens, int64_t dim,
+                         int64_t hidden, int num_experts, int topk,
+                         const void* indices, int indices_are_int64,
+                         const float* top_scores, int score_before,
+                         float swiglu_limit, const void* w13,
+                         const void* w13_exponents, const void* w2,
+                         const void* w2_exponents, int64_t shared_hidden,
+                         const void* w13_shared, const void* w13_shared_exponents,
+                         const void* w2_shared, const void* w2_shared_exponents,
+                         const float* shared_gate, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * Both in one call: router of the tokens, then their expert stage.  w_gate (bf16
+ * [dim], nullable) needs shared_hidden > 0.  top_scores fp32 and top_indices int64
+ * [T, K] are outputs.  workspace: ttamd_moe_decode_workspace_bytes.
+ */
+size_t ttamd_moe_decode_workspace_bytes(int64_t num_tokens, int64_t dim,
+                                        int64_t hidden, int num_experts,
+                                        int topk, int64_t shared_hidden);
+int ttamd_moe_decode(const void* x, int64_t num_tokens, int64_t dim,
+                     int64_t hidden, int num_experts, int topk,
+                     const void* w_router, const float* expert_bias,
+                     int num_groups, int topk_groups, int group_score,
+                     int score_func, int renormalize, float renorm_eps,
+                     float route_scale, int score_before, float swiglu_limit,
+                     const void* w13, const void* w13_exponents, const void* w2,
+                     const void* w2_exponents, int64_t shared_hidden,
+                     const void* w13_shared, const void* w13_shared_exponents,
+                     const void* w2_shared, const void* w2_shared_exponents,
+                     const void* w_gate, float* top_scores, int64_t* top_indices,
+                     void* out, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+
 /*
  * ttamd_grouped_mm_dgrad_swiglu with the saved pre-activation packed: h is
  * codes uint8 [M, 2H] with exponents uint8 [M, 2H / 128]; everything else as

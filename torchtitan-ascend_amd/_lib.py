@@ -167,6 +167,32 @@ SIGNATURES: dict[str, tuple] = {
         _i32,
         [_c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i64, _i64, _c_void_p, _i32, _c_void_p, _sz, _c_void_p],
     ),
+    "ttamd_pack_e2m1": (_i32, [_c_void_p, _i32, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p]),
+    "ttamd_unpack_e2m1": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p]),
+    "ttamd_grouped_mm_e2m1": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32, _i64, _i64, _c_void_p, _c_void_p],
+    ),
+    "ttamd_router_decode_workspace_bytes": (_sz, [_i64, _i32]),
+    "ttamd_router_decode": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _f32,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p],
+    ),
+    "ttamd_experts_decode_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i64]),
+    "ttamd_experts_decode": (
+        _i32,
+        [_c_void_p, _i64, _i64, _i64, _i32, _i32, _c_void_p, _i32, _c_void_p, _i32, _f32, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz,
+         _c_void_p],
+    ),
+    "ttamd_moe_decode_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32, _i64]),
+    "ttamd_moe_decode": (
+        _i32,
+        [_c_void_p, _i64, _i64, _i64, _i32, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _i32, _f32, _f32, _i32,
+         _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p],
+    ),
     "ttamd_pack_e4m3": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p]),
     "ttamd_unpack_e4m3": (
         _i32, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i32, _c_void_p, _i64, _c_void_p, _c_void_p]

@@ -1006,6 +1006,243 @@ int ttamd_unpack_e4m3(const void* codes, const void* exponents, int64_t num_src_
                    fn);
 }
 
+// ---------------------------------------------------------------------------
+// 4-bit weights, the layer for a few tokens
+// ---------------------------------------------------------------------------
+namespace {
+
+// Matrices [E, n, k] of 4-bit weights: columns in whole groups, rows padded to
+// tiles; the codes' bytes stay countable.
+int check_fp4(const char* fn, int64_t E, int64_t n, int64_t k) {
+  TRY(check_dim(fn, "k", k, 32));
+  TRY(check_dim(fn, "n", n, 1));
+  REQUIRE(E >= 0 && E <= (1 << 20) && E * ((n + 15) / 16) <= (1 << 26), "%s: too many matrices (%lld of %lld x %lld)",
+          fn, (long long)E, (long long)n, (long long)k);
+  REQUIRE(E * ((n + 15) / 16) * ((k + 127) / 128) <= (int64_t(1) << 32), "%s: weights too large", fn);
+  return TTAMD_OK;
+}
+
+int check_ptr16(const char* fn, const char* name, const void* p) {
+  REQUIRE(p != nullptr, "%s: %s is null", fn, name);
+  REQUIRE(aligned16(p), "%s: %s must be 16-byte aligned", fn, name);
+  return TTAMD_OK;
+}
+
+int check_decode(const char* fn, int64_t T, int64_t D, int64_t H, int E, int K, int64_t Hs) {
+  REQUIRE(T >= 0 && T <= ttamd::kDecodeMaxTokens, "%s: num_tokens must be in [0, %d] (got %lld)", fn,
+          ttamd::kDecodeMaxTokens, (long long)T);
+  REQUIRE(E >= 1 && E <= 1024, "%s: num_experts must be in [1, 1024] (got %d)", fn, E);
+  REQUIRE(K >= 1 && K <= ttamd::kDecodeMaxTopk, "%s: topk must be in [1, %d] (got %d)", fn, ttamd::kDecodeMaxTopk, K);
+  TRY(check_dim(fn, "dim", D, 32));
+  TRY(check_dim(fn, "hidden", H, 32));
+  REQUIRE(Hs == 0 || (Hs > 0 && Hs % 32 == 0 && Hs <= (1 << 20)),
+          "%s: shared_hidden must be 0 or a positive multiple of 32 (got %lld)", fn, (long long)Hs);
+  REQUIRE(E * H * D < (int64_t(1) << 40) && Hs * D < (int64_t(1) << 40), "%s: weights too large", fn);
+  return TTAMD_OK;
+}
+
+struct DecodeWeights {
+  const void *w13, *e13, *w2, *e2, *s13, *es13, *s2, *es2;
+};
+
+int check_decode_weights(const char* fn, const DecodeWeights& w, int64_t Hs) {
+  TRY(check_ptr16(fn, "w13", w.w13));
+  TRY(check_ptr16(fn, "w2", w.w2));
+  const bool fp4 = w.e13 != nullptr;
+  REQUIRE((w.e2 != nullptr) == fp4, "%s: w13 and w2 must be of one type (exponents of one only)", fn);
+  if (fp4) {
+    TRY(check_ptr16(fn, "w13_exponents", w.e13));
+    TRY(check_ptr16(fn, "w2_exponents", w.e2));
+  }
+  if (Hs > 0) {
+    TRY(check_ptr16(fn, "w13_shared", w.s13));
+    TRY(check_ptr16(fn, "w2_shared", w.s2));
+    REQUIRE((w.es13 != nullptr) == fp4 && (w.es2 != nullptr) == fp4,
+            "%s: the shared expert's weights must be of the experts' type", fn);
+    if (fp4) {
+      TRY(check_ptr16(fn, "w13_shared_exponents", w.es13));
+      TRY(check_ptr16(fn, "w2_shared_exponents", w.es2));
+    }
+  }
+  return TTAMD_OK;
+}
+
+ttamd::ExpertsDecode decode_args(const DecodeWeights& w, const void* x, int64_t T, int64_t D, int64_t H, int E, int K,
+                                 int64_t Hs, const void* idx, bool is64, const float* scores, int before, float limit,
+                                 const float* gate, void* out) {
+  ttamd::ExpertsDecode c{};
+  c.T = (int)T, c.D = (int)D, c.H = (int)H, c.E = E, c.K = K, c.Hs = (int)Hs;
+  c.x = x, c.idx = idx, c.is64 = is64, c.before = before != 0, c.fp4 = w.e13 != nullptr;
+  c.scores = scores, c.limit = limit;
+  c.w13 = w.w13, c.w2 = w.w2, c.s13 = w.s13, c.s2 = w.s2;
+  c.e13 = (const uint8_t*)w.e13, c.e2 = (const uint8_t*)w.e2;
+  c.es13 = (const uint8_t*)w.es13, c.es2 = (const uint8_t*)w.es2;
+  c.gate = gate, c.out = out;
+  return c;
+}
+
+int check_router_decode(const char* fn, int64_t T, int E, int64_t D, int K, int groups, int kept, int group_score,
+                        int score_func) {
+  REQUIRE(T >= 0 && T <= ttamd::kDecodeMaxTokens, "%s: num_tokens must be in [0, %d] (got %lld)", fn,
+          ttamd::kDecodeMaxTokens, (long long)T);
+  REQUIRE(E >= 1 && E <= 1024, "%s: num_experts must be in [1, 1024] (got %d)", fn, E);
+  TRY(check_dim(fn, "dim", D, 8));
+  TRY(check_groups(fn, E, K, groups, kept, group_score));
+  REQUIRE(score_func == TTAMD_SCORE_SOFTMAX || score_func == TTAMD_SCORE_SIGMOID, "%s: unknown score_func %d", fn,
+          score_func);
+  return TTAMD_OK;
+}
+
+}  // namespace
+
+int ttamd_pack_e2m1(const void* w, int w_is_fp32, int64_t num_matrices, int64_t n, int64_t k, void* codes,
+                    void* exponents, void* stream) {
+  const char* fn = "ttamd_pack_e2m1";
+  TRY(check_fp4(fn, num_matrices, n, k));
+  if (num_matrices == 0) return TTAMD_OK;
+  TRY(check_ptr16(fn, "w", w));
+  TRY(check_ptr16(fn, "codes", codes));
+  TRY(check_ptr16(fn, "exponents", exponents));
+  return check_hip(ttamd::launch_pack_fp4(w, w_is_fp32 != 0, num_matrices, (int)n, (int)k, codes, exponents,
+                                          (hipStream_t)stream),
+                   fn);
+}
+
+int ttamd_unpack_e2m1(const void* codes, const void* exponents, int64_t num_matrices, int64_t n, int64_t k, void* out,
+                      void* stream) {
+  const char* fn = "ttamd_unpack_e2m1";
+  TRY(check_fp4(fn, num_matrices, n, k));
+  if (num_matrices == 0) return TTAMD_OK;
+  TRY(check_ptr16(fn, "codes", codes));
+  TRY(check_ptr16(fn, "exponents", exponents));
+  TRY(check_ptr16(fn, "out", out));
+  return check_hip(ttamd::launch_unpack_fp4(codes, exponents, num_matrices, (int)n, (int)k, out, (hipStream_t)stream),
+                   fn);
+}
+
+int ttamd_grouped_mm_e2m1(const void* x, const void* codes, const void* exponents, const int32_t* offs,
+                          const void* bias, int bias_is_fp32, int64_t num_rows, int num_experts, int64_t n, int64_t k,
+                          void* out, void* stream) {
+  const char* fn = "ttamd_grouped_mm_e2m1";
+  REQUIRE(num_experts >= 1 && num_experts <= 1024, "%s: num_experts must be in [1, 1024] (got %d)", fn, num_experts);
+  REQUIRE(num_rows >= 0 && num_rows <= (1 << 28), "%s: num_rows out of range (%lld)", fn, (long long)num_rows);
+  TRY(check_fp4(fn, num_experts, n, k));
+  REQUIRE(offs || num_experts == 1, "%s: offs is null with %d experts", fn, num_experts);
+  REQUIRE(!offs || !bias, "%s: bias is for a call without offs", fn);
+  if (num_rows == 0) return TTAMD_OK;
+  TRY(check_ptr16(fn, "x", x));
+  TRY(check_ptr16(fn, "codes", codes));
+  TRY(check_ptr16(fn, "exponents", exponents));
+  TRY(check_ptr16(fn, "out", out));
+  return check_hip(ttamd::launch_grouped_mm_fp4(x, codes, exponents, offs, bias, bias_is_fp32 != 0, (int)num_rows,
+                                                num_experts, (int)n, (int)k, out, (hipStream_t)stream),
+                   fn);
+}
+
+size_t ttamd_router_decode_workspace_bytes(int64_t num_tokens, int num_experts) {
+  if (num_tokens < 0 || num_experts < 1) return 0;
+  return ttamd::router_decode_workspace_bytes(num_tokens, num_experts);
+}
+
+int ttamd_router_decode(const void* x, const void* w_router, const float* expert_bias, const void* w_gate,
+                        int64_t num_tokens, int num_experts, int64_t dim, int topk, int num_groups, int topk_groups,
+                        int group_score, int score_func, int renormalize, float renorm_eps, float route_scale,
+                        float* top_scores, int64_t* top_indices, float* gate_out, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  const char* fn = "ttamd_router_decode";
+  TRY(check_router_decode(fn, num_tokens, num_experts, dim, topk, num_groups, topk_groups, group_score, score_func));
+  if (num_tokens == 0) return TTAMD_OK;
+  TRY(check_ptr16(fn, "x", x));
+  TRY(check_ptr16(fn, "w_router", w_router));
+  REQUIRE(top_scores && top_indices, "%s: null pointer argument", fn);
+  REQUIRE((w_gate != nullptr) == (gate_out != nullptr), "%s: give w_gate and gate_out together", fn);
+  REQUIRE(aligned16(w_gate), "%s: w_gate must be 16-byte aligned", fn);
+  TRY(check_ws(fn, workspace, workspace_bytes, ttamd::router_decode_workspace_bytes(num_tokens, num_experts)));
+  const ttamd::RouterGroups g = {num_groups, topk_groups, group_score == TTAMD_GROUP_TOP2};
+  return check_hip(ttamd::launch_router_decode(x, w_router, w_gate, expert_bias, (int)num_tokens, num_experts, (int)dim,
+                                               topk, g, score_func, renormalize, renorm_eps, route_scale, top_scores,
+                                               top_indices, gate_out, workspace, (hipStream_t)stream),
+                   fn);
+}
+
+size_t ttamd_experts_decode_workspace_bytes(int64_t num_tokens, int64_t dim, int64_t hidden, int topk,
+                                            int64_t shared_hidden) {
+  if (num_tokens < 0 || dim < 1 || hidden < 1 || topk < 1 || shared_hidden < 0) return 0;
+  return ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden);
+}
+
+int ttamd_experts_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts, int topk,
+                         const void* indices, int indices_are_int64, const float* top_scores, int score_before,
+                         float swiglu_limit, const void* w13, const void* w13_exponents, const void* w2,
+                         const void* w2_exponents, int64_t shared_hidden, const void* w13_shared,
+                         const void* w13_shared_exponents, const void* w2_shared, const void* w2_shared_exponents,
+                         const float* shared_gate, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "ttamd_experts_decode";
+  TRY(check_decode(fn, num_tokens, dim, hidden, num_experts, topk, shared_hidden));
+  REQUIRE(std::isnan(swiglu_limit) || swiglu_limit >= 0.f, "%s: swiglu_limit must be >= 0 or NaN", fn);
+  REQUIRE(!shared_gate || shared_hidden > 0, "%s: shared_gate without a shared expert", fn);
+  if (num_tokens == 0) return TTAMD_OK;
+  const DecodeWeights w = {w13,        w13_exponents,        w2,        w2_exponents,
+                           w13_shared, w13_shared_exponents, w2_shared, w2_shared_exponents};
+  TRY(check_decode_weights(fn, w, shared_hidden));
+  TRY(check_ptr16(fn, "x", x));
+  TRY(check_ptr16(fn, "out", out));
+  REQUIRE(indices && top_scores, "%s: null pointer argument", fn);
+  TRY(check_ws(fn, workspace, workspace_bytes,
+               ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden)));
+  return check_hip(ttamd::launch_experts_decode(decode_args(w, x, num_tokens, dim, hidden, num_experts, topk,
+                                                            shared_hidden, indices, indices_are_int64 != 0, top_scores,
+                                                            score_before, swiglu_limit, shared_gate, out),
+                                                workspace, (hipStream_t)stream),
+                   fn);
+}
+
+size_t ttamd_moe_decode_workspace_bytes(int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts, int topk,
+                                        int64_t shared_hidden) {
+  if (num_tokens < 0 || dim < 1 || hidden < 1 || num_experts < 1 || topk < 1 || shared_hidden < 0) return 0;
+  return align256((size_t)num_tokens * 4) + ttamd::router_decode_workspace_bytes(num_tokens, num_experts) +
+         ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden);
+}
+
+int ttamd_moe_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts, int topk,
+                     const void* w_router, const float* expert_bias, int num_groups, int topk_groups, int group_score,
+                     int score_func, int renormalize, float renorm_eps, float route_scale, int score_before,
+                     float swiglu_limit, const void* w13, const void* w13_exponents, const void* w2,
+                     const void* w2_exponents, int64_t shared_hidden, const void* w13_shared,
+                     const void* w13_shared_exponents, const void* w2_shared, const void* w2_shared_exponents,
+                     const void* w_gate, float* top_scores, int64_t* top_indices, void* out, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  const char* fn = "ttamd_moe_decode";
+  TRY(check_decode(fn, num_tokens, dim, hidden, num_experts, topk, shared_hidden));
+  TRY(check_router_decode(fn, num_tokens, num_experts, dim, topk, num_groups, topk_groups, group_score, score_func));
+  REQUIRE(std::isnan(swiglu_limit) || swiglu_limit >= 0.f, "%s: swiglu_limit must be >= 0 or NaN", fn);
+  REQUIRE(!w_gate || shared_hidden > 0, "%s: w_gate without a shared expert", fn);
+  if (num_tokens == 0) return TTAMD_OK;
+  const DecodeWeights w = {w13,        w13_exponents,        w2,        w2_exponents,
+                           w13_shared, w13_shared_exponents, w2_shared, w2_shared_exponents};
+  TRY(check_decode_weights(fn, w, shared_hidden));
+  TRY(check_ptr16(fn, "x", x));
+  TRY(check_ptr16(fn, "w_router", w_router));
+  TRY(check_ptr16(fn, "out", out));
+  REQUIRE(aligned16(w_gate), "%s: w_gate must be 16-byte aligned", fn);
+  REQUIRE(top_scores && top_indices, "%s: null pointer argument", fn);
+  TRY(check_ws(fn, workspace, workspace_bytes,
+               ttamd_moe_decode_workspace_bytes(num_tokens, dim, hidden, num_experts, topk, shared_hidden)));
+  float* const gate = w_gate ? (float*)workspace : nullptr;
+  char* const logits = (char*)workspace + align256((size_t)num_tokens * 4);
+  const ttamd::RouterGroups g = {num_groups, topk_groups, group_score == TTAMD_GROUP_TOP2};
+  TRY(check_hip(ttamd::launch_router_decode(x, w_router, w_gate, expert_bias, (int)num_tokens, num_experts, (int)dim,
+                                            topk, g, score_func, renormalize, renorm_eps, route_scale, top_scores,
+                                            top_indices, gate, logits, (hipStream_t)stream),
+                fn));
+  return check_hip(
+      ttamd::launch_experts_decode(decode_args(w, x, num_tokens, dim, hidden, num_experts, topk, shared_hidden,
+                                               top_indices, true, top_scores, score_before, swiglu_limit, gate, out),
+                                   logits + ttamd::router_decode_workspace_bytes(num_tokens, num_experts),
+                                   (hipStream_t)stream),
+      fn);
+}
+
 int ttamd_grouped_mm_dgrad_swiglu_packed(const void* dy, const void* w2, const void* codes, const void* exponents,
                                          const int32_t* offs, int64_t num_rows, int num_experts, int64_t dim,
                                          int64_t hidden, float swiglu_limit, void* dh, void* a_out, void* workspace,

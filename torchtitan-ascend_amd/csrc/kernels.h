@@ -203,6 +203,39 @@ hipError_t launch_grouped_mm_wgrad_packed(const void* dy, const void* codes, con
                                           int M, int E, int N, int K, void* dw, bool fp32, void* ws,
                                           hipStream_t stream);
 
+// 4-bit weights (fp4.hip): tiles of 16 rows x 128 columns.
+hipError_t launch_pack_fp4(const void* in, bool f32, int64_t E, int N, int K, void* codes, void* exps,
+                           hipStream_t stream);
+hipError_t launch_unpack_fp4(const void* codes, const void* exps, int64_t E, int N, int K, void* out,
+                             hipStream_t stream);
+
+// The layer for a few tokens, products with 4-bit weights (decode.hip).
+constexpr int kDecodeMaxTokens = 64;
+constexpr int kDecodeMaxTopk = 16;
+size_t router_decode_workspace_bytes(int64_t T, int E);
+// logits: router_decode_workspace_bytes; w_gate (nullable): gate[t] = sigmoid of
+// the token's product with it.
+hipError_t launch_router_decode(const void* x, const void* w_router, const void* w_gate, const float* bias, int T, int E,
+                                int D, int K, const RouterGroups& groups, int score_func, int renorm, float renorm_eps,
+                                float route_scale, float* top_scores, int64_t* top_idx, float* gate, void* logits,
+                                hipStream_t stream);
+struct ExpertsDecode {
+  int T, D, H, E, K, Hs;
+  const void* x;
+  const void* idx;
+  int is64, before, fp4;
+  const float* scores;
+  float limit;
+  const void *w13, *w2, *s13, *s2;
+  const uint8_t *e13, *e2, *es13, *es2;  // exponents of 4-bit weights
+  const float* gate;
+  void* out;
+};
+size_t experts_decode_workspace_bytes(int64_t T, int64_t D, int64_t H, int K, int64_t Hs);
+hipError_t launch_experts_decode(const ExpertsDecode& c, void* ws, hipStream_t stream);
+hipError_t launch_grouped_mm_fp4(const void* x, const void* codes, const void* exps, const int* offs, const void* bias,
+                                 bool bias32, int M, int E, int N, int K, void* out, hipStream_t stream);
+
 // fp8 e4m3 path (quant.hip, gemm_fp8.hip via gemm.hip)
 hipError_t launch_quantize_rows(const void* in, const int* src_index, int src_div, const float* row_mul,
                                 int n_in, int R, int K, void* q_out, float* scale_t, hipStream_t stream);

@@ -1,0 +1,352 @@
+"""The MoE layer for a few tokens (a decode batch), and 4-bit weights.
+
+A batch of at most 64 tokens streams the weights of the experts it hits once
+and computes almost nothing with them, so it takes other kernels than the
+grouped GEMMs of `ops`: `moe_decode` is the whole layer (router, experts,
+combine, shared expert), `experts_decode` its expert stage on given picks, both
+with bf16 or 4-bit weights; `pack_e2m1` makes the latter, `grouped_mm_e2m1`
+multiplies a few rows with them.  For serving: none has a backward, and a call
+under autograd with a tensor that requires a gradient raises.
+
+Like `ops`, every function allocates with torch's caching allocator and calls
+the C ABI on torch's current stream of its tensors' device; there is no
+fallback.  Reference: NpuGroupedExperts.forward with its router
+(torchtitanturbo/models/common/npu_gmm.py:100-110; models/qwen3_5/model.py:752-809).
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib, ops
+from .ops import _call, _gpu, _groups, _limit, _p, _same_device, _stream, _want, _ws
+
+_BF16 = torch.bfloat16
+MAX_TOKENS = 64
+
+
+class PackedWeights(NamedTuple):
+    """Weights [E, N, K] (or [N, K] as E = 1) in 4 bits: e2m1 codes with one
+    power-of-two scale per row and 32 columns, value = code * 2^(exponent - 127),
+    exact in bf16 (tile layout: ttamd_pack_e2m1)."""
+
+    codes: torch.Tensor  # uint8 [E, ceil(N / 16), ceil(K / 128), 64, 16]
+    exponents: torch.Tensor  # uint8 [E, ceil(N / 16), ceil(K / 512), 64, 4]
+    rows: int  # N
+    cols: int  # K
+
+
+def _no_grad(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} is for inference (it has no backward); call it under torch.no_grad()")
+
+
+def _shapes(E: int, N: int, K: int) -> tuple[tuple, tuple]:
+    nb, nc = (N + 15) // 16, (K + 127) // 128
+    return (E, nb, nc, 64, 16), (E, nb, (nc + 3) // 4, 64, 4)
+
+
+def _packed(name: str, w: PackedWeights, dev: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    codes = _want(f"{name}.codes", w.codes, torch.uint8)
+    exps = _want(f"{name}.exponents", w.exponents, torch.uint8)
+    _same_device(dev, **{f"{name}.codes": codes, f"{name}.exponents": exps})
+    if w.rows < 1 or w.cols < 1 or codes.dim() != 5 or \
+            (tuple(codes.shape), tuple(exps.shape)) != _shapes(codes.shape[0], w.rows, w.cols):
+        raise ValueError(f"{name}: codes {tuple(codes.shape)} and exponents {tuple(exps.shape)} are not those of "
+                         f"[E, {w.rows}, {w.cols}] weights")
+    return codes, exps
+
+
+def pack_e2m1(w: torch.Tensor) -> PackedWeights:
+    """4-bit form of weights w [E, N, K] or [N, K], bf16 or fp32, K % 32 == 0
+    (ttamd_pack_e2m1): 17/32 byte per value, each within a quarter of its
+    magnitude, or within 2^-2 of a 32-column group's scale where that is more.
+    A group that holds a NaN or an infinity becomes NaN."""
+    dev = _gpu("w", w)
+    _no_grad("pack_e2m1", w)
+    if w.dim() not in (2, 3):
+        raise ValueError(f"w must be [E, N, K] or [N, K], got {tuple(w.shape)}")
+    if w.dtype not in (_BF16, torch.float32):
+        raise TypeError(f"w must be bfloat16 or float32, got {w.dtype}")
+    w = w.contiguous()
+    E, (N, K) = (w.shape[0] if w.dim() == 3 else 1), w.shape[-2:]
+    codes_shape, exps_shape = _shapes(E, N, K)
+    codes = torch.empty(codes_shape, dtype=torch.uint8, device=dev)
+    exps = torch.empty(exps_shape, dtype=torch.uint8, device=dev)
+    _call(dev, "ttamd_pack_e2m1", _p(w), int(w.dtype == torch.float32), E, N, K, _p(codes), _p(exps), _stream(dev))
+    return PackedWeights(codes, exps, N, K)
+
+
+def unpack_e2m1(w: PackedWeights) -> torch.Tensor:
+    """The bf16 values [E, N, K] of packed weights, exactly (ttamd_unpack_e2m1):
+    for prompts, whose rows fill the grouped GEMMs."""
+    dev = _gpu("w.codes", w.codes)
+    codes, exps = _packed("w", w, dev)
+    E = codes.shape[0]
+    out = torch.empty(E, w.rows, w.cols, dtype=_BF16, device=dev)
+    _call(dev, "ttamd_unpack_e2m1", _p(codes), _p(exps), E, w.rows, w.cols, _p(out), _stream(dev))
+    return out
+
+
+def tile_e2m1(codes: torch.Tensor, exponents: torch.Tensor) -> PackedWeights:
+    """PackedWeights from row-major 4-bit weights, as checkpoints hold them: codes
+    uint8 [..., N, K / 2], two to a byte, the even column in the low half, and
+    exponent bytes uint8 [..., N, K / 32] (value = code * 2^(byte - 127)).  A
+    re-ordering by torch operations, done once when weights are loaded."""
+    dev = _gpu("codes", codes)
+    _same_device(dev, exponents=exponents)
+    if codes.dtype != torch.uint8 or exponents.dtype != torch.uint8:
+        raise TypeError("codes and exponents must be uint8")
+    if codes.dim() not in (2, 3) or codes.shape[-1] % 16 or \
+            tuple(exponents.shape) != (*codes.shape[:-1], codes.shape[-1] // 16):
+        raise ValueError(f"codes [..., N, K / 2] {tuple(codes.shape)} and exponents [..., N, K / 32] "
+                         f"{tuple(exponents.shape)} do not match")
+    N, K = codes.shape[-2], 2 * codes.shape[-1]
+    E = codes.shape[0] if codes.dim() == 3 else 1
+    (_, nb, nc, _, _), exps_shape = _shapes(E, N, K)
+    pad = torch.nn.functional.pad
+    c = pad(codes.reshape(E, N, K // 2), (0, nc * 64 - K // 2, 0, nb * 16 - N))
+    c = c.view(E, nb, 16, nc, 4, 16).permute(0, 1, 3, 4, 2, 5).reshape(E, nb, nc, 64, 16).contiguous()
+    x = pad(exponents.reshape(E, N, K // 32), (0, 16 * exps_shape[2] - K // 32, 0, nb * 16 - N), value=127)
+    x = x.view(E, nb, 16, exps_shape[2], 4, 4).permute(0, 1, 3, 5, 2, 4).reshape(exps_shape).contiguous()
+    return PackedWeights(c, x, N, K)
+
+
+def grouped_mm_e2m1(
+    x: torch.Tensor, w: PackedWeights, offs: torch.Tensor | None = None, bias: torch.Tensor | None = None
+) -> torch.Tensor:
+    """out[m] = x[m] @ w[e]^T (+ bias) with 4-bit weights (ttamd_grouped_mm_e2m1):
+    x bf16 [M, K] (without offs also [..., K]); expert e's rows end at offs[e]
+    (int32 [E]) as in grouped_mm, or all rows take the one matrix of w.  bias [N]
+    bf16 or fp32, without offs.  For few rows: every 64 of an expert read its
+    weights again, so a prompt takes unpack_e2m1 and a matrix product.  Rows at or
+    past offs[-1] are not written."""
+    dev = _gpu("x", x)
+    _no_grad("grouped_mm_e2m1", x, bias)
+    x = _want("x", x, _BF16)
+    codes, exps = _packed("w", w, dev)
+    E = codes.shape[0]
+    if x.shape[-1] != w.cols or (offs is not None and x.dim() != 2):
+        raise ValueError(f"x must be [M, {w.cols}], got {tuple(x.shape)}")
+    if offs is None and E != 1:
+        raise ValueError(f"w holds {E} matrices: give offs")
+    if offs is not None:
+        _same_device(dev, offs=offs)
+        offs = _want("offs", offs, torch.int32)
+        if offs.numel() != E:
+            raise ValueError(f"offs has {offs.numel()} entries, w holds {E} matrices")
+        if bias is not None:
+            raise ValueError("bias is for a call without offs")
+    if bias is not None:
+        _same_device(dev, bias=bias)
+        if bias.dtype not in (_BF16, torch.float32) or bias.numel() != w.rows:
+            raise ValueError(f"bias must be [{w.rows}], bfloat16 or float32")
+        bias = bias.contiguous()
+    out = torch.empty(*x.shape[:-1], w.rows, dtype=_BF16, device=dev)
+    _call(dev, "ttamd_grouped_mm_e2m1", _p(x), _p(codes), _p(exps), _p(offs), _p(bias),
+          int(bias is not None and bias.dtype == torch.float32), x.numel() // w.cols, E, w.rows, w.cols, _p(out),
+          _stream(dev))
+    return out
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    x = _want("x", x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), _BF16)
+    if x.shape[0] > MAX_TOKENS:
+        raise ValueError(f"at most {MAX_TOKENS} tokens, got {x.shape[0]}: a longer batch fills the grouped GEMMs "
+                         "(functional.moe_decode chooses)")
+    return x
+
+
+def _bias(expert_bias: torch.Tensor | None, E: int, dev: torch.device) -> torch.Tensor | None:
+    if expert_bias is None:
+        return None
+    _same_device(dev, expert_bias=expert_bias)
+    expert_bias = expert_bias.float().contiguous()
+    if expert_bias.shape != (E,):
+        raise ValueError("expert_bias must be [E]")
+    return expert_bias
+
+
+def _gate_row(shared_gate: torch.Tensor | None, D: int, dev: torch.device) -> torch.Tensor | None:
+    if shared_gate is None:
+        return None
+    _same_device(dev, shared_gate=shared_gate)
+    shared_gate = _want("shared_gate", shared_gate, _BF16)
+    if shared_gate.numel() != D:
+        raise ValueError(f"shared_gate must be [1, {D}], got {tuple(shared_gate.shape)}")
+    return shared_gate
+
+
+def _weight(name: str, w, dev: torch.device) -> tuple[torch.Tensor, torch.Tensor | None, tuple]:
+    """(tensor, exponents or None, (E, N, K)) of bf16 [E, N, K] / [N, K] or packed weights."""
+    if isinstance(w, PackedWeights):
+        codes, exps = _packed(name, w, dev)
+        return codes, exps, (codes.shape[0], w.rows, w.cols)
+    _gpu(name, w)
+    w = _want(name, w, _BF16)
+    _same_device(dev, **{name: w})
+    if w.dim() not in (2, 3):
+        raise ValueError(f"{name} must be [E, N, K], got {tuple(w.shape)}")
+    return w, None, (w.shape[0] if w.dim() == 3 else 1, *w.shape[-2:])
+
+
+def _experts(w13, w2, shared_w13, shared_w2, D: int, dev: torch.device):
+    """(E, H, Hs, the eight weight tensors) of the layer's weights, checked."""
+    t13, e13, s13 = _weight("w13", w13, dev)
+    t2, e2, s2 = _weight("w2", w2, dev)
+    E, H = s13[0], s13[1] // 2
+    if s13[2] != D or s13[1] % 2 or s2 != (E, D, H):
+        raise ValueError(f"w13 must be [E, 2H, {D}] and w2 [E, {D}, H]; got {s13}, {s2}")
+    if (e13 is None) != (e2 is None):
+        raise TypeError("w13 and w2 must both be bfloat16 or both packed")
+    if (shared_w13 is None) != (shared_w2 is None):
+        raise ValueError("give shared_w13 and shared_w2 together")
+    Hs, shared = 0, (None, None, None, None)
+    if shared_w13 is not None:
+        u13, f13, z13 = _weight("shared_w13", shared_w13, dev)
+        u2, f2, z2 = _weight("shared_w2", shared_w2, dev)
+        Hs = z13[1] // 2
+        if z13[0] != 1 or z13[2] != D or z13[1] % 2 or z2 != (1, D, Hs):
+            raise ValueError(f"shared_w13 must be [2Hs, {D}] and shared_w2 [{D}, Hs]; got {z13}, {z2}")
+        if (f13 is None) != (e13 is None) or (f2 is None) != (e13 is None):
+            raise TypeError("the shared expert's weights must be of the experts' type")
+        shared = (u13, f13, u2, f2)
+    return E, H, Hs, (t13, e13, t2, e2), shared
+
+
+def router_decode(
+    x: torch.Tensor,
+    w_router: torch.Tensor,
+    top_k: int,
+    score_func: str = "softmax",
+    route_norm: bool = False,
+    route_scale: float = 1.0,
+    expert_bias: torch.Tensor | None = None,
+    norm_eps: float = 1e-20,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
+    shared_gate: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """Router of at most 64 tokens (ttamd_router_decode): (top_scores fp32 [T, K],
+    selected_experts_indices int64 [T, K], gate fp32 [T] or None).  Arguments as
+    ops.router_fused; the bf16 logits come from 64-bit sums and the selection is
+    ops.router_topk's with groups (one group without num_groups).  shared_gate [1,
+    D] bf16: gate = sigmoid of the token's bf16 product with it."""
+    dev = _gpu("x", x)
+    _no_grad("router_decode", x, w_router, shared_gate)
+    x = _rows(x)
+    w_router = _want("w_router", w_router, _BF16)
+    _same_device(dev, w_router=w_router)
+    T, D = x.shape
+    E = w_router.shape[0]
+    if w_router.dim() != 2 or w_router.shape[1] != D:
+        raise ValueError(f"w_router must be [E, {D}], got {tuple(w_router.shape)}")
+    if score_func not in ops._SCORE_FUNCS:
+        raise ValueError(f"score_func must be one of {sorted(ops._SCORE_FUNCS)}")
+    groups = _groups(num_groups, topk_groups, group_score) or (1, 1, 0)
+    expert_bias = _bias(expert_bias, E, dev)
+    shared_gate = _gate_row(shared_gate, D, dev)
+    scores = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+    idx = torch.empty(T, top_k, dtype=torch.int64, device=dev)
+    gate = None if shared_gate is None else torch.empty(T, dtype=torch.float32, device=dev)
+    ws = _ws(_lib.load().ttamd_router_decode_workspace_bytes(T, E), dev)
+    _call(dev, "ttamd_router_decode", _p(x), _p(w_router), _p(expert_bias), _p(shared_gate), T, E, D, top_k, *groups,
+          ops._SCORE_FUNCS[score_func], int(bool(route_norm)), float(norm_eps), float(route_scale), _p(scores), _p(idx),
+          _p(gate), _p(ws), ws.numel(), _stream(dev))
+    return scores, idx, gate
+
+
+def experts_decode(
+    x: torch.Tensor,
+    top_scores: torch.Tensor,
+    selected_experts_indices: torch.Tensor,
+    w13: torch.Tensor | PackedWeights,
+    w2: torch.Tensor | PackedWeights,
+    score_before_experts: bool = False,
+    swiglu_limit: float | None = None,
+    shared_w13: torch.Tensor | PackedWeights | None = None,
+    shared_w2: torch.Tensor | PackedWeights | None = None,
+    shared_scale: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Expert stage of at most 64 tokens on given picks, in two kernels
+    (ttamd_experts_decode): x bf16 [T, D], scores and indices [T, K] (int64 or
+    int32; one outside [0, E) adds nothing) -> bf16 [T, D].  Weights bf16 (w13 [E,
+    2H, D], w2 [E, D, H]) or all packed.  A shared expert [2Hs, D] / [D, Hs] is added
+    times shared_scale fp32 [T] (None: 1)."""
+    dev = _gpu("x", x)
+    _no_grad("experts_decode", x, top_scores, w13, w2, shared_w13, shared_w2, shared_scale)
+    x = _rows(x)
+    T, D = x.shape
+    idx = selected_experts_indices
+    if idx.dtype not in (torch.int64, torch.int32):
+        raise TypeError("expert indices must be int64 or int32")
+    K = idx.shape[-1]
+    _same_device(dev, top_scores=top_scores, selected_experts_indices=idx, shared_scale=shared_scale)
+    if idx.numel() != T * K or top_scores.numel() != T * K:
+        raise ValueError(f"scores and indices must be [{T}, K], got {tuple(top_scores.shape)} and {tuple(idx.shape)}")
+    idx, top_scores = idx.contiguous(), top_scores.float().contiguous()
+    E, H, Hs, weights, shared = _experts(w13, w2, shared_w13, shared_w2, D, dev)
+    if shared_scale is not None:
+        shared_scale = shared_scale.float().contiguous()
+        if Hs == 0 or shared_scale.numel() != T:
+            raise ValueError(f"shared_scale must be [{T}] and needs a shared expert")
+    out = torch.empty(T, D, dtype=_BF16, device=dev)
+    ws = _ws(_lib.load().ttamd_experts_decode_workspace_bytes(T, D, H, K, Hs), dev)
+    _call(dev, "ttamd_experts_decode", _p(x), T, D, H, E, K, _p(idx), int(idx.dtype == torch.int64), _p(top_scores),
+          int(bool(score_before_experts)), _limit(swiglu_limit), *map(_p, weights), Hs, *map(_p, shared),
+          _p(shared_scale), _p(out), _p(ws), ws.numel(), _stream(dev))
+    return out
+
+
+def moe_decode(
+    x: torch.Tensor,
+    w_router: torch.Tensor,
+    w13: torch.Tensor | PackedWeights,
+    w2: torch.Tensor | PackedWeights,
+    top_k: int,
+    score_func: str = "softmax",
+    route_norm: bool = False,
+    route_scale: float = 1.0,
+    expert_bias: torch.Tensor | None = None,
+    norm_eps: float = 1e-20,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
+    score_before_experts: bool = False,
+    swiglu_limit: float | None = None,
+    shared_w13: torch.Tensor | PackedWeights | None = None,
+    shared_w2: torch.Tensor | PackedWeights | None = None,
+    shared_gate: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The MoE layer of at most 64 tokens in one call (ttamd_moe_decode): x bf16
+    [T, D] to (out bf16 [T, D], top_scores fp32 [T, K], selected_experts_indices
+    int64 [T, K]).  Router arguments as router_decode, expert arguments as
+    experts_decode; shared_gate [1, D] scales the shared expert by sigmoid(x .
+    shared_gate)."""
+    dev = _gpu("x", x)
+    _no_grad("moe_decode", x, w_router, w13, w2, shared_w13, shared_w2, shared_gate)
+    x = _rows(x)
+    w_router = _want("w_router", w_router, _BF16)
+    _same_device(dev, w_router=w_router)
+    T, D = x.shape
+    E, H, Hs, weights, shared = _experts(w13, w2, shared_w13, shared_w2, D, dev)
+    if tuple(w_router.shape) != (E, D):
+        raise ValueError(f"w_router must be [{E}, {D}] for these experts, got {tuple(w_router.shape)}")
+    if score_func not in ops._SCORE_FUNCS:
+        raise ValueError(f"score_func must be one of {sorted(ops._SCORE_FUNCS)}")
+    groups = _groups(num_groups, topk_groups, group_score) or (1, 1, 0)
+    expert_bias = _bias(expert_bias, E, dev)
+    shared_gate = _gate_row(shared_gate, D, dev)
+    if shared_gate is not None and Hs == 0:
+        raise ValueError("shared_gate needs a shared expert")
+    scores = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+    idx = torch.empty(T, top_k, dtype=torch.int64, device=dev)
+    out = torch.empty(T, D, dtype=_BF16, device=dev)
+    ws = _ws(_lib.load().ttamd_moe_decode_workspace_bytes(T, D, H, E, top_k, Hs), dev)
+    _call(dev, "ttamd_moe_decode", _p(x), T, D, H, E, top_k, _p(w_router), _p(expert_bias), *groups,
+          ops._SCORE_FUNCS[score_func], int(bool(route_norm)), float(norm_eps), float(route_scale),
+          int(bool(score_before_experts)), _limit(swiglu_limit), *map(_p, weights), Hs, *map(_p, shared),
+          _p(shared_gate), _p(scores), _p(idx), _p(out), _p(ws), ws.numel(), _stream(dev))
+    return out, scores, idx
