@@ -324,7 +324,9 @@ def test_router(decode, ops, T, E, K, D, func):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
-@pytest.mark.parametrize("T,E,K,D,H", [(1, 128, 8, 2048, 768), (17, 60, 4, 1440, 544), (64, 8, 2, 256, 512)])
+@pytest.mark.parametrize("T,E,K,D,H", [(1, 128, 8, 2048, 768), (17, 60, 4, 1440, 544), (64, 8, 2, 256, 512),
+                                       (3, 16, 2, 128, 96), (20, 160, 6, 64, 32), (64, 256, 8, 64, 32),
+                                       (33, 1024, 16, 64, 32), (5, 300, 9, 32, 64), (40, 64, 12, 96, 32)])
 def test_whole_layer(decode, T, E, K, D, H, bits):
     rng = np.random.default_rng(T)
     w, wb = build(decode, rng, E, D, H, bits, 96)
@@ -337,6 +339,12 @@ def test_whole_layer(decode, T, E, K, D, H, bits):
     assert torch.equal(out, decode.experts_decode(x, s, i, *w[:2], False, None, w[2], w[3], gate))
     ref, bound = layer_ref(x, s, i, *wb[:2], False, None, wb[2:], gate)
     assert ((out.double() - ref).abs() - bound).max() <= 0
+    if E % 4 == 0 and K <= E // 2:
+        groups = dict(num_groups=4, topk_groups=2, group_score="max")
+        out, scores, idx = decode.moe_decode(x, wr, *w[:2], K, "sigmoid", **groups)
+        s, i, _ = decode.router_decode(x, wr, K, "sigmoid", **groups)
+        assert torch.equal(scores, s) and torch.equal(idx, i)
+        assert torch.equal(out, decode.experts_decode(x, s, i, *w[:2]))
 
 
 def test_without_tokens(decode):

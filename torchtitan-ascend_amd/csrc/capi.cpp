@@ -1038,6 +1038,8 @@ int check_decode(const char* fn, int64_t T, int64_t D, int64_t H, int E, int K, 
   REQUIRE(Hs == 0 || (Hs > 0 && Hs % 32 == 0 && Hs <= (1 << 20)),
           "%s: shared_hidden must be 0 or a positive multiple of 32 (got %lld)", fn, (long long)Hs);
   REQUIRE(E * H * D < (int64_t(1) << 40) && Hs * D < (int64_t(1) << 40), "%s: weights too large", fn);
+  REQUIRE(2 * T * (K * H + Hs) <= kI32Max, "%s: too many activations (%lld tokens of %d x %lld)", fn, (long long)T, K,
+          (long long)H);
   return TTAMD_OK;
 }
 
@@ -1158,16 +1160,18 @@ int ttamd_router_decode(const void* x, const void* w_router, const float* expert
   REQUIRE((w_gate != nullptr) == (gate_out != nullptr), "%s: give w_gate and gate_out together", fn);
   REQUIRE(aligned16(w_gate), "%s: w_gate must be 16-byte aligned", fn);
   TRY(check_ws(fn, workspace, workspace_bytes, ttamd::router_decode_workspace_bytes(num_tokens, num_experts)));
-  const ttamd::RouterGroups g = {num_groups, topk_groups, group_score == TTAMD_GROUP_TOP2};
-  return check_hip(ttamd::launch_router_decode(x, w_router, w_gate, expert_bias, (int)num_tokens, num_experts, (int)dim,
-                                               topk, g, score_func, renormalize, renorm_eps, route_scale, top_scores,
-                                               top_indices, gate_out, workspace, (hipStream_t)stream),
+  const ttamd::RouterDecode r = {x, w_router, w_gate, expert_bias,
+                                 {num_groups, topk_groups, group_score == TTAMD_GROUP_TOP2}, score_func, renormalize,
+                                 renorm_eps, route_scale, top_scores, top_indices, gate_out, workspace};
+  return check_hip(ttamd::launch_router_decode(r, (int)num_tokens, num_experts, (int)dim, topk, (hipStream_t)stream),
                    fn);
 }
 
 size_t ttamd_experts_decode_workspace_bytes(int64_t num_tokens, int64_t dim, int64_t hidden, int topk,
                                             int64_t shared_hidden) {
-  if (num_tokens < 0 || dim < 1 || hidden < 1 || topk < 1 || shared_hidden < 0) return 0;
+  if (num_tokens < 0 || num_tokens > ttamd::kDecodeMaxTokens || dim < 1 || hidden < 1 || topk < 1 ||
+      topk > ttamd::kDecodeMaxTopk || shared_hidden < 0)
+    return 0;
   return ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden);
 }
 
@@ -1193,13 +1197,15 @@ int ttamd_experts_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t
   return check_hip(ttamd::launch_experts_decode(decode_args(w, x, num_tokens, dim, hidden, num_experts, topk,
                                                             shared_hidden, indices, indices_are_int64 != 0, top_scores,
                                                             score_before, swiglu_limit, shared_gate, out),
-                                                workspace, (hipStream_t)stream),
+                                                nullptr, workspace, (hipStream_t)stream),
                    fn);
 }
 
 size_t ttamd_moe_decode_workspace_bytes(int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts, int topk,
                                         int64_t shared_hidden) {
-  if (num_tokens < 0 || dim < 1 || hidden < 1 || num_experts < 1 || topk < 1 || shared_hidden < 0) return 0;
+  if (num_tokens < 0 || num_tokens > ttamd::kDecodeMaxTokens || dim < 1 || hidden < 1 || num_experts < 1 ||
+      topk < 1 || topk > ttamd::kDecodeMaxTopk || shared_hidden < 0)
+    return 0;
   return align256((size_t)num_tokens * 4) + ttamd::router_decode_workspace_bytes(num_tokens, num_experts) +
          ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden);
 }
@@ -1230,15 +1236,13 @@ int ttamd_moe_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t hid
                ttamd_moe_decode_workspace_bytes(num_tokens, dim, hidden, num_experts, topk, shared_hidden)));
   float* const gate = w_gate ? (float*)workspace : nullptr;
   char* const logits = (char*)workspace + align256((size_t)num_tokens * 4);
-  const ttamd::RouterGroups g = {num_groups, topk_groups, group_score == TTAMD_GROUP_TOP2};
-  TRY(check_hip(ttamd::launch_router_decode(x, w_router, w_gate, expert_bias, (int)num_tokens, num_experts, (int)dim,
-                                            topk, g, score_func, renormalize, renorm_eps, route_scale, top_scores,
-                                            top_indices, gate, logits, (hipStream_t)stream),
-                fn));
+  const ttamd::RouterDecode r = {x, w_router, w_gate, expert_bias,
+                                 {num_groups, topk_groups, group_score == TTAMD_GROUP_TOP2}, score_func, renormalize,
+                                 renorm_eps, route_scale, top_scores, top_indices, gate, logits};
   return check_hip(
       ttamd::launch_experts_decode(decode_args(w, x, num_tokens, dim, hidden, num_experts, topk, shared_hidden,
                                                top_indices, true, top_scores, score_before, swiglu_limit, gate, out),
-                                   logits + ttamd::router_decode_workspace_bytes(num_tokens, num_experts),
+                                   &r, logits + ttamd::router_decode_workspace_bytes(num_tokens, num_experts),
                                    (hipStream_t)stream),
       fn);
 }

@@ -34,6 +34,7 @@
 #include "fp4.h"
 #include "gemm_common.h"
 #include "kernels.h"
+#include "router_select.h"
 
 namespace ttamd {
 namespace {
@@ -226,7 +227,22 @@ struct DecodeArgs {
   int ncount;
   bf16_t* out;          // [T, D]
   int log_ks, cap, smem_rows;
+  const char* plan;
+  int plan_lds;         // its bytes in LDS
 };
+
+// silu(min(gate, L)) * clamp(up, -L, L) in bf16: rounded for the matrix cores, the
+// only rounding between x and the output.
+__device__ __forceinline__ u32x2_t activate(const floatx4_t& g, const floatx4_t& u, float limit) {
+  float o[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    float gate = g[v], up = u[v];
+    if (limit == limit) gate = clamp_max_nan(gate, limit), up = clamp_nan(up, limit);
+    o[v] = silu_f(gate) * up;
+  }
+  return u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+}
 
 // The labels of the call, and which experts they hit.
 struct Labels {
@@ -348,15 +364,7 @@ __global__ __launch_bounds__(kThreads, 4) void decode_w13_kernel(const DecodeArg
     if (group >= H / 16) return;
     const int slot = shared ? i : s.slots[i];
     const float sc = a.before && !shared ? a.scores[slot] : 1.f;
-    float o[4];
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      float gate = v0[v] * sc, up = v1[v] * sc;
-      if (a.limit == a.limit) gate = clamp_max_nan(gate, a.limit), up = clamp_nan(up, a.limit);
-      o[v] = silu_f(gate) * up;
-    }
-    // rounded for the matrix cores, the only rounding between x and the output
-    *(u32x2_t*)(dst + (int64_t)slot * H + 16 * group + 4 * quad) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+    *(u32x2_t*)(dst + (int64_t)slot * H + 16 * group + 4 * quad) = activate(v0 * sc, v1 * sc, a.limit);
   };
   stream_rows<WT, NT>(pair, live, a.D, cnt, a.cap, a.log_ks, rows, a.smem_rows, 0, a.cap, src, emit);
 }
@@ -415,167 +423,246 @@ __global__ __launch_bounds__(kThreads, 4) void decode_w2_kernel(const DecodeArgs
 }
 
 // ---------------------------------------------------------------------------
-// bf16 weights: every wave streams its own row pairs through a ring in LDS
+// The plan: which experts are hit, and by which slots
 // ---------------------------------------------------------------------------
-// What a workgroup knows of the call's labels: the hit experts in order of their
-// first slot, and the slots sorted by expert.
-struct Plan {
-  int hit;
-  short list[kMaxE];       // the j-th hit expert
-  short start[kMaxE + 1];  // its first place in `sorted`
-  short sorted[kMaxSlots];
-  float score[kMaxSlots];  // factor of the slot at a place
-  float gate[kDecodeMaxTokens];
-  uint32_t valid[kDecodeMaxTokens];
+// One workgroup makes it (with the selection, where the router runs), the two
+// streaming kernels copy it to LDS.  Hit experts in order; slots sorted by expert
+// ("places").
+struct PlanMap {
+  int T, S;
+  __host__ __device__ constexpr int valid() const { return 16; }                   // uint32 [T]: choices that name an expert
+  __host__ __device__ constexpr int gate() const { return valid() + 4 * T; }       // float [T]: factor of the shared expert
+  __host__ __device__ constexpr int score() const { return gate() + 4 * T; }       // float [S], by place
+  __host__ __device__ constexpr int sorted() const { return score() + 4 * S; }     // short [S]: slot at a place
+  __host__ __device__ constexpr int inverse() const { return sorted() + 2 * S; }   // short [S]: place of a slot
+  __host__ __device__ constexpr int list() const { return inverse() + 2 * S; }     // short [hit]: experts
+  __host__ __device__ constexpr int start() const { return list() + 2 * S; }       // short [hit + 1]: their first places
+  __host__ __device__ constexpr int bytes() const { return (start() + 2 * (S + 1) + 15) & ~15; }  // int hit at 0
 };
-struct PlanScratch {
-  int first[kMaxE], count[kMaxE];
-  short lab[kMaxSlots], pos[kMaxSlots];
+constexpr int kMaxPlanBytes = PlanMap{kDecodeMaxTokens, kMaxSlots}.bytes();
+
+struct Plan : PlanMap {
+  char* p;
+  __device__ Plan(char* p_, int T_, int S_) : PlanMap{T_, S_}, p(p_) {}
+  __device__ int& hit() const { return *(int*)p; }
+  __device__ uint32_t& valid(int i) const { return ((uint32_t*)(p + PlanMap::valid()))[i]; }
+  __device__ float& gate(int i) const { return ((float*)(p + PlanMap::gate()))[i]; }
+  __device__ float& score(int i) const { return ((float*)(p + PlanMap::score()))[i]; }
+  __device__ short& sorted(int i) const { return ((short*)(p + PlanMap::sorted()))[i]; }
+  __device__ short& inverse(int i) const { return ((short*)(p + PlanMap::inverse()))[i]; }
+  __device__ short& list(int i) const { return ((short*)(p + PlanMap::list()))[i]; }
+  __device__ short& start(int i) const { return ((short*)(p + PlanMap::start()))[i]; }
 };
 
-__device__ __forceinline__ void build_plan(const DecodeArgs& a, Plan& p, PlanScratch& t, bool scored) {
-  const int S = a.T * a.K, tid = threadIdx.x;
-  for (int i = tid; i < S; i += kThreads) {
-    const int64_t v = a.is64 ? ((const int64_t*)a.idx)[i] : (int64_t)((const int*)a.idx)[i];
-    const bool in = v >= 0 && v < a.E;
-    t.lab[i] = in ? (short)v : (short)-1;
-    if (in) t.first[v] = S, t.count[v] = 0;
-  }
-  __syncthreads();
-  for (int i = tid; i < S; i += kThreads)
-    if (t.lab[i] >= 0) {
-      atomicMin(&t.first[t.lab[i]], i);
-      t.pos[i] = (short)atomicAdd(&t.count[t.lab[i]], 1);  // (columns of a tile: any order gives the same sums)
-    }
-  __syncthreads();
-  if (tid < 64) {
-    int hit = 0, base = 0;
-    for (int i0 = 0; i0 < S; i0 += 64) {
-      const int i = i0 + tid, lab = i < S ? t.lab[i] : -1;
-      const bool lead = lab >= 0 && t.first[max(lab, 0)] == i;
-      const uint64_t m = ballot64(lead);
-      const int n = lead ? t.count[lab] : 0, upto = wave_inclusive_scan(n);
-      if (lead) {
-        const int j = hit + __popcll(m & lanemask_lt());
-        p.list[j] = (short)lab;
-        p.start[j] = (short)(base + upto - n);
-        t.count[lab] = base + upto - n;  // from here on the expert's first place
+constexpr int kPlanThreads = 1024;
+
+struct PlanArgs {
+  select::GroupTopkArgs topk;  // of the selection (its scores and idx are outputs)
+  const void* idx;             // without it: given picks
+  int is64;
+  const float* scores;
+  const float* gate;           // [T] or null: 1
+  int T, E, K;
+  char* plan;
+  int* count;                  // cleared for the kernels after this one
+  int ncount;
+};
+
+// LPT = 0: given picks.  One thread per slot, then one per expert.  Barriers wait
+// for LDS alone: the picks' stores need not land in between.
+template <int LPT, int PL, int KL>
+__global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(const PlanArgs a) {
+  __shared__ int total[kMaxE];
+  __shared__ float score[kMaxSlots];
+  __shared__ short lab[kMaxSlots];
+  __shared__ int wave_hit[kPlanThreads / 64], wave_rows[kPlanThreads / 64];
+  const int S = a.T * a.K, tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  const Plan p(a.plan, a.T, S);
+  if (tid < a.E) total[tid] = 0;
+  for (int i = tid; i < a.ncount; i += kPlanThreads) a.count[i] = 0;
+  float gate = 1.f;
+  if (tid < a.T && a.gate) gate = a.gate[tid];
+  if constexpr (LPT > 0) {
+    constexpr int TPB = kPlanThreads / LPT;
+    const int gi = tid & (LPT - 1);
+    for (int t0 = 0; t0 < a.T; t0 += TPB) {
+      const int t = t0 + tid / LPT;
+      if (t0 + ((tid & ~63) / LPT) >= a.T) break;  // no token for this wave
+      int pick;
+      double weight;
+      select::select_token<LPT, PL, KL, select::SRC_BF16>(a.topk, min(t, a.T - 1), t < a.T, pick, weight, [](int) {});
+      if (gi < a.K && t < a.T) {
+        const float sc = (float)(weight * (double)a.topk.route_scale);
+        a.topk.scores[t * a.K + gi] = score[t * a.K + gi] = sc;
+        a.topk.idx[t * a.K + gi] = pick;
+        lab[t * a.K + gi] = (short)pick;
       }
-      hit += __popcll(m);
-      base += __shfl(upto, 63, 64);
     }
-    if (tid == 0) p.hit = hit, p.start[hit] = (short)base;
+  } else if (tid < S) {  // (S <= kPlanThreads)
+    const int64_t v = a.is64 ? ((const int64_t*)a.idx)[tid] : (int64_t)((const int*)a.idx)[tid];
+    lab[tid] = v >= 0 && v < a.E ? (short)v : (short)-1;
+    score[tid] = a.scores[tid];
   }
-  __syncthreads();
-  for (int i = tid; i < S; i += kThreads)
-    if (t.lab[i] >= 0) {
-      const int at = t.count[t.lab[i]] + t.pos[i];
-      p.sorted[at] = (short)i;
-      p.score[at] = scored ? a.scores[i] : 1.f;
-    }
-  if (a.gate && tid < a.T) p.gate[tid] = a.gate[tid];
-  note_valid(a, t.lab, p.valid);
-  __syncthreads();
+  dma::lds_barrier();
+  const int mine = tid < S ? lab[tid] : -1;
+  int pos = 0;
+  if (mine >= 0) pos = atomicAdd(&total[mine], 1);  // (columns of a product: any order gives the same sums)
+  if (tid < a.T) {
+    uint32_t m = (1u << a.K) - 1;
+    if (LPT == 0)
+      for (int k = 0; k < a.K; ++k) m &= ~((lab[tid * a.K + k] < 0 ? 1u : 0u) << k);
+    p.valid(tid) = m;
+    p.gate(tid) = gate;
+  }
+  dma::lds_barrier();
+  const int n = tid < a.E ? total[tid] : 0, upto = wave_inclusive_scan(n);
+  const uint64_t m = ballot64(n > 0);
+  if (l == 63) wave_hit[w] = __popcll(m), wave_rows[w] = upto;
+  dma::lds_barrier();
+  int hit = 0, base = 0, hits = 0;
+#pragma unroll
+  for (int v = 0; v < kPlanThreads / 64; ++v) {
+    const int h = wave_hit[v], r = wave_rows[v];
+    if (v < w) hit += h, base += r;
+    hits += h;
+  }
+  if (n > 0) {
+    const int j = hit + __popcll(m & lanemask_lt()), first = base + upto - n;
+    p.list(j) = (short)tid;
+    p.start(j) = (short)first;
+    if (j == hits - 1) p.start(hits) = (short)(first + n);
+    total[tid] = first;
+  }
+  if (tid == 0) p.hit() = hits;
+  dma::lds_barrier();
+  if (mine >= 0) {
+    const int at = total[mine] + pos;
+    p.sorted(at) = (short)tid;
+    p.inverse(tid) = (short)at;
+    p.score(at) = score[tid];
+  }
 }
 
-// One item of a workgroup: kWaves / KS row pairs of one expert (or the shared one).
-struct Item {
-  uint64_t base0, base1;  // this wave's two row blocks
-  int cnt;                // token rows
-  int start;              // their places in Plan::sorted; -1: the shared expert, row = token
-  int rb;                 // which run of row pairs
-  int K;
-  bool live;              // this wave's pair exists
+// ---------------------------------------------------------------------------
+// Streams: every wave pulls its own weight rows through a ring in LDS
+// ---------------------------------------------------------------------------
+// A stage of a wave: its weight rows and the token rows over kCols columns (bf16: a
+// 128-byte line of every row; 4 bits: one tile and its exponents).  A DMA
+// instruction moves 8 bf16 weight rows, one 4-bit tile of 16, or 8 (4) token rows of
+// 128 (256) bytes; BL and NB count the instructions.
+template <int WT, int BL, int NB, int NS>
+struct Ring {
+  static constexpr int kCols = WT == W_BF16 ? 64 : 128;
+  static constexpr int kBlocks = WT == W_BF16 ? (BL + 1) / 2 : BL;  // of 16 rows
+  static constexpr int kExps = BL * 1024;                           // 4 bits: 256 bytes of exponents per block
+  static constexpr int kRowsAt = kExps + (WT == W_BF16 ? 0 : 256 * BL);
+  static constexpr int kBytes = kRowsAt + 1024 * NB;
+  static constexpr int kOps = (WT == W_BF16 ? BL : 2 * BL) + NB;
+  static constexpr int kRows = NB * (WT == W_BF16 ? 8 : 4);
+  static constexpr int NT = (kRows + 15) / 16;
+  static constexpr int kAll = kWaves * NS * kBytes;
 };
 
-constexpr int kStageCols = 64;  // a 128-byte line of every row
+// One item of a wave: rows of one expert (or the shared one) times its token rows.
+template <int BL>
+struct Item {
+  uint64_t base[BL];  // per load: bf16, its first row of 8; 4 bits, its first tile
+  uint64_t exps[BL];  // 4 bits: its exponents
+  int cnt;            // token rows
+  int start;          // their first place in the plan; -1: the shared expert, row = token
+  int rb;             // which run of rows (the caller's)
+  int K;
+  bool live;          // the wave has rows here
+};
 
-// Waves that share a row pair (log2): rounds of the walk times a wave's stages in
-// one (a stage is 1.4 us where HBM bounds it), the meeting of KS waves as half a
-// stage.  From the experts really hit, so that the last round is full: 112 experts
-// of 1536 x 2048 make 2.6 rounds with whole pairs and 21.0 with eighths.
-__device__ __forceinline__ int split_log(int pairs, int K) {
-  const int stages = (K + kStageCols - 1) / kStageCols, slots = kWaves * gridDim.x;
-  int best = 0, cost = 0x7fffffff;
-  for (int k = 0; k <= 3 && (1 << k) <= stages; ++k) {
-    const int rounds = ((pairs << k) + slots - 1) / slots;
-    const int c = rounds * (2 * ((stages + (1 << k) - 1) >> k) + (k > 0));
-    if (c < cost) best = k, cost = c;
-  }
-  return best;
-}
-
-// Token rows that the partial sums of KS waves meet over at a time.
-template <int NB>
-constexpr int kMeetRows = NB == 1 ? 8 : NB == 2 ? 4 : 16;
-
-// The wave's stages (32 weight rows and 8 NB token rows, 64 columns) in a ring of
-// NS, filled by LDS DMA: whole 128-byte lines, eight rows an instruction, the
-// 16-byte chunk c of row r at c ^ cswz(r).  The DMAs run over the flattened
-// sequence of all its items' stages, NS ahead, so neither an epilogue nor the next
-// expert's start empties the pipe; a wave meets the others only where KS > 1.
-// item(i): the i-th item; src(item, i): byte offset of its token row i from xbase.
-template <int NB, int NS, class ItemOf, class Src, class Emit>
-__device__ __forceinline__ void stream_items(char* ring, floatx4_t* red, int nitems, int log_ks, uint64_t xbase,
-                                             ItemOf item_of, Src src, Emit emit) {
+// Runs the items first, first + step, ... < nitems.  Of a item's stages the wave
+// takes every KS-th from ks on.  The DMAs run over the flattened sequence of all
+// its stages, NS ahead, so neither an epilogue nor the next expert's start empties
+// the pipe, and no wave waits for another here.  item_of(i): the i-th item;
+// src(item, i): byte offset of its token row i from xbase; done(item, c0, rows,
+// acc): the sums of its token rows c0 .. c0 + rows - 1 (lane l, block b, tile t:
+// weight rows 4 (l / 16) .. + 3, token row c0 + 16 t + l % 16).
+template <int WT, int BL, int NB, int NS, class ItemOf, class Src, class Done>
+__device__ __forceinline__ void stream_items(char* ring, int first, int step, int nitems, int ks, int KS,
+                                             uint64_t xbase, ItemOf item_of, Src src, Done done) {
   using namespace dma;
-  constexpr int OPS = 4 + NB, SB = 1024 * OPS, NT = (NB + 1) / 2, ROWS = 8 * NB;
-  const int tid = threadIdx.x, l = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int KS = 1 << log_ks, ks = w & (KS - 1), G = gridDim.x;
+  using R = Ring<WT, BL, NB, NS>;
+  constexpr int NT = R::NT, MB = R::kBlocks;
+  const int l = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = l & 15, q = l >> 4;
-  const int lr = l >> 3;
-  ring += w * (NS * SB);
+  ring += w * (NS * R::kBytes);
   const uint32_t lds0 = lds_addr(ring);
 
+  // 16-byte chunk of its row that lane l moves in instruction i: LDS holds chunk c
+  // of row r at c ^ cswz(r) (8 chunks a row) or c ^ r (16), so that the fragment
+  // reads of 16 rows meet no bank twice
+  auto chunk8 = [&](int i) { return (l & 7) ^ cswz(8 * i + (l >> 3)); };
+  auto chunk16 = [&](int i) { return (l & 15) ^ ((4 * i + (l >> 4)) & 15); };
+
   // the issuing end
-  int it = blockIdx.x, n0 = 0, s = ks;
+  int it = first, n0 = 0, s = ks;
   bool more = it < nitems;
-  Item in;
-  uint32_t va[4], vb[NB];
+  Item<BL> in;
+  uint32_t va[BL], vb[NB];
   auto rows = [&]() {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int r = 8 * b + lr;
-      vb[b] = src(in, min(n0 + r, in.cnt - 1)) + (uint32_t)(((l & 7) ^ cswz(r)) * 16);
+      const int r = WT == W_BF16 ? 8 * b + (l >> 3) : 4 * b + (l >> 4);
+      const int ch = WT == W_BF16 ? chunk8(b) : chunk16(b);
+      vb[b] = src(in, min(n0 + r, in.cnt - 1)) + (uint32_t)(16 * ch);
     }
   };
   auto enter = [&]() {  // item `it`, or the next with a stage for this wave
-    for (;; it += G) {
+    for (;; it += step) {
       more = it < nitems;
       if (!more) return;
       in = item_of(it);
-      if (in.live && in.cnt > 0 && ks * kStageCols < in.K) break;
+      if (in.live && in.cnt > 0 && ks * R::kCols < in.K) break;
     }
     n0 = 0, s = ks;
+    if constexpr (WT == W_BF16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      va[i] = (uint32_t)((8 * (i & 1) + lr) * in.K * 2) + (uint32_t)(((l & 7) ^ cswz(8 * i + lr)) * 16);
+      for (int i = 0; i < BL; ++i) va[i] = (uint32_t)((l >> 3) * in.K * 2) + (uint32_t)(16 * chunk8(i));
+    }
     rows();
   };
   auto issue = [&](int slot) {
-    const uint32_t at = lds0 + (uint32_t)(slot * SB);
-    const uint64_t k = (uint64_t)s * (kStageCols * 2);
-    // a row's last 32 columns: the upper chunks load the lower ones again
-    const bool half = (s + 1) * kStageCols > in.K;
+    const uint32_t at = lds0 + (uint32_t)(slot * R::kBytes);
+    const int left = in.K - s * R::kCols;  // columns of the row from this stage on, a multiple of 32
+    if constexpr (WT == W_BF16) {
+      const uint64_t k = (uint64_t)s * 128;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t back = half && (((l & 7) ^ cswz(8 * i + lr)) & 4) ? 64u : 0u;
-      dma16(va[i] - back, (i < 2 ? in.base0 : in.base1) + k, at + i * 1024);
-    }
+      for (int i = 0; i < BL; ++i) {  // past the row's end: the chunk 64 bytes before once more
+        const uint32_t back = left < 64 && (chunk8(i) & 4) ? 64u : 0u;
+        dma16(va[i] - back, in.base[i] + k, at + i * 1024);
+      }
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const uint32_t back = half && (((l & 7) ^ cswz(8 * b + lr)) & 4) ? 64u : 0u;
-      dma16(vb[b] - back, xbase + k, at + (4 + b) * 1024);
+      for (int b = 0; b < NB; ++b) {
+        const uint32_t back = left < 64 && (chunk8(b) & 4) ? 64u : 0u;
+        dma16(vb[b] - back, xbase + k, at + R::kRowsAt + b * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < BL; ++b) dma16((uint32_t)(16 * l), in.base[b] + (uint64_t)s * 1024, at + b * 1024);
+#pragma unroll
+      for (int b = 0; b < BL; ++b)
+        dma4((uint32_t)(4 * l), in.exps[b] + (uint64_t)(s >> 2) * 256, at + R::kExps + b * 256);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int ch = chunk16(b);
+        const uint32_t back = 8 * ch >= left ? (uint32_t)(16 * (ch & ~3)) : 0u;
+        dma16(vb[b] - back, xbase + (uint64_t)s * 256, at + R::kRowsAt + b * 1024);
+      }
     }
     s += KS;
-    if (s * kStageCols < in.K) return;
+    if (s * R::kCols < in.K) return;
     s = ks;
-    n0 += ROWS;
+    n0 += R::kRows;
     if (n0 < in.cnt) {
       rows();
     } else {
-      it += G;
+      it += step;
       enter();
     }
   };
@@ -587,210 +674,303 @@ __device__ __forceinline__ void stream_items(char* ring, floatx4_t* red, int nit
 
   // the consuming end
   int slot = 0;
-  for (int ci = blockIdx.x; ci < nitems; ci += G) {
-    const Item c = item_of(ci);
-    for (int c0 = 0; c0 < c.cnt; c0 += ROWS) {
-      const int rows_here = min(c.cnt - c0, ROWS);
-      floatx4_t acc[2][NT];
+  for (int ci = first; ci < nitems; ci += step) {
+    const Item<BL> c = item_of(ci);
+    for (int c0 = 0; c0 < c.cnt; c0 += R::kRows) {
+      floatx4_t acc[MB][NT];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < MB; ++b)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[b][t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
       if (c.live)
-        for (int cs = ks; cs * kStageCols < c.K; cs += KS) {
-          if (ahead == NS) wait_vm<(NS - 1) * OPS>();
+        for (int cs = ks; cs * R::kCols < c.K; cs += KS) {
+          if (ahead == NS) wait_vm<(NS - 1) * R::kOps>();
           else wait_vm<0>();
-          const char* st = ring + slot * SB;
-          bf16x8_t a0[2], a1[2], bx[2][NT];
+          const char* st = ring + slot * R::kBytes;
+          const int left = c.K - cs * R::kCols;
+          if constexpr (WT == W_BF16) {
+            bf16x8_t aw[MB][2], bx[2][NT];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int ch = 4 * h + q;
-            a0[h] = *(const bf16x8_t*)(st + n * 128 + ((ch ^ cswz(n)) << 4));
-            a1[h] = *(const bf16x8_t*)(st + (16 + n) * 128 + ((ch ^ cswz(16 + n)) << 4));
+            for (int h = 0; h < 2; ++h) {
+              const int ch = 4 * h + q;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              const int r = (16 * t + n) & (ROWS - 1);
-              bx[h][t] = *(const bf16x8_t*)(st + 4096 + r * 128 + ((ch ^ cswz(r)) << 4));
+              for (int b = 0; b < MB; ++b) {  // (the second half of a last block of 8 rows: the first once more)
+                const int r = 16 * b + (2 * b + 1 < BL ? n : n & 7);
+                aw[b][h] = *(const bf16x8_t*)(st + r * 128 + ((ch ^ cswz(r)) << 4));
+              }
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                const int r = (16 * t + n) & (R::kRows - 1);
+                bx[h][t] = *(const bf16x8_t*)(st + R::kRowsAt + r * 128 + ((ch ^ cswz(r)) << 4));
+              }
+            }
+            lds_wait();  // the slot is free
+            if (more) issue(slot);
+            else --ahead;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h == 1 && left < 64) break;
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int b = 0; b < MB; ++b)
+                  acc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(aw[b][h], bx[h][t], acc[b][t], 0, 0, 0);
+            }
+          } else {
+            uint4 qw[BL];
+            float scale[BL];
+            bf16x8_t bx[4][NT];
+#pragma unroll
+            for (int b = 0; b < BL; ++b) {
+              qw[b] = *(const uint4*)(st + b * 1024 + 16 * l);
+              scale[b] = fp4_scale(*(const uint32_t*)(st + R::kExps + b * 256 + 4 * l), cs & 3);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                const int r = (16 * t + n) & (R::kRows - 1);
+                bx[j][t] = *(const bf16x8_t*)(st + R::kRowsAt + r * 256 + (((4 * q + j) ^ (r & 15)) << 4));
+              }
+            lds_wait();
+            if (more) issue(slot);
+            else --ahead;
+            if (left < 128 && 32 * q >= left) {  // (codes past the row's end are zeros; so must be what they meet)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) bx[j][t] = __builtin_bit_cast(bf16x8_t, make_uint4(0u, 0u, 0u, 0u));
+            }
+#pragma unroll
+            for (int b = 0; b < BL; ++b) {
+              const uint32_t d[4] = {qw[b].x, qw[b].y, qw[b].z, qw[b].w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const bf16x8_t aw = fp4_frag(d[j], scale[b]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                  acc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(aw, bx[j][t], acc[b][t], 0, 0, 0);
+              }
             }
           }
-          lds_wait();  // the slot is free
-          if (more) issue(slot);
-          else --ahead;
           slot = slot == NS - 1 ? 0 : slot + 1;
-          const bool half = (cs + 1) * kStageCols > c.K;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h == 1 && half) break;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0[h], bx[h][t], acc[0][t], 0, 0, 0);
-              acc[1][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1[h], bx[h][t], acc[1][t], 0, 0, 0);
-            }
-          }
         }
-      if (log_ks == 0) {
-        if (c.live) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-            if (16 * t + n < rows_here) emit(c, w, c0 + 16 * t + n, q, acc[0][t], acc[1][t]);
-        }
-        continue;
-      }
-      // the KS partial sums of a pair, in order
-      constexpr int MR = kMeetRows<NB>;
-      for (int m0 = 0; m0 < rows_here; m0 += MR) {
-        const int mr = min(rows_here - m0, MR), per = mr * 4, total = (kWaves >> log_ks) * per;
-        if (c.live) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const int i = 16 * t + n - m0;
-            if (i >= 0 && i < mr) {
-              red[(w * 2 + 0) * per + i * 4 + q] = acc[0][t];
-              red[(w * 2 + 1) * per + i * 4 + q] = acc[1][t];
-            }
-          }
-        }
-        lds_barrier();
-        for (int i = tid; i < total; i += kThreads) {
-          const int r = i / per, at = i - r * per;
-          const floatx4_t* p = red + (r << log_ks) * 2 * per + at;
-          floatx4_t v0 = p[0], v1 = p[per];
-          for (int j = 1; j < KS; ++j) v0 += p[2 * j * per], v1 += p[2 * j * per + per];
-          emit(c, r, c0 + m0 + (at >> 2), at & 3, v0, v1);
-        }
-        lds_barrier();
-      }
+      done(c, c0, min(c.cnt - c0, R::kRows), acc);
     }
   }
   wait_vm<0>();
 }
 
-template <int NB, int NS>
-constexpr int ring_bytes() {
-  return kWaves * NS * 1024 * (4 + NB);
+// Waves that share an item (log2) out of kWaves: rounds of the walk times a wave's
+// stages in one, twice, with `meet` for the meeting of KS waves.  From the experts
+// really hit, so that the last round is full: 112 experts of 1536 x 2048 make 2.6
+// rounds with whole row pairs and 21.0 with eighths.
+__device__ __forceinline__ int split_log(int items, int slots, int stages, int most, int meet) {
+  int best = 0, cost = 0x7fffffff;
+  for (int k = 0; k <= most && (1 << k) <= stages; ++k) {
+    const int rounds = ((items << k) + slots - 1) / slots;
+    const int c = rounds * (2 * ((stages + (1 << k) - 1) >> k) + (k > 0 ? meet : 0));
+    if (c < cost) best = k, cost = c;
+  }
+  return best;
 }
-constexpr int kPlanBytes = (sizeof(Plan) + 1023) & ~1023;
 
-template <int NB, int NS>
-__global__ __launch_bounds__(kThreads, 2) void decode_w13_bf16_kernel(const DecodeArgs a) {
+// Load b of an item: 8 rows (bf16) or 16 (4 bits) of expert e's [N, K] weights from
+// row `row` on.
+template <int WT, int BL>
+__device__ __forceinline__ void set_load(Item<BL>& c, int b, const Weights& m, int64_t e, int N, int K, int row) {
+  if constexpr (WT == W_BF16) {
+    c.base[b] = (uint64_t)((const bf16_t*)m.w + (e * N + row) * K);
+  } else {
+    const int C = (K + 127) / 128, C4 = (C + 3) / 4;
+    const int64_t at = e * ((N + 15) / 16) + row / 16;
+    c.base[b] = (uint64_t)((const char*)m.w + at * C * 1024);
+    c.exps[b] = (uint64_t)(m.exps + at * C4 * 256);
+  }
+}
+
+__device__ __forceinline__ void load_plan(const DecodeArgs& a, char* smem) {
+  const int n = PlanMap{a.T, a.T * a.K}.bytes() / 16;
+  for (int i = threadIdx.x; i < n; i += kThreads) ((uint4*)smem)[i] = ((const uint4*)a.plan)[i];
+  __syncthreads();
+}
+
+// Token rows that the partial sums of KS waves meet over at a time (1 KB each).
+constexpr int kMeetRows = 4;
+
+// gate and up rows of 16 hidden units
+template <int WT>
+constexpr int kPairLoads = WT == W_BF16 ? 4 : 2;
+
+template <int WT, int NB, int NS>
+__global__ __launch_bounds__(kThreads, 2) void stream_w13_kernel(const DecodeArgs a) {
+  constexpr int BL = kPairLoads<WT>;
+  using Rg = Ring<WT, BL, NB, NS>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  Plan& p = *(Plan*)smem;
-  char* const ring = smem + kPlanBytes;
-  const int S = a.T * a.K;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < a.ncount; i += kThreads) a.count[i] = 0;
-  build_plan(a, p, *(PlanScratch*)ring, a.before != 0);
-  const int hit = __builtin_amdgcn_readfirstlane(p.hit);
-  const int log_ks = split_log(hit * (a.H / 16) + a.Hs / 16, a.D);
-  const int R = kWaves >> log_ks, r0 = w >> log_ks;
+  const int S = a.T * a.K, tid = threadIdx.x, l = tid & 63;
+  const Plan p(smem, a.T, S);
+  char* const ring = smem + a.plan_lds;
+  floatx4_t* const red = (floatx4_t*)(ring + Rg::kAll);
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  load_plan(a, smem);
+  const int hit = __builtin_amdgcn_readfirstlane(p.hit());
+  const int log_ks = split_log(hit * (a.H / 16) + a.Hs / 16, kWaves * gridDim.x,
+                               (a.D + Rg::kCols - 1) / Rg::kCols, 3, 1);
+  const int KS = 1 << log_ks, R = kWaves >> log_ks, r0 = w >> log_ks;
   const int nsh = (a.Hs / 16 + R - 1) / R, nrb = (a.H / 16 + R - 1) / R;
-  const int nitems = nsh + hit * nrb;
   auto item_of = [&](int i) {
-    Item c;
+    Item<BL> c;
     const bool shared = i < nsh;
     const int j = shared ? 0 : (i - nsh) / nrb;
-    const int e = shared ? 0 : __builtin_amdgcn_readfirstlane(p.list[j]);
+    const int e = shared ? 0 : __builtin_amdgcn_readfirstlane(p.list(j));
     const int H = shared ? a.Hs : a.H;
     c.rb = shared ? i : i - nsh - j * nrb;
-    c.start = shared ? -1 : __builtin_amdgcn_readfirstlane(p.start[j]);
-    c.cnt = shared ? a.T : __builtin_amdgcn_readfirstlane(p.start[j + 1]) - c.start;
+    c.start = shared ? -1 : __builtin_amdgcn_readfirstlane(p.start(j));
+    c.cnt = shared ? a.T : __builtin_amdgcn_readfirstlane(p.start(j + 1)) - c.start;
     c.K = a.D;
     const int g = c.rb * R + r0;
     c.live = g < H / 16;
-    c.base0 = (uint64_t)((const bf16_t*)(shared ? a.s13 : a.w13).w + ((int64_t)e * 2 * H + 16 * g) * a.D);
-    c.base1 = c.base0 + (uint64_t)H * a.D * 2;
+    const Weights& m = shared ? a.s13 : a.w13;
+#pragma unroll
+    for (int b = 0; b < BL; ++b)
+      set_load<WT>(c, b, m, e, 2 * H, a.D, (b < BL / 2 ? 0 : H) + 16 * g + (WT == W_BF16 ? 8 * (b & 1) : 0));
     return c;
   };
-  auto src = [&](const Item& c, int i) {
-    return (uint32_t)(c.start < 0 ? i : p.sorted[c.start + i] / a.K) * (uint32_t)a.D * 2u;
+  auto src = [&](const Item<BL>& c, int i) {
+    return (uint32_t)(c.start < 0 ? i : p.sorted(c.start + i) / a.K) * (uint32_t)a.D * 2u;
   };
-  auto emit = [&](const Item& c, int r, int i, int quad, const floatx4_t& v0, const floatx4_t& v1) {
+  auto emit = [&](const Item<BL>& c, int r, int i, int quad, const floatx4_t& v0, const floatx4_t& v1) {
     const bool shared = c.start < 0;
     const int H = shared ? a.Hs : a.H, group = c.rb * R + r;
     if (group >= H / 16) return;
-    const int slot = shared ? i : p.sorted[c.start + i];
-    const float sc = shared ? 1.f : p.score[c.start + i];
+    const int slot = shared ? i : p.sorted(c.start + i);
+    const float sc = shared || !a.before ? 1.f : p.score(c.start + i);
     bf16_t* const dst = a.a + (shared ? (int64_t)S * a.H : 0) + (int64_t)slot * H + 16 * group + 4 * quad;
-    float o[4];
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      float gate = v0[v] * sc, up = v1[v] * sc;
-      if (a.limit == a.limit) gate = clamp_max_nan(gate, a.limit), up = clamp_nan(up, a.limit);
-      o[v] = silu_f(gate) * up;
-    }
-    // rounded for the matrix cores, the only rounding between x and the output
-    *(u32x2_t*)dst = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+    *(u32x2_t*)dst = activate(v0 * sc, v1 * sc, a.limit);
   };
-  stream_items<NB, NS>(ring, (floatx4_t*)(ring + ring_bytes<NB, NS>()), nitems, log_ks, (uint64_t)a.x, item_of, src,
-                       emit);
+  stream_items<WT, BL, NB, NS>(
+      ring, blockIdx.x, gridDim.x, nsh + hit * nrb, w & (KS - 1), KS, (uint64_t)a.x, item_of, src,
+      [&](const Item<BL>& c, int c0, int rows, const floatx4_t (&acc)[2][Rg::NT]) {
+        constexpr int NT = Rg::NT;
+        const int n = l & 15, q = l >> 4;
+        if (log_ks == 0) {
+          if (c.live) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              if (16 * t + n < rows) emit(c, w, c0 + 16 * t + n, q, acc[0][t], acc[1][t]);
+          }
+          return;
+        }
+        // the KS partial sums of a pair, in order
+        for (int m0 = 0; m0 < rows; m0 += kMeetRows) {
+          const int mr = min(rows - m0, kMeetRows), per = mr * 4, total = R * per;
+          if (c.live) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              const int i = 16 * t + n - m0;
+              if (i >= 0 && i < mr) {
+                red[(w * 2 + 0) * per + i * 4 + q] = acc[0][t];
+                red[(w * 2 + 1) * per + i * 4 + q] = acc[1][t];
+              }
+            }
+          }
+          dma::lds_barrier();
+          for (int i = tid; i < total; i += kThreads) {
+            const int r = i / per, at = i - r * per;
+            const floatx4_t* v = red + (r << log_ks) * 2 * per + at;
+            floatx4_t v0 = v[0], v1 = v[per];
+            for (int j = 1; j < KS; ++j) v0 += v[2 * j * per], v1 += v[2 * j * per + per];
+            emit(c, r, c0 + m0 + (at >> 2), at & 3, v0, v1);
+          }
+          dma::lds_barrier();
+        }
+      });
 }
 
-template <int NB, int NS>
-__global__ __launch_bounds__(kThreads, 2) void decode_w2_bf16_kernel(const DecodeArgs a) {
+// A workgroup owns the output rows of BL loads (8 each, 4 bits: 16) for every
+// expert; its waves (KS to a share of
+// the columns) take the hit experts in turn, the weighted rows of all slots meet in
+// LDS and leave as the tokens' sums: nothing goes through memory, no workgroup
+// waits for another, every sum has its order.
+template <int WT, int BL, int NB, int NS>
+__global__ __launch_bounds__(kThreads, 2) void stream_w2_kernel(const DecodeArgs a) {
+  using Rg = Ring<WT, BL, NB, NS>;
+  constexpr int MB = Rg::kBlocks, LR = WT == W_BF16 ? 8 : 16;  // rows of a load
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  __shared__ int nlast;
-  Plan& p = *(Plan*)smem;
-  char* const ring = smem + kPlanBytes;
-  const int S = a.T * a.K;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  build_plan(a, p, *(PlanScratch*)ring, a.before == 0);
-  const int hit = __builtin_amdgcn_readfirstlane(p.hit);
-  const int log_ks = split_log((hit + (a.Hs > 0)) * (a.D / 32), hit > 0 ? a.H : a.Hs);
-  const int R = kWaves >> log_ks, r0 = w >> log_ks;
-  const int nrb = (a.D / 32 + R - 1) / R, nsh = a.Hs > 0 ? nrb : 0;
-  const int nitems = nsh + hit * nrb;
+  const int S = a.T * a.K, tid = threadIdx.x, l = tid & 63;
+  const Plan p(smem, a.T, S);
+  char* const ring = smem + a.plan_lds;
+  floatx4_t* const sums = (floatx4_t*)(ring + Rg::kAll);  // [KS][place][MB][4]
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  load_plan(a, smem);
+  const int hit = __builtin_amdgcn_readfirstlane(p.hit());
+  const int nsh = a.Hs > 0, places = S + (nsh ? a.T : 0);
+  constexpr int C = Rg::kCols;
+  const int log_ks = split_log(hit + nsh, kWaves, ((hit > 0 ? a.H : a.Hs) + C - 1) / C, a.log_ks, 0);
+  const int KS = 1 << log_ks, R = kWaves >> log_ks, ks = w & (KS - 1);
+  const int row0 = blockIdx.x * BL * LR;
   auto item_of = [&](int i) {
-    Item c;
+    Item<BL> c;
     const bool shared = i < nsh;
-    const int j = shared ? 0 : (i - nsh) / nrb;
-    const int e = shared ? 0 : __builtin_amdgcn_readfirstlane(p.list[j]);
-    c.rb = shared ? i : i - nsh - j * nrb;
-    c.start = shared ? -1 : __builtin_amdgcn_readfirstlane(p.start[j]);
-    c.cnt = shared ? a.T : __builtin_amdgcn_readfirstlane(p.start[j + 1]) - c.start;
+    const int e = shared ? 0 : __builtin_amdgcn_readfirstlane(p.list(i - nsh));
+    c.rb = 0;
+    c.start = shared ? -1 : __builtin_amdgcn_readfirstlane(p.start(i - nsh));
+    c.cnt = shared ? a.T : __builtin_amdgcn_readfirstlane(p.start(i - nsh + 1)) - c.start;
     c.K = shared ? a.Hs : a.H;
-    const int g = c.rb * R + r0;
-    c.live = g < a.D / 32;
-    c.base0 = (uint64_t)((const bf16_t*)(shared ? a.s2 : a.w2).w + ((int64_t)e * a.D + 32 * g) * c.K);
-    c.base1 = c.base0 + (uint64_t)c.K * 32;
+    c.live = true;
+#pragma unroll
+    for (int b = 0; b < BL; ++b)  // (rows past the last: the last ones again, not stored)
+      set_load<WT>(c, b, shared ? a.s2 : a.w2, e, a.D, c.K, min(row0 + b * LR, a.D - LR));
     return c;
   };
   const uint32_t shared_at = (uint32_t)S * (uint32_t)a.H * 2u;
-  auto src = [&](const Item& c, int i) {
+  auto src = [&](const Item<BL>& c, int i) {
     return c.start < 0 ? shared_at + (uint32_t)i * (uint32_t)a.Hs * 2u
-                       : (uint32_t)p.sorted[c.start + i] * (uint32_t)a.H * 2u;
+                       : (uint32_t)p.sorted(c.start + i) * (uint32_t)a.H * 2u;
   };
-  auto emit = [&](const Item& c, int r, int i, int quad, const floatx4_t& v0, const floatx4_t& v1) {
-    const int group = c.rb * R + r;
-    if (group >= a.D / 32) return;
-    const bool shared = c.start < 0;
-    const int slot = shared ? S + i : p.sorted[c.start + i];
-    const float sc = shared ? (a.gate ? p.gate[i] : 1.f) : p.score[c.start + i];
-    float* y = a.y + (int64_t)slot * a.D + 32 * group + 4 * quad;
-    store_agent(y, v0 * sc);
-    store_agent(y + 16, v1 * sc);
-  };
-  if (threadIdx.x == 0) nlast = 0;
-  stream_items<NB, NS>(ring, (floatx4_t*)(ring + ring_bytes<NB, NS>()), nitems, log_ks, (uint64_t)a.a, item_of, src,
-                       emit);
-  // Arrivals: the workgroup's sums are in memory (the stream ends waiting for its
-  // stores) before its items are counted; who brings a run of rows to its count
-  // reads the others' sums after that.
+  stream_items<WT, BL, NB, NS>(
+      ring, w >> log_ks, R, nsh + hit, ks, KS, (uint64_t)a.a, item_of, src,
+      [&](const Item<BL>& c, int c0, int rows, const floatx4_t (&acc)[MB][Rg::NT]) {
+#pragma unroll
+        for (int t = 0; t < Rg::NT; ++t) {
+          const int i = 16 * t + (l & 15);
+          if (i < rows) {
+            const int place = (c.start < 0 ? S : c.start) + c0 + i;
+#pragma unroll
+            for (int b = 0; b < MB; ++b) sums[((ks * places + place) * MB + b) * 4 + (l >> 4)] = acc[b][t];
+          }
+        }
+      });
   __syncthreads();
-  short* const last = (short*)ring;
-  const int all = hit + (nsh > 0);
-  if (all > 0) {
-    for (int i = threadIdx.x; i * (int)gridDim.x + (int)blockIdx.x < nitems; i += kThreads) {
-      const int it = i * gridDim.x + blockIdx.x, rb = it < nsh ? it : (it - nsh) % nrb;
-      if (__hip_atomic_fetch_add(a.count + rb, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1)
-        last[atomicAdd(&nlast, 1)] = (short)rb;
+  constexpr int quads = BL * LR / 4, room = 4 * MB;
+  for (int i = tid; i < a.T * quads; i += kThreads) {
+    const int t = i / quads, d = i % quads;
+    if (row0 + 4 * d >= a.D) continue;
+    auto row = [&](int place) {  // the KS shares in order
+      floatx4_t v = sums[place * room + d];
+      for (int j = 1; j < KS; ++j) v += sums[(j * places + place) * room + d];
+      return v;
+    };
+    const uint32_t ok = p.valid(t);
+    floatx4_t sum = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < a.K; k0 += 8) {
+      int place[8];
+      float sc[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const bool in = k0 + k < a.K && (ok >> (k0 + k) & 1);
+        place[k] = in ? p.inverse(t * a.K + k0 + k) : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sc[k] = a.before || place[k] < 0 ? 1.f : p.score(place[k]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (place[k] >= 0) sum += row(place[k]) * sc[k];
     }
-  } else {  // no expert at all: the rows are zeros
-    for (int rb = blockIdx.x + threadIdx.x * gridDim.x; rb < nrb; rb += kThreads * gridDim.x)
-      last[atomicAdd(&nlast, 1)] = (short)rb;
+    if (nsh) sum += row(S + t) * p.gate(t);
+    *(u32x2_t*)(a.out + (int64_t)t * a.D + row0 + 4 * d) =
+        u32x2_t{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
   }
-  __syncthreads();
-  for (int f = 0; f < nlast; ++f) sum_rows(a, p.valid, 32 * R * last[f], 32 * R, nsh > 0);
 }
 
 // z[t, e] = bf16(sum_d x[t, d] w[e, d]).  Products of bf16 pairs are exact in 64
@@ -923,7 +1103,7 @@ int row_bytes(int cap, int K, int log_ks, int unit) {
   return (int)std::min<int64_t>(kRowBytes, std::max(all, red));
 }
 
-hipError_t launch_experts_fp4(DecodeArgs a, hipStream_t stream) {
+hipError_t launch_experts_fp4_many(DecodeArgs a, hipStream_t stream) {
   constexpr int WT = W_FP4, U = kUnit<WT>;
   const int S = a.T * a.K, hit = std::min(a.E, S);
   const bool few = a.T <= 16;
@@ -952,30 +1132,111 @@ hipError_t launch_experts_fp4(DecodeArgs a, hipStream_t stream) {
   return launch_k(false, k2, grid, dim3(kThreads), lds2, stream, a);
 }
 
-template <int NB, int NS>
-hipError_t launch_bf16(DecodeArgs a, hipStream_t stream) {
-  constexpr uint32_t lds = kPlanBytes + ring_bytes<NB, NS>() + kMeetRows<NB> * kWaves * 128;
-  static_assert(lds + 1024 <= 160 * 1024, "LDS");
-  const int hit = std::min(a.E, a.T * a.K), G = num_cus();
-  a.ncount = a.D / 32;
-  auto k13 = decode_w13_bf16_kernel<NB, NS>;
-  auto k2 = decode_w2_bf16_kernel<NB, NS>;
-  // (one item per row pair at the finest)
-  hipError_t err = hipFuncSetAttribute((const void*)k13, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (err != hipSuccess) return err;
-  err = launch_k(false, k13, dim3(std::min<int64_t>((int64_t)hit * (a.H / 16) + a.Hs / 16, G)), dim3(kThreads), lds, stream, a);
-  if (err != hipSuccess) return err;
-  err = hipFuncSetAttribute((const void*)k2, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (err != hipSuccess) return err;
-  return launch_k(false, k2, dim3(std::min<int64_t>((int64_t)(hit + (a.Hs > 0)) * (a.D / 32), G)), dim3(kThreads), lds, stream, a);
+constexpr int kLds = 160 * 1024;
+
+hipError_t launch_lds(void (*kernel)(DecodeArgs), int64_t grid, int lds, hipStream_t stream, const DecodeArgs& a) {
+  if (lds > 64 * 1024) {
+    const hipError_t err = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (err != hipSuccess) return err;
+  }
+  return launch_k(false, kernel, dim3((unsigned)grid), dim3(kThreads), lds, stream, a);
 }
 
-// Token rows per pass, by the rows that an expert gets on average: a pass more
-// streams its weights again, a larger one takes LDS from the ring.
+template <int WT, int NB, int NS>
+bool stream_w13(const DecodeArgs& a, hipStream_t stream, hipError_t& err) {
+  const int lds = a.plan_lds + Ring<WT, kPairLoads<WT>, NB, NS>::kAll + kMeetRows * 1024;
+  if (lds > kLds) return false;
+  const int64_t pairs = (int64_t)std::min(a.E, a.T * a.K) * (a.H / 16) + a.Hs / 16;  // at the finest
+  err = launch_lds(stream_w13_kernel<WT, NB, NS>, std::min<int64_t>(pairs, num_cus()), lds, stream, a);
+  return true;
+}
+
+template <int WT, int BL, int NB, int NS>
+bool stream_w2(DecodeArgs a, hipStream_t stream, hipError_t& err) {
+  using Rg = Ring<WT, BL, NB, NS>;
+  const int base = a.plan_lds + Rg::kAll;
+  const int sums = (a.T * a.K + (a.Hs > 0 ? a.T : 0)) * Rg::kBlocks * 64;  // of one of KS shares
+  if (base + sums > kLds) return false;
+  a.log_ks = 0;
+  while (a.log_ks < 3 && base + (sums << (a.log_ks + 1)) <= kLds) ++a.log_ks;
+  err = launch_lds(stream_w2_kernel<WT, BL, NB, NS>, ceil_div(a.D, BL * (WT == W_BF16 ? 8 : 16)),
+                   base + (sums << a.log_ks), stream, a);
+  return true;
+}
+
+// bf16.  Token rows per pass by the rows that an expert gets on average: a pass
+// more streams its weights again, a larger one takes LDS from the ring.  The second
+// product takes as few output rows per workgroup as give one workgroup per CU at
+// most, where the slots' sums leave the room.
+template <int BL>
+bool w2_bf16(const DecodeArgs& a, int rows, hipStream_t stream, hipError_t& err) {
+  if (rows <= 4)
+    return stream_w2<W_BF16, BL, 1, BL == 1 ? 7 : BL == 2 ? 5 : 3>(a, stream, err) ||
+           stream_w2<W_BF16, BL, 1, BL == 1 ? 4 : BL == 2 ? 3 : 2>(a, stream, err);
+  if (rows <= 10)
+    return stream_w2<W_BF16, BL, 2, BL == 1 ? 5 : BL == 2 ? 4 : 2>(a, stream, err) ||
+           stream_w2<W_BF16, BL, 2, 2>(a, stream, err);
+  return BL <= 2 && stream_w2<W_BF16, BL, 4, 2>(a, stream, err);
+}
+
 hipError_t launch_experts_bf16(const DecodeArgs& a, hipStream_t stream) {
-  const int most = a.Hs > 0 ? a.T : 0, rows = std::max(most, ceil_div(a.T * a.K, a.E));
-  if (a.T <= 8 || rows <= 4) return launch_bf16<1, 3>(a, stream);
-  return rows <= 10 ? launch_bf16<2, 3>(a, stream) : launch_bf16<4, 2>(a, stream);
+  const int rows = a.T <= 8 ? 1 : ceil_div(a.T * a.K, a.E);
+  hipError_t err = hipSuccess;
+  if (rows <= 4) stream_w13<W_BF16, 1, 3>(a, stream, err);
+  else if (rows <= 10) stream_w13<W_BF16, 2, 3>(a, stream, err) || stream_w13<W_BF16, 2, 2>(a, stream, err);
+  else stream_w13<W_BF16, 4, 2>(a, stream, err);
+  if (err != hipSuccess) return err;
+  const int loads = ceil_div(a.D, 8 * num_cus());
+  const bool ok = (loads <= 1 && w2_bf16<1>(a, rows, stream, err)) || (loads <= 2 && w2_bf16<2>(a, rows, stream, err)) ||
+                  (loads <= 3 && w2_bf16<3>(a, rows, stream, err)) || w2_bf16<4>(a, rows, stream, err) ||
+                  stream_w2<W_BF16, 2, 4, 2>(a, stream, err) || stream_w2<W_BF16, 2, 1, 2>(a, stream, err);
+  return ok ? err : hipErrorInvalidValue;
+}
+
+// 4 bits.  The token rows of a stage take as much LDS as its weights, so the
+// streams are for few rows; more share theirs between a workgroup's waves.
+hipError_t launch_experts_fp4(const DecodeArgs& a, hipStream_t stream) {
+  const int rows = a.T <= 4 ? 1 : ceil_div(a.T * a.K, a.E);
+  if (rows > 4 || (a.Hs > 0 && a.T > 16)) return launch_experts_fp4_many(a, stream);
+  hipError_t err = hipSuccess;
+  if (rows <= 1) stream_w13<W_FP4, 1, 4>(a, stream, err);
+  else stream_w13<W_FP4, 2, 3>(a, stream, err);
+  if (err != hipSuccess) return err;
+  const bool one = a.D / 16 <= num_cus();
+  bool ok;
+  if (rows <= 1)
+    ok = (one && stream_w2<W_FP4, 1, 1, 5>(a, stream, err)) || (!one && stream_w2<W_FP4, 2, 1, 4>(a, stream, err)) ||
+         stream_w2<W_FP4, 1, 2, 3>(a, stream, err);
+  else
+    ok = (!one && stream_w2<W_FP4, 2, 2, 3>(a, stream, err)) || stream_w2<W_FP4, 1, 2, 3>(a, stream, err);
+  return ok ? err : hipErrorInvalidValue;
+}
+
+template <int LPT, int PL>
+hipError_t go_plan(const PlanArgs& a, hipStream_t stream) {
+  auto kernel = a.K <= 8 ? decode_plan_kernel<LPT, PL, 8> : decode_plan_kernel<LPT, PL, 16>;
+  return launch_k(false, kernel, dim3(1), dim3(kPlanThreads), 0, stream, a);
+}
+
+// The selection and the plan.  A wave per token (16 at a time) while that is one
+// round, else 16 lanes (64 tokens at a time) where they can hold the experts.
+hipError_t launch_plan_topk(PlanArgs a, hipStream_t stream) {
+  select::GroupTopkArgs& t = a.topk;
+  int lr16 = 0, lr64 = 0;
+  const int p16 = select::experts_per_lane(16, t.G, t.EG, &lr16), p64 = select::experts_per_lane(64, t.G, t.EG, &lr64);
+  const bool narrow = p16 > 0 && p16 <= 16 && (p16 <= 4 || a.T > 16);
+  t.log_run = narrow ? lr16 : lr64;
+  t.per_lane = narrow ? p16 : p64;
+  if (narrow) {
+    if (p16 <= 4) return go_plan<16, 4>(a, stream);
+    if (p16 <= 8) return go_plan<16, 8>(a, stream);
+    if (p16 <= 12) return go_plan<16, 12>(a, stream);
+    return go_plan<16, 16>(a, stream);
+  }
+  if (p64 <= 4) return go_plan<64, 4>(a, stream);
+  if (p64 <= 8) return go_plan<64, 8>(a, stream);
+  if (p64 <= 16) return go_plan<64, 16>(a, stream);
+  return go_plan<64, 32>(a, stream);  // E <= 1024, G <= 64: at most 32 per lane
 }
 
 size_t al256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -984,30 +1245,35 @@ size_t al256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 size_t router_decode_workspace_bytes(int64_t T, int E) { return al256((size_t)T * E * 2); }
 
-hipError_t launch_router_decode(const void* x, const void* w_router, const void* w_gate, const float* bias, int T, int E,
-                                int D, int K, const RouterGroups& groups, int score_func, int renorm, float renorm_eps,
-                                float route_scale, float* top_scores, int64_t* top_idx, float* gate, void* logits,
-                                hipStream_t stream) {
-  const int rows = E + (w_gate != nullptr);
+namespace {
+
+hipError_t launch_logits(const RouterDecode& r, int T, int E, int D, hipStream_t stream) {
+  const int rows = E + (r.w_gate != nullptr);
   const int tb = T >= 4 ? 4 : T >= 2 ? 2 : 1;
   const dim3 grid(ceil_div(rows, 4), ceil_div(T, tb));
   auto kernel = tb == 4 ? router_logits_kernel<4> : tb == 2 ? router_logits_kernel<2> : router_logits_kernel<1>;
-  hipError_t err = launch_k(false, kernel, grid, dim3(256), 0, stream, (const bf16_t*)x, (const bf16_t*)w_router,
-                            (const bf16_t*)w_gate, T, E, D, (bf16_t*)logits, gate);
-  if (err != hipSuccess) return err;
-  return launch_router_topk_grouped(logits, true, bias, T, E, K, groups, score_func, renorm, renorm_eps, route_scale,
-                                    top_scores, top_idx, stream);
+  return launch_k(false, kernel, grid, dim3(256), 0, stream, (const bf16_t*)r.x, (const bf16_t*)r.w_router,
+                  (const bf16_t*)r.w_gate, T, E, D, (bf16_t*)r.logits, r.gate);
 }
 
-// Workspace: activations of the slots and of the shared expert, their fp32 output
-// rows, arrival counters.
+}  // namespace
+
+hipError_t launch_router_decode(const RouterDecode& r, int T, int E, int D, int K, hipStream_t stream) {
+  const hipError_t err = launch_logits(r, T, E, D, stream);
+  if (err != hipSuccess) return err;
+  return launch_router_topk_grouped(r.logits, true, r.bias, T, E, K, r.groups, r.score_func, r.renorm, r.eps, r.scale,
+                                    r.top_scores, r.top_idx, stream);
+}
+
+// Workspace: the plan, activations of the slots and of the shared expert, their
+// fp32 output rows, arrival counters.
 size_t experts_decode_workspace_bytes(int64_t T, int64_t D, int64_t H, int K, int64_t Hs) {
   const int64_t S = T * K;
-  return al256((size_t)(S * H + (Hs > 0 ? T * Hs : 0)) * 2) + al256((size_t)(S + (Hs > 0 ? T : 0)) * D * 4) +
-         al256((size_t)(D / 32) * 4);
+  return al256(PlanMap{(int)T, (int)S}.bytes()) + al256((size_t)(S * H + (Hs > 0 ? T * Hs : 0)) * 2) +
+         al256((size_t)(S + (Hs > 0 ? T : 0)) * D * 4) + al256((size_t)(D / 32) * 4);
 }
 
-hipError_t launch_experts_decode(const ExpertsDecode& c, void* ws, hipStream_t stream) {
+hipError_t launch_experts_decode(const ExpertsDecode& c, const RouterDecode* router, void* ws, hipStream_t stream) {
   DecodeArgs a{};
   a.T = c.T, a.D = c.D, a.H = c.H, a.E = c.E, a.K = c.K, a.Hs = c.Hs;
   a.x = (const bf16_t*)c.x;
@@ -1015,13 +1281,39 @@ hipError_t launch_experts_decode(const ExpertsDecode& c, void* ws, hipStream_t s
   a.scores = c.scores, a.limit = c.limit, a.gate = c.gate;
   a.w13 = {c.w13, c.e13}, a.w2 = {c.w2, c.e2}, a.s13 = {c.s13, c.es13}, a.s2 = {c.s2, c.es2};
   const int64_t S = (int64_t)a.T * a.K, Ts = a.Hs > 0 ? a.T : 0;
+  const PlanMap map{a.T, (int)S};
   char* p = (char*)ws;
+  a.plan = p;
+  a.plan_lds = (map.bytes() + 127) & ~127;
+  p += al256(map.bytes());
   a.a = (bf16_t*)p;
   p += al256((size_t)(S * a.H + Ts * a.Hs) * 2);
   a.y = (float*)p;
   p += al256((size_t)(S + Ts) * a.D * 4);
   a.count = (int*)p;
   a.out = (bf16_t*)c.out;
+
+  PlanArgs pa{};
+  pa.idx = c.idx, pa.is64 = c.is64, pa.scores = c.scores, pa.gate = c.gate;
+  pa.T = a.T, pa.E = a.E, pa.K = a.K, pa.plan = (char*)ws;
+  pa.count = a.count, pa.ncount = a.D / 32;
+  hipError_t err;
+  if (router) {
+    err = launch_logits(*router, a.T, a.E, a.D, stream);
+    if (err != hipSuccess) return err;
+    select::GroupTopkArgs& t = pa.topk;
+    t.z = router->logits;
+    t.S = 1, t.T = a.T, t.E = a.E, t.K = a.K;
+    t.aligned = ((uintptr_t)router->logits & 15) == 0;
+    t.G = router->groups.groups, t.EG = a.E / t.G, t.kept = router->groups.kept, t.top2 = router->groups.top2;
+    t.bias = router->bias;
+    t.score_func = router->score_func, t.renorm = router->renorm, t.eps = router->eps, t.route_scale = router->scale;
+    t.scores = router->top_scores, t.idx = router->top_idx;
+    err = launch_plan_topk(pa, stream);
+  } else {
+    err = go_plan<0, 4>(pa, stream);
+  }
+  if (err != hipSuccess) return err;
   return c.fp4 ? launch_experts_fp4(a, stream) : launch_experts_bf16(a, stream);
 }
 

@@ -213,12 +213,19 @@ hipError_t launch_unpack_fp4(const void* codes, const void* exps, int64_t E, int
 constexpr int kDecodeMaxTokens = 64;
 constexpr int kDecodeMaxTopk = 16;
 size_t router_decode_workspace_bytes(int64_t T, int E);
-// logits: router_decode_workspace_bytes; w_gate (nullable): gate[t] = sigmoid of
-// the token's product with it.
-hipError_t launch_router_decode(const void* x, const void* w_router, const void* w_gate, const float* bias, int T, int E,
-                                int D, int K, const RouterGroups& groups, int score_func, int renorm, float renorm_eps,
-                                float route_scale, float* top_scores, int64_t* top_idx, float* gate, void* logits,
-                                hipStream_t stream);
+struct RouterDecode {
+  const void *x, *w_router;
+  const void* w_gate;  // nullable: gate[t] = sigmoid of the token's product with it
+  const float* bias;
+  RouterGroups groups;
+  int score_func, renorm;
+  float eps, scale;
+  float* top_scores;
+  int64_t* top_idx;
+  float* gate;
+  void* logits;        // router_decode_workspace_bytes
+};
+hipError_t launch_router_decode(const RouterDecode& r, int T, int E, int D, int K, hipStream_t stream);
 struct ExpertsDecode {
   int T, D, H, E, K, Hs;
   const void* x;
@@ -232,7 +239,8 @@ struct ExpertsDecode {
   void* out;
 };
 size_t experts_decode_workspace_bytes(int64_t T, int64_t D, int64_t H, int K, int64_t Hs);
-hipError_t launch_experts_decode(const ExpertsDecode& c, void* ws, hipStream_t stream);
+// router (nullable): its picks are made first (c.idx, c.scores and c.gate are its outputs).
+hipError_t launch_experts_decode(const ExpertsDecode& c, const RouterDecode* router, void* ws, hipStream_t stream);
 hipError_t launch_grouped_mm_fp4(const void* x, const void* codes, const void* exps, const int* offs, const void* bias,
                                  bool bias32, int M, int E, int N, int K, void* out, hipStream_t stream);
 
