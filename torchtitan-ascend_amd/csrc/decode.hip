@@ -1082,6 +1082,17 @@ __global__ __launch_bounds__(kThreads, 4) void grouped_mm_fp4_kernel(const Fp4Ar
   stream_rows<W_FP4, NT>(pair, live, a.K, cnt, a.cap, a.log_ks, smem, a.smem_rows, first, a.cap * gridDim.y, src, emit);
 }
 
+constexpr int kLds = 160 * 1024;
+
+// MOST: the kernel's largest dynamic LDS (its static LDS beside it).
+template <auto KERNEL, int MOST = kLds, class Args>
+hipError_t launch_lds(dim3 grid, int lds, hipStream_t stream, const Args& a) {
+  static const hipError_t attr_err =
+      hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, MOST);
+  if (attr_err != hipSuccess) return attr_err;
+  return launch_k(false, KERNEL, grid, dim3(kThreads), lds, stream, a);
+}
+
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Waves that share a row pair (log2): as many as bring the launch to two
@@ -1116,30 +1127,16 @@ hipError_t launch_experts_fp4_many(DecodeArgs a, hipStream_t stream) {
   const int R2 = kWaves >> log_ks2, nrb2 = ceil_div(a.D / 32, R2);
   a.ncount = nrb2;
   dim3 grid(ceil_div(a.Hs / 16, R) + hit * ceil_div(a.H / 16, R));
-  auto k13 = few ? decode_w13_kernel<WT, 1> : decode_w13_kernel<WT, 4>;
   const uint32_t lds13 = sizeof(Labels) + a.smem_rows;
-  hipError_t err = hipFuncSetAttribute((const void*)k13, hipFuncAttributeMaxDynamicSharedMemorySize, lds13);
-  if (err != hipSuccess) return err;
-  err = launch_k(false, k13, grid, dim3(kThreads), lds13, stream, a);
+  hipError_t err = few ? launch_lds<decode_w13_kernel<WT, 1>>(grid, lds13, stream, a)
+                       : launch_lds<decode_w13_kernel<WT, 4>>(grid, lds13, stream, a);
   if (err != hipSuccess) return err;
   a.log_ks = log_ks2;
   a.smem_rows = row_bytes(a.cap, std::max(a.H, a.Hs), log_ks2, U);
   grid = dim3(((a.Hs > 0) + hit) * nrb2);
-  auto k2 = few ? decode_w2_kernel<WT, 1> : decode_w2_kernel<WT, 4>;
   const uint32_t lds2 = sizeof(Labels) + a.smem_rows;
-  err = hipFuncSetAttribute((const void*)k2, hipFuncAttributeMaxDynamicSharedMemorySize, lds2);
-  if (err != hipSuccess) return err;
-  return launch_k(false, k2, grid, dim3(kThreads), lds2, stream, a);
-}
-
-constexpr int kLds = 160 * 1024;
-
-hipError_t launch_lds(void (*kernel)(DecodeArgs), int64_t grid, int lds, hipStream_t stream, const DecodeArgs& a) {
-  if (lds > 64 * 1024) {
-    const hipError_t err = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (err != hipSuccess) return err;
-  }
-  return launch_k(false, kernel, dim3((unsigned)grid), dim3(kThreads), lds, stream, a);
+  return few ? launch_lds<decode_w2_kernel<WT, 1>, kLds / 2>(grid, lds2, stream, a)
+             : launch_lds<decode_w2_kernel<WT, 4>, kLds / 2>(grid, lds2, stream, a);
 }
 
 template <int WT, int NB, int NS>
@@ -1147,7 +1144,7 @@ bool stream_w13(const DecodeArgs& a, hipStream_t stream, hipError_t& err) {
   const int lds = a.plan_lds + Ring<WT, kPairLoads<WT>, NB, NS>::kAll + kMeetRows * 1024;
   if (lds > kLds) return false;
   const int64_t pairs = (int64_t)std::min(a.E, a.T * a.K) * (a.H / 16) + a.Hs / 16;  // at the finest
-  err = launch_lds(stream_w13_kernel<WT, NB, NS>, std::min<int64_t>(pairs, num_cus()), lds, stream, a);
+  err = launch_lds<stream_w13_kernel<WT, NB, NS>>(dim3((unsigned)std::min<int64_t>(pairs, num_cus())), lds, stream, a);
   return true;
 }
 
@@ -1159,8 +1156,8 @@ bool stream_w2(DecodeArgs a, hipStream_t stream, hipError_t& err) {
   if (base + sums > kLds) return false;
   a.log_ks = 0;
   while (a.log_ks < 3 && base + (sums << (a.log_ks + 1)) <= kLds) ++a.log_ks;
-  err = launch_lds(stream_w2_kernel<WT, BL, NB, NS>, ceil_div(a.D, BL * (WT == W_BF16 ? 8 : 16)),
-                   base + (sums << a.log_ks), stream, a);
+  err = launch_lds<stream_w2_kernel<WT, BL, NB, NS>>(dim3(ceil_div(a.D, BL * (WT == W_BF16 ? 8 : 16))),
+                                                     base + (sums << a.log_ks), stream, a);
   return true;
 }
 
@@ -1327,12 +1324,9 @@ hipError_t launch_grouped_mm_fp4(const void* x, const void* codes, const void* e
   const int pairs = ceil_div(ceil_div(N, 16), 2), tiles = std::min(ceil_div(M, a.cap), 1024);
   a.log_ks = pick_log_ks((int64_t)pairs * (offs ? std::min(E, M) : tiles), K, kUnit<W_FP4>, a.cap);
   a.smem_rows = row_bytes(a.cap, K, a.log_ks, kUnit<W_FP4>);
-  auto kernel = few ? grouped_mm_fp4_kernel<1> : grouped_mm_fp4_kernel<4>;
-  const hipError_t err =
-      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, a.smem_rows);
-  if (err != hipSuccess) return err;
   const dim3 grid(E * ceil_div(pairs, kWaves >> a.log_ks), offs ? std::min(tiles, 8) : tiles);
-  return launch_k(false, kernel, grid, dim3(kThreads), a.smem_rows, stream, a);
+  return few ? launch_lds<grouped_mm_fp4_kernel<1>>(grid, a.smem_rows, stream, a)
+             : launch_lds<grouped_mm_fp4_kernel<4>>(grid, a.smem_rows, stream, a);
 }
 
 }  // namespace ttamd

@@ -20,9 +20,10 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, ops
-from .ops import _call, _gpu, _groups, _limit, _p, _same_device, _stream, _want, _ws
+from .ops import _call, _gpu, _groups, _limit, _p, _same_device, _stream, _want
 
 _BF16 = torch.bfloat16
+_U8 = torch.uint8
 MAX_TOKENS = 64
 
 
@@ -38,8 +39,10 @@ class PackedWeights(NamedTuple):
 
 
 def _no_grad(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} is for inference (it has no backward); call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and getattr(t, "requires_grad", False):
+                raise RuntimeError(f"{name} is for inference (it has no backward); call it under torch.no_grad()")
 
 
 def _shapes(E: int, N: int, K: int) -> tuple[tuple, tuple]:
@@ -47,15 +50,21 @@ def _shapes(E: int, N: int, K: int) -> tuple[tuple, tuple]:
     return (E, nb, nc, 64, 16), (E, nb, (nc + 3) // 4, 64, 4)
 
 
-def _packed(name: str, w: PackedWeights, dev: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
-    codes = _want(f"{name}.codes", w.codes, torch.uint8)
-    exps = _want(f"{name}.exponents", w.exponents, torch.uint8)
-    _same_device(dev, **{f"{name}.codes": codes, f"{name}.exponents": exps})
-    if w.rows < 1 or w.cols < 1 or codes.dim() != 5 or \
-            (tuple(codes.shape), tuple(exps.shape)) != _shapes(codes.shape[0], w.rows, w.cols):
+# (device and dtype comparisons written out here and below: a call on one token is
+# bound by the host, and keyword helpers take half a microsecond each)
+def _packed(name: str, w: PackedWeights, dev: torch.device) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """(codes, exponents, E) of packed weights, checked."""
+    codes, exps, N, K = w
+    if codes.dtype is not _U8 or exps.dtype is not _U8:
+        raise TypeError(f"{name}: codes and exponents must be uint8, got {codes.dtype} and {exps.dtype}")
+    if codes.device != dev or exps.device != dev:
+        raise RuntimeError(f"{name} is on {codes.device} and {exps.device}, expected {dev}")
+    E = codes.shape[0] if codes.dim() == 5 else 0
+    nb, nc = (N + 15) // 16, (K + 127) // 128
+    if N < 1 or K < 1 or codes.shape != (E, nb, nc, 64, 16) or exps.shape != (E, nb, (nc + 3) // 4, 64, 4):
         raise ValueError(f"{name}: codes {tuple(codes.shape)} and exponents {tuple(exps.shape)} are not those of "
-                         f"[E, {w.rows}, {w.cols}] weights")
-    return codes, exps
+                         f"[E, {N}, {K}] weights")
+    return codes.contiguous(), exps.contiguous(), E
 
 
 def pack_e2m1(w: torch.Tensor) -> PackedWeights:
@@ -82,8 +91,7 @@ def unpack_e2m1(w: PackedWeights) -> torch.Tensor:
     """The bf16 values [E, N, K] of packed weights, exactly (ttamd_unpack_e2m1):
     for prompts, whose rows fill the grouped GEMMs."""
     dev = _gpu("w.codes", w.codes)
-    codes, exps = _packed("w", w, dev)
-    E = codes.shape[0]
+    codes, exps, E = _packed("w", w, dev)
     out = torch.empty(E, w.rows, w.cols, dtype=_BF16, device=dev)
     _call(dev, "ttamd_unpack_e2m1", _p(codes), _p(exps), E, w.rows, w.cols, _p(out), _stream(dev))
     return out
@@ -125,13 +133,15 @@ def grouped_mm_e2m1(
     dev = _gpu("x", x)
     _no_grad("grouped_mm_e2m1", x, bias)
     x = _want("x", x, _BF16)
-    codes, exps = _packed("w", w, dev)
-    E = codes.shape[0]
-    if x.shape[-1] != w.cols or (offs is not None and x.dim() != 2):
-        raise ValueError(f"x must be [M, {w.cols}], got {tuple(x.shape)}")
-    if offs is None and E != 1:
-        raise ValueError(f"w holds {E} matrices: give offs")
-    if offs is not None:
+    codes, exps, E = _packed("w", w, dev)
+    N, K = w.rows, w.cols
+    shape = x.shape
+    if shape[-1] != K or (offs is not None and len(shape) != 2):
+        raise ValueError(f"x must be [M, {K}], got {tuple(shape)}")
+    if offs is None:
+        if E != 1:
+            raise ValueError(f"w holds {E} matrices: give offs")
+    else:
         _same_device(dev, offs=offs)
         offs = _want("offs", offs, torch.int32)
         if offs.numel() != E:
@@ -140,12 +150,12 @@ def grouped_mm_e2m1(
             raise ValueError("bias is for a call without offs")
     if bias is not None:
         _same_device(dev, bias=bias)
-        if bias.dtype not in (_BF16, torch.float32) or bias.numel() != w.rows:
-            raise ValueError(f"bias must be [{w.rows}], bfloat16 or float32")
+        if bias.dtype not in (_BF16, torch.float32) or bias.numel() != N:
+            raise ValueError(f"bias must be [{N}], bfloat16 or float32")
         bias = bias.contiguous()
-    out = torch.empty(*x.shape[:-1], w.rows, dtype=_BF16, device=dev)
-    _call(dev, "ttamd_grouped_mm_e2m1", _p(x), _p(codes), _p(exps), _p(offs), _p(bias),
-          int(bias is not None and bias.dtype == torch.float32), x.numel() // w.cols, E, w.rows, w.cols, _p(out),
+    out = torch.empty((*shape[:-1], N), dtype=_BF16, device=dev)
+    _call(dev, "ttamd_grouped_mm_e2m1", x.data_ptr(), codes.data_ptr(), exps.data_ptr(), _p(offs), _p(bias),
+          1 if bias is not None and bias.dtype is torch.float32 else 0, x.numel() // K, E, N, K, out.data_ptr(),
           _stream(dev))
     return out
 
@@ -181,38 +191,43 @@ def _gate_row(shared_gate: torch.Tensor | None, D: int, dev: torch.device) -> to
 def _weight(name: str, w, dev: torch.device) -> tuple[torch.Tensor, torch.Tensor | None, tuple]:
     """(tensor, exponents or None, (E, N, K)) of bf16 [E, N, K] / [N, K] or packed weights."""
     if isinstance(w, PackedWeights):
-        codes, exps = _packed(name, w, dev)
-        return codes, exps, (codes.shape[0], w.rows, w.cols)
-    _gpu(name, w)
+        codes, exps, E = _packed(name, w, dev)
+        return codes, exps, (E, w.rows, w.cols)
+    if w.device != dev:
+        _gpu(name, w)
+        raise RuntimeError(f"{name} is on {w.device}, expected {dev}")
     w = _want(name, w, _BF16)
-    _same_device(dev, **{name: w})
-    if w.dim() not in (2, 3):
-        raise ValueError(f"{name} must be [E, N, K], got {tuple(w.shape)}")
-    return w, None, (w.shape[0] if w.dim() == 3 else 1, *w.shape[-2:])
+    shape = w.shape
+    if len(shape) == 3:
+        return w, None, shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} must be [E, N, K], got {tuple(shape)}")
+    return w, None, (1, *shape)
 
 
 def _experts(w13, w2, shared_w13, shared_w2, D: int, dev: torch.device):
-    """(E, H, Hs, the eight weight tensors) of the layer's weights, checked."""
+    """(E, H, Hs, the data pointers of the eight weight tensors, the tensors) of the layer's weights, checked."""
     t13, e13, s13 = _weight("w13", w13, dev)
     t2, e2, s2 = _weight("w2", w2, dev)
     E, H = s13[0], s13[1] // 2
-    if s13[2] != D or s13[1] % 2 or s2 != (E, D, H):
-        raise ValueError(f"w13 must be [E, 2H, {D}] and w2 [E, {D}, H]; got {s13}, {s2}")
+    if s13[2] != D or s13[1] % 2 or tuple(s2) != (E, D, H):
+        raise ValueError(f"w13 must be [E, 2H, {D}] and w2 [E, {D}, H]; got {tuple(s13)}, {tuple(s2)}")
     if (e13 is None) != (e2 is None):
         raise TypeError("w13 and w2 must both be bfloat16 or both packed")
-    if (shared_w13 is None) != (shared_w2 is None):
+    keep = (t13, e13, t2, e2)
+    if shared_w13 is None and shared_w2 is None:
+        return E, H, 0, (t13.data_ptr(), _p(e13), t2.data_ptr(), _p(e2)), (None, None, None, None), keep
+    if shared_w13 is None or shared_w2 is None:
         raise ValueError("give shared_w13 and shared_w2 together")
-    Hs, shared = 0, (None, None, None, None)
-    if shared_w13 is not None:
-        u13, f13, z13 = _weight("shared_w13", shared_w13, dev)
-        u2, f2, z2 = _weight("shared_w2", shared_w2, dev)
-        Hs = z13[1] // 2
-        if z13[0] != 1 or z13[2] != D or z13[1] % 2 or z2 != (1, D, Hs):
-            raise ValueError(f"shared_w13 must be [2Hs, {D}] and shared_w2 [{D}, Hs]; got {z13}, {z2}")
-        if (f13 is None) != (e13 is None) or (f2 is None) != (e13 is None):
-            raise TypeError("the shared expert's weights must be of the experts' type")
-        shared = (u13, f13, u2, f2)
-    return E, H, Hs, (t13, e13, t2, e2), shared
+    u13, f13, z13 = _weight("shared_w13", shared_w13, dev)
+    u2, f2, z2 = _weight("shared_w2", shared_w2, dev)
+    Hs = z13[1] // 2
+    if z13[0] != 1 or z13[2] != D or z13[1] % 2 or tuple(z2) != (1, D, Hs):
+        raise ValueError(f"shared_w13 must be [2Hs, {D}] and shared_w2 [{D}, Hs]; got {tuple(z13)}, {tuple(z2)}")
+    if (f13 is None) != (e13 is None) or (f2 is None) != (e13 is None):
+        raise TypeError("the shared expert's weights must be of the experts' type")
+    return (E, H, Hs, (t13.data_ptr(), _p(e13), t2.data_ptr(), _p(e2)),
+            (u13.data_ptr(), _p(f13), u2.data_ptr(), _p(f2)), (*keep, u13, f13, u2, f2))
 
 
 def router_decode(
@@ -251,7 +266,7 @@ def router_decode(
     scores = torch.empty(T, top_k, dtype=torch.float32, device=dev)
     idx = torch.empty(T, top_k, dtype=torch.int64, device=dev)
     gate = None if shared_gate is None else torch.empty(T, dtype=torch.float32, device=dev)
-    ws = _ws(_lib.load().ttamd_router_decode_workspace_bytes(T, E), dev)
+    ws = torch.empty(max(16, _lib.load().ttamd_router_decode_workspace_bytes(T, E)), dtype=_U8, device=dev)
     _call(dev, "ttamd_router_decode", _p(x), _p(w_router), _p(expert_bias), _p(shared_gate), T, E, D, top_k, *groups,
           ops._SCORE_FUNCS[score_func], int(bool(route_norm)), float(norm_eps), float(route_scale), _p(scores), _p(idx),
           _p(gate), _p(ws), ws.numel(), _stream(dev))
@@ -287,16 +302,18 @@ def experts_decode(
     if idx.numel() != T * K or top_scores.numel() != T * K:
         raise ValueError(f"scores and indices must be [{T}, K], got {tuple(top_scores.shape)} and {tuple(idx.shape)}")
     idx, top_scores = idx.contiguous(), top_scores.float().contiguous()
-    E, H, Hs, weights, shared = _experts(w13, w2, shared_w13, shared_w2, D, dev)
+    E, H, Hs, weights, shared, _keep = _experts(w13, w2, shared_w13, shared_w2, D, dev)
     if shared_scale is not None:
         shared_scale = shared_scale.float().contiguous()
         if Hs == 0 or shared_scale.numel() != T:
             raise ValueError(f"shared_scale must be [{T}] and needs a shared expert")
-    out = torch.empty(T, D, dtype=_BF16, device=dev)
-    ws = _ws(_lib.load().ttamd_experts_decode_workspace_bytes(T, D, H, K, Hs), dev)
-    _call(dev, "ttamd_experts_decode", _p(x), T, D, H, E, K, _p(idx), int(idx.dtype == torch.int64), _p(top_scores),
-          int(bool(score_before_experts)), _limit(swiglu_limit), *map(_p, weights), Hs, *map(_p, shared),
-          _p(shared_scale), _p(out), _p(ws), ws.numel(), _stream(dev))
+    lib = _lib._lib or _lib.load()
+    out = torch.empty_like(x)
+    ws = torch.empty(lib.ttamd_experts_decode_workspace_bytes(T, D, H, K, Hs), dtype=_U8, device=dev)
+    _call(dev, "ttamd_experts_decode", x.data_ptr(), T, D, H, E, K, idx.data_ptr(),
+          1 if idx.dtype is torch.int64 else 0, top_scores.data_ptr(), 1 if score_before_experts else 0,
+          _limit(swiglu_limit), *weights, Hs, *shared, _p(shared_scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
+          _stream(dev))
     return out
 
 
@@ -328,25 +345,30 @@ def moe_decode(
     dev = _gpu("x", x)
     _no_grad("moe_decode", x, w_router, w13, w2, shared_w13, shared_w2, shared_gate)
     x = _rows(x)
-    w_router = _want("w_router", w_router, _BF16)
-    _same_device(dev, w_router=w_router)
     T, D = x.shape
-    E, H, Hs, weights, shared = _experts(w13, w2, shared_w13, shared_w2, D, dev)
-    if tuple(w_router.shape) != (E, D):
+    E, H, Hs, weights, shared, _keep = _experts(w13, w2, shared_w13, shared_w2, D, dev)
+    w_router = _want("w_router", w_router, _BF16)
+    if w_router.device != dev:
+        raise RuntimeError(f"w_router is on {w_router.device}, expected {dev}")
+    if w_router.shape != (E, D):
         raise ValueError(f"w_router must be [{E}, {D}] for these experts, got {tuple(w_router.shape)}")
-    if score_func not in ops._SCORE_FUNCS:
+    func = ops._SCORE_FUNCS.get(score_func)
+    if func is None:
         raise ValueError(f"score_func must be one of {sorted(ops._SCORE_FUNCS)}")
     groups = _groups(num_groups, topk_groups, group_score) or (1, 1, 0)
-    expert_bias = _bias(expert_bias, E, dev)
-    shared_gate = _gate_row(shared_gate, D, dev)
-    if shared_gate is not None and Hs == 0:
-        raise ValueError("shared_gate needs a shared expert")
-    scores = torch.empty(T, top_k, dtype=torch.float32, device=dev)
-    idx = torch.empty(T, top_k, dtype=torch.int64, device=dev)
-    out = torch.empty(T, D, dtype=_BF16, device=dev)
-    ws = _ws(_lib.load().ttamd_moe_decode_workspace_bytes(T, D, H, E, top_k, Hs), dev)
-    _call(dev, "ttamd_moe_decode", _p(x), T, D, H, E, top_k, _p(w_router), _p(expert_bias), *groups,
-          ops._SCORE_FUNCS[score_func], int(bool(route_norm)), float(norm_eps), float(route_scale),
-          int(bool(score_before_experts)), _limit(swiglu_limit), *map(_p, weights), Hs, *map(_p, shared),
-          _p(shared_gate), _p(scores), _p(idx), _p(out), _p(ws), ws.numel(), _stream(dev))
+    if expert_bias is not None:
+        expert_bias = _bias(expert_bias, E, dev)
+    if shared_gate is not None:
+        shared_gate = _gate_row(shared_gate, D, dev)
+        if Hs == 0:
+            raise ValueError("shared_gate needs a shared expert")
+    lib = _lib._lib or _lib.load()
+    scores = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    idx = torch.empty((T, top_k), dtype=torch.int64, device=dev)
+    out = torch.empty_like(x)
+    ws = torch.empty(lib.ttamd_moe_decode_workspace_bytes(T, D, H, E, top_k, Hs), dtype=_U8, device=dev)
+    _call(dev, "ttamd_moe_decode", x.data_ptr(), T, D, H, E, top_k, w_router.data_ptr(), _p(expert_bias), *groups,
+          func, 1 if route_norm else 0, norm_eps, route_scale, 1 if score_before_experts else 0, _limit(swiglu_limit),
+          *weights, Hs, *shared, _p(shared_gate), scores.data_ptr(), idx.data_ptr(), out.data_ptr(), ws.data_ptr(),
+          ws.numel(), _stream(dev))
     return out, scores, idx
