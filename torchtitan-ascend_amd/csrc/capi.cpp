@@ -1129,6 +1129,8 @@ int ttamd_grouped_mm_e2m1(const void* x, const void* codes, const void* exponent
   REQUIRE(num_experts >= 1 && num_experts <= 1024, "%s: num_experts must be in [1, 1024] (got %d)", fn, num_experts);
   REQUIRE(num_rows >= 0 && num_rows <= (1 << 28), "%s: num_rows out of range (%lld)", fn, (long long)num_rows);
   TRY(check_fp4(fn, num_experts, n, k));
+  REQUIRE((num_rows / 16 + num_experts) * (n / 32 + 1) <= (int64_t(1) << 30), "%s: too many outputs (%lld x %lld)", fn,
+          (long long)num_rows, (long long)n);
   REQUIRE(offs || num_experts == 1, "%s: offs is null with %d experts", fn, num_experts);
   REQUIRE(!offs || !bias, "%s: bias is for a call without offs", fn);
   if (num_rows == 0) return TTAMD_OK;
@@ -1172,7 +1174,7 @@ size_t ttamd_experts_decode_workspace_bytes(int64_t num_tokens, int64_t dim, int
   if (num_tokens < 0 || num_tokens > ttamd::kDecodeMaxTokens || dim < 1 || hidden < 1 || topk < 1 ||
       topk > ttamd::kDecodeMaxTopk || shared_hidden < 0)
     return 0;
-  return ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden);
+  return ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden, true);
 }
 
 int ttamd_experts_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts, int topk,
@@ -1193,7 +1195,7 @@ int ttamd_experts_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t
   TRY(check_ptr16(fn, "out", out));
   REQUIRE(indices && top_scores, "%s: null pointer argument", fn);
   TRY(check_ws(fn, workspace, workspace_bytes,
-               ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden)));
+               ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden, true)));
   return check_hip(ttamd::launch_experts_decode(decode_args(w, x, num_tokens, dim, hidden, num_experts, topk,
                                                             shared_hidden, indices, indices_are_int64 != 0, top_scores,
                                                             score_before, swiglu_limit, shared_gate, out),
@@ -1207,7 +1209,7 @@ size_t ttamd_moe_decode_workspace_bytes(int64_t num_tokens, int64_t dim, int64_t
       topk < 1 || topk > ttamd::kDecodeMaxTopk || shared_hidden < 0)
     return 0;
   return align256((size_t)num_tokens * 4) + ttamd::router_decode_workspace_bytes(num_tokens, num_experts) +
-         ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden);
+         ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden, true);
 }
 
 int ttamd_moe_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts, int topk,

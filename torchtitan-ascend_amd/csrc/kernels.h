@@ -209,7 +209,7 @@ hipError_t launch_pack_fp4(const void* in, bool f32, int64_t E, int N, int K, vo
 hipError_t launch_unpack_fp4(const void* codes, const void* exps, int64_t E, int N, int K, void* out,
                              hipStream_t stream);
 
-// The layer for a few tokens, products with 4-bit weights (decode.hip).
+// The layer for a few tokens (decode.hip), products with 4-bit weights (fp4_mm.hip).
 constexpr int kDecodeMaxTokens = 64;
 constexpr int kDecodeMaxTopk = 16;
 size_t router_decode_workspace_bytes(int64_t T, int E);
@@ -238,7 +238,7 @@ struct ExpertsDecode {
   const float* gate;
   void* out;
 };
-size_t experts_decode_workspace_bytes(int64_t T, int64_t D, int64_t H, int K, int64_t Hs);
+size_t experts_decode_workspace_bytes(int64_t T, int64_t D, int64_t H, int K, int64_t Hs, bool fp4);
 // router (nullable): its picks are made first (c.idx, c.scores and c.gate are its outputs).
 hipError_t launch_experts_decode(const ExpertsDecode& c, const RouterDecode* router, void* ws, hipStream_t stream);
 hipError_t launch_grouped_mm_fp4(const void* x, const void* codes, const void* exps, const int* offs, const void* bias,
