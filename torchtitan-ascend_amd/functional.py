@@ -18,14 +18,17 @@ plus the reference's own NPUMoeTokenUnpermute (npu_permute.py:15-53), the
 norms around the block (models/common/npu_rmsnorm.py:15-37) and `moe_block`,
 the whole of them.
 `moe_experts_forward` chains them; without autograd it takes the fused
-inference op (one C-ABI call for the whole expert stage).
+inference op (one C-ABI call for the whole expert stage).  `moe_decode` is a
+serving step's layer, `experts_decode` its expert stage for a few tokens.
 """
 from __future__ import annotations
 
 import torch
 
+from . import decode
 from . import library  # noqa: F401  (registers the ttamd::* ops)
 from . import ops
+from .decode import PackedWeights
 
 _BF16 = torch.bfloat16
 _T = torch.ops.ttamd
@@ -297,6 +300,96 @@ def moe_experts_forward(
     y = experts(routed, w13, w2, offs, swiglu_limit)
     out = combine(y, scores_flat, sorted_idx, inverse, K, not score_before_experts)
     return out.to(x.dtype)
+
+
+def _tensors(w) -> tuple:
+    """(weights or codes, exponents or None) of weights in either form, or of None."""
+    return (w.codes, w.exponents) if isinstance(w, PackedWeights) else (w, None)
+
+
+def _bf16_weights(w):
+    return decode.unpack_e2m1(w) if isinstance(w, PackedWeights) else w
+
+
+def _hidden(w13) -> int:
+    return 0 if w13 is None else (w13.rows if isinstance(w13, PackedWeights) else w13.shape[-2]) // 2
+
+
+def experts_decode(
+    x: torch.Tensor,
+    top_scores: torch.Tensor,
+    selected_experts_indices: torch.Tensor,
+    w13: torch.Tensor | PackedWeights,
+    w2: torch.Tensor | PackedWeights,
+    score_before_experts: bool = False,
+    swiglu_limit: float | None = None,
+    shared_w13: torch.Tensor | PackedWeights | None = None,
+    shared_w2: torch.Tensor | PackedWeights | None = None,
+    shared_scale: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """decode.experts_decode; under torch.compile as the op ttamd::experts_decode
+    (whose dispatch costs a call on one token more than its kernels take)."""
+    if not torch.compiler.is_compiling():
+        return decode.experts_decode(x, top_scores, selected_experts_indices, w13, w2, score_before_experts,
+                                     swiglu_limit, shared_w13, shared_w2, shared_scale)
+    (t13, e13), (t2, e2), (u13, f13), (u2, f2) = map(_tensors, (w13, w2, shared_w13, shared_w2))
+    return _T.experts_decode(x, top_scores, selected_experts_indices, t13, t2, _hidden(w13), score_before_experts,
+                             swiglu_limit, e13, e2, _hidden(shared_w13), u13, u2, f13, f2, shared_scale)
+
+
+def moe_decode(
+    x: torch.Tensor,
+    w_router: torch.Tensor,
+    w13: torch.Tensor | PackedWeights,
+    w2: torch.Tensor | PackedWeights,
+    top_k: int,
+    score_func: str = "softmax",
+    route_norm: bool = False,
+    route_scale: float = 1.0,
+    expert_bias: torch.Tensor | None = None,
+    norm_eps: float = 1e-20,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
+    score_before_experts: bool = False,
+    swiglu_limit: float | None = None,
+    shared_w13: torch.Tensor | PackedWeights | None = None,
+    shared_w2: torch.Tensor | PackedWeights | None = None,
+    shared_gate: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The MoE layer of a serving step on one GPU, for batches of any length: x bf16
+    [T, D] to (out bf16 [T, D], top_scores fp32 [T, K], selected_experts_indices
+    int64 [T, K]); arguments as decode.moe_decode.  At most 64 tokens stream the
+    weights (decode.moe_decode; under torch.compile ttamd::moe_decode); a prompt takes
+    the router, the grouped GEMMs and the shared expert's pass, 4-bit weights
+    restored to bf16 for the call (D % 128 == 0 and H % 128 == 0 there).  The two sum
+    a logit in other orders, so tokens whose experts nearly tie may pick others.  No
+    backward."""
+    decode._no_grad("moe_decode", x, w_router, w13, w2, shared_w13, shared_w2, shared_gate)
+    if x.dim() != 2 or x.dtype != _BF16:
+        raise TypeError(f"x must be bfloat16 [T, D], got {x.dtype} {tuple(x.shape)}")
+    if x.shape[0] > decode.MAX_TOKENS:
+        if (shared_w13 is None) != (shared_w2 is None):
+            raise ValueError("give shared_w13 and shared_w2 together")
+        if shared_gate is not None and shared_w13 is None:
+            raise ValueError("shared_gate needs a shared expert")
+        scores, idx = router(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps,
+                             num_groups, topk_groups, group_score)
+        out = moe_experts_forward(x, scores, idx, _bf16_weights(w13), _bf16_weights(w2), w_router.shape[0],
+                                  score_before_experts, swiglu_limit)
+        if shared_w13 is not None:
+            s13, s2 = (w.reshape(w.shape[-2:]) for w in map(_bf16_weights, (shared_w13, shared_w2)))
+            logits = None if shared_gate is None else x @ shared_gate.reshape(-1)
+            out = shared_expert_combine(out, x, s13, s2, logits, swiglu_limit)
+        return out, scores, idx
+    if not torch.compiler.is_compiling():
+        return decode.moe_decode(x, w_router, w13, w2, top_k, score_func, route_norm, route_scale, expert_bias,
+                                 norm_eps, num_groups, topk_groups, group_score, score_before_experts, swiglu_limit,
+                                 shared_w13, shared_w2, shared_gate)
+    (t13, e13), (t2, e2), (u13, f13), (u2, f2) = map(_tensors, (w13, w2, shared_w13, shared_w2))
+    return _T.moe_decode(x, w_router, t13, t2, top_k, _hidden(w13), score_func, route_norm, route_scale, expert_bias,
+                         norm_eps, num_groups, topk_groups, group_score, score_before_experts, swiglu_limit, e13, e2,
+                         _hidden(shared_w13), u13, u2, f13, f2, shared_gate)
 
 
 def moe_block(

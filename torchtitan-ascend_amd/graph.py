@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import torch
 
+from . import decode as _few
 from . import ops
 from .functional import moe_block
 
@@ -37,6 +38,9 @@ class MoELayerGraph:
     the block around the layer (functional.moe_block: norm, layer, norm, gate,
     residual sum, next norm; the gate is read in place too) and returns (u, n);
     x, the residual stream, is then bf16 or fp32.
+
+    With ``decode`` the step is decode.moe_decode (at most 64 tokens): its weights may
+    be packed in 4 bits, and it takes a shared expert.
     """
 
     def __init__(
@@ -64,15 +68,31 @@ class MoELayerGraph:
         next_weight: torch.Tensor | None = None,
         eps: float = 1e-6,
         residual: bool = False,
+        decode: bool = False,
+        shared_w13: torch.Tensor | _few.PackedWeights | None = None,
+        shared_w2: torch.Tensor | _few.PackedWeights | None = None,
+        shared_gate: torch.Tensor | None = None,
     ):
         block = residual or any(t is not None for t in (pre_weight, post_weight, gate, next_weight))
         if x.dim() != 2 or x.dtype != _BF16 and not (block and x.dtype == torch.float32):
             raise TypeError("x must be a bf16 [T, D] tensor, or an fp32 one with the block around the layer")
         if not block and (residual_scale != 1.0 or gate_func != "identity"):
             raise ValueError("residual_scale and gate_func need the block: residual=True, a norm weight or a gate")
-        for name, t in (("w_router", w_router), ("w13", w13), ("w2", w2)):
-            if t.dtype != _BF16 or not t.is_contiguous():
+        shared = (shared_w13, shared_w2, shared_gate)
+        if decode and block:
+            raise ValueError("decode is for the layer alone, without the block around it")
+        if not decode and any(t is not None for t in shared):
+            raise ValueError("a shared expert needs decode=True")
+        for name, t in zip(("w_router", "w13", "w2", "shared_w13", "shared_w2", "shared_gate"),
+                           (w_router, w13, w2, *shared)):
+            if isinstance(t, _few.PackedWeights):
+                if not decode:
+                    raise TypeError(f"{name}: 4-bit weights need decode=True")
+                if not (t.codes.is_contiguous() and t.exponents.is_contiguous()):
+                    raise TypeError(f"{name} must be contiguous (read in place by the graph)")
+            elif t is not None and (t.dtype != _BF16 or not t.is_contiguous()):
                 raise TypeError(f"{name} must be a contiguous bf16 tensor (read in place by the graph)")
+        self._shared = dict(zip(("shared_w13", "shared_w2", "shared_gate"), shared)) if decode else None
         self._args = (w_router, w13, w2, top_k, score_func, route_norm, score_before_experts, route_scale,
                       expert_bias, swiglu_limit)
         self._groups = dict(num_groups=num_groups, topk_groups=topk_groups, group_score=group_score)
@@ -98,6 +118,9 @@ class MoELayerGraph:
             return moe_block(x, w_router, w13, w2, top_k, score_func=func, route_norm=norm, route_scale=scale,
                              expert_bias=bias, score_before_experts=before, swiglu_limit=limit, **self._block,
                              **self._groups)
+        if self._shared is not None:
+            return _few.moe_decode(x, w_router, w13, w2, top_k, func, norm, scale, bias, score_before_experts=before,
+                                   swiglu_limit=limit, **self._groups, **self._shared)[0]
         _, _, r = ops.router_route(x, w_router, top_k, func, norm, scale, bias, with_inverse=False,
                                     **self._groups)
         return ops.experts_forward(x, r, w13, w2, top_k, before, limit)

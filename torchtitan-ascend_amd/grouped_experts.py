@@ -19,7 +19,8 @@ from typing import Any
 import torch
 from torch import nn
 
-from .functional import moe_experts_forward, run_experts_grouped_mm
+from . import decode
+from .functional import experts_decode, moe_experts_forward, run_experts_grouped_mm
 from .protocol import GroupedExperts, Module, ModelConfigConverter
 from .state_dict import upstream_to_fused
 from .token_dispatcher import HipTokenDispatcher
@@ -65,14 +66,23 @@ class HipGroupedExperts(Module):
         # (functional.moe_experts_forward, so with a local HipTokenDispatcher
         # only); None: in bf16
         activation_checkpoint: str | None = None
+        # how at most 64 tokens without autograd run on a local HipTokenDispatcher:
+        # "bf16": from the parameters (where they are bf16) through
+        # decode.experts_decode; "e2m1": through it from 4-bit copies, which
+        # pack_weights() makes; None: as every other batch
+        decode_weights: str | None = None
 
     def __init__(self, config: "HipGroupedExperts.Config"):
         super().__init__()
+        if config.decode_weights not in (None, "bf16", "e2m1"):
+            raise ValueError(f"decode_weights must be 'bf16', 'e2m1' or None, got {config.decode_weights!r}")
         if config.activation_checkpoint not in (None, "e4m3"):
             raise ValueError(f"activation_checkpoint must be 'e4m3' or None, got {config.activation_checkpoint!r}")
         self.num_experts = config.num_experts
         self.swiglu_limit = config.swiglu_limit
         self.activation_checkpoint = config.activation_checkpoint
+        self.decode_weights = config.decode_weights
+        self._packed = None  # (stamps of the parameters, packed w13, packed w2)
         E, D, H = config.num_experts, config.dim, config.hidden_dim
         self.w13 = nn.Parameter(torch.empty(E, 2 * H, D))
         self.w2 = nn.Parameter(torch.empty(E, D, H))
@@ -92,6 +102,35 @@ class HipGroupedExperts(Module):
                 "across the TP group; this build runs the experts of one GPU")
         return w13, w2
 
+    def _stamps(self):
+        # (an inference tensor counts no versions)
+        return tuple((p, None if p.is_inference() else p._version) for p in (self.w13, self.w2))
+
+    @torch.no_grad()
+    def pack_weights(self):
+        """Make the 4-bit copies that decode_weights="e2m1" runs a few tokens on
+        (17/64 of the bf16 parameters' memory more).  Call it again after the
+        parameters changed: forward refuses copies that are older than a change that
+        torch counts (not one through .data)."""
+        if self.decode_weights != "e2m1":
+            raise RuntimeError(f"pack_weights is for decode_weights='e2m1', not {self.decode_weights!r}")
+        w13, w2 = self._weights()
+        self._packed = (self._stamps(), decode.pack_e2m1(w13), decode.pack_e2m1(w2))
+
+    def _decode_weights(self):
+        """The weights that a few tokens stream, or None: the regular path."""
+        if self.decode_weights is None:
+            return None
+        if self.decode_weights == "bf16":
+            w13, w2 = self._weights()
+            return (w13, w2) if w13.dtype == w2.dtype == torch.bfloat16 else None
+        if self._packed is None:
+            raise RuntimeError("decode_weights='e2m1': call pack_weights() first")
+        stamps, w13, w2 = self._packed
+        if any(a is not b or v != u for (a, v), (b, u) in zip(stamps, self._stamps())):
+            raise RuntimeError("the parameters changed after pack_weights(); call it again")
+        return w13, w2
+
     def _experts_forward(self, x, num_tokens_per_expert):
         w13, w2 = self._weights()
         return run_experts_grouped_mm(w13, w2, x, num_tokens_per_expert, self.swiglu_limit)
@@ -104,6 +143,12 @@ class HipGroupedExperts(Module):
         selected_experts_indices = selected_experts_indices.view(bs * slen, top_k)
         disp = self.token_dispatcher
         if isinstance(disp, HipTokenDispatcher) and disp.is_local:
+            if self.decode_weights is not None and x.shape[0] <= decode.MAX_TOKENS and not torch.is_grad_enabled():
+                few = self._decode_weights()
+                if few is not None:
+                    out = experts_decode(x.to(torch.bfloat16), top_scores, selected_experts_indices, *few,
+                                         disp.score_before_experts, self.swiglu_limit)
+                    return out.to(x.dtype)
             w13, w2 = self._weights()
             return moe_experts_forward(
                 x, top_scores, selected_experts_indices, w13, w2, self.num_experts,
@@ -133,9 +178,11 @@ class HipGroupedExpertsConverter(ModelConfigConverter):
     class Config(ModelConfigConverter.Config):
         swiglu_limit: float | None = None
         activation_checkpoint: str | None = None
+        decode_weights: str | None = None
 
     def __init__(self, config: "HipGroupedExpertsConverter.Config"):
         self.config = config
+        self.decode_weights = config.decode_weights
         self.swiglu_limit = config.swiglu_limit
         self.activation_checkpoint = config.activation_checkpoint
 
@@ -149,6 +196,7 @@ class HipGroupedExpertsConverter(ModelConfigConverter):
                 token_dispatcher=cfg.token_dispatcher,
                 swiglu_limit=self.swiglu_limit,
                 activation_checkpoint=self.activation_checkpoint,
+                decode_weights=self.decode_weights,
             )
             for extra in ("param_init", "sharding_config"):
                 if hasattr(cfg, extra):

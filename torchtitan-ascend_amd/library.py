@@ -28,6 +28,9 @@ Reference ops these stand for (torchtitanturbo/models/common/):
   * ttamd::moe_experts_forward        the fused inference expert stage
   * ttamd::moe_block_forward          the inference block: norms, router, experts, residual
   * ttamd::shared_expert_add          shared-expert tail, qwen3_5/model.py:796-809
+  * ttamd::moe_decode / experts_decode / grouped_mm_e2m1
+                                      the layer, its expert stage and a product for a few
+                                      tokens, 4-bit weights as (codes, exponents) tensors
   * ttamd::token_permute / token_unpermute (+ backward)
                                       npu_moe_token_permute / unpermute, npu_permute.py:74-88
 """
@@ -38,7 +41,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from . import ops
+from . import decode, ops
 
 _BF16 = torch.bfloat16
 _F32 = torch.float32
@@ -638,6 +641,72 @@ def shared_expert_add(routed_out: Tensor, x: Tensor, w13_shared: Tensor, w2_shar
 @shared_expert_add.register_fake
 def _(routed_out, x, w13_shared, w2_shared, gate_logits, swiglu_limit):
     return routed_out.new_empty(routed_out.shape, dtype=_BF16)
+
+
+# ---------------------------------------------------------------------------
+# A few tokens (no gradient).  Weights are bf16 [E, N, K], or the codes of 4-bit
+# weights with their exponents; what a tile's padding hides of N and K follows from
+# x, w13's hidden size and the other weights
+# ---------------------------------------------------------------------------
+def _packed_or(w: Optional[Tensor], exps: Optional[Tensor], rows: int, cols: int):
+    return w if exps is None or w is None else decode.PackedWeights(w, exps, rows, cols)
+
+
+@torch.library.custom_op("ttamd::grouped_mm_e2m1", mutates_args=())
+def grouped_mm_e2m1(x: Tensor, codes: Tensor, exponents: Tensor, rows: int, offs: Optional[Tensor],
+                    bias: Optional[Tensor]) -> Tensor:
+    """x bf16 [M, K] (without offs [..., K]) times 4-bit weights [E, rows, K]."""
+    return decode.grouped_mm_e2m1(x, decode.PackedWeights(codes, exponents, rows, x.shape[-1]), offs, bias)
+
+
+@grouped_mm_e2m1.register_fake
+def _(x, codes, exponents, rows, offs, bias):
+    return x.new_empty((*x.shape[:-1], rows))
+
+
+@torch.library.custom_op("ttamd::experts_decode", mutates_args=())
+def experts_decode(x: Tensor, top_scores: Tensor, idx: Tensor, w13: Tensor, w2: Tensor, hidden: int,
+                   score_before: bool, swiglu_limit: Optional[float], e13: Optional[Tensor] = None,
+                   e2: Optional[Tensor] = None, shared_hidden: int = 0, shared_w13: Optional[Tensor] = None,
+                   shared_w2: Optional[Tensor] = None, shared_e13: Optional[Tensor] = None,
+                   shared_e2: Optional[Tensor] = None, shared_scale: Optional[Tensor] = None) -> Tensor:
+    """Expert stage of at most 64 tokens on given picks."""
+    D = x.shape[-1]
+    return decode.experts_decode(x, top_scores, idx, _packed_or(w13, e13, 2 * hidden, D),
+                                 _packed_or(w2, e2, D, hidden), score_before, swiglu_limit,
+                                 _packed_or(shared_w13, shared_e13, 2 * shared_hidden, D),
+                                 _packed_or(shared_w2, shared_e2, D, shared_hidden), shared_scale)
+
+
+@experts_decode.register_fake
+def _(x, top_scores, idx, w13, w2, hidden, score_before, swiglu_limit, e13=None, e2=None, shared_hidden=0,
+      shared_w13=None, shared_w2=None, shared_e13=None, shared_e2=None, shared_scale=None):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("ttamd::moe_decode", mutates_args=())
+def moe_decode(x: Tensor, w_router: Tensor, w13: Tensor, w2: Tensor, top_k: int, hidden: int, score_func: str,
+               route_norm: bool, route_scale: float, expert_bias: Optional[Tensor], norm_eps: float,
+               num_groups: Optional[int], topk_groups: Optional[int], group_score: str, score_before: bool,
+               swiglu_limit: Optional[float], e13: Optional[Tensor] = None, e2: Optional[Tensor] = None,
+               shared_hidden: int = 0, shared_w13: Optional[Tensor] = None, shared_w2: Optional[Tensor] = None,
+               shared_e13: Optional[Tensor] = None, shared_e2: Optional[Tensor] = None,
+               shared_gate: Optional[Tensor] = None) -> tuple[Tensor, Tensor, Tensor]:
+    """The layer of at most 64 tokens: (out [T, D], top_scores fp32 [T, K], indices int64 [T, K])."""
+    D = x.shape[-1]
+    return decode.moe_decode(x, w_router, _packed_or(w13, e13, 2 * hidden, D), _packed_or(w2, e2, D, hidden), top_k,
+                             score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups, topk_groups,
+                             group_score, score_before, swiglu_limit,
+                             _packed_or(shared_w13, shared_e13, 2 * shared_hidden, D),
+                             _packed_or(shared_w2, shared_e2, D, shared_hidden), shared_gate)
+
+
+@moe_decode.register_fake
+def _(x, w_router, w13, w2, top_k, hidden, score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups,
+      topk_groups, group_score, score_before, swiglu_limit, e13=None, e2=None, shared_hidden=0, shared_w13=None,
+      shared_w2=None, shared_e13=None, shared_e2=None, shared_gate=None):
+    T = x.shape[0]
+    return (x.new_empty(x.shape), x.new_empty((T, top_k), dtype=_F32), x.new_empty((T, top_k), dtype=torch.int64))
 
 
 # ---------------------------------------------------------------------------
