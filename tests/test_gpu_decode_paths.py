@@ -432,3 +432,46 @@ def test_a_serving_step(decode, functional):
         ref, bound = layer_ref(z, s, i, *wb[:2], False, None, wb[2:], gate)
         assert ((out.double() - ref).abs() - bound).max() <= 0, n
         last = want[0]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("picks", [[3, 3, 1, 3], [-1, 2, 4, 1], [4, 9, -7, 2 ** 33], [0, 1, 2, 3]])
+@pytest.mark.parametrize("shared", [0, 64])
+def test_one_token_of_any_picks(decode, bits, picks, shared):
+    """Repeated picks and picks of no expert, none left at all."""
+    rng = np.random.default_rng(31)
+    E, D, H = 4, 288, 160
+    w, wb = build(decode, rng, E, D, H, bits, shared)
+    x, scores = weights(rng, 1, D, scale=1.0), torch.rand(1, 4, device=DEV)
+    idx = torch.tensor([picks], device=DEV)
+    scale = torch.rand(1, device=DEV) if shared else None
+    announce(f"one token {picks} bits={bits} shared={shared}")
+    y = decode.experts_decode(x, scores, idx, *w[:2], False, None, *(w[2:] or (None, None)), scale)
+    ref, bound = layer_ref(x, scores, idx, *wb[:2], False, None, wb[2:] or None, scale)
+    assert ((y.double() - ref).abs() - bound).max() <= 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("E,K,kw", [
+    (1, 1, {}), (256, 8, {}), (257, 8, {}), (128, 9, {}), (60, 4, dict(score_func="sigmoid", route_norm=True)),
+    (64, 6, dict(num_groups=8, topk_groups=3)), (96, 8, dict(num_groups=4, topk_groups=2, group_score="max")),
+    (16, 2, dict(score_before_experts=True, swiglu_limit=0.5))])
+@pytest.mark.parametrize("biased", [False, True])
+def test_one_token_of_any_router(decode, ops, bits, E, K, kw, biased):
+    """The selection made with the first product against the router's own, and both
+    forms of the expert stage against each other."""
+    rng = np.random.default_rng(E + K)
+    D, H = 160, 64
+    x, wr, w, shared, _ = layer(decode, rng, 1, E, D, H, bits, 32)
+    kw = dict(kw, expert_bias=torch.randn(E, device=DEV) * 0.1) if biased else kw
+    route = {k: v for k, v in kw.items() if k not in ("score_before_experts", "swiglu_limit")}
+    announce(f"one token E={E} K={K} {kw.keys()} bits={bits}")
+    out, s, i = decode.moe_decode(x, wr, *w, K, **kw, **shared)
+    s2, i2, gate = decode.router_decode(x, wr, K, shared_gate=shared["shared_gate"], **route)
+    assert torch.equal(s, s2) and torch.equal(i, i2)
+    want = decode.experts_decode(x, s2, i2, *w, kw.get("score_before_experts", False), kw.get("swiglu_limit"),
+                                 shared["shared_w13"], shared["shared_w2"], gate)
+    assert torch.equal(out, want)
+    # the same token twice: the plan's kernel instead
+    both = decode.moe_decode(x.expand(2, -1), wr, *w, K, **kw, **shared)
+    assert torch.equal(both[1], s.expand(2, -1)) and torch.equal(both[2], i.expand(2, -1))

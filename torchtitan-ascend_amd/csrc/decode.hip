@@ -6,10 +6,11 @@
 //   a[s]    = silu(min(g, L)) * clamp(u, -L, L)              slot s = t K + k
 //   out[t]  = sum_k score[s] w2[e_s] a[s]  (+ gate[t] * shared expert of x[t])
 //
-// Four launches:
-//   router_logits_kernel  one wave per row of the gate and up to 4 tokens
+// Four launches, three for one token:
+//   router_logits_kernel  a workgroup per row of the gate and up to 4 tokens
 //   decode_plan_kernel    one workgroup: the selection, and which slots each hit
-//                         expert has (for given picks only that)
+//                         expert has (for given picks only that); for one token the
+//                         next two do it themselves (select_w13_kernel, plan_one)
 //   stream_w13_kernel     persistent workgroups over (hit expert, row pairs)
 //   stream_w2_kernel      a workgroup owns output rows, for every hit expert
 // The streams: decode_stream.h.  With 4-bit weights and more than a few rows per
@@ -40,8 +41,11 @@ struct DecodeArgs {
   bf16_t* a;            // [T K, H], then [T, Hs]
   float* y;             // lock_w2_kernel: [T K (+ T), D]
   bf16_t* out;          // [T, D]
-  const char* plan;
+  const char* plan;     // null (one token): made by each workgroup from the picks
   int plan_lds;         // its bytes in LDS
+  const void* idx;      // one token: its picks and weights, the shared expert's factor
+  const float *scores, *gate;
+  int is64, split[2];   // log2 of KS: w13, w2
 };
 
 // silu(min(gate, L)) * clamp(up, -L, L) in bf16: rounded for the matrix cores, the
@@ -191,11 +195,52 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(const PlanArg
   }
 }
 
-// The second operand of the layer's kernels: LDS from the plan on.
+// One token needs no sorting: each of its slots is a run, in order (a repeated pick
+// streams its expert again).  The first wave's lane k has choice k.
+__device__ __forceinline__ void plan_one(const DecodeArgs& a, char* smem, int64_t pick, float score) {
+  const Plan p(smem, 1, a.K);
+  const int k = threadIdx.x;
+  const bool ok = k < a.K && pick >= 0 && pick < a.E;
+  const uint64_t m = ballot64(ok);
+  if (ok) {
+    const int j = __popcll(m & lanemask_lt());
+    p.list(j) = (short)pick;
+    p.score(j) = score;
+    p.start(j) = (short)j;
+    p.sorted(j) = (short)k;
+    p.token(j) = 0;
+    p.inverse(k) = (short)j;
+  }
+  if (k == 0) {
+    const int hits = __popcll(m);
+    p.hit() = hits;
+    p.start(hits) = (short)hits;
+    p.valid(0) = (uint32_t)m;
+    p.gate(0) = a.gate ? a.gate[0] : 1.f;
+    p.split(0) = a.split[0], p.split(1) = a.split[1];
+  }
+}
+
+// The plan in LDS.
 __device__ __forceinline__ void load_plan(const DecodeArgs& a, char* smem) {
-  const int n = PlanMap{a.T, a.T * a.K}.bytes() / 16;
-  for (int i = threadIdx.x; i < n; i += kThreads) ((uint4*)smem)[i] = ((const uint4*)a.plan)[i];
+  if (!a.plan) {
+    if (threadIdx.x < 64) {
+      const int k = min((int)threadIdx.x, a.K - 1);
+      plan_one(a, smem, a.is64 ? ((const int64_t*)a.idx)[k] : (int64_t)((const int*)a.idx)[k], a.scores[k]);
+    }
+  } else {
+    const int n = PlanMap{a.T, a.T * a.K}.bytes() / 16;
+    for (int i = threadIdx.x; i < n; i += kThreads) ((uint4*)smem)[i] = ((const uint4*)a.plan)[i];
+  }
   __syncthreads();
+}
+
+// c ? x : y by value (a branch would become one between the members' addresses, and
+// they, the kernel's arguments, a copy in scratch)
+__device__ __forceinline__ Weights either(bool c, const Weights& x, const Weights& y) {
+  const uint64_t m = c ? ~0ull : 0ull;
+  auto one = [&](const void* p, const void* q) { return (const void*)((uint64_t)q ^ (((uint64_t)p ^ (uint64_t)q) & m)); };
+  return {one(x.w, y.w), (const uint8_t*)one(x.exps, y.exps)};
 }
 
 // w13's items: R row pairs (gate and up rows of the same 16 hidden units) of an
@@ -228,7 +273,7 @@ struct W13 {
     c.pair = r;
     const int g = c.rb * R + r;
     c.live = g < H / 16;
-    const Weights& m = shared ? a.s13 : a.w13;
+    const Weights m = either(shared, a.s13, a.w13);
 #pragma unroll
     for (int b = 0; b < BL; ++b)
       set_load<WT>(c, b, m, e, 2 * H, a.D,
@@ -255,27 +300,59 @@ template <int WT>
 constexpr int kPairLoads = WT == W_BF16 ? 4 : 2;
 
 template <int WT, int NB, int NS>
-__global__ __launch_bounds__(kThreads, 2) void stream_w13_kernel(const DecodeArgs a) {
+__device__ __forceinline__ void stream_w13(const DecodeArgs& a, char* smem) {
   constexpr int BL = kPairLoads<WT>;
   using Rg = Ring<WT, BL, NB, NS>;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
   const Plan p(smem, a.T, a.T * a.K);
   char* const ring = smem + a.plan_lds;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  load_plan(a, smem);
   const int log_ks = __builtin_amdgcn_readfirstlane(p.split(0)), KS = 1 << log_ks;
   const W13<WT, BL> items(a, p, kWaves >> log_ks);
   int turn = 0;
   stream_items<WT, BL, NB, NS>(
       ring, blockIdx.x, gridDim.x, items.items(__builtin_amdgcn_readfirstlane(p.hit())), w & (KS - 1), KS,
-      [&](int i) __attribute__((always_inline)) { return items(i, w >> log_ks); }, [](const Item<BL>& c, int) { return c.x; },
-      [&](const Item<BL>& c, int, int i) { return items.src(c, i); },
-      [&](const Item<BL>& c, int c0, int rows, const floatx4_t (&acc)[2][Rg::NT]) {
+      [&](int i) __attribute__((always_inline)) { return items(i, w >> log_ks); },
+      [](const Item<BL>& c, int) { return c.x; },
+      [&](const Item<BL>& c, int, int i) __attribute__((always_inline)) { return items.src(c, i); },
+      [&](const Item<BL>& c, int c0, int rows, const floatx4_t (&acc)[2][Rg::NT]) __attribute__((always_inline)) {
         meet_pairs(ring + Rg::kAll, turn, log_ks, c, c0, rows, acc,
-                   [&](const Item<BL>& it, int r, int i, int quad, const floatx4_t& v0, const floatx4_t& v1) {
-                     items.emit(it, r, i, quad, v0, v1);
-                   });
+                   [&](const Item<BL>& it, int r, int i, int quad, const floatx4_t& v0, const floatx4_t& v1)
+                       __attribute__((always_inline)) { items.emit(it, r, i, quad, v0, v1); });
       });
+}
+
+template <int WT, int NB, int NS>
+__global__ __launch_bounds__(kThreads, 2) void stream_w13_kernel(const DecodeArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  load_plan(a, smem);
+  stream_w13<WT, NB, NS>(a, smem);
+}
+
+// One token: every workgroup makes the selection for itself (the first wave; equal
+// bits in all), which costs it 2 to 3 us; a launch for it cost 6.5.
+struct SelectArgs {
+  DecodeArgs d;
+  select::GroupTopkArgs topk;
+};
+constexpr int kSelectPerLane = 4, kSelectK = 8;  // experts of a lane, picks
+
+template <int WT, int NB, int NS>
+__global__ __launch_bounds__(kThreads, 2) void select_w13_kernel(const SelectArgs s) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int k = threadIdx.x;
+  if (k < 64) {
+    int pick;
+    double weight;
+    select::select_token<64, kSelectPerLane, kSelectK, select::SRC_BF16>(s.topk, 0, true, pick, weight, [](int) {});
+    const float score = (float)(weight * (double)s.topk.route_scale);
+    plan_one(s.d, smem, pick, score);
+    if (blockIdx.x == 0 && k < s.d.K) {
+      s.topk.scores[k] = score;
+      s.topk.idx[k] = pick;
+    }
+  }
+  __syncthreads();
+  stream_w13<WT, NB, NS>(s.d, smem);
 }
 
 // More rows per expert, 4 bits.
@@ -509,6 +586,7 @@ size_t al256(size_t n) { return (n + 255) & ~(size_t)255; }
 // A call's kernels, chosen before the plan is made (it takes their splits).
 struct Choice {
   hipError_t (*w13)(const DecodeArgs&, hipStream_t);
+  hipError_t (*select_w13)(const SelectArgs&, hipStream_t);  // one token (null: not that form)
   hipError_t (*w2)(const DecodeArgs&, hipStream_t);
   Split split[2];
 };
@@ -522,11 +600,20 @@ hipError_t go_w13(const DecodeArgs& a, hipStream_t stream) {
 }
 
 template <int WT, int NB, int NS>
+hipError_t go_select_w13(const SelectArgs& s, hipStream_t stream) {
+  const int64_t pairs = (int64_t)s.d.K * (s.d.H / 16) + s.d.Hs / 16;
+  return launch_lds<select_w13_kernel<WT, NB, NS>>(
+      dim3((unsigned)std::min<int64_t>(pairs, num_cus())),
+      s.d.plan_lds + Ring<WT, kPairLoads<WT>, NB, NS>::kAll + kMeetBytes, stream, s);
+}
+
+template <int WT, int NB, int NS>
 bool use_w13(const DecodeArgs& a, Choice& c) {
   using Rg = Ring<WT, kPairLoads<WT>, NB, NS>;
   if (a.plan_lds + Rg::kAll + kMeetBytes > kLds) return false;
   const int64_t pairs = (int64_t)std::min(a.E, a.T * a.K) * (a.H / 16) + a.Hs / 16;
   c.w13 = go_w13<WT, NB, NS>;
+  if constexpr (NB == 1 && NS == (WT == W_BF16 ? 3 : 5)) c.select_w13 = go_select_w13<WT, NB, NS>;
   c.split[0] = {a.H / 16, a.Hs / 16, kWaves * (int)std::min<int64_t>(pairs, num_cus()), ceil_div(a.D, Rg::kCols), 3, kMeet<WT>};
   return true;
 }
@@ -699,15 +786,10 @@ hipError_t launch_experts_decode(const ExpertsDecode& c, const RouterDecode* rou
   Choice choice{};
   if (!(c.fp4 ? choose_fp4(a, choice) : choose_bf16(a, choice))) return hipErrorInvalidValue;
 
-  PlanArgs pa{};
-  pa.idx = c.idx, pa.is64 = c.is64, pa.scores = c.scores, pa.gate = c.gate;
-  pa.T = a.T, pa.E = a.E, pa.K = a.K, pa.plan = (char*)ws;
-  pa.split[0] = choice.split[0], pa.split[1] = choice.split[1];
-  hipError_t err;
+  hipError_t err = router ? launch_logits(*router, a.T, a.E, a.D, stream) : hipSuccess;
+  if (err != hipSuccess) return err;
+  select::GroupTopkArgs t{};
   if (router) {
-    err = launch_logits(*router, a.T, a.E, a.D, stream);
-    if (err != hipSuccess) return err;
-    select::GroupTopkArgs& t = pa.topk;
     t.z = router->logits;
     t.S = 1, t.T = a.T, t.E = a.E, t.K = a.K;
     t.aligned = ((uintptr_t)router->logits & 15) == 0;
@@ -715,10 +797,35 @@ hipError_t launch_experts_decode(const ExpertsDecode& c, const RouterDecode* rou
     t.bias = router->bias;
     t.score_func = router->score_func, t.renorm = router->renorm, t.eps = router->eps, t.route_scale = router->scale;
     t.scores = router->top_scores, t.idx = router->top_idx;
-    err = launch_plan_topk(pa, stream);
-  } else {
-    err = go_plan<0, 4>(pa, stream);
   }
+  if (a.T == 1 && choice.select_w13) {
+    int log_run = 0;
+    const int per_lane = router ? select::experts_per_lane(64, t.G, t.EG, &log_run) : 0;
+    if (!router || (per_lane > 0 && per_lane <= kSelectPerLane && a.K <= kSelectK)) {
+      a.plan = nullptr;
+      a.idx = router ? (const void*)router->top_idx : c.idx, a.is64 = router || c.is64;
+      a.scores = router ? router->top_scores : c.scores;
+      a.gate = c.gate;
+      for (int i = 0; i < 2; ++i) {
+        const Split& sp = choice.split[i];
+        a.split[i] = split_log(a.K * sp.items + sp.shared, sp.slots, sp.stages, sp.most, sp.meet);
+      }
+      if (router) {
+        t.log_run = log_run, t.per_lane = per_lane;
+        err = choice.select_w13(SelectArgs{a, t}, stream);
+      } else {
+        err = choice.w13(a, stream);
+      }
+      return err != hipSuccess ? err : choice.w2(a, stream);
+    }
+  }
+
+  PlanArgs pa{};
+  pa.topk = t;
+  pa.idx = c.idx, pa.is64 = c.is64, pa.scores = c.scores, pa.gate = c.gate;
+  pa.T = a.T, pa.E = a.E, pa.K = a.K, pa.plan = (char*)ws;
+  pa.split[0] = choice.split[0], pa.split[1] = choice.split[1];
+  err = router ? launch_plan_topk(pa, stream) : go_plan<0, 4>(pa, stream);
   if (err != hipSuccess) return err;
   err = choice.w13(a, stream);
   return err != hipSuccess ? err : choice.w2(a, stream);

@@ -280,7 +280,7 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
 // us and the DMAs go on meanwhile, four of the 4-bit stages.
 template <int WT>
 constexpr int kMeet = WT == W_BF16 ? 1 : 8;
-__device__ __forceinline__ int split_log(int items, int slots, int stages, int most, int meet) {
+__host__ __device__ inline int split_log(int items, int slots, int stages, int most, int meet) {
   int best = 0, cost = 0x7fffffff;
   for (int k = 0; k <= most && (1 << k) <= stages; ++k) {
     const int rounds = ((items << k) + slots - 1) / slots;
