@@ -299,6 +299,8 @@ struct W13 {
 template <int WT>
 constexpr int kPairLoads = WT == W_BF16 ? 4 : 2;
 
+constexpr int kMeetRows = 4;  // (the rings leave room for no more)
+
 template <int WT, int NB, int NS>
 __device__ __forceinline__ void stream_w13(const DecodeArgs& a, char* smem) {
   constexpr int BL = kPairLoads<WT>;
@@ -315,7 +317,7 @@ __device__ __forceinline__ void stream_w13(const DecodeArgs& a, char* smem) {
       [](const Item<BL>& c, int) { return c.x; },
       [&](const Item<BL>& c, int, int i) __attribute__((always_inline)) { return items.src(c, i); },
       [&](const Item<BL>& c, int c0, int rows, const floatx4_t (&acc)[2][Rg::NT]) __attribute__((always_inline)) {
-        meet_pairs(ring + Rg::kAll, turn, log_ks, c, c0, rows, acc,
+        meet_pairs<kMeetRows>(ring + Rg::kAll, turn, log_ks, c, c0, rows, acc,
                    [&](const Item<BL>& it, int r, int i, int quad, const floatx4_t& v0, const floatx4_t& v1)
                        __attribute__((always_inline)) { items.emit(it, r, i, quad, v0, v1); });
       });
@@ -595,7 +597,7 @@ template <int WT, int NB, int NS>
 hipError_t go_w13(const DecodeArgs& a, hipStream_t stream) {
   const int64_t pairs = (int64_t)std::min(a.E, a.T * a.K) * (a.H / 16) + a.Hs / 16;  // items at the finest
   return launch_lds<stream_w13_kernel<WT, NB, NS>>(dim3((unsigned)std::min<int64_t>(pairs, num_cus())),
-                                                   a.plan_lds + Ring<WT, kPairLoads<WT>, NB, NS>::kAll + kMeetBytes,
+                                                   a.plan_lds + Ring<WT, kPairLoads<WT>, NB, NS>::kAll + meet_bytes(kMeetRows),
                                                    stream, a);
 }
 
@@ -604,17 +606,17 @@ hipError_t go_select_w13(const SelectArgs& s, hipStream_t stream) {
   const int64_t pairs = (int64_t)s.d.K * (s.d.H / 16) + s.d.Hs / 16;
   return launch_lds<select_w13_kernel<WT, NB, NS>>(
       dim3((unsigned)std::min<int64_t>(pairs, num_cus())),
-      s.d.plan_lds + Ring<WT, kPairLoads<WT>, NB, NS>::kAll + kMeetBytes, stream, s);
+      s.d.plan_lds + Ring<WT, kPairLoads<WT>, NB, NS>::kAll + meet_bytes(kMeetRows), stream, s);
 }
 
 template <int WT, int NB, int NS>
 bool use_w13(const DecodeArgs& a, Choice& c) {
   using Rg = Ring<WT, kPairLoads<WT>, NB, NS>;
-  if (a.plan_lds + Rg::kAll + kMeetBytes > kLds) return false;
+  if (a.plan_lds + Rg::kAll + meet_bytes(kMeetRows) > kLds) return false;
   const int64_t pairs = (int64_t)std::min(a.E, a.T * a.K) * (a.H / 16) + a.Hs / 16;
   c.w13 = go_w13<WT, NB, NS>;
   if constexpr (NB == 1 && NS == (WT == W_BF16 ? 3 : 5)) c.select_w13 = go_select_w13<WT, NB, NS>;
-  c.split[0] = {a.H / 16, a.Hs / 16, kWaves * (int)std::min<int64_t>(pairs, num_cus()), ceil_div(a.D, Rg::kCols), 3, kMeet<WT>};
+  c.split[0] = {a.H / 16, a.Hs / 16, kWaves * (int)std::min<int64_t>(pairs, num_cus()), ceil_div(a.D, Rg::kCols), 3, 1};
   return true;
 }
 

@@ -276,11 +276,13 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
 // stages in one, twice, with `meet` for the meeting of KS waves.  From the experts
 // really hit, so that the last round is full: 112 experts of 1536 x 2048 make 2.6
 // rounds with whole row pairs and 21.0 with eighths.
-// A meeting costs about 1.5 us of latency: half a stage where HBM gives a stage in 1.4
-// us and the DMAs go on meanwhile, four of the 4-bit stages.
-template <int WT>
-constexpr int kMeet = WT == W_BF16 ? 1 : 8;
-__host__ __device__ inline int split_log(int items, int slots, int stages, int most, int meet) {
+// A meeting counts as half a stage: its 1.5 us of latency pass while the next stages
+// load (96 rows of 68 experts of 1536 x 2048 in 4 bits: whole pairs 35.0 us, quarters,
+// which this chooses, 32.2).  One round that half the waves share already has the
+// chip's requests, and no next stages for a meeting to hide behind (41 experts' w13 of
+// 544 x 1440 in 4 bits: whole 12.9 us, quarters 14.4).
+__host__ __device__ inline int split_log(int items, int slots, int stages, int most, int meet = 1) {
+  if (items <= slots && 2 * items >= slots) return 0;
   int best = 0, cost = 0x7fffffff;
   for (int k = 0; k <= most && (1 << k) <= stages; ++k) {
     const int rounds = ((items << k) + slots - 1) / slots;
@@ -304,13 +306,12 @@ __device__ __forceinline__ void set_load(Item<BL>& c, int b, const Weights& m, i
   }
 }
 
-// The KS partial sums of row pairs (two blocks each), added in order: kMeetRows token
-// rows at a time, two rounds of LDS in turn (a round is read before the next one's
+// The KS partial sums of row pairs (two blocks each), added in order: MR token rows at
+// a time (13 rows of 1000 x 1440 in 4 bits: 4 at a time 10.5 us, 16 6.7), two rounds of LDS in turn (a round is read before the next one's
 // barrier and written after it).  emit(item, r, i, quad, v0, v1): rows 4 quad .. + 3
 // of the blocks of the workgroup's pair r, token row i.  Every wave calls it.
-constexpr int kMeetRows = 4;
-constexpr int kMeetBytes = 2 * kMeetRows * kWaves * 128;
-template <int BL, int NT, class Emit>
+constexpr int meet_bytes(int rows) { return 2 * rows * kWaves * 128; }
+template <int MR, int BL, int NT, class Emit>
 __device__ __forceinline__ void meet_pairs(char* lds, int& turn, int log_ks, const Item<BL>& c, int c0, int rows,
                                            const floatx4_t (&acc)[2][NT], Emit emit) {
   const int tid = threadIdx.x, l = tid & 63, n = l & 15, q = l >> 4;
@@ -323,22 +324,22 @@ __device__ __forceinline__ void meet_pairs(char* lds, int& turn, int log_ks, con
     }
     return;
   }
-  constexpr int per = 4 * kMeetRows;
-  for (int m0 = 0; m0 < rows; m0 += kMeetRows) {
-    floatx4_t* const red = (floatx4_t*)(lds + turn * (kMeetBytes / 2));
+  constexpr int per = 4 * MR;
+  for (int m0 = 0; m0 < rows; m0 += MR) {
+    floatx4_t* const red = (floatx4_t*)(lds + turn * (meet_bytes(MR) / 2));
     turn ^= 1;
     if (c.live) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int i = 16 * t + n - m0;
-        if (i >= 0 && i < kMeetRows) {
+        if (i >= 0 && i < MR) {
           red[(w * 2 + 0) * per + i * 4 + q] = acc[0][t];
           red[(w * 2 + 1) * per + i * 4 + q] = acc[1][t];
         }
       }
     }
     dma::lds_barrier();
-    // (kWaves per / KS <= 64 places: the first wave)
+    // (kWaves per / KS places, at most 256)
     const int r = tid / per, at = tid % per, i = m0 + (at >> 2);
     if (r < kWaves >> log_ks && i < rows) {
       const floatx4_t* v = red + (r << log_ks) * 2 * per + at;
@@ -472,7 +473,7 @@ __device__ __forceinline__ void lock_items(char* ring, int all, int stages, Item
   wait_vm<0>();
   if (nitems == all) return;
   __syncthreads();
-  static_assert(TailRing::kAll + kMeetBytes <= L::kAll, "LDS");
+  static_assert(TailRing::kAll + meet_bytes(TailRing::kRows) <= L::kAll, "LDS");
   const int pairs = (all - nitems) * kWaves, parts = 2 * pairs <= (int)gridDim.x ? 2 : 1;
   int turn = 0;
   stream_items<W_FP4, 2, kTailNB, kTailNS>(
@@ -490,7 +491,7 @@ __device__ __forceinline__ void lock_items(char* ring, int all, int stages, Item
       origin, src,
       [&](const Item<2>& c, int c0, int rows, const floatx4_t (&acc)[2][TailRing::NT]) __attribute__((always_inline)) {
         if (!c.live) return;  // (of the whole workgroup: the item is all waves')
-        meet_pairs(ring + TailRing::kAll, turn, 3, c, c0, rows, acc,
+        meet_pairs<TailRing::kRows>(ring + TailRing::kAll, turn, 3, c, c0, rows, acc,
                    [&](const Item<2>& it, int, int i, int quad, const floatx4_t& v0, const floatx4_t& v1)
                        __attribute__((always_inline)) { emit(it, i, quad, v0, v1); });
       });

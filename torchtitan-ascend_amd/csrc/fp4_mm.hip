@@ -141,7 +141,7 @@ __global__ __launch_bounds__(kThreads, 2) void stream_mm_kernel(const MmArgs a) 
     find_runs(a, s);
     runs = __builtin_amdgcn_readfirstlane(s.n);
   }
-  const int log_ks = split_log(runs * (((a.N + 15) / 16 + 1) / 2), kWaves * gridDim.x, (a.K + 127) / 128, 3, kMeet<W_FP4>);
+  const int log_ks = split_log(runs * (((a.N + 15) / 16 + 1) / 2), kWaves * gridDim.x, (a.K + 127) / 128, 3);
   const int KS = 1 << log_ks;
   const MmItems items(a, s, kWaves >> log_ks);
   int turn = 0;
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kThreads, 2) void stream_mm_kernel(const MmArgs a) 
       [&](const Item<2>& c, int n0) __attribute__((always_inline)) { return items.origin(c, n0); },
       [&](const Item<2>&, int n0, int i) __attribute__((always_inline)) { return items.src(n0, i); },
       [&](const Item<2>& c, int c0, int rows, const floatx4_t (&acc)[2][Rg::NT]) __attribute__((always_inline)) {
-        meet_pairs(ring + Rg::kAll, turn, log_ks, c, c0, rows, acc,
+        meet_pairs<Rg::kRows>(ring + Rg::kAll, turn, log_ks, c, c0, rows, acc,
                    [&](const Item<2>& it, int r, int i, int quad, const floatx4_t& v0, const floatx4_t& v1)
                        __attribute__((always_inline)) {
                      items.emit(it, r, i, quad, v0, v1);
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kThreads, 2) void lock_mm_kernel(const MmArgs a) {
 
 template <int NB, int NS>
 hipError_t go_stream(const MmArgs& a, int64_t pairs, hipStream_t stream) {
-  constexpr int lds = Ring<W_FP4, 2, NB, NS>::kAll + kMeetBytes;
+  constexpr int lds = Ring<W_FP4, 2, NB, NS>::kAll + meet_bytes(Ring<W_FP4, 2, NB, NS>::kRows);
   static_assert(lds + kRunsBytes <= kLds, "LDS");
   return launch_lds<stream_mm_kernel<NB, NS>>(dim3((unsigned)std::min<int64_t>(pairs, num_cus())),
                                               lds + (a.offs ? kRunsBytes : 0), stream, a);
