@@ -235,12 +235,26 @@ __device__ __forceinline__ void load_plan(const DecodeArgs& a, char* smem) {
   __syncthreads();
 }
 
-// c ? x : y by value (a branch would become one between the members' addresses, and
-// they, the kernel's arguments, a copy in scratch)
+// c ? x : y by value.  (A branch would become one between the members' addresses: the
+// kernel's arguments loaded again for every item, or copied to scratch.)
+__device__ __forceinline__ int either(bool c, int x, int y) { return y ^ ((x ^ y) & -(int)c); }
 __device__ __forceinline__ Weights either(bool c, const Weights& x, const Weights& y) {
   const uint64_t m = c ? ~0ull : 0ull;
   auto one = [&](const void* p, const void* q) { return (const void*)((uint64_t)q ^ (((uint64_t)p ^ (uint64_t)q) & m)); };
   return {one(x.w, y.w), (const uint8_t*)one(x.exps, y.exps)};
+}
+
+// The hit expert at j and its rows, or the shared one: one round of LDS reads, not
+// one per branch (an item of a few stages waits for them; 32 tokens of 128 experts'
+// w2 of 2048 x 768 in 4 bits: 45 -> 41 us).
+struct Run {
+  int e, start, cnt;
+};
+__device__ __forceinline__ Run run_of(const DecodeArgs& a, const Plan& p, bool shared, int j) {
+  j = shared ? 0 : j;
+  const int e = __builtin_amdgcn_readfirstlane(p.list(j)), first = __builtin_amdgcn_readfirstlane(p.start(j)),
+            end = __builtin_amdgcn_readfirstlane(p.start(j + 1));
+  return {shared ? 0 : e, shared ? -1 : first, shared ? a.T : end - first};
 }
 
 // w13's items: R row pairs (gate and up rows of the same 16 hidden units) of an
@@ -262,12 +276,12 @@ struct W13 {
     const bool shared = LAST ? i >= sh0 : i < nsh;
     const int r0 = LAST ? i : i - nsh;
     const int j = shared ? 0 : r0 / nrb;
-    const int e = shared ? 0 : __builtin_amdgcn_readfirstlane(p.list(j));
-    const int H = shared ? a.Hs : a.H;
+    const Run run = run_of(a, p, shared, j);
+    const int e = run.e, H = either(shared, a.Hs, a.H);
     c.rb = shared ? i - sh0 : r0 - j * nrb;
-    c.start = shared ? -1 : __builtin_amdgcn_readfirstlane(p.start(j));
+    c.start = run.start;
     c.lo = 0;
-    c.cnt = shared ? a.T : __builtin_amdgcn_readfirstlane(p.start(j + 1)) - c.start;
+    c.cnt = run.cnt;
     c.K = a.D;
     c.x = (uint64_t)a.x;
     c.pair = r;
@@ -281,7 +295,8 @@ struct W13 {
     return c;
   }
   __device__ __forceinline__ uint32_t src(const Item<BL>& c, int i) const {
-    return (uint32_t)(c.start < 0 ? i : p.token(c.start + i)) * (uint32_t)a.D * 2u;
+    const int t = p.token(max(c.start, 0) + i);  // (in the plan; the shared expert's rows are the tokens)
+    return (uint32_t)(c.start < 0 ? i : t) * (uint32_t)a.D * 2u;
   }
   __device__ __forceinline__ void emit(const Item<BL>& c, int pair, int i, int quad, const floatx4_t& v0,
                                        const floatx4_t& v1) const {
@@ -381,7 +396,7 @@ __global__ __launch_bounds__(kThreads, 2) void lock_w13_kernel(const DecodeArgs 
 template <int WT, int BL, int NB, int NS>
 __global__ __launch_bounds__(kThreads, 2) void stream_w2_kernel(const DecodeArgs a) {
   using Rg = Ring<WT, BL, NB, NS>;
-  constexpr int MB = Rg::kBlocks, LR = WT == W_BF16 ? 8 : 16;  // rows of a load
+  constexpr int MB = Rg::kBlocks, LR = load_rows(WT);
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int S = a.T * a.K, tid = threadIdx.x, l = tid & 63;
   const Plan p(smem, a.T, S);
@@ -397,23 +412,24 @@ __global__ __launch_bounds__(kThreads, 2) void stream_w2_kernel(const DecodeArgs
   auto item_of = [&](int i) {
     Item<BL> c;
     const bool shared = i < nsh;
-    const int e = shared ? 0 : __builtin_amdgcn_readfirstlane(p.list(i - nsh));
+    const Run run = run_of(a, p, shared, i - nsh);
     c.rb = 0;
-    c.start = shared ? -1 : __builtin_amdgcn_readfirstlane(p.start(i - nsh));
+    c.start = run.start;
     c.lo = 0;
-    c.cnt = shared ? a.T : __builtin_amdgcn_readfirstlane(p.start(i - nsh + 1)) - c.start;
-    c.K = shared ? a.Hs : a.H;
+    c.cnt = run.cnt;
+    c.K = either(shared, a.Hs, a.H);
     c.x = (uint64_t)(shared ? a.a + (int64_t)S * a.H : a.a);
     c.live = true;
 #pragma unroll
     for (int b = 0; b < BL; ++b)  // (rows past the last: the last ones again, not stored)
-      set_load<WT>(c, b, shared ? a.s2 : a.w2, e, a.D, c.K, min(row0 + b * LR, a.D - LR));
+      set_load<WT>(c, b, either(shared, a.s2, a.w2), run.e, a.D, c.K, min(row0 + b * LR, a.D - LR));
     return c;
   };
   stream_items<WT, BL, NB, NS>(
       ring, w >> log_ks, R, nsh + hit, ks, KS, item_of, [](const Item<BL>& c, int) { return c.x; },
       [&](const Item<BL>& c, int, int i) {
-        return c.start < 0 ? (uint32_t)i * (uint32_t)a.Hs * 2u : (uint32_t)p.sorted(c.start + i) * (uint32_t)a.H * 2u;
+        const int slot = p.sorted(max(c.start, 0) + i);
+        return (uint32_t)(c.start < 0 ? i : slot) * (uint32_t)c.K * 2u;
       },
       [&](const Item<BL>& c, int c0, int rows, const floatx4_t (&acc)[MB][Rg::NT]) {
 #pragma unroll
@@ -439,18 +455,22 @@ __global__ __launch_bounds__(kThreads, 2) void stream_w2_kernel(const DecodeArgs
     const uint32_t ok = p.valid(t);
     floatx4_t sum = {0.f, 0.f, 0.f, 0.f};
     for (int k0 = 0; k0 < a.K; k0 += 8) {
-      int place[8];
+      bool in[8];
+      int place[8];  // (reads without branches, at place 0 for no expert: one wait for all)
       float sc[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const bool in = k0 + k < a.K && (ok >> (k0 + k) & 1);
-        place[k] = in ? p.inverse(t * a.K + k0 + k) : -1;
+        const int inv = p.inverse(t * a.K + min(k0 + k, a.K - 1));
+        in[k] = k0 + k < a.K && (ok >> (k0 + k) & 1);
+        place[k] = in[k] ? inv : 0;
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sc[k] = a.before || place[k] < 0 ? 1.f : p.score(place[k]);
+      for (int k = 0; k < 8; ++k) sc[k] = p.score(place[k]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (place[k] >= 0) sum += row(place[k]) * sc[k];
+      for (int k = 0; k < 8; ++k) {
+        const floatx4_t next = sum + row(place[k]) * (a.before ? 1.f : sc[k]);
+        sum = in[k] ? next : sum;
+      }
     }
     if (nsh) sum += row(S + t) * p.gate(t);
     *(u32x2_t*)(a.out + (int64_t)t * a.D + row0 + 4 * d) =
@@ -473,24 +493,25 @@ __global__ __launch_bounds__(kThreads, 2) void lock_w2_kernel(const DecodeArgs a
         Item<2> c;
         const bool shared = i < nsh;
         const int j = shared ? 0 : (i - nsh) / nrb;
-        const int e = shared ? 0 : __builtin_amdgcn_readfirstlane(p.list(j));
+        const Run run = run_of(a, p, shared, j);
         c.rb = shared ? i : i - nsh - j * nrb;
-        c.start = shared ? -1 : __builtin_amdgcn_readfirstlane(p.start(j));
+        c.start = run.start;
         c.lo = 0;
-        c.cnt = shared ? a.T : __builtin_amdgcn_readfirstlane(p.start(j + 1)) - c.start;
-        c.K = shared ? a.Hs : a.H;
+        c.cnt = run.cnt;
+        c.K = either(shared, a.Hs, a.H);
         c.x = (uint64_t)(shared ? a.a + (int64_t)S * a.H : a.a);
         c.pair = r;
         const int g = c.rb * kWaves + r;
         c.live = g < a.D / 32;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          set_load<W_FP4>(c, b, shared ? a.s2 : a.w2, e, a.D, c.K, c.live ? 32 * g + 16 * b : 0);
+          set_load<W_FP4>(c, b, either(shared, a.s2, a.w2), run.e, a.D, c.K, c.live ? 32 * g + 16 * b : 0);
         return c;
       },
       [](const Item<2>& c, int) { return c.x; },
       [&](const Item<2>& c, int, int i) {
-        return c.start < 0 ? (uint32_t)i * (uint32_t)a.Hs * 2u : (uint32_t)p.sorted(c.start + i) * (uint32_t)a.H * 2u;
+        const int slot = p.sorted(max(c.start, 0) + i);
+        return (uint32_t)(c.start < 0 ? i : slot) * (uint32_t)c.K * 2u;
       },
       [&](const Item<2>& c, int i, int quad, const floatx4_t& v0, const floatx4_t& v1) __attribute__((always_inline)) {
         const bool shared = c.start < 0;
@@ -634,7 +655,7 @@ template <int WT, int BL, int NB, int NS>
 hipError_t go_w2(const DecodeArgs& a, hipStream_t stream) {
   using Rg = Ring<WT, BL, NB, NS>;
   const int sums = (a.T * a.K + (a.Hs > 0 ? a.T : 0)) * Rg::kBlocks * 64;
-  return launch_lds<stream_w2_kernel<WT, BL, NB, NS>>(dim3(ceil_div(a.D, BL * (WT == W_BF16 ? 8 : 16))),
+  return launch_lds<stream_w2_kernel<WT, BL, NB, NS>>(dim3(ceil_div(a.D, BL * load_rows(WT))),
                                                       a.plan_lds + Rg::kAll + (sums << w2_log<WT, BL, NB, NS>(a)),
                                                       stream, a);
 }
@@ -702,12 +723,18 @@ bool choose_fp4(const DecodeArgs& a, Choice& c) {
     static_assert(((kMaxPlanBytes + 127) & ~127) + Lock<1, 5>::kAll <= kLds, "LDS");
     return true;
   }
-  const bool two = a.D / 16 > num_cus();
+  // The second product's workgroups own 16 output rows, or 32 where 16 would make more
+  // of them than the chip has CUs, or 8 where 16 would leave half of it idle (17 tokens
+  // of 60 experts, 1440 rows: 18.2 us by 16, 17.2 by 8; 32 of 128, 2048 rows: 52 and 45).
+  const int blocks = a.D / 16, cus = num_cus();
   if (rows <= 2)
-    return (use_w13<W_FP4, 1, 5>(a, c) || use_w13<W_FP4, 1, 4>(a, c)) && ((!two && use_w2<W_FP4, 1, 1, 7>(a, c)) || (two && use_w2<W_FP4, 2, 1, 4>(a, c)) ||
-                                          use_w2<W_FP4, 1, 2, 3>(a, c));
-  return (use_w13<W_FP4, 2, 4>(a, c) || use_w13<W_FP4, 2, 3>(a, c)) && ((!two && use_w2<W_FP4, 1, 2, 5>(a, c)) || (two && use_w2<W_FP4, 2, 2, 3>(a, c)) ||
-                                        use_w2<W_FP4, 1, 2, 3>(a, c));
+    return (use_w13<W_FP4, 1, 5>(a, c) || use_w13<W_FP4, 1, 4>(a, c)) &&
+           ((2 * blocks <= cus && use_w2<W_FP4_8, 1, 2, 5>(a, c)) ||
+            (blocks <= cus && use_w2<W_FP4, 1, 1, 7>(a, c)) ||
+            (blocks > cus && use_w2<W_FP4, 2, 1, 4>(a, c)) || use_w2<W_FP4, 1, 2, 3>(a, c));
+  return (use_w13<W_FP4, 2, 4>(a, c) || use_w13<W_FP4, 2, 3>(a, c)) &&
+         ((2 * blocks <= cus && use_w2<W_FP4_8, 1, 4, 3>(a, c)) || (blocks <= cus && use_w2<W_FP4, 1, 2, 5>(a, c)) ||
+          (blocks > cus && use_w2<W_FP4, 2, 2, 3>(a, c)) || use_w2<W_FP4, 1, 2, 3>(a, c));
 }
 
 template <int LPT, int PL>

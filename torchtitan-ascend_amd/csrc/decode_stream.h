@@ -24,7 +24,10 @@ constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kLds = 160 * 1024;
 
-enum WeightType { W_BF16 = 0, W_FP4 = 1 };
+// W_FP4_8: 4-bit tiles by their upper or lower 8 rows, two tiles of a row of tiles at a
+// time (for a workgroup that owns 8 output rows).
+enum WeightType { W_BF16 = 0, W_FP4 = 1, W_FP4_8 = 2 };
+constexpr int load_rows(int wt) { return wt == W_FP4 ? 16 : 8; }
 
 // Weights [E, N, K]: bf16 rows, or 4-bit tiles and their exponents (fp4.hip).
 struct Weights {
@@ -34,20 +37,21 @@ struct Weights {
 
 // ---- streams: every wave pulls its own weight rows through a ring in LDS --------
 // A stage of a wave: its weight rows and the token rows over kCols columns (bf16: a
-// 128-byte line of every row; 4 bits: one tile and its exponents).  A DMA
-// instruction moves 8 bf16 weight rows, one 4-bit tile of 16, or 8 (4) token rows of
-// 128 (256) bytes; BL and NB count the instructions.
+// 128-byte line of every row; 4 bits: one tile, or two halves, and the exponents).  A
+// DMA instruction moves 8 bf16 weight rows, one 4-bit tile of 16, or 8 (4, 2) token
+// rows of 128 (256, 512) bytes; BL and NB count the instructions.
 template <int WT, int BL, int NB, int NS>
 struct Ring {
-  static constexpr int kCols = WT == W_BF16 ? 64 : 128;
+  static constexpr int kCols = WT == W_BF16 ? 64 : WT == W_FP4 ? 128 : 256;
   static constexpr int kBlocks = WT == W_BF16 ? (BL + 1) / 2 : BL;  // of 16 rows
   static constexpr int kExps = BL * 1024;                           // 4 bits: 256 bytes of exponents per block
   static constexpr int kRowsAt = kExps + (WT == W_BF16 ? 0 : 256 * BL);
   static constexpr int kBytes = kRowsAt + 1024 * NB;
   static constexpr int kOps = (WT == W_BF16 ? BL : 2 * BL) + NB;
-  static constexpr int kRows = NB * (WT == W_BF16 ? 8 : 4);
+  static constexpr int kRows = NB * (512 / kCols);
   static constexpr int NT = (kRows + 15) / 16;
   static constexpr int kAll = kWaves * NS * kBytes;
+  static_assert(WT != W_FP4_8 || BL == 1);
 };
 
 // One item of a wave: rows of one expert (or the shared one) times its token rows.
@@ -117,6 +121,36 @@ __device__ __forceinline__ void consume_tiles(floatx4_t (&acc)[BL][ALL], const c
   }
 }
 
+// acc += stage cs of 8 rows' halves of two tiles times the token rows (512 bytes each).
+template <int ROWS, class Free>
+__device__ __forceinline__ void consume_halves(floatx4_t& acc, const char* st, int exps_at, const char* rows_at, int cs,
+                                               int left, Free free) {
+  const int l = threadIdx.x & 63, n = l & 15, q = l >> 4, r = n & (ROWS - 1);
+  const uint32_t ex = *(const uint32_t*)(st + exps_at + 4 * l);
+  uint4 qw[2];
+  bf16x8_t bx[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    qw[h] = *(const uint4*)(st + (32 * h + 8 * q + (n & 7)) * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bx[h][j] = *(const bf16x8_t*)(rows_at + r * 512 + (((16 * h + 4 * q + j) ^ r) << 4));
+  }
+  free();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (128 * h >= left) break;
+    if (128 * h + 32 * q >= left) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bx[h][j] = __builtin_bit_cast(bf16x8_t, make_uint4(0u, 0u, 0u, 0u));
+    }
+    const uint32_t d[4] = {qw[h].x, qw[h].y, qw[h].z, qw[h].w};
+    const float scale = fp4_scale(ex, (2 * cs + h) & 3);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_frag(d[j], scale), bx[h][j], acc, 0, 0, 0);
+  }
+}
+
 // Runs the items first, first + step, ... < nitems.  Of a item's stages the wave
 // takes every KS-th from ks on.  The DMAs run over the flattened sequence of all
 // its stages, NS ahead, so neither an epilogue nor the next expert's start empties
@@ -142,6 +176,9 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
   // reads of 16 rows meet no bank twice
   auto chunk8 = [&](int i) { return (l & 7) ^ cswz(8 * i + (l >> 3)); };
   auto chunk16 = [&](int i) { return (l & 15) ^ ((4 * i + (l >> 4)) & 15); };
+  auto chunk32 = [&](int i) { return (l & 31) ^ ((2 * i + (l >> 5)) & 15); };
+  auto row_of = [&](int i) { return WT == W_BF16 ? 8 * i + (l >> 3) : WT == W_FP4 ? 4 * i + (l >> 4) : 2 * i + (l >> 5); };
+  auto chunk_of = [&](int i) { return WT == W_BF16 ? chunk8(i) : WT == W_FP4 ? chunk16(i) : chunk32(i); };
 
   // the issuing end
   int it = first, n0 = 0, s = ks;
@@ -153,9 +190,7 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
     xbase = origin(in, n0);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int r = WT == W_BF16 ? 8 * b + (l >> 3) : 4 * b + (l >> 4);
-      const int ch = WT == W_BF16 ? chunk8(b) : chunk16(b);
-      vb[b] = src(in, n0, min(n0 + r, in.cnt - 1)) + (uint32_t)(16 * ch);
+      vb[b] = src(in, n0, min(n0 + row_of(b), in.cnt - 1)) + (uint32_t)(16 * chunk_of(b));
     }
   };
   auto enter = [&]() __attribute__((always_inline)) {  // item `it`, or the next with a stage for this wave
@@ -189,12 +224,18 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
           dma16(vb[b] - (chunk8(b) & 4 ? 64u : 0u), xbase + k, at + R::kRowsAt + b * 1024);
       }
     } else {
-      issue_tiles<BL>(in, s, at, R::kExps);
+      if constexpr (WT == W_FP4) {
+        issue_tiles<BL>(in, s, at, R::kExps);
+      } else {  // (past the last tile: the first once more)
+        const int h = left > 128 ? l >> 5 : 0;
+        dma16((uint32_t)(1024 * h + 256 * (l >> 3 & 3) + 16 * (l & 7)), in.base[0] + (uint64_t)s * 2048, at);
+        dma4((uint32_t)(4 * (l & 0x37)), in.exps[0] + (uint64_t)(s >> 1) * 256, at + R::kExps);
+      }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const int ch = chunk16(b);
+        const int ch = chunk_of(b);
         const uint32_t back = 8 * ch >= left ? (uint32_t)(16 * (ch & ~3)) : 0u;
-        dma16(vb[b] - back, xbase + (uint64_t)s * 256, at + R::kRowsAt + b * 1024);
+        dma16(vb[b] - back, xbase + (uint64_t)s * (2 * R::kCols), at + R::kRowsAt + b * 1024);
       }
     }
     s += KS;
@@ -258,11 +299,13 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
                   acc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(aw[b][h], bx[h][t], acc[b][t], 0, 0, 0);
             }
           } else {
-            consume_tiles<BL, NT, R::kRows>(acc, st, R::kExps, st + R::kRowsAt, cs, left, [&]() __attribute__((always_inline)) {
+            auto free = [&]() __attribute__((always_inline)) {
               lds_wait();
               if (more) issue(slot);
               else --ahead;
-            });
+            };
+            if constexpr (WT == W_FP4) consume_tiles<BL, NT, R::kRows>(acc, st, R::kExps, st + R::kRowsAt, cs, left, free);
+            else consume_halves<R::kRows>(acc[0][0], st, R::kExps, st + R::kRowsAt, cs, left, free);
           }
           slot = slot == NS - 1 ? 0 : slot + 1;
         }
@@ -292,8 +335,7 @@ __host__ __device__ inline int split_log(int items, int slots, int stages, int m
   return best;
 }
 
-// Load b of an item: 8 rows (bf16) or 16 (4 bits) of expert e's [N, K] weights from
-// row `row` on.
+// Load b of an item: load_rows(WT) rows of expert e's [N, K] weights from row `row` on.
 template <int WT, int BL>
 __device__ __forceinline__ void set_load(Item<BL>& c, int b, const Weights& m, int64_t e, int N, int K, int row) {
   if constexpr (WT == W_BF16) {
@@ -301,8 +343,9 @@ __device__ __forceinline__ void set_load(Item<BL>& c, int b, const Weights& m, i
   } else {
     const int C = (K + 127) / 128, C4 = (C + 3) / 4;
     const int64_t at = e * ((N + 15) / 16) + row / 16;
-    c.base[b] = (uint64_t)((const char*)m.w + at * C * 1024);
-    c.exps[b] = (uint64_t)(m.exps + at * C4 * 256);
+    const int half = WT == W_FP4_8 ? row >> 3 & 1 : 0;  // (8 places of 16 and of 4 bytes)
+    c.base[b] = (uint64_t)((const char*)m.w + at * C * 1024 + half * 128);
+    c.exps[b] = (uint64_t)(m.exps + at * C4 * 256 + half * 32);
   }
 }
 
