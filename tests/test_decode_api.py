@@ -249,6 +249,7 @@ def test_python_refusals(monkeypatch):
         refused(TypeError, "x must be", functional.moe_decode, x[None], wr, w13, w2, K)
         refused(ValueError, "together", functional.moe_decode, t(65, D), wr, w13, w2, K, shared_w13=t(64, D))
         refused(ValueError, "shared_gate needs", functional.moe_decode, t(65, D), wr, w13, w2, K, shared_gate=t(1, D))
+        refused(TypeError, "w13 must be bfloat16", functional.moe_decode, t(65, D), wr, w13.float(), w2, K)
         # no backward
         g = lambda v: v.requires_grad_(True)  # noqa: E731
         refused(RuntimeError, "inference", ed, x, sc, idx, g(t(E, 2 * H, D)), w2)

@@ -153,7 +153,7 @@ def grouped_mm_e2m1(
         if bias.dtype not in (_BF16, torch.float32) or bias.numel() != N:
             raise ValueError(f"bias must be [{N}], bfloat16 or float32")
         bias = bias.contiguous()
-    out = torch.empty((*shape[:-1], N), dtype=_BF16, device=dev)
+    out = x.new_empty((*shape[:-1], N))
     _call(dev, "ttamd_grouped_mm_e2m1", x.data_ptr(), codes.data_ptr(), exps.data_ptr(), _p(offs), _p(bias),
           1 if bias is not None and bias.dtype is torch.float32 else 0, x.numel() // K, E, N, K, out.data_ptr(),
           _stream(dev))
@@ -285,11 +285,11 @@ def experts_decode(
     shared_w2: torch.Tensor | PackedWeights | None = None,
     shared_scale: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """Expert stage of at most 64 tokens on given picks, in two kernels
-    (ttamd_experts_decode): x bf16 [T, D], scores and indices [T, K] (int64 or
-    int32; one outside [0, E) adds nothing) -> bf16 [T, D].  Weights bf16 (w13 [E,
-    2H, D], w2 [E, D, H]) or all packed.  A shared expert [2Hs, D] / [D, Hs] is added
-    times shared_scale fp32 [T] (None: 1)."""
+    """Expert stage of at most 64 tokens on given picks (ttamd_experts_decode): x bf16
+    [T, D], scores and indices [T, K] (int64 or int32; one outside [0, E) adds
+    nothing) -> bf16 [T, D].  Weights bf16 (w13 [E, 2H, D], w2 [E, D, H]) or all
+    packed.  A shared expert [2Hs, D] / [D, Hs] is added times shared_scale fp32 [T]
+    (None: 1)."""
     dev = _gpu("x", x)
     _no_grad("experts_decode", x, top_scores, w13, w2, shared_w13, shared_w2, shared_scale)
     x = _rows(x)
@@ -308,8 +308,8 @@ def experts_decode(
         if Hs == 0 or shared_scale.numel() != T:
             raise ValueError(f"shared_scale must be [{T}] and needs a shared expert")
     lib = _lib._lib or _lib.load()
-    out = torch.empty_like(x)
-    ws = torch.empty(lib.ttamd_experts_decode_workspace_bytes(T, D, H, K, Hs), dtype=_U8, device=dev)
+    out = x.new_empty((T, D))
+    ws = x.new_empty(lib.ttamd_experts_decode_workspace_bytes(T, D, H, K, Hs), dtype=_U8)
     _call(dev, "ttamd_experts_decode", x.data_ptr(), T, D, H, E, K, idx.data_ptr(),
           1 if idx.dtype is torch.int64 else 0, top_scores.data_ptr(), 1 if score_before_experts else 0,
           _limit(swiglu_limit), *weights, Hs, *shared, _p(shared_scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
@@ -363,10 +363,10 @@ def moe_decode(
         if Hs == 0:
             raise ValueError("shared_gate needs a shared expert")
     lib = _lib._lib or _lib.load()
-    scores = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-    idx = torch.empty((T, top_k), dtype=torch.int64, device=dev)
-    out = torch.empty_like(x)
-    ws = torch.empty(lib.ttamd_moe_decode_workspace_bytes(T, D, H, E, top_k, Hs), dtype=_U8, device=dev)
+    scores = x.new_empty((T, top_k), dtype=torch.float32)
+    idx = x.new_empty((T, top_k), dtype=torch.int64)
+    out = x.new_empty((T, D))
+    ws = x.new_empty(lib.ttamd_moe_decode_workspace_bytes(T, D, H, E, top_k, Hs), dtype=_U8)
     _call(dev, "ttamd_moe_decode", x.data_ptr(), T, D, H, E, top_k, w_router.data_ptr(), _p(expert_bias), *groups,
           func, 1 if route_norm else 0, norm_eps, route_scale, 1 if score_before_experts else 0, _limit(swiglu_limit),
           *weights, Hs, *shared, _p(shared_gate), scores.data_ptr(), idx.data_ptr(), out.data_ptr(), ws.data_ptr(),
