@@ -99,10 +99,9 @@ struct Plan : PlanMap {
 constexpr int kPlanThreads = 1024;
 
 // What split_log needs beside the number of hit experts: items of an expert and of
-// the shared one, waves to share them, stages of an item, largest log2, cost of KS
-// waves' meeting.
+// the shared one, waves to share them, stages of an item, largest log2.
 struct Split {
-  int items, shared, slots, stages, most, meet;
+  int items, shared, slots, stages, most;
 };
 
 struct PlanArgs {
@@ -183,7 +182,7 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(const PlanArg
   if (tid == kPlanThreads - 1) p.hit() = hits;
   if (l == 0 && w >= kPlanThreads / 64 - 2) {  // (waves with little else to do)
     const Split& sp = a.split[w - (kPlanThreads / 64 - 2)];
-    p.split(w - (kPlanThreads / 64 - 2)) = split_log(hits * sp.items + sp.shared, sp.slots, sp.stages, sp.most, sp.meet);
+    p.split(w - (kPlanThreads / 64 - 2)) = split_log(hits * sp.items + sp.shared, sp.slots, sp.stages, sp.most);
   }
   dma::lds_barrier();
   if (mine >= 0) {
@@ -637,7 +636,7 @@ bool use_w13(const DecodeArgs& a, Choice& c) {
   const int64_t pairs = (int64_t)std::min(a.E, a.T * a.K) * (a.H / 16) + a.Hs / 16;
   c.w13 = go_w13<WT, NB, NS>;
   if constexpr (NB == 1 && NS == (WT == W_BF16 ? 3 : 5)) c.select_w13 = go_select_w13<WT, NB, NS>;
-  c.split[0] = {a.H / 16, a.Hs / 16, kWaves * (int)std::min<int64_t>(pairs, num_cus()), ceil_div(a.D, Rg::kCols), 3, 1};
+  c.split[0] = {a.H / 16, a.Hs / 16, kWaves * (int)std::min<int64_t>(pairs, num_cus()), ceil_div(a.D, Rg::kCols), 3};
   return true;
 }
 
@@ -665,7 +664,7 @@ bool use_w2(const DecodeArgs& a, Choice& c) {
   const int most = w2_log<WT, BL, NB, NS>(a);
   if (most < 0) return false;
   c.w2 = go_w2<WT, BL, NB, NS>;
-  c.split[1] = {1, a.Hs > 0, kWaves, ceil_div(std::max(a.H, a.Hs), Ring<WT, BL, NB, NS>::kCols), most, 0};
+  c.split[1] = {1, a.Hs > 0, kWaves, ceil_div(std::max(a.H, a.Hs), Ring<WT, BL, NB, NS>::kCols), most};
   return true;
 }
 
@@ -686,8 +685,8 @@ bool use_w2_bf16(const DecodeArgs& a, int rows, Choice& c) {
 
 bool choose_bf16(const DecodeArgs& a, Choice& c) {
   const int rows = a.T <= 8 ? 1 : ceil_div(a.T * a.K, a.E);
-  const bool first = rows <= 4    ? use_w13<W_BF16, 1, 3>(a, c)
-                     : rows <= 10 ? use_w13<W_BF16, 2, 3>(a, c) || use_w13<W_BF16, 2, 2>(a, c)
+  const bool first = rows <= 2   ? use_w13<W_BF16, 1, 3>(a, c)
+                     : rows <= 8 ? use_w13<W_BF16, 2, 3>(a, c) || use_w13<W_BF16, 2, 2>(a, c)
                                   : use_w13<W_BF16, 4, 2>(a, c);
   const int loads = ceil_div(a.D, 8 * num_cus());
   return first && ((loads <= 1 && use_w2_bf16<1>(a, rows, c)) || (loads <= 2 && use_w2_bf16<2>(a, rows, c)) ||
@@ -727,14 +726,25 @@ bool choose_fp4(const DecodeArgs& a, Choice& c) {
   // of them than the chip has CUs, or 8 where 16 would leave half of it idle (17 tokens
   // of 60 experts, 1440 rows: 18.2 us by 16, 17.2 by 8; 32 of 128, 2048 rows: 52 and 45).
   const int blocks = a.D / 16, cus = num_cus();
-  if (rows <= 2)
-    return (use_w13<W_FP4, 1, 5>(a, c) || use_w13<W_FP4, 1, 4>(a, c)) &&
-           ((2 * blocks <= cus && use_w2<W_FP4_8, 1, 2, 5>(a, c)) ||
-            (blocks <= cus && use_w2<W_FP4, 1, 1, 7>(a, c)) ||
-            (blocks > cus && use_w2<W_FP4, 2, 1, 4>(a, c)) || use_w2<W_FP4, 1, 2, 3>(a, c));
-  return (use_w13<W_FP4, 2, 4>(a, c) || use_w13<W_FP4, 2, 3>(a, c)) &&
-         ((2 * blocks <= cus && use_w2<W_FP4_8, 1, 4, 3>(a, c)) || (blocks <= cus && use_w2<W_FP4, 1, 2, 5>(a, c)) ||
-          (blocks > cus && use_w2<W_FP4, 2, 2, 3>(a, c)) || use_w2<W_FP4, 1, 2, 3>(a, c));
+  // lock_w2_kernel and its sums instead where items are a few stages, so that a stream
+  // waits for the plan more than for weights, and slots enough to pay for the launch (32
+  // tokens of 128 experts, 2048 x 768: 41 us, so 32; 8 tokens 18.9 and 19.4; 8 of 32
+  // experts, 7168 x 2048: 37 and 51), and where the LDS has no room for all slots' sums
+  // beside a ring (64 tokens of 128 experts: a ring of 3 stages 70 us, so 33).
+  bool first, second;
+  if (rows <= 2) {
+    first = use_w13<W_FP4, 1, 5>(a, c) || use_w13<W_FP4, 1, 4>(a, c);
+    second = 2 * blocks <= cus ? use_w2<W_FP4_8, 1, 2, 5>(a, c)
+             : blocks <= cus   ? use_w2<W_FP4, 1, 1, 7>(a, c)
+                               : use_w2<W_FP4, 2, 1, 4>(a, c);
+  } else {
+    first = use_w13<W_FP4, 2, 4>(a, c) || use_w13<W_FP4, 2, 3>(a, c);
+    second = 2 * blocks <= cus ? use_w2<W_FP4_8, 1, 4, 3>(a, c)
+             : blocks <= cus   ? use_w2<W_FP4, 1, 2, 5>(a, c)
+                               : use_w2<W_FP4, 2, 2, 3>(a, c);
+  }
+  if (!second || (S > 64 && std::max(a.H, a.Hs) <= 1024)) c.w2 = go_lock_w2<1, 5>;
+  return first;
 }
 
 template <int LPT, int PL>
@@ -837,7 +847,7 @@ hipError_t launch_experts_decode(const ExpertsDecode& c, const RouterDecode* rou
       a.gate = c.gate;
       for (int i = 0; i < 2; ++i) {
         const Split& sp = choice.split[i];
-        a.split[i] = split_log(a.K * sp.items + sp.shared, sp.slots, sp.stages, sp.most, sp.meet);
+        a.split[i] = split_log(a.K * sp.items + sp.shared, sp.slots, sp.stages, sp.most);
       }
       if (router) {
         t.log_run = log_run, t.per_lane = per_lane;

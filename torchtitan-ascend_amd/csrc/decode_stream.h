@@ -315,21 +315,21 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
   wait_vm<0>();
 }
 
-// Waves that share an item (log2) out of kWaves: rounds of the walk times a wave's
-// stages in one, twice, with `meet` for the meeting of KS waves.  From the experts
-// really hit, so that the last round is full: 112 experts of 1536 x 2048 make 2.6
-// rounds with whole row pairs and 21.0 with eighths.
-// A meeting counts as half a stage: its 1.5 us of latency pass while the next stages
-// load (96 rows of 68 experts of 1536 x 2048 in 4 bits: whole pairs 35.0 us, quarters,
-// which this chooses, 32.2).  One round that half the waves share already has the
-// chip's requests, and no next stages for a meeting to hide behind (41 experts' w13 of
-// 544 x 1440 in 4 bits: whole 12.9 us, quarters 14.4).
-__host__ __device__ inline int split_log(int items, int slots, int stages, int most, int meet = 1) {
+// Waves that share an item (log2): rounds of the walk times a wave's stages in one,
+// twice; half a stage for a meeting of KS waves, whose 1.5 us of latency pass while the
+// next stages load; half an item for the last round, where items of more rows end late.
+// From the experts really hit.  (128 experts of 1536 x 2048, 64 tokens, exactly 3 rounds
+// of whole pairs: whole 161 us, eighths, which this chooses, 134; 96 rows of 68
+// experts in 4 bits: whole 35.0 us, quarters 32.2.)  One round that half the waves share
+// already has the chip's requests, and no next stages for a meeting to hide behind (41
+// experts' w13 of 544 x 1440 in 4 bits: whole 12.9 us, quarters 14.4).
+__host__ __device__ inline int split_log(int items, int slots, int stages, int most) {
   if (items <= slots && 2 * items >= slots) return 0;
   int best = 0, cost = 0x7fffffff;
   for (int k = 0; k <= most && (1 << k) <= stages; ++k) {
     const int rounds = ((items << k) + slots - 1) / slots;
-    const int c = rounds * (2 * ((stages + (1 << k) - 1) >> k) + (k > 0 ? meet : 0));
+    const int st = (stages + (1 << k) - 1) >> k;
+    const int c = rounds * (2 * st + (k > 0)) + (rounds > 1 ? st : 0);
     if (c < cost) best = k, cost = c;
   }
   return best;
