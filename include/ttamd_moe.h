@@ -804,18 +804,21 @@ int ttamd_router_decode(const void* x, const void* w_router,
                         size_t workspace_bytes, void* stream);
 
 /*
- * The expert stage for a few tokens (at most 64) in two kernels: dispatch ->
- * w13 + SwiGLU -> w2 + score -> combine (npu_gmm.py:100-110 with :21-40) on given
- * picks; out bf16 [T, D].
+ * The expert stage for a few tokens (at most 64): dispatch -> w13 + SwiGLU -> w2 +
+ * score -> combine (npu_gmm.py:100-110 with :21-40) on given picks; out bf16 [T, D].
  *   a[s] = bf16(silu(min(g, L)) clamp(u, -L, L)), (g, u) = w13[e_s] x[t]
  *   out[t] = sum_k score[t, k] w2[e] a[t K + k] (+ gate[t] shared(x[t]))
  * with the score on g and u instead when score_before (npu_gmm.py dispatches
- * score * x).  All else is fp32, added over k in order, rounded once.
- *   indices: int64 or int32 [T, K]; one outside [0, E) adds nothing, a repeated
- *   one counts each time.  w13 [E, 2H, D] and w2 [E, D, H] in bf16 (exponents
- *   NULL), or all weights as 4-bit codes with their exponents.
+ * score * x).  All else is fp32, added over k in order, rounded once.  Equal calls
+ * give equal bits; a token's sums may be taken in other shares, and so differ in
+ * their last bits, when the other tokens hit other experts.
+ *   indices: int64 or int32 [T, K]; one outside [0, E) adds nothing (a token without
+ *   any gets zeros), a repeated one counts each time.  w13 [E, 2H, D] and w2 [E, D, H]
+ *   in bf16 (exponents NULL), or all weights as 4-bit codes with their exponents.
  *   shared_hidden > 0: a shared expert w13_shared [2 Hs, D], w2_shared [D, Hs] of
  *   the same type, times shared_gate fp32 [T] (nullable).
+ * A value that is not finite reaches its token's output, or that of the tokens that
+ * chose its expert, and no other.
  * topk <= 16, E <= 1024; D, H and Hs multiples of 32; swiglu_limit NaN: none.
  * workspace: ttamd_experts_decode_workspace_bytes (contents need no
  * initialisation; one call at a time).
@@ -836,9 +839,9 @@ int ttamd_experts_decode(const void* x, int64_t num_tokens, int64_t dim,
                          size_t workspace_bytes, void* stream);
 
 /*
- * Both in one call: router of the tokens, then their expert stage.  w_gate (bf16
- * [dim], nullable) needs shared_hidden > 0.  top_scores fp32 and top_indices int64
- * [T, K] are outputs.  workspace: ttamd_moe_decode_workspace_bytes.
+ * Both in one call: router of the tokens, then their expert stage (three to five
+ * kernels, capturable).  w_gate (bf16 [dim], nullable) needs shared_hidden > 0.
+ * top_scores fp32 and top_indices int64 [T, K] are outputs.  workspace: ttamd_moe_decode_workspace_bytes.
  */
 size_t ttamd_moe_decode_workspace_bytes(int64_t num_tokens, int64_t dim,
                                         int64_t hidden, int num_experts,

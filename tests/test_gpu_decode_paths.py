@@ -475,3 +475,23 @@ def test_one_token_of_any_router(decode, ops, bits, E, K, kw, biased):
     # the same token twice: the plan's kernel instead
     both = decode.moe_decode(x.expand(2, -1), wr, *w, K, **kw, **shared)
     assert torch.equal(both[1], s.expand(2, -1)) and torch.equal(both[2], i.expand(2, -1))
+
+
+@pytest.mark.parametrize("option", ["bf16", "e2m1"])
+def test_module_option_under_torch_compile(option):
+    pkg = importlib.import_module("torchtitan-ascend_amd")
+    E, K, D, H = 8, 2, 256, 128
+    rng = np.random.default_rng(5)
+    dispatcher = pkg.HipTokenDispatcher.Config(num_experts=E, top_k=K)
+    m = pkg.HipGroupedExperts(pkg.HipGroupedExperts.Config(
+        dim=D, hidden_dim=H, num_experts=E, token_dispatcher=dispatcher, decode_weights=option)).to(DEV).bfloat16()
+    m.init_weights()
+    if option == "e2m1":
+        m.pack_weights()
+    idx = torch.from_numpy(np.argsort(rng.random((2, 9, E)), axis=-1)[..., :K].copy()).to(DEV)
+    scores, x = torch.rand(2, 9, K, device=DEV), weights(rng, 2, 9, D, scale=1.0)
+    announce(f"compiled module {option}")
+    with torch.no_grad():
+        want = m(x, scores, idx)
+        # (the check that the 4-bit copies are of the present parameters breaks the graph)
+        assert torch.equal(torch.compile(m, backend="aot_eager", fullgraph=option == "bf16")(x, scores, idx), want)

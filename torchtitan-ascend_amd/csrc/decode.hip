@@ -669,8 +669,8 @@ bool use_w2(const DecodeArgs& a, Choice& c) {
 }
 
 // bf16.  Token rows per pass by the rows that an expert gets on average: a pass
-// more streams its weights again, a larger one takes LDS from the ring.  The second
-// product takes as few output rows per workgroup as give one workgroup per CU at
+// more streams its weights again, a larger one takes LDS from the ring (64 tokens, 4
+// rows each of 128 experts: w13 by 8 rows 176 us, by 16 161).  The second product takes as few output rows per workgroup as give one workgroup per CU at
 // most, where the slots' sums leave the room.
 template <int BL>
 bool use_w2_bf16(const DecodeArgs& a, int rows, Choice& c) {
@@ -723,8 +723,8 @@ bool choose_fp4(const DecodeArgs& a, Choice& c) {
     return true;
   }
   // The second product's workgroups own 16 output rows, or 32 where 16 would make more
-  // of them than the chip has CUs, or 8 where 16 would leave half of it idle (17 tokens
-  // of 60 experts, 1440 rows: 18.2 us by 16, 17.2 by 8; 32 of 128, 2048 rows: 52 and 45).
+  // of them than the chip has CUs, or 8 where 16 would leave half of it idle (2048 rows of
+  // 768: one token's 8 experts 7.3 us by 16, 6.3 by 8; 8 tokens' 50 experts 30 and 21).
   const int blocks = a.D / 16, cus = num_cus();
   // lock_w2_kernel and its sums instead where items are a few stages, so that a stream
   // waits for the plan more than for weights, and slots enough to pay for the launch (32
@@ -743,7 +743,7 @@ bool choose_fp4(const DecodeArgs& a, Choice& c) {
              : blocks <= cus   ? use_w2<W_FP4, 1, 2, 5>(a, c)
                                : use_w2<W_FP4, 2, 2, 3>(a, c);
   }
-  if (!second || (S > 64 && std::max(a.H, a.Hs) <= 1024)) c.w2 = go_lock_w2<1, 5>;
+  if (!second || (S > 64 && std::max(a.H, a.Hs) <= 1024)) c.w2 = go_lock_w2<1, 5>, c.select_w13 = nullptr;
   return first;
 }
 

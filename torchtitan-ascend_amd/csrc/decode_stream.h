@@ -320,11 +320,13 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
 // next stages load; half an item for the last round, where items of more rows end late.
 // From the experts really hit.  (128 experts of 1536 x 2048, 64 tokens, exactly 3 rounds
 // of whole pairs: whole 161 us, eighths, which this chooses, 134; 96 rows of 68
-// experts in 4 bits: whole 35.0 us, quarters 32.2.)  One round that half the waves share
-// already has the chip's requests, and no next stages for a meeting to hide behind (41
-// experts' w13 of 544 x 1440 in 4 bits: whole 12.9 us, quarters 14.4).
+// experts in 4 bits: whole 35.0 us, quarters 32.2.)  One round that half the chip's
+// waves share already has its requests, and no next stages for a meeting to hide behind
+// (41 experts' w13 of 544 x 1440 in 4 bits: whole 12.9 us, quarters 14.4); not so the
+// eight waves of a workgroup that walks by itself (5 experts and the shared one, w2 of
+// 5120 x 8192: whole 90 us, shared 75).
 __host__ __device__ inline int split_log(int items, int slots, int stages, int most) {
-  if (items <= slots && 2 * items >= slots) return 0;
+  if (slots > kWaves && items <= slots && 2 * items >= slots) return 0;
   int best = 0, cost = 0x7fffffff;
   for (int k = 0; k <= most && (1 << k) <= stages; ++k) {
     const int rounds = ((items << k) + slots - 1) / slots;
