@@ -495,3 +495,54 @@ def test_module_option_under_torch_compile(option):
         want = m(x, scores, idx)
         # (the check that the 4-bit copies are of the present parameters breaks the graph)
         assert torch.equal(torch.compile(m, backend="aot_eager", fullgraph=option == "bf16")(x, scores, idx), want)
+
+
+@pytest.mark.parametrize("T", [1, 5, 64])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_weights_past_32_bits(decode, T, bits):
+    """Experts that lie 5 GB apart give what they give side by side."""
+    E, K, D, H = (40, 2, 8192, 4096) if bits == 16 else (80, 2, 16384, 4096)
+    g = torch.Generator(DEV).manual_seed(T)
+    if bits == 16:
+        w = [torch.empty(E, 2 * H, D, dtype=BF16, device=DEV), torch.empty(E, D, H, dtype=BF16, device=DEV)]
+    else:
+        w = [decode.PackedWeights(torch.empty(c, dtype=torch.uint8, device=DEV),
+                                  torch.empty(e, dtype=torch.uint8, device=DEV), n, k)
+             for n, k in ((2 * H, D), (D, H)) for c, e in (decode._shapes(E, n, k),)]
+        assert w[0].codes.numel() > 2 ** 32
+    at = [0, E // 2, E - 1]
+    for t in w:
+        for e in at:
+            if bits == 16:
+                t[e] = torch.randn(t.shape[1:], generator=g, device=DEV) * 0.02
+            else:
+                t.codes[e] = torch.randint(0, 256, t.codes.shape[1:], generator=g, device=DEV, dtype=torch.uint8)
+                t.exponents[e] = 120
+    if bits == 16:
+        near = [t[at].clone() for t in w]
+        assert w[0].numel() * 2 > 2 ** 32
+    else:
+        near = [decode.PackedWeights(t.codes[at].clone(), t.exponents[at].clone(), t.rows, t.cols) for t in w]
+    x = torch.randn(T, D, generator=g, device=DEV).to(BF16)
+    idx = torch.stack([torch.arange(T, device=DEV) % 3, (torch.arange(T, device=DEV) + 2) % 3], 1)
+    scores = torch.rand(T, K, device=DEV)
+    announce(f"past 32 bits T={T} bits={bits}")
+    pad = torch.tensor(at, device=DEV)
+    y = decode.experts_decode(x, scores, pad[idx], *w)
+    z = decode.experts_decode(x, scores, idx, *near)
+    ref, bound = layer_ref(x, scores, idx, *(near if bits == 16 else map(decode.unpack_e2m1, near)), False, None)
+    for got in (y, z):  # (not the same bits: the choice of kernels goes by tokens per expert)
+        assert ((got.double() - ref).abs() - bound).max() <= 0
+
+
+@pytest.mark.parametrize("option", [None, "bf16"])
+def test_module_without_tokens(option):
+    pkg = importlib.import_module("torchtitan-ascend_amd")
+    m = pkg.HipGroupedExperts(pkg.HipGroupedExperts.Config(
+        dim=128, hidden_dim=128, num_experts=4, decode_weights=option,
+        token_dispatcher=pkg.HipTokenDispatcher.Config(num_experts=4, top_k=2))).to(DEV).bfloat16()
+    m.init_weights()
+    with torch.no_grad():
+        y = m(torch.empty(0, 3, 128, dtype=BF16, device=DEV), torch.empty(0, 3, 2, device=DEV),
+              torch.empty(0, 3, 2, dtype=torch.int64, device=DEV))
+    assert y.shape == (0, 128)
