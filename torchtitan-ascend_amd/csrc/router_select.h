@@ -358,15 +358,16 @@ __device__ __forceinline__ void select_token(const GroupTopkArgs& a, int64_t t, 
           z[m] = bf16_to_f32(q.x & 0xffff), z[m + 1] = bf16_to_f32(q.x >> 16);
           z[m + 2] = bf16_to_f32(q.y & 0xffff), z[m + 3] = bf16_to_f32(q.y >> 16);
         } else {
-          float4 q = *(const float4*)((const float*)a.z + at);
+          // (a vector, not a struct of floats, whose loads would be merged with the other
+          // branch's into 16 single ones: 16384 tokens of 256 experts 15.6 us so, 20.6)
+          floatx4_t q = *(const floatx4_t*)((const float*)a.z + at);
           if constexpr (SRC == SRC_PARTIALS) {
             for (int s = 1; s < a.S; ++s) {
-              const float4 p = *(const float4*)((const float*)a.z + at + (int64_t)s * a.T * a.E);
-              q.x += p.x, q.y += p.y, q.z += p.z, q.w += p.w;
+              q += *(const floatx4_t*)((const float*)a.z + at + (int64_t)s * a.T * a.E);
             }
-            q.x = round_bf16(q.x), q.y = round_bf16(q.y), q.z = round_bf16(q.z), q.w = round_bf16(q.w);
+            q = floatx4_t{round_bf16(q[0]), round_bf16(q[1]), round_bf16(q[2]), round_bf16(q[3])};
           }
-          z[m] = q.x, z[m + 1] = q.y, z[m + 2] = q.z, z[m + 3] = q.w;
+          z[m] = q[0], z[m + 1] = q[1], z[m + 2] = q[2], z[m + 3] = q[3];
         }
       }
     }
