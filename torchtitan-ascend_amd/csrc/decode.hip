@@ -18,6 +18,10 @@
 // adds the slots.  No kernel waits for another workgroup; every sum has its order, so
 // a call gives the same bits every time.  Labels outside [0, E) name no expert and add
 // nothing.
+// Measured, experts of 1536 x 2048 and 2048 x 768, 8 picks: one token 3.2 + 15 + 8 us
+// (bf16; 50 and 25 MB: each kernel's start and end are 3 to 4 us of it), 32 tokens of
+// 128 experts 6 + 7 + 118 + 60 us (5.9 TB/s); in 4 bits 3 + 11 + 6 and, with the sums,
+// 6 + 7 + 49 + 27 + 5.  Loads in flight bound all but the lock step (decode_stream.h).
 #include <algorithm>
 
 #include "decode_stream.h"

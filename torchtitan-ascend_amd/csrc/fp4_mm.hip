@@ -5,6 +5,9 @@
 // Bound by the weights' bytes (17/32 per value); the streams of decode_stream.h.  With
 // few rows per matrix a wave streams 32 output rows by itself, or KS waves together
 // where that fills the chip; with more, a workgroup's waves share the token rows.
+// Measured: 1 x 5120 x 8192 9.8 us (22 MB; 160 workgroups have rows), 13 x 1000 x 1440
+// 6.7, 96 rows of 68 of 128 matrices of 1536 x 2048 31.7 (114 MB, 4.5 TB/s between
+// start and end).
 #include <algorithm>
 
 #include "decode_stream.h"
