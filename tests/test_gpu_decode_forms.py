@@ -1,0 +1,83 @@
+"""The few-token operators and 4-bit weights in the forms beside the plain call: recorded
+and replayed, at the ends of the prompt's path, in every kernel that a size may take.
+
+Bounds: test_gpu_decode.py."""
+from __future__ import annotations
+
+import importlib
+import warnings
+
+import numpy as np
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from gpu_util import DEV, announce
+from test_gpu_decode import build, weights
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def decode():
+    return importlib.import_module("torchtitan-ascend_amd.decode")
+
+
+@pytest.fixture(scope="module")
+def functional():
+    return importlib.import_module("torchtitan-ascend_amd.functional")
+
+
+def equal(got, want):
+    got, want = (v if isinstance(v, tuple) else (v,) for v in (got, want))
+    assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------
+# Recordings
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [1, 9, 65])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_recordings_compute(decode, functional, T, bits):
+    """make_fx, torch.jit.trace and torch.compile of the layer on one input, replayed on
+    others, give the eager call's bits."""
+    rng = np.random.default_rng(T)
+    E, K, D, H = 8, 2, 256, 128
+    w, _ = build(decode, rng, E, D, H, bits, 128)
+    wr, wg = weights(rng, E, D), weights(rng, 1, D)
+    proj = decode.pack_e2m1(weights(rng, D, D))
+
+    def step(x):
+        h = functional.grouped_mm_e2m1(x, proj)
+        return functional.moe_decode(h, wr, *w[:2], K, shared_w13=w[2], shared_w2=w[3], shared_gate=wg)
+
+    x = weights(rng, T, D, scale=1.0)
+    announce(f"recordings T={T} bits={bits}")
+    with torch.no_grad(), warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        forms = [make_fx(step)(x), torch.jit.trace(step, (x,), check_trace=False),
+                 torch.compile(step, backend="aot_eager", fullgraph=True)]
+        for i in range(3):
+            xi = weights(rng, T, D, scale=1.0 + i)
+            want = step(xi)
+            for f in forms:
+                equal(f(xi), want)
+
+
+@pytest.mark.parametrize("name", ["pack", "pack_matrix", "unpack", "router", "router_gate"])
+def test_opcheck_of_weights_and_router(decode, name):
+    importlib.import_module("torchtitan-ascend_amd.library")
+    rng = np.random.default_rng(1)
+    x, wr, wg, w = (weights(rng, *s) for s in ((6, 96), (4, 96), (1, 96), (3, 20, 160)))
+    p = decode.pack_e2m1(w)
+    ops = torch.ops.ttamd
+    op, args = {
+        "pack": (ops.pack_e2m1, (w,)),
+        "pack_matrix": (ops.pack_e2m1, (w[0].float(),)),
+        "unpack": (ops.unpack_e2m1, (p.codes, p.exponents, p.rows, p.cols)),
+        "router": (ops.router_decode, (x, wr, 2, "softmax", False, 1.0, None, 1e-20, None, None, "top2", None)),
+        "router_gate": (ops.router_decode, (x, wr, 2, "sigmoid", True, 2.5, torch.rand(4, device=DEV), 1e-20, 2, 1,
+                                            "max", wg)),
+    }[name]
+    announce(f"opcheck {name}")
+    torch.library.opcheck(op, args)

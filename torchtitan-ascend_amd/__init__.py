@@ -10,9 +10,9 @@ The directory name is not a Python identifier; import it with
 `importlib.import_module("torchtitan-ascend_amd")`.  Importing it has no
 side effects: nothing is patched, nothing is loaded until an op runs.
 """
-from .decode import PackedWeights, grouped_mm_e2m1, pack_e2m1, tile_e2m1, unpack_e2m1
-from .functional import (HIPMoeTokenUnpermute, moe_block, moe_decode, moe_experts_forward,
-                         run_experts_grouped_mm)
+from .decode import PackedWeights, tile_e2m1
+from .functional import (HIPMoeTokenUnpermute, grouped_mm_e2m1, moe_block, moe_decode, moe_experts_forward,
+                         pack_e2m1, run_experts_grouped_mm, unpack_e2m1)
 from .grouped_experts import HipGroupedExperts, HipGroupedExpertsConverter
 from .protocol import HAVE_TORCHTITAN
 from . import state_dict

@@ -10,7 +10,9 @@ under autograd with a tensor that requires a gradient raises.
 
 Like `ops`, every function allocates with torch's caching allocator and calls
 the C ABI on torch's current stream of its tensors' device; there is no
-fallback.  Reference: NpuGroupedExperts.forward with its router
+fallback.  A tracer sees nothing of such a call, so the functions refuse to run under
+one; those of the same names in `functional` take the registered ops there.
+Reference: NpuGroupedExperts.forward with its router
 (torchtitanturbo/models/common/npu_gmm.py:100-110; models/qwen3_5/model.py:752-809).
 """
 from __future__ import annotations
@@ -36,6 +38,18 @@ class PackedWeights(NamedTuple):
     exponents: torch.Tensor  # uint8 [E, ceil(N / 16), ceil(K / 512), 64, 4]
     rows: int  # N
     cols: int  # K
+
+
+_tracing, _included = torch._C._get_tracing_state, torch._C._dispatch_tls_is_dispatch_key_included
+_mode_count, _mode = torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode
+_PRE_DISPATCH, _PROXY = torch._C.DispatchKey.PreDispatch, torch._C._TorchDispatchModeKey.PROXY
+
+
+def _direct(name: str) -> None:
+    """Refuse a call under torch.jit.trace or make_fx, whose recording would hold the
+    outputs' allocation and not the kernels."""
+    if _tracing() is not None or _included(_PRE_DISPATCH) or _mode_count() and _mode(_PROXY) is not None:
+        raise RuntimeError(f"decode.{name} cannot be recorded by a tracer: call functional.{name}")
 
 
 def _no_grad(name: str, *tensors) -> None:
@@ -73,6 +87,7 @@ def pack_e2m1(w: torch.Tensor) -> PackedWeights:
     magnitude, or within 2^-2 of a 32-column group's scale where that is more.
     A group that holds a NaN or an infinity becomes NaN."""
     dev = _gpu("w", w)
+    _direct("pack_e2m1")
     _no_grad("pack_e2m1", w)
     if w.dim() not in (2, 3):
         raise ValueError(f"w must be [E, N, K] or [N, K], got {tuple(w.shape)}")
@@ -91,6 +106,7 @@ def unpack_e2m1(w: PackedWeights) -> torch.Tensor:
     """The bf16 values [E, N, K] of packed weights, exactly (ttamd_unpack_e2m1):
     for prompts, whose rows fill the grouped GEMMs."""
     dev = _gpu("w.codes", w.codes)
+    _direct("unpack_e2m1")
     codes, exps, E = _packed("w", w, dev)
     out = torch.empty(E, w.rows, w.cols, dtype=_BF16, device=dev)
     _call(dev, "ttamd_unpack_e2m1", _p(codes), _p(exps), E, w.rows, w.cols, _p(out), _stream(dev))
@@ -131,6 +147,7 @@ def grouped_mm_e2m1(
     weights again, so a prompt takes unpack_e2m1 and a matrix product.  Rows at or
     past offs[-1] are not written."""
     dev = _gpu("x", x)
+    _direct("grouped_mm_e2m1")
     _no_grad("grouped_mm_e2m1", x, bias)
     x = _want("x", x, _BF16)
     codes, exps, E = _packed("w", w, dev)
@@ -250,6 +267,7 @@ def router_decode(
     ops.router_topk's with groups (one group without num_groups).  shared_gate [1,
     D] bf16: gate = sigmoid of the token's bf16 product with it."""
     dev = _gpu("x", x)
+    _direct("router_decode")
     _no_grad("router_decode", x, w_router, shared_gate)
     x = _rows(x)
     w_router = _want("w_router", w_router, _BF16)
@@ -291,6 +309,7 @@ def experts_decode(
     packed.  A shared expert [2Hs, D] / [D, Hs] is added times shared_scale fp32 [T]
     (None: 1)."""
     dev = _gpu("x", x)
+    _direct("experts_decode")
     _no_grad("experts_decode", x, top_scores, w13, w2, shared_w13, shared_w2, shared_scale)
     x = _rows(x)
     T, D = x.shape
@@ -343,6 +362,7 @@ def moe_decode(
     experts_decode; shared_gate [1, D] scales the shared expert by sigmoid(x .
     shared_gate)."""
     dev = _gpu("x", x)
+    _direct("moe_decode")
     _no_grad("moe_decode", x, w_router, w13, w2, shared_w13, shared_w2, shared_gate)
     x = _rows(x)
     T, D = x.shape

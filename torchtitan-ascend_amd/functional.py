@@ -308,11 +308,78 @@ def _tensors(w) -> tuple:
 
 
 def _bf16_weights(w):
-    return decode.unpack_e2m1(w) if isinstance(w, PackedWeights) else w
+    return unpack_e2m1(w) if isinstance(w, PackedWeights) else w
 
 
 def _hidden(w13) -> int:
     return 0 if w13 is None else (w13.rows if isinstance(w13, PackedWeights) else w13.shape[-2]) // 2
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
+_transforms = torch._C._functorch.peek_interpreter_stack
+
+
+def _as_op(*args) -> bool:
+    """Whether something sees the call before the device does (torch.compile, a tracer,
+    a dispatch mode, a function transform, a tensor subclass): it takes the registered
+    op then.  Else the C call at once: an op's dispatch costs a call on one token more
+    than its kernels take, this check 0.8 us."""
+    if torch.compiler.is_compiling() or decode._mode_count() or decode._tracing() is not None:
+        return True
+    if decode._included(decode._PRE_DISPATCH) or _transforms() is not None:
+        return True
+    for t in args:
+        if type(t) not in _PLAIN and (type(t) is not PackedWeights or type(t.codes) is not torch.Tensor
+                                      or type(t.exponents) is not torch.Tensor):
+            return True
+    return False
+
+
+def pack_e2m1(w: torch.Tensor) -> PackedWeights:
+    """decode.pack_e2m1, or ttamd::pack_e2m1 under a tracer."""
+    if not _as_op(w):
+        return decode.pack_e2m1(w)
+    decode._no_grad("pack_e2m1", w)
+    return PackedWeights(*_T.pack_e2m1(w), *w.shape[-2:])
+
+
+def unpack_e2m1(w: PackedWeights) -> torch.Tensor:
+    """decode.unpack_e2m1, or ttamd::unpack_e2m1 under a tracer."""
+    return _T.unpack_e2m1(*w) if _as_op(w) else decode.unpack_e2m1(w)
+
+
+def grouped_mm_e2m1(
+    x: torch.Tensor, w: PackedWeights, offs: torch.Tensor | None = None, bias: torch.Tensor | None = None
+) -> torch.Tensor:
+    """decode.grouped_mm_e2m1, or ttamd::grouped_mm_e2m1 under a tracer."""
+    if not _as_op(x, w, offs, bias):
+        return decode.grouped_mm_e2m1(x, w, offs, bias)
+    decode._no_grad("grouped_mm_e2m1", x, bias)
+    return _T.grouped_mm_e2m1(x, w.codes, w.exponents, w.rows, offs, bias)
+
+
+def router_decode(
+    x: torch.Tensor,
+    w_router: torch.Tensor,
+    top_k: int,
+    score_func: str = "softmax",
+    route_norm: bool = False,
+    route_scale: float = 1.0,
+    expert_bias: torch.Tensor | None = None,
+    norm_eps: float = 1e-20,
+    num_groups: int | None = None,
+    topk_groups: int | None = None,
+    group_score: str = "top2",
+    shared_gate: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """decode.router_decode, or ttamd::router_decode under a tracer."""
+    args = (x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups, topk_groups,
+            group_score, shared_gate)
+    if not _as_op(x, w_router, expert_bias, shared_gate):
+        return decode.router_decode(*args)
+    decode._no_grad("router_decode", x, w_router, shared_gate)
+    scores, idx, gate = _T.router_decode(*args)
+    return scores, idx, None if shared_gate is None else gate
 
 
 def experts_decode(
@@ -327,11 +394,11 @@ def experts_decode(
     shared_w2: torch.Tensor | PackedWeights | None = None,
     shared_scale: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """decode.experts_decode; under torch.compile as the op ttamd::experts_decode
-    (whose dispatch costs a call on one token more than its kernels take)."""
-    if not torch.compiler.is_compiling():
+    """decode.experts_decode, or ttamd::experts_decode under a tracer."""
+    if not _as_op(x, top_scores, selected_experts_indices, w13, w2, shared_w13, shared_w2, shared_scale):
         return decode.experts_decode(x, top_scores, selected_experts_indices, w13, w2, score_before_experts,
                                      swiglu_limit, shared_w13, shared_w2, shared_scale)
+    decode._no_grad("experts_decode", x, top_scores, w13, w2, shared_w13, shared_w2, shared_scale)
     (t13, e13), (t2, e2), (u13, f13), (u2, f2) = map(_tensors, (w13, w2, shared_w13, shared_w2))
     return _T.experts_decode(x, top_scores, selected_experts_indices, t13, t2, _hidden(w13), score_before_experts,
                              swiglu_limit, e13, e2, _hidden(shared_w13), u13, u2, f13, f2, shared_scale)
@@ -360,7 +427,7 @@ def moe_decode(
     """The MoE layer of a serving step on one GPU, for batches of any length: x bf16
     [T, D] to (out bf16 [T, D], top_scores fp32 [T, K], selected_experts_indices
     int64 [T, K]); arguments as decode.moe_decode.  At most 64 tokens stream the
-    weights (decode.moe_decode; under torch.compile ttamd::moe_decode); a prompt takes
+    weights (decode.moe_decode; under a tracer ttamd::moe_decode); a prompt takes
     the router, the grouped GEMMs and the shared expert's pass, 4-bit weights
     restored to bf16 for the call (D % 128 == 0 and H % 128 == 0 there).  The two sum
     a logit in other orders, so tokens whose experts nearly tie may pick others.  No
@@ -386,7 +453,7 @@ def moe_decode(
             logits = None if shared_gate is None else x @ shared_gate.reshape(-1)
             out = shared_expert_combine(out, x, s13, s2, logits, swiglu_limit)
         return out, scores, idx
-    if not torch.compiler.is_compiling():
+    if not _as_op(x, w_router, w13, w2, expert_bias, shared_w13, shared_w2, shared_gate):
         return decode.moe_decode(x, w_router, w13, w2, top_k, score_func, route_norm, route_scale, expert_bias,
                                  norm_eps, num_groups, topk_groups, group_score, score_before_experts, swiglu_limit,
                                  shared_w13, shared_w2, shared_gate)

@@ -28,9 +28,10 @@ Reference ops these stand for (torchtitanturbo/models/common/):
   * ttamd::moe_experts_forward        the fused inference expert stage
   * ttamd::moe_block_forward          the inference block: norms, router, experts, residual
   * ttamd::shared_expert_add          shared-expert tail, qwen3_5/model.py:796-809
-  * ttamd::moe_decode / experts_decode / grouped_mm_e2m1
-                                      the layer, its expert stage and a product for a few
-                                      tokens, 4-bit weights as (codes, exponents) tensors
+  * ttamd::moe_decode / experts_decode / router_decode / grouped_mm_e2m1
+                                      the layer, its expert stage, its router and a product for
+                                      a few tokens, 4-bit weights as (codes, exponents) tensors
+  * ttamd::pack_e2m1 / unpack_e2m1    those weights from and to their values
   * ttamd::token_permute / token_unpermute (+ backward)
                                       npu_moe_token_permute / unpermute, npu_permute.py:74-88
 """
@@ -650,6 +651,48 @@ def _(routed_out, x, w13_shared, w2_shared, gate_logits, swiglu_limit):
 # ---------------------------------------------------------------------------
 def _packed_or(w: Optional[Tensor], exps: Optional[Tensor], rows: int, cols: int):
     return w if exps is None or w is None else decode.PackedWeights(w, exps, rows, cols)
+
+
+@torch.library.custom_op("ttamd::pack_e2m1", mutates_args=())
+def pack_e2m1(w: Tensor) -> tuple[Tensor, Tensor]:
+    """(codes, exponents) of weights [E, N, K] or [N, K]."""
+    return decode.pack_e2m1(w)[:2]
+
+
+@pack_e2m1.register_fake
+def _(w):
+    codes, exps = decode._shapes(w.shape[0] if w.dim() == 3 else 1, *w.shape[-2:])
+    return w.new_empty(codes, dtype=torch.uint8), w.new_empty(exps, dtype=torch.uint8)
+
+
+@torch.library.custom_op("ttamd::unpack_e2m1", mutates_args=())
+def unpack_e2m1(codes: Tensor, exponents: Tensor, rows: int, cols: int) -> Tensor:
+    """bf16 [E, rows, cols] of 4-bit weights."""
+    return decode.unpack_e2m1(decode.PackedWeights(codes, exponents, rows, cols))
+
+
+@unpack_e2m1.register_fake
+def _(codes, exponents, rows, cols):
+    return codes.new_empty((codes.shape[0], rows, cols), dtype=_BF16)
+
+
+@torch.library.custom_op("ttamd::router_decode", mutates_args=())
+def router_decode(x: Tensor, w_router: Tensor, top_k: int, score_func: str, route_norm: bool, route_scale: float,
+                  expert_bias: Optional[Tensor], norm_eps: float, num_groups: Optional[int],
+                  topk_groups: Optional[int], group_score: str,
+                  shared_gate: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
+    """Router of at most 64 tokens: (top_scores fp32 [T, K], indices int64 [T, K], gate fp32 [T] or empty)."""
+    scores, idx, gate = decode.router_decode(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias,
+                                             norm_eps, num_groups, topk_groups, group_score, shared_gate)
+    return scores, idx, scores.new_empty((0,)) if gate is None else gate
+
+
+@router_decode.register_fake
+def _(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups, topk_groups,
+      group_score, shared_gate):
+    T = x.shape[0]
+    return (x.new_empty((T, top_k), dtype=_F32), x.new_empty((T, top_k), dtype=torch.int64),
+            x.new_empty((0 if shared_gate is None else T,), dtype=_F32))
 
 
 @torch.library.custom_op("ttamd::grouped_mm_e2m1", mutates_args=())
