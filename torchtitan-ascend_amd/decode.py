@@ -40,15 +40,20 @@ class PackedWeights(NamedTuple):
     cols: int  # K
 
 
-_tracing, _included = torch._C._get_tracing_state, torch._C._dispatch_tls_is_dispatch_key_included
-_mode_count, _mode = torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode
+_tracing, _mode = torch._C._get_tracing_state, torch._C._get_dispatch_mode
+_included, _mode_count = torch._C._dispatch_tls_is_dispatch_key_included, torch._C._len_torch_dispatch_stack
 _PRE_DISPATCH, _PROXY = torch._C.DispatchKey.PreDispatch, torch._C._TorchDispatchModeKey.PROXY
+
+
+def _seen() -> bool:
+    """Whether a tracer or another dispatch mode is at work."""
+    return _mode_count() > 0 or _tracing() is not None or _included(_PRE_DISPATCH)
 
 
 def _direct(name: str) -> None:
     """Refuse a call under torch.jit.trace or make_fx, whose recording would hold the
     outputs' allocation and not the kernels."""
-    if _tracing() is not None or _included(_PRE_DISPATCH) or _mode_count() and _mode(_PROXY) is not None:
+    if _seen() and (_tracing() is not None or _included(_PRE_DISPATCH) or _mode(_PROXY) is not None):
         raise RuntimeError(f"decode.{name} cannot be recorded by a tracer: call functional.{name}")
 
 

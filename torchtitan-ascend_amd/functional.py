@@ -315,22 +315,20 @@ def _hidden(w13) -> int:
     return 0 if w13 is None else (w13.rows if isinstance(w13, PackedWeights) else w13.shape[-2]) // 2
 
 
-_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
 _transforms = torch._C._functorch.peek_interpreter_stack
+_PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
 
 
 def _as_op(*args) -> bool:
     """Whether something sees the call before the device does (torch.compile, a tracer,
     a dispatch mode, a function transform, a tensor subclass): it takes the registered
     op then.  Else the C call at once: an op's dispatch costs a call on one token more
-    than its kernels take, this check 0.8 us."""
-    if torch.compiler.is_compiling() or decode._mode_count() or decode._tracing() is not None:
-        return True
-    if decode._included(decode._PRE_DISPATCH) or _transforms() is not None:
+    than its kernels take."""
+    if torch.compiler.is_compiling() or decode._seen() or _transforms() is not None:
         return True
     for t in args:
-        if type(t) not in _PLAIN and (type(t) is not PackedWeights or type(t.codes) is not torch.Tensor
-                                      or type(t.exponents) is not torch.Tensor):
+        if type(t) not in _PLAIN and not (
+                type(t) is PackedWeights and type(t.codes) is type(t.exponents) is torch.Tensor):
             return True
     return False
 
