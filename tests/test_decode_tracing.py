@@ -209,3 +209,22 @@ def test_direct_calls_refuse_to_be_recorded(library):
                 with pytest.raises(RuntimeError, match=f"functional.{name}"):
                     trace(x)
             fn(x)
+
+
+@pytest.mark.parametrize("shape", [(9,), (3, 3), (1, 9), (0, 4)])
+def test_fakes_have_the_shapes_of_the_calls(library, shape):
+    """Rows [..., D] come back flat, traced or not."""
+    t = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype)  # noqa: E731
+    wr, gate, w, q = t(E, D), t(1, D), (t(E, 2 * H, D), t(E, D, H)), packed("cpu", 1, 2 * H, D)
+    idx, scores = t(*shape, K, dtype=torch.int64), t(*shape, K, dtype=F32)
+    o = torch.ops.ttamd
+    route = ("softmax", False, 1.0, None, 1e-20, None, None, "top2")
+    fns = [lambda x: (o.experts_decode(x, scores, idx, *w, H, False, None),),
+           lambda x: o.moe_decode(x, wr, *w, K, H, *route, False, None),
+           lambda x: o.router_decode(x, wr, K, *route, gate),
+           lambda x: (o.grouped_mm_e2m1(x, q.codes, q.exponents, 2 * H, None, None),)]
+    x = t(*shape, D)
+    for fn in fns:
+        real = [(v.shape, v.stride(), v.dtype) for v in fn(x)]
+        with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            assert [(v.shape, v.stride(), v.dtype) for v in fn(mode.from_tensor(x))] == real

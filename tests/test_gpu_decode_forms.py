@@ -81,3 +81,23 @@ def test_opcheck_of_weights_and_router(decode, name):
     }[name]
     announce(f"opcheck {name}")
     torch.library.opcheck(op, args)
+
+
+@pytest.mark.parametrize("name", ["experts", "layer", "router"])
+def test_opcheck_of_rows_in_a_batch(decode, name):
+    """x [B, S, D]: the rows come back flat, as the ops' shapes say."""
+    importlib.import_module("torchtitan-ascend_amd.library")
+    rng = np.random.default_rng(2)
+    E, K, D, H = 4, 2, 96, 64
+    w, _ = build(decode, rng, E, D, H, 16)
+    x, wr, wg = weights(rng, 2, 3, D, scale=1.0), weights(rng, E, D), weights(rng, 1, D)
+    idx = torch.from_numpy(np.argsort(rng.random((2, 3, E)), axis=2)[..., :K].copy()).to(DEV)
+    ops = torch.ops.ttamd
+    route = ("softmax", True, 1.0, None, 1e-20, None, None, "top2")
+    op, args = {
+        "experts": (ops.experts_decode, (x, torch.rand(2, 3, K, device=DEV), idx, *w, H, False, None)),
+        "layer": (ops.moe_decode, (x, wr, *w, K, H, *route, False, None)),
+        "router": (ops.router_decode, (x, wr, K, *route, wg)),
+    }[name]
+    announce(f"opcheck rows in a batch {name}")
+    torch.library.opcheck(op, args)

@@ -37,6 +37,7 @@ Reference ops these stand for (torchtitanturbo/models/common/):
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -649,6 +650,11 @@ def _(routed_out, x, w13_shared, w2_shared, gate_logits, swiglu_limit):
 # weights with their exponents; what a tile's padding hides of N and K follows from
 # x, w13's hidden size and the other weights
 # ---------------------------------------------------------------------------
+def _num_tokens(x: Tensor) -> int:
+    """Rows of x [..., D]; the operators below take and return them flat."""
+    return math.prod(x.shape[:-1])
+
+
 def _packed_or(w: Optional[Tensor], exps: Optional[Tensor], rows: int, cols: int):
     return w if exps is None or w is None else decode.PackedWeights(w, exps, rows, cols)
 
@@ -690,7 +696,7 @@ def router_decode(x: Tensor, w_router: Tensor, top_k: int, score_func: str, rout
 @router_decode.register_fake
 def _(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups, topk_groups,
       group_score, shared_gate):
-    T = x.shape[0]
+    T = _num_tokens(x)
     return (x.new_empty((T, top_k), dtype=_F32), x.new_empty((T, top_k), dtype=torch.int64),
             x.new_empty((0 if shared_gate is None else T,), dtype=_F32))
 
@@ -724,7 +730,7 @@ def experts_decode(x: Tensor, top_scores: Tensor, idx: Tensor, w13: Tensor, w2: 
 @experts_decode.register_fake
 def _(x, top_scores, idx, w13, w2, hidden, score_before, swiglu_limit, e13=None, e2=None, shared_hidden=0,
       shared_w13=None, shared_w2=None, shared_e13=None, shared_e2=None, shared_scale=None):
-    return x.new_empty(x.shape)
+    return x.new_empty((_num_tokens(x), x.shape[-1]))
 
 
 @torch.library.custom_op("ttamd::moe_decode", mutates_args=())
@@ -748,8 +754,9 @@ def moe_decode(x: Tensor, w_router: Tensor, w13: Tensor, w2: Tensor, top_k: int,
 def _(x, w_router, w13, w2, top_k, hidden, score_func, route_norm, route_scale, expert_bias, norm_eps, num_groups,
       topk_groups, group_score, score_before, swiglu_limit, e13=None, e2=None, shared_hidden=0, shared_w13=None,
       shared_w2=None, shared_e13=None, shared_e2=None, shared_gate=None):
-    T = x.shape[0]
-    return (x.new_empty(x.shape), x.new_empty((T, top_k), dtype=_F32), x.new_empty((T, top_k), dtype=torch.int64))
+    T = _num_tokens(x)
+    return (x.new_empty((T, x.shape[-1])), x.new_empty((T, top_k), dtype=_F32),
+            x.new_empty((T, top_k), dtype=torch.int64))
 
 
 # ---------------------------------------------------------------------------
