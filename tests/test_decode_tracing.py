@@ -228,3 +228,17 @@ def test_fakes_have_the_shapes_of_the_calls(library, shape):
         real = [(v.shape, v.stride(), v.dtype) for v in fn(x)]
         with FakeTensorMode(allow_non_fake_inputs=True) as mode:
             assert [(v.shape, v.stride(), v.dtype) for v in fn(mode.from_tensor(x))] == real
+
+
+@pytest.mark.parametrize("experts,runs", [(256, 0), (257, 2), (300, 2), (1024, 4)])
+@pytest.mark.parametrize("groups", [{}, dict(num_groups=1, topk_groups=1)])
+def test_prompts_of_more_experts_than_the_fused_router_takes(library, experts, runs, groups):
+    t = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
+    wr, w = t(experts, D), (t(experts, 2, D), t(experts, D, 1))
+    with torch.no_grad():
+        graph = make_fx(lambda x: functional.moe_decode(x, wr, *w, K, **groups))(t(65, D))
+    routers = ["router"] * runs + ["router_topk"] if runs else ["router"]
+    assert recorded(graph.graph) == [*routers, "route", "moe_experts_forward"]
+    sizes = [n.args[1].meta["val"].shape[0] if runs else experts for n in graph.graph.nodes
+             if str(n.target) == "ttamd.router.default"]
+    assert sum(sizes) == experts and max(sizes) <= 256

@@ -101,3 +101,50 @@ def test_opcheck_of_rows_in_a_batch(decode, name):
     }[name]
     announce(f"opcheck rows in a batch {name}")
     torch.library.opcheck(op, args)
+
+
+# ---------------------------------------------------------------------------
+# Prompts
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("T,E,K", [(65, 257, 2), (65, 300, 8), (200, 1024, 16), (130, 512, 1)])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("form", ["plain", "groups", "bias"])
+def test_prompts_of_many_experts(decode, functional, T, E, K, bits, form):
+    """The prompt's path takes as many experts as the few-token layer.  A logit is the
+    bf16 of an fp32 sum, within b = 2^-8 |z| + (D + 8) 2^-24 sum |x w| (1 + 2^-8) of the
+    64-bit z; picks are right within b, scores within a factor e^(2 b) and fp32."""
+    rng = np.random.default_rng(T + E)
+    D, H = 128, 128
+    w, wb = build(decode, rng, E, D, H, bits)
+    x, wr = weights(rng, T, D, scale=1.0), weights(rng, E, D)
+    kw, func = {}, "softmax"
+    if form == "groups":
+        G = 4 if E % 4 == 0 else 1
+        kw = dict(num_groups=G, topk_groups=max(1, G // 2), group_score="max")
+    if form == "bias":
+        kw, func = dict(expert_bias=torch.randn(E, device=DEV) * 0.05), "sigmoid"
+    announce(f"prompt T={T} E={E} K={K} bits={bits} {form}")
+    out, s, i = functional.moe_decode(x, wr, *w, K, func, **kw)
+    with torch.no_grad():
+        assert torch.equal(out, functional.moe_experts_forward(x, s, i, *wb, E, False))
+    z = x.double() @ wr.double().t()
+    size = x.double().abs() @ wr.double().abs().t()
+    b = (2.0 ** -8 * z.abs() + (1 + 2.0 ** -8) * (D + 8) * 2.0 ** -24 * size).amax().item()
+    p = torch.softmax(z, 1) if func == "softmax" else torch.sigmoid(z)
+    near = np.exp(2 * b) * (1 + 2.0 ** -20)
+    ratio = s.double() / p.gather(1, i)
+    assert ratio.max() <= near and ratio.min() >= 1 / near
+    # selection values: b moves a sigmoid by at most b / 4, a softmax score by the factor above
+    v = p if form != "bias" else p + kw["expert_bias"].double()
+    slack = b / 4 + 2.0 ** -20 if form == "bias" else (near - 1) * p.amax().item()
+    if form == "groups" and kw["num_groups"] > 1:
+        best = v.view(T, kw["num_groups"], -1).amax(2)
+        kept = torch.zeros_like(best, dtype=torch.bool).scatter_(1, i // (E // kw["num_groups"]), True)
+        assert (kept.sum(1) <= kw["topk_groups"]).all()
+        last = best.topk(kw["topk_groups"], 1).values[:, -1]
+        assert (torch.where(kept, best, torch.inf).amin(1) >= last - 2 * slack).all()
+        v = torch.where(kept.repeat_interleave(E // kw["num_groups"], 1), v, -torch.inf)
+    worst = v.gather(1, i).amin(1)
+    rest = v.scatter(1, i, -torch.inf).amax(1)
+    assert (rest - worst <= 2 * slack).all()
+    assert (i.sort(1).values.diff(dim=1) > 0).all()  # no expert twice

@@ -402,6 +402,19 @@ def experts_decode(
                              swiglu_limit, e13, e2, _hidden(shared_w13), u13, u2, f13, f2, shared_scale)
 
 
+def _prompt_router(x, w_router, top_k, func, norm, scale, bias, eps, num_groups, topk_groups, group_score):
+    """functional.router for as many experts as the few-token layer takes: the fused gate
+    holds 256, so of more the logits come from it run by run, and the selection from them
+    (with groups, whose 64-bit form that layer's selection is)."""
+    if w_router.shape[0] <= 256:
+        return router(x, w_router, top_k, func, norm, scale, bias, eps, num_groups, topk_groups, group_score)
+    x = x.contiguous()
+    logits = torch.cat([_T.router(x, w, 1, func, False, 1.0, None, eps)[2] for w in w_router.split(256)], 1)
+    if num_groups is None and topk_groups is None:
+        num_groups = topk_groups = 1
+    return router_topk(logits, top_k, func, norm, scale, bias, eps, num_groups, topk_groups, group_score)
+
+
 def moe_decode(
     x: torch.Tensor,
     w_router: torch.Tensor,
@@ -442,8 +455,8 @@ def moe_decode(
                         ("shared_w2", shared_w2), ("shared_gate", shared_gate)):
             if w is not None and not isinstance(w, PackedWeights) and w.dtype != _BF16:
                 raise TypeError(f"{name} must be bfloat16, got {w.dtype}")
-        scores, idx = router(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps,
-                             num_groups, topk_groups, group_score)
+        scores, idx = _prompt_router(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps,
+                                     num_groups, topk_groups, group_score)
         out = moe_experts_forward(x, scores, idx, _bf16_weights(w13), _bf16_weights(w2), w_router.shape[0],
                                   score_before_experts, swiglu_limit)
         if shared_w13 is not None:
