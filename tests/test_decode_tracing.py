@@ -155,6 +155,23 @@ def test_the_modules_option_is_recorded(library):
         assert recorded(graph.graph) == ["experts_decode"]
 
 
+@pytest.mark.parametrize("choices,ops", [(16, ["experts_decode"]), (17, ["route", "moe_experts_forward"]),
+                                         (64, ["route", "moe_experts_forward"])])
+@pytest.mark.parametrize("option", ["bf16", "e2m1"])
+def test_the_modules_option_leaves_many_choices_to_the_regular_path(library, option, choices, ops):
+    """More than 16 choices a token run as they do without the option."""
+    pkg = importlib.import_module("torchtitan-ascend_amd")
+    dispatcher = pkg.HipTokenDispatcher.Config(num_experts=64, top_k=choices)
+    m = pkg.HipGroupedExperts(pkg.HipGroupedExperts.Config(
+        dim=D, hidden_dim=64, num_experts=64, token_dispatcher=dispatcher, decode_weights=option)).bfloat16()
+    if option == "e2m1":
+        m.pack_weights()
+    idx, scores = torch.zeros(3, 3, choices, dtype=torch.int64), torch.zeros(3, 3, choices)
+    with torch.no_grad():
+        graph = make_fx(lambda x: m(x, scores, idx))(torch.zeros(3, 3, D, dtype=BF16))
+    assert recorded(graph.graph) == ops
+
+
 class Seen(TorchDispatchMode):
     def __init__(self):
         super().__init__()

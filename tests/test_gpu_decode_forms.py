@@ -148,3 +148,27 @@ def test_prompts_of_many_experts(decode, functional, T, E, K, bits, form):
     rest = v.scatter(1, i, -torch.inf).amax(1)
     assert (rest - worst <= 2 * slack).all()
     assert (i.sort(1).values.diff(dim=1) > 0).all()  # no expert twice
+
+
+@pytest.mark.parametrize("option", ["bf16", "e2m1"])
+def test_module_of_many_choices(option):
+    """More than 16 choices a token: the module's option changes nothing."""
+    pkg = importlib.import_module("torchtitan-ascend_amd")
+    E, K, D, H, T = 40, 20, 128, 64, 7
+    rng = np.random.default_rng(3)
+    idx = torch.from_numpy(np.argsort(rng.random((1, T, E)), axis=2)[..., :K].copy()).to(DEV)
+    scores, x = torch.rand(1, T, K, device=DEV), weights(rng, 1, T, D, scale=1.0)
+    w13, w2 = weights(rng, E, 2 * H, D), weights(rng, E, D, H)
+    out = []
+    for o in (None, option):
+        m = pkg.HipGroupedExperts(pkg.HipGroupedExperts.Config(
+            dim=D, hidden_dim=H, num_experts=E, decode_weights=o,
+            token_dispatcher=pkg.HipTokenDispatcher.Config(num_experts=E, top_k=K))).to(DEV).bfloat16()
+        with torch.no_grad():
+            m.w13.copy_(w13)
+            m.w2.copy_(w2)
+            if o == "e2m1":
+                m.pack_weights()
+            announce(f"module K={K} {o}")
+            out.append(m(x, scores, idx))
+    assert torch.equal(*out)

@@ -27,6 +27,7 @@ from .ops import _call, _gpu, _groups, _limit, _p, _same_device, _stream, _want
 _BF16 = torch.bfloat16
 _U8 = torch.uint8
 MAX_TOKENS = 64
+MAX_TOPK = 16
 
 
 class PackedWeights(NamedTuple):

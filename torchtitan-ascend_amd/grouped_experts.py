@@ -66,7 +66,7 @@ class HipGroupedExperts(Module):
         # (functional.moe_experts_forward, so with a local HipTokenDispatcher
         # only); None: in bf16
         activation_checkpoint: str | None = None
-        # how at most 64 tokens without autograd run on a local HipTokenDispatcher:
+        # how at most 64 tokens of 16 choices without autograd run on a local HipTokenDispatcher:
         # "bf16": from the parameters (where they are bf16) through
         # decode.experts_decode; "e2m1": through it from 4-bit copies, which
         # pack_weights() makes; None: as every other batch
@@ -143,7 +143,8 @@ class HipGroupedExperts(Module):
         selected_experts_indices = selected_experts_indices.view(bs * slen, top_k)
         disp = self.token_dispatcher
         if isinstance(disp, HipTokenDispatcher) and disp.is_local:
-            if self.decode_weights is not None and x.shape[0] <= decode.MAX_TOKENS and not torch.is_grad_enabled():
+            few_tokens = x.shape[0] <= decode.MAX_TOKENS and top_k <= decode.MAX_TOPK
+            if self.decode_weights is not None and few_tokens and not torch.is_grad_enabled():
                 few = self._decode_weights()
                 if few is not None:
                     out = experts_decode(x.to(torch.bfloat16), top_scores, selected_experts_indices, *few,
