@@ -13,7 +13,7 @@ import torch
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from gpu_util import DEV, announce
-from test_gpu_decode import build, weights
+from test_gpu_decode import BF16, build, check_product, layer_ref, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -172,3 +172,130 @@ def test_module_of_many_choices(option):
             announce(f"module K={K} {o}")
             out.append(m(x, scores, idx))
     assert torch.equal(*out)
+
+
+# ---------------------------------------------------------------------------
+# What a call writes
+# ---------------------------------------------------------------------------
+GUARD = 4096
+
+
+class Guarded:
+    """A tensor between two guards, all of one byte value; written() after a call: which
+    rows changed, with the guards checked."""
+
+    def __init__(self, shape, dtype, fill=0xA5):
+        n = int(np.prod(shape)) * dtype.itemsize
+        self.raw = torch.full((2 * GUARD + n,), fill, dtype=torch.uint8, device=DEV)
+        self.fill, self.t = fill, self.raw[GUARD:GUARD + n].view(dtype).view(shape)
+
+    def check(self, rows):
+        """The guards and all rows but the given ones hold the fill, bit for bit."""
+        torch.cuda.synchronize()
+        assert (self.raw[:GUARD] == self.fill).all() and (self.raw[-GUARD:] == self.fill).all()
+        left = torch.ones(self.t.shape[0], dtype=torch.bool)
+        left[rows] = False
+        assert (self.t.view(torch.uint8).cpu()[left] == self.fill).all()
+
+
+def call(name, *args):
+    lib = importlib.import_module("torchtitan-ascend_amd._lib")
+    lib.call(name, *(a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args),
+             torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("counts,N,K", [
+    ([1], 40, 64), ([0, 3, 0, 1], 97, 1056), ([5, 0, 17, 64, 65, 2], 131, 512), ([0, 0, 0], 32, 32), ([1] * 60, 1536, 2048),
+    ([200, 1, 300], 31, 160), ([2] * 20, 18, 96), ([4, 3] * 8, 50, 288), ([30] * 5, 75, 544), ([100], 1003, 128)])
+@pytest.mark.parametrize("past", [0, 1, 5, 70])
+def test_rows_behind_the_last_run_stay(decode, counts, N, K, past):
+    """Rows at or past offs[-1], and what lies in front of and behind the output, hold
+    what they held."""
+    rng = np.random.default_rng(sum(counts) + N)
+    M, E = sum(counts) + past, len(counts)
+    x, p = weights(rng, M, K, scale=1.0), decode.pack_e2m1(weights(rng, E, N, K))
+    offs = torch.tensor(counts, device=DEV).cumsum(0).int()
+    announce(f"rows behind counts={counts[:8]} N={N} K={K} past={past}")
+    out = Guarded((M, N), BF16)
+    call("ttamd_grouped_mm_e2m1", x, p.codes, p.exponents, offs, None, 0, M, E, N, K, out.t)
+    out.check(slice(0, sum(counts)))
+    w, r = decode.unpack_e2m1(p), 0
+    for e, c in enumerate(counts):
+        if c:
+            check_product(x[r:r + c], w[e], out.t[r:r + c])
+        r += c
+
+
+def test_offsets_out_of_order_leave_rows(decode):
+    """Ends that fall, pass the rows or are negative: rows of no run, and all around the
+    output, stay."""
+    rng = np.random.default_rng(0)
+    E, M, N, K = 5, 12, 49, 96
+    p, x = decode.pack_e2m1(weights(rng, E, N, K)), weights(rng, M, K, scale=1.0)
+    w = decode.unpack_e2m1(p)
+    for offs, runs in (([-3, 4, 2, 99, 99], {1: (0, 4), 3: (2, 12)}), ([0, 0, -5, -1, 3], {4: (0, 3)}),
+                       ([7, 5, 5, 2, 2], {0: (0, 7)}), ([-9, -9, -9, -9, -9], {}),
+                       ([2 ** 31 - 1, -2 ** 31, 1, 3, 3], {0: (0, 12), 2: (0, 1), 3: (1, 3)})):
+        announce(f"offsets {offs}")
+        out = Guarded((M, N), BF16)
+        call("ttamd_grouped_mm_e2m1", x, p.codes, p.exponents, torch.tensor(offs, dtype=torch.int32, device=DEV), None, 0,
+             M, E, N, K, out.t)
+        rows = sorted({r for a, b in runs.values() for r in range(a, b)})
+        out.check(rows)
+        for e, (a, b) in runs.items():  # (rows of two runs hold either's)
+            own = [r for r in range(a, b) if sum(lo <= r < hi for lo, hi in runs.values()) == 1]
+            if own:
+                check_product(x[own], w[e], out.t[own])
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 5121, 160), (3, 17, 96), (13, 1001, 1440), (16, 33, 512), (17, 31, 288),
+                                   (40, 65, 96), (64, 15, 1056), (100, 130, 128)])
+def test_dense_products_write_their_rows_alone(decode, M, N, K):
+    rng = np.random.default_rng(M + N)
+    x, p, b = weights(rng, M, K, scale=1.0), decode.pack_e2m1(weights(rng, N, K)), Guarded((N,), BF16, 0x7F)
+    b.t.copy_(weights(rng, N))
+    announce(f"dense M={M} N={N} K={K}")
+    out = Guarded((M, N), BF16)
+    call("ttamd_grouped_mm_e2m1", x, p.codes, p.exponents, None, b.t, 0, M, 1, N, K, out.t)
+    out.check(slice(0, M))
+    check_product(x, decode.unpack_e2m1(p)[0], out.t, b.t)  # (the bias' guards are NaN)
+
+
+@pytest.mark.parametrize("E,N,K", [(1, 1, 32), (3, 17, 160), (2, 15, 1056), (1, 33, 96), (2, 100, 544)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_packing_writes_its_tiles_alone(decode, E, N, K, dtype):
+    rng = np.random.default_rng(N + K)
+    w = weights(rng, E, N, K).to(dtype)
+    want = decode.pack_e2m1(w)
+    codes, exps = (Guarded(s, torch.uint8) for s in decode._shapes(E, N, K))
+    out = Guarded((E, N, K), BF16)
+    announce(f"pack E={E} N={N} K={K} {dtype}")
+    call("ttamd_pack_e2m1", w, int(dtype == torch.float32), E, N, K, codes.t, exps.t)
+    call("ttamd_unpack_e2m1", codes.t, exps.t, E, N, K, out.t)
+    for g in (codes, exps, out):
+        g.check(slice(0, E))
+    assert torch.equal(codes.t, want.codes) and torch.equal(exps.t, want.exponents)
+    assert torch.equal(out.t, decode.unpack_e2m1(want))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("T,E,K,D,H,shared", [(1, 8, 2, 160, 96, 0), (5, 8, 2, 288, 32, 64), (33, 3, 3, 96, 64, 0),
+                                              (64, 40, 16, 64, 32, 32), (64, 2, 1, 2080, 288, 96)])
+def test_the_layer_writes_its_rows_and_its_workspace_alone(decode, T, E, K, D, H, shared, bits):
+    lib = importlib.import_module("torchtitan-ascend_amd._lib").load()
+    rng = np.random.default_rng(T + D)
+    w, _ = build(decode, rng, E, D, H, bits, shared)
+    x, wr = weights(rng, T, D, scale=1.0), weights(rng, E, D)
+    tensors = [t for p in w for t in ((p.codes, p.exponents) if bits == 4 else (p, None))]
+    tensors += [None] * (8 - len(tensors))
+    announce(f"layer writes T={T} E={E} D={D} bits={bits}")
+    out, scores, idx = Guarded((T, D), BF16), Guarded((T, K), torch.float32), Guarded((T, K), torch.int64)
+    nbytes = lib.ttamd_moe_decode_workspace_bytes(T, D, H, E, K, shared)
+    ws = Guarded((nbytes,), torch.uint8)
+    call("ttamd_moe_decode", x, T, D, H, E, K, wr, None, 1, 1, 0, 0, 0, 1e-20, 1.0, 0, float("nan"), *tensors[:4], shared,
+         *tensors[4:], None, scores.t, idx.t, out.t, ws.t, nbytes)
+    for g in (out, scores, idx):
+        g.check(slice(0, T))
+    ws.check(slice(0, nbytes))
+    want = decode.moe_decode(x, wr, *w[:2], K, shared_w13=w[2] if shared else None, shared_w2=w[3] if shared else None)
+    equal((out.t, scores.t, idx.t), want)
