@@ -299,3 +299,79 @@ def test_the_layer_writes_its_rows_and_its_workspace_alone(decode, T, E, K, D, H
     ws.check(slice(0, nbytes))
     want = decode.moe_decode(x, wr, *w[:2], K, shared_w13=w[2] if shared else None, shared_w2=w[3] if shared else None)
     equal((out.t, scores.t, idx.t), want)
+
+
+# ---------------------------------------------------------------------------
+# Every kernel that sizes choose
+# ---------------------------------------------------------------------------
+def gpu_weights(gen, *shape, scale=0.05):
+    return (torch.randn(*shape, device=DEV, generator=gen) * scale).to(BF16)
+
+
+# T, E, K, D, H, Hs; on 256 CUs these take each ring of both products in either type
+FORMS16 = [
+    (1, 4, 1, 96, 2080, 0), (1, 4, 1, 96, 288, 288), (1, 4, 3, 2080, 2080, 0), (1, 4, 1, 2080, 96, 288),
+    (1, 4, 2, 2880, 1440, 0), (1, 2, 2, 4096, 2080, 0), (1, 4, 1, 4128, 2080, 0), (1, 4, 1, 4128, 96, 288),
+    (1, 4, 1, 6400, 2080, 0), (1, 4, 1, 6400, 96, 288), (12, 4, 4, 2080, 1056, 64), (16, 4, 3, 96, 2080, 0),
+    (16, 4, 3, 2080, 2080, 0), (17, 4, 1, 2080, 2080, 0), (17, 4, 1, 2080, 96, 288), (9, 1, 1, 4096, 1056, 0),
+    (17, 4, 1, 4128, 2080, 0), (17, 4, 1, 4128, 96, 288), (17, 4, 1, 6400, 2080, 0), (9, 1, 1, 7168, 544, 0),
+    (17, 4, 1, 6400, 96, 288), (24, 4, 2, 96, 544, 288), (24, 128, 12, 6400, 96, 0), (32, 128, 16, 5120, 64, 0),
+    (32, 128, 16, 7168, 96, 0), (33, 4, 1, 96, 2080, 0), (33, 4, 1, 96, 288, 64), (33, 60, 13, 2080, 288, 0),
+    (33, 128, 14, 4128, 96, 0), (33, 128, 15, 2080, 96, 64), (33, 256, 16, 2080, 96, 0), (48, 128, 9, 4128, 96, 288),
+    (48, 128, 12, 96, 96, 64), (63, 16, 16, 96, 544, 64), (63, 60, 6, 2080, 288, 64), (63, 64, 4, 6400, 96, 64),
+    (63, 128, 9, 96, 288, 0), (64, 16, 14, 2080, 544, 0), (64, 16, 16, 128, 96, 96), (64, 256, 9, 96, 96, 288),
+    (64, 256, 10, 96, 288, 0),
+]
+FORMS4 = [
+    (1, 4, 1, 96, 2080, 0), (1, 4, 1, 96, 288, 288), (1, 4, 3, 2080, 2080, 0), (1, 4, 1, 2080, 96, 288),
+    (1, 4, 2, 2880, 1440, 0), (1, 2, 2, 4096, 2080, 0), (1, 4, 1, 4128, 2080, 0), (1, 4, 1, 4128, 96, 288),
+    (9, 4, 1, 96, 2080, 0), (9, 4, 1, 96, 288, 288), (9, 4, 1, 2080, 2080, 0), (9, 4, 1, 2080, 96, 288),
+    (5, 2, 1, 2880, 1056, 0), (5, 2, 1, 4096, 1056, 0), (16, 4, 1, 2880, 1056, 96), (9, 4, 1, 4128, 2080, 0),
+    (9, 4, 1, 4128, 96, 288), (17, 4, 1, 96, 2080, 0), (17, 4, 1, 96, 288, 288), (63, 256, 9, 96, 288, 0),
+    (63, 512, 14, 96, 96, 0), (4, 60, 4, 2080, 1056, 32), (8, 60, 2, 4128, 544, 0), (16, 64, 4, 2880, 1440, 0),
+]
+
+
+@pytest.mark.parametrize("bits,form", [(16, f) for f in FORMS16] + [(4, f) for f in FORMS4])
+@pytest.mark.parametrize("before", [False, True])
+def test_every_stream(decode, bits, form, before):
+    T, E, K, D, H, Hs = form
+    gen = torch.Generator(DEV).manual_seed(T + D + H)
+    w = [gpu_weights(gen, E, 2 * H, D), gpu_weights(gen, E, D, H)]
+    w += [gpu_weights(gen, 2 * Hs, D), gpu_weights(gen, D, Hs)] if Hs else []
+    wb, limit = w, 0.9 if before else None
+    if bits == 4:
+        w = [decode.pack_e2m1(t) for t in w]
+        wb = [decode.unpack_e2m1(p).view(t.shape) for p, t in zip(w, wb)]
+    x = gpu_weights(gen, T, D, scale=1.0)
+    idx = torch.rand(T, E, device=DEV, generator=gen).argsort(1)[:, :K].contiguous()
+    scores = torch.rand(T, K, device=DEV, generator=gen)
+    announce(f"streams T={T} E={E} K={K} D={D} H={H} Hs={Hs} bits={bits} before={before}")
+    y = decode.experts_decode(x, scores, idx, *w[:2], before, limit, *(w[2:] or (None, None)))
+    ref, bound = layer_ref(x, scores, idx, *wb[:2], before, limit, wb[2:] or None)
+    off = ((y.double() - ref).abs() - bound).max().item()
+    assert off <= 0, f"{off:.3e} past the bound"
+    again = decode.experts_decode(x, scores, idx, *w[:2], before, limit, *(w[2:] or (None, None)))
+    assert torch.equal(y, again)
+
+
+@pytest.mark.parametrize("T,E,K,groups", [
+    (61, 8, 1, None), (9, 64, 12, None), (32, 128, 8, None), (32, 128, 12, (4, 2)), (20, 160, 6, (8, 3)), (20, 192, 16, None),
+    (17, 256, 8, (8, 4)), (17, 256, 16, None), (9, 200, 8, (8, 4)), (9, 256, 16, (64, 20)), (5, 300, 4, (3, 2)),
+    (5, 512, 16, None), (33, 1024, 8, (64, 7)), (33, 1024, 16, None), (7, 990, 8, (33, 4)), (64, 1023, 16, (33, 20)),
+    (2, 961, 3, (31, 1)), (64, 63, 3, (63, 5)),
+])
+@pytest.mark.parametrize("func", ["softmax", "sigmoid"])
+def test_every_plan(decode, T, E, K, groups, func):
+    """The selection within the plan against the router's own kernel, and the stage on
+    the plan's picks against the one that is given them."""
+    rng = np.random.default_rng(T + E)
+    D, H = 64, 32
+    w, _ = build(decode, rng, E, D, H, 16)
+    x, wr = weights(rng, T, D, scale=1.0), weights(rng, E, D)
+    kw = {} if groups is None else dict(num_groups=groups[0], topk_groups=groups[1])
+    bias = torch.randn(E, device=DEV) * 0.05 if T % 2 else None
+    announce(f"plan T={T} E={E} K={K} {groups} {func}")
+    out, s, i = decode.moe_decode(x, wr, *w, K, func, True, 2.5, bias, **kw)
+    equal((s, i), decode.router_decode(x, wr, K, func, True, 2.5, bias, **kw)[:2])
+    assert torch.equal(out, decode.experts_decode(x, s, i, *w))
