@@ -172,6 +172,27 @@ def test_the_modules_option_leaves_many_choices_to_the_regular_path(library, opt
     assert recorded(graph.graph) == ops
 
 
+@pytest.mark.parametrize("tokens", [64, 65])
+def test_layers_refuse_weights_on_another_device(tokens):
+    """At either length, before a kernel gets their pointers."""
+    with FakeTensorMode(), torch.no_grad():
+        t = lambda *s, dev="cuda:0", dtype=BF16: torch.empty(*s, dtype=dtype, device=dev)  # noqa: E731
+        x, good = t(tokens, D), dict(w_router=(E, D), w13=(E, 2 * H, D), w2=(E, D, H), shared_w13=(2 * H, D),
+                                     shared_w2=(D, H), shared_gate=(1, D), expert_bias=(E,))
+        call = functional.moe_decode if tokens > 64 else decode.moe_decode
+        for dev in ("cpu", "cuda:1"):
+            for name in good:
+                kw = {n: t(*s, dev=dev if n == name else "cuda:0", dtype=F32 if n == "expert_bias" else BF16)
+                      for n, s in good.items()}
+                with pytest.raises(RuntimeError, match=name):
+                    call(x, top_k=K, **kw)
+            p = dict(w13=packed("cuda:0", E, 2 * H, D), w2=packed("cuda:0", E, D, H))
+            for name, field in (("w13", "codes"), ("w13", "exponents"), ("w2", "codes"), ("w2", "exponents")):
+                w = p[name]._replace(**{field: getattr(p[name], field).to(dev)})
+                with pytest.raises(RuntimeError, match=name):
+                    call(x, t(E, D), top_k=K, **(p | {name: w}))
+
+
 class Seen(TorchDispatchMode):
     def __init__(self):
         super().__init__()

@@ -452,9 +452,13 @@ def moe_decode(
         if shared_gate is not None and shared_w13 is None:
             raise ValueError("shared_gate needs a shared expert")
         for name, w in (("w_router", w_router), ("w13", w13), ("w2", w2), ("shared_w13", shared_w13),
-                        ("shared_w2", shared_w2), ("shared_gate", shared_gate)):
-            if w is not None and not isinstance(w, PackedWeights) and w.dtype != _BF16:
+                        ("shared_w2", shared_w2), ("shared_gate", shared_gate), ("expert_bias", expert_bias)):
+            packed = isinstance(w, PackedWeights)
+            if w is not None and not packed and w.dtype != _BF16 and w is not expert_bias:
                 raise TypeError(f"{name} must be bfloat16, got {w.dtype}")
+            for t in w[:2] if packed else (w,):
+                if t is not None and t.device != x.device:  # (a kernel would read through its pointer)
+                    raise RuntimeError(f"{name} is on {t.device}, expected {x.device}")
         scores, idx = _prompt_router(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps,
                                      num_groups, topk_groups, group_score)
         out = moe_experts_forward(x, scores, idx, _bf16_weights(w13), _bf16_weights(w2), w_router.shape[0],
