@@ -150,6 +150,33 @@ def test_prompts_of_many_experts(decode, functional, T, E, K, bits, form):
     assert (i.sort(1).values.diff(dim=1) > 0).all()  # no expert twice
 
 
+@pytest.mark.parametrize("T", [64, 65])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("Hs", [0, 192])
+def test_prompt_of_one_expert(decode, functional, T, bits, Hs):
+    """Weights [N, K] are one expert's; widths that are multiples of 64."""
+    rng = np.random.default_rng(T)
+    D, H = 256, 192
+    w, wb = build(decode, rng, 1, D, H, 16, Hs)
+    w = [t.reshape(t.shape[-2:]) for t in w]
+    if bits == 4:
+        w = [decode.pack_e2m1(t) for t in w]
+        wb = [decode.unpack_e2m1(p).view(t.shape) for p, t in zip(w, wb)]
+    x, wr = weights(rng, T, D, scale=1.0), weights(rng, 1, D)
+    announce(f"one expert T={T} bits={bits} Hs={Hs}")
+    kw = dict(shared_w13=w[2], shared_w2=w[3]) if Hs else {}
+    out, s, i = functional.moe_decode(x, wr, *w[:2], 1, **kw)
+    assert (s == 1).all() and (i == 0).all()
+    if T > 64:
+        with torch.no_grad():
+            want = functional.moe_experts_forward(x, s, i, *wb[:2], 1, False)
+            want = functional.shared_expert_combine(want, x, *wb[2:]) if Hs else want
+        assert torch.equal(out, want)
+        return
+    ref, bound = layer_ref(x, s, i, *wb[:2], False, None, wb[2:] or None)
+    assert ((out.double() - ref).abs() - bound).max() <= 0
+
+
 @pytest.mark.parametrize("option", ["bf16", "e2m1"])
 def test_module_of_many_choices(option):
     """More than 16 choices a token: the module's option changes nothing."""

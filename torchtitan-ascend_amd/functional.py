@@ -308,7 +308,9 @@ def _tensors(w) -> tuple:
 
 
 def _bf16_weights(w):
-    return unpack_e2m1(w) if isinstance(w, PackedWeights) else w
+    """bf16 [E, N, K] of weights in either form; [N, K] is one expert."""
+    w = unpack_e2m1(w) if isinstance(w, PackedWeights) else w
+    return w if w.dim() == 3 else w.unsqueeze(0)
 
 
 def _hidden(w13) -> int:
@@ -459,6 +461,11 @@ def moe_decode(
             for t in w[:2] if packed else (w,):
                 if t is not None and t.device != x.device:  # (a kernel would read through its pointer)
                     raise RuntimeError(f"{name} is on {t.device}, expected {x.device}")
+        if isinstance(w13, PackedWeights) != isinstance(w2, PackedWeights):
+            raise TypeError("w13 and w2 must both be bfloat16 or both packed")
+        if any(w is not None and isinstance(w, PackedWeights) != isinstance(w13, PackedWeights)
+               for w in (shared_w13, shared_w2)):
+            raise TypeError("the shared expert's weights must be of the experts' type")
         scores, idx = _prompt_router(x, w_router, top_k, score_func, route_norm, route_scale, expert_bias, norm_eps,
                                      num_groups, topk_groups, group_score)
         out = moe_experts_forward(x, scores, idx, _bf16_weights(w13), _bf16_weights(w2), w_router.shape[0],
