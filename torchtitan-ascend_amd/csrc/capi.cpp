@@ -1174,7 +1174,7 @@ size_t ttamd_experts_decode_workspace_bytes(int64_t num_tokens, int64_t dim, int
   if (num_tokens < 0 || num_tokens > ttamd::kDecodeMaxTokens || dim < 1 || hidden < 1 || topk < 1 ||
       topk > ttamd::kDecodeMaxTopk || shared_hidden < 0)
     return 0;
-  return ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden, true);
+  return ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden);
 }
 
 int ttamd_experts_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts, int topk,
@@ -1195,7 +1195,7 @@ int ttamd_experts_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t
   TRY(check_ptr16(fn, "out", out));
   REQUIRE(indices && top_scores, "%s: null pointer argument", fn);
   TRY(check_ws(fn, workspace, workspace_bytes,
-               ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden, true)));
+               ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden)));
   return check_hip(ttamd::launch_experts_decode(decode_args(w, x, num_tokens, dim, hidden, num_experts, topk,
                                                             shared_hidden, indices, indices_are_int64 != 0, top_scores,
                                                             score_before, swiglu_limit, shared_gate, out),
@@ -1209,7 +1209,7 @@ size_t ttamd_moe_decode_workspace_bytes(int64_t num_tokens, int64_t dim, int64_t
       topk < 1 || topk > ttamd::kDecodeMaxTopk || shared_hidden < 0)
     return 0;
   return align256((size_t)num_tokens * 4) + ttamd::router_decode_workspace_bytes(num_tokens, num_experts) +
-         ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden, true);
+         ttamd::experts_decode_workspace_bytes(num_tokens, dim, hidden, topk, shared_hidden);
 }
 
 int ttamd_moe_decode(const void* x, int64_t num_tokens, int64_t dim, int64_t hidden, int num_experts, int topk,

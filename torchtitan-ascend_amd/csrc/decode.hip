@@ -803,11 +803,11 @@ hipError_t launch_router_decode(const RouterDecode& r, int T, int E, int D, int 
 }
 
 // Workspace: the plan, activations of the slots and of the shared expert, their
-// fp32 output rows.
-size_t experts_decode_workspace_bytes(int64_t T, int64_t D, int64_t H, int K, int64_t Hs, bool fp4) {
+// fp32 output rows (lock_w2_kernel's; of 4-bit weights, but one size serves both types).
+size_t experts_decode_workspace_bytes(int64_t T, int64_t D, int64_t H, int K, int64_t Hs) {
   const int64_t S = T * K;
   return al256(PlanMap{(int)T, (int)S}.bytes()) + al256((size_t)(S * H + (Hs > 0 ? T * Hs : 0)) * 2) +
-         (fp4 ? al256((size_t)(S + (Hs > 0 ? T : 0)) * D * 4) : 0);
+         al256((size_t)(S + (Hs > 0 ? T : 0)) * D * 4);
 }
 
 hipError_t launch_experts_decode(const ExpertsDecode& c, const RouterDecode* router, void* ws, hipStream_t stream) {

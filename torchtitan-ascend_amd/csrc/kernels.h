@@ -238,7 +238,7 @@ struct ExpertsDecode {
   const float* gate;
   void* out;
 };
-size_t experts_decode_workspace_bytes(int64_t T, int64_t D, int64_t H, int K, int64_t Hs, bool fp4);
+size_t experts_decode_workspace_bytes(int64_t T, int64_t D, int64_t H, int K, int64_t Hs);
 // router (nullable): its picks are made first (c.idx, c.scores and c.gate are its outputs).
 hipError_t launch_experts_decode(const ExpertsDecode& c, const RouterDecode* router, void* ws, hipStream_t stream);
 hipError_t launch_grouped_mm_fp4(const void* x, const void* codes, const void* exps, const int* offs, const void* bias,
