@@ -760,8 +760,8 @@ int ttamd_unpack_e4m3(const void* codes, const void* exponents,
  *              32 (l / 16) .. + 31 of the tile; byte b columns 2 b (low half) and
  *              2 b + 1
  *   exponents  uint8 [E, NB, ceil(C / 4), 64, 4]: place l of four tiles along K
- * Places outside [N, K] hold zeros.  K % 32 == 0; w bf16 or fp32 (w_is_fp32 = 1);
- * codes, exponents and w 16-byte aligned.
+ * Codes outside [N, K] are zeros; exponents there any byte but 255.  K % 32 == 0; w
+ * bf16 or fp32 (w_is_fp32 = 1); codes, exponents and w 16-byte aligned.
  */
 int ttamd_pack_e2m1(const void* w, int w_is_fp32, int64_t num_matrices,
                     int64_t n, int64_t k, void* codes, void* exponents,
@@ -776,8 +776,10 @@ int ttamd_unpack_e2m1(const void* codes, const void* exponents,
  * [M, K], out bf16 [M, N], sums in fp32, rounded once.  offs int32 [E] as in
  * ttamd_grouped_mm (rows at or past offs[E-1] are not written), or NULL with
  * num_experts = 1: all rows.  bias [N] (bias_is_fp32: fp32, else bf16) or NULL;
- * only without offs.  Meant for few rows: every 64 rows of an expert stream its
- * weights again.  K % 32 == 0.
+ * only without offs.  Meant for few rows: an expert's weights are streamed again for
+ * every 4, 8, 32 or 64 of its rows, where an expert has up to 2, 4, 32 or more rows on
+ * average (without offs 4, 8, 16, 32 or 64 for up to 2, 8, 16, 32 or more rows).
+ * K % 32 == 0.
  */
 int ttamd_grouped_mm_e2m1(const void* x, const void* codes,
                           const void* exponents, const int32_t* offs,

@@ -73,15 +73,16 @@ __device__ __forceinline__ u32x2_t activate(const floatx4_t& g, const floatx4_t&
 // ("places").
 struct PlanMap {
   int T, S;
-  __host__ __device__ constexpr int valid() const { return 16; }                   // uint32 [T]: choices that name an expert
-  __host__ __device__ constexpr int gate() const { return valid() + 4 * T; }       // float [T]: factor of the shared expert
-  __host__ __device__ constexpr int score() const { return gate() + 4 * T; }       // float [S], by place
-  __host__ __device__ constexpr int sorted() const { return score() + 4 * S; }     // short [S]: slot at a place
-  __host__ __device__ constexpr int inverse() const { return sorted() + 2 * S; }   // short [S]: place of a slot
-  __host__ __device__ constexpr int token() const { return inverse() + 2 * S; }    // short [S]: token at a place
-  __host__ __device__ constexpr int list() const { return token() + 2 * S; }       // short [hit]: experts
-  __host__ __device__ constexpr int start() const { return list() + 2 * S; }       // short [hit + 1]: their first places
-  __host__ __device__ constexpr int bytes() const { return (start() + 2 * (S + 1) + 15) & ~15; }  // at 0: hit, the splits
+  // at 0: hit, the splits
+  __host__ __device__ constexpr int valid() const { return 16; }  // uint32 [T]: which choices name an expert
+  __host__ __device__ constexpr int gate() const { return valid() + 4 * T; }      // float [T]: factor of the shared one
+  __host__ __device__ constexpr int score() const { return gate() + 4 * T; }      // float [S], by place
+  __host__ __device__ constexpr int sorted() const { return score() + 4 * S; }    // short [S]: slot at a place
+  __host__ __device__ constexpr int inverse() const { return sorted() + 2 * S; }  // short [S]: place of a slot
+  __host__ __device__ constexpr int token() const { return inverse() + 2 * S; }   // short [S]: token at a place
+  __host__ __device__ constexpr int list() const { return token() + 2 * S; }      // short [hit]: experts
+  __host__ __device__ constexpr int start() const { return list() + 2 * S; }      // short [hit + 1]: first places
+  __host__ __device__ constexpr int bytes() const { return (start() + 2 * (S + 1) + 15) & ~15; }
 };
 constexpr int kMaxPlanBytes = PlanMap{kDecodeMaxTokens, kMaxSlots}.bytes();
 
@@ -243,7 +244,9 @@ __device__ __forceinline__ void load_plan(const DecodeArgs& a, char* smem) {
 __device__ __forceinline__ int either(bool c, int x, int y) { return y ^ ((x ^ y) & -(int)c); }
 __device__ __forceinline__ Weights either(bool c, const Weights& x, const Weights& y) {
   const uint64_t m = c ? ~0ull : 0ull;
-  auto one = [&](const void* p, const void* q) { return (const void*)((uint64_t)q ^ (((uint64_t)p ^ (uint64_t)q) & m)); };
+  auto one = [&](const void* p, const void* q) {
+    return (const void*)((uint64_t)q ^ (((uint64_t)p ^ (uint64_t)q) & m));
+  };
   return {one(x.w, y.w), (const uint8_t*)one(x.exps, y.exps)};
 }
 
@@ -385,17 +388,17 @@ __global__ __launch_bounds__(kThreads, 2) void lock_w13_kernel(const DecodeArgs 
   lock_items<NR, NS>(
       smem + a.plan_lds, items.items(__builtin_amdgcn_readfirstlane(p.hit())), (a.D + 127) / 128,
       [&](int i, int r) __attribute__((always_inline)) { return items(i, r); },
-      [](const Item<2>& c, int) { return c.x; }, [&](const Item<2>& c, int, int i) __attribute__((always_inline)) { return items.src(c, i); },
+      [](const Item<2>& c, int) { return c.x; },
+      [&](const Item<2>& c, int, int i) __attribute__((always_inline)) { return items.src(c, i); },
       [&](const Item<2>& c, int i, int quad, const floatx4_t& v0, const floatx4_t& v1) __attribute__((always_inline)) {
         items.emit(c, c.pair, i, quad, v0, v1);
       });
 }
 
 // A workgroup owns the output rows of BL loads (8 each, 4 bits: 16) for every
-// expert; its waves (KS to a share of
-// the columns) take the hit experts in turn, the weighted rows of all slots meet in
-// LDS and leave as the tokens' sums: nothing goes through memory, no workgroup
-// waits for another, every sum has its order.
+// expert; its waves (KS to a share of the columns) take the hit experts in turn, the
+// weighted rows of all slots meet in LDS and leave as the tokens' sums: nothing goes
+// through memory, no workgroup waits for another, every sum has its order.
 template <int WT, int BL, int NB, int NS>
 __global__ __launch_bounds__(kThreads, 2) void stream_w2_kernel(const DecodeArgs a) {
   using Rg = Ring<WT, BL, NB, NS>;
@@ -620,9 +623,9 @@ struct Choice {
 template <int WT, int NB, int NS>
 hipError_t go_w13(const DecodeArgs& a, hipStream_t stream) {
   const int64_t pairs = (int64_t)std::min(a.E, a.T * a.K) * (a.H / 16) + a.Hs / 16;  // items at the finest
-  return launch_lds<stream_w13_kernel<WT, NB, NS>>(dim3((unsigned)std::min<int64_t>(pairs, num_cus())),
-                                                   a.plan_lds + Ring<WT, kPairLoads<WT>, NB, NS>::kAll + meet_bytes(kMeetRows),
-                                                   stream, a);
+  return launch_lds<stream_w13_kernel<WT, NB, NS>>(
+      dim3((unsigned)std::min<int64_t>(pairs, num_cus())),
+      a.plan_lds + Ring<WT, kPairLoads<WT>, NB, NS>::kAll + meet_bytes(kMeetRows), stream, a);
 }
 
 template <int WT, int NB, int NS>
@@ -672,10 +675,19 @@ bool use_w2(const DecodeArgs& a, Choice& c) {
   return true;
 }
 
-// bf16.  Token rows per pass by the rows that an expert gets on average: a pass
-// more streams its weights again, a larger one takes LDS from the ring (64 tokens, 4
-// rows each of 128 experts: w13 by 8 rows 176 us, by 16 161).  The second product takes as few output rows per workgroup as give one workgroup per CU at
-// most, where the slots' sums leave the room.
+// bf16.  Token rows per pass by the rows that an expert gets on average (up to 8
+// tokens fit one pass of 8 anyway): a pass more streams its weights again, a larger one
+// takes LDS from the ring.  The second product takes as few output rows per workgroup as
+// give one workgroup per CU at most, where the slots' sums leave the room.
+// Both sides (the stage of 8 picks from 32 experts of 1536 x 2048, captured, us; the
+// other product as chosen):
+//   w13, 8 / 16 rows a pass    average 4: 70 / 70, 5: 91 / 74
+//   w13, 16 / 32               average 10: 78 / 80, 12: 100 / 85
+//   w2, 8 / 16                 average 4: 71 / 71, 5: 74 / 74, 8: 85 / 76
+//   w2, 16 / 32                average 10: 81 / 84, 12: 86 / 85, 16: 89 / 84
+// The average counts the routed experts: a shared one of more tokens than a pass holds
+// is streamed again for every pass (16 experts of 5120 x 8192, one pick and a shared one
+// as wide: 32 tokens 827 us, 526 without it).
 template <int BL>
 bool use_w2_bf16(const DecodeArgs& a, int rows, Choice& c) {
   if (rows <= 4)
@@ -716,7 +728,11 @@ hipError_t go_lock_w2(const DecodeArgs& a, hipStream_t stream) {
 }
 
 // 4 bits.  A stream's token rows take as much LDS as its weights: for few rows per
-// expert, else all waves of a workgroup share them.
+// expert (up to 4 tokens fit one pass of 4), else all waves of a workgroup share them, as
+// they do for a shared expert of many tokens.  Both sides, streams / lock step (8 picks,
+// captured, us): 32 experts of 1536 x 2048, average 4: 36 / 39, 5: 45 / 39; 4096 x 7168, 4:
+// 148 / 162, 6: 171 / 164; with a shared expert, 16 tokens 169 / 170, 20 186 / 170 (128 of
+// 1536 x 2048: 12 tokens 68 / 64, 16 76 / 71, 20 86 / 80).
 bool choose_fp4(const DecodeArgs& a, Choice& c) {
   const int64_t S = (int64_t)a.T * a.K;
   const int rows = a.T <= 4 ? 1 : ceil_div(S, a.E);
@@ -735,6 +751,10 @@ bool choose_fp4(const DecodeArgs& a, Choice& c) {
   // tokens of 128 experts, 2048 x 768: 41 us, so 32; 8 tokens 18.9 and 19.4; 8 of 32
   // experts, 7168 x 2048: 37 and 51), and where the LDS has no room for all slots' sums
   // beside a ring (64 tokens of 128 experts: a ring of 3 stages 70 us, so 33).
+  // Around these bounds (the stage, captured, streams / lock step, us): 2048 x 768, 64 slots
+  // 52.5 / 51.8, 96 63.6 / 61.9, 128 68.0 / 63.3; 128 slots, H = 1024 83.6 / 79.3, H = 1280
+  // 98.4 / 89.7, so that 2048 columns would gain past 1024 too; 4096 columns do not below:
+  // 96 slots of 4096 x 768 89.6 / 92.2, x 1024 107.5 / 111.7.
   bool first, second;
   if (rows <= 2) {
     first = use_w13<W_FP4, 1, 5>(a, c) || use_w13<W_FP4, 1, 4>(a, c);

@@ -84,8 +84,8 @@ __device__ __forceinline__ void issue_tiles(const Item<BL>& c, int s, uint32_t a
 // of its token rows (256 bytes each at rows_at, chunk c of row r at c ^ r); ROWS: how
 // many rows the stage holds.
 template <int BL, int NT, int ROWS, int ALL, class Free>
-__device__ __forceinline__ void consume_tiles(floatx4_t (&acc)[BL][ALL], const char* st, int exps_at, const char* rows_at,
-                                              int cs, int left, Free free) {
+__device__ __forceinline__ void consume_tiles(floatx4_t (&acc)[BL][ALL], const char* st, int exps_at,
+                                              const char* rows_at, int cs, int left, Free free) {
   const int l = threadIdx.x & 63, n = l & 15, q = l >> 4;
   uint4 qw[BL];
   float scale[BL];
@@ -177,7 +177,9 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
   auto chunk8 = [&](int i) { return (l & 7) ^ cswz(8 * i + (l >> 3)); };
   auto chunk16 = [&](int i) { return (l & 15) ^ ((4 * i + (l >> 4)) & 15); };
   auto chunk32 = [&](int i) { return (l & 31) ^ ((2 * i + (l >> 5)) & 15); };
-  auto row_of = [&](int i) { return WT == W_BF16 ? 8 * i + (l >> 3) : WT == W_FP4 ? 4 * i + (l >> 4) : 2 * i + (l >> 5); };
+  auto row_of = [&](int i) {
+    return WT == W_BF16 ? 8 * i + (l >> 3) : WT == W_FP4 ? 4 * i + (l >> 4) : 2 * i + (l >> 5);
+  };
   auto chunk_of = [&](int i) { return WT == W_BF16 ? chunk8(i) : WT == W_FP4 ? chunk16(i) : chunk32(i); };
 
   // the issuing end
@@ -304,8 +306,9 @@ __device__ __forceinline__ void stream_items(char* ring, int first, int step, in
               if (more) issue(slot);
               else --ahead;
             };
-            if constexpr (WT == W_FP4) consume_tiles<BL, NT, R::kRows>(acc, st, R::kExps, st + R::kRowsAt, cs, left, free);
-            else consume_halves<R::kRows>(acc[0][0], st, R::kExps, st + R::kRowsAt, cs, left, free);
+            const char* rows_at = st + R::kRowsAt;
+            if constexpr (WT == W_FP4) consume_tiles<BL, NT, R::kRows>(acc, st, R::kExps, rows_at, cs, left, free);
+            else consume_halves<R::kRows>(acc[0][0], st, R::kExps, rows_at, cs, left, free);
           }
           slot = slot == NS - 1 ? 0 : slot + 1;
         }
@@ -352,9 +355,10 @@ __device__ __forceinline__ void set_load(Item<BL>& c, int b, const Weights& m, i
 }
 
 // The KS partial sums of row pairs (two blocks each), added in order: MR token rows at
-// a time (13 rows of 1000 x 1440 in 4 bits: 4 at a time 10.5 us, 16 6.7), two rounds of LDS in turn (a round is read before the next one's
-// barrier and written after it).  emit(item, r, i, quad, v0, v1): rows 4 quad .. + 3
-// of the blocks of the workgroup's pair r, token row i.  Every wave calls it.
+// a time (13 rows of 1000 x 1440 in 4 bits: 4 at a time 10.5 us, 16 6.7), two rounds of
+// LDS in turn (a round is read before the next one's barrier and written after it).
+// emit(item, r, i, quad, v0, v1): rows 4 quad .. + 3 of the blocks of the workgroup's
+// pair r, token row i.  Every wave calls it.
 constexpr int meet_bytes(int rows) { return 2 * rows * kWaves * 128; }
 template <int MR, int BL, int NT, class Emit>
 __device__ __forceinline__ void meet_pairs(char* lds, int& turn, int log_ks, const Item<BL>& c, int c0, int rows,
@@ -427,7 +431,8 @@ using TailRing = Ring<W_FP4, 2, kTailNB, kTailNS>;
 // the workgroup (a wave with none takes part with any blocks, its sums dropped).
 // emit(item, i, quad, v0, v1): rows 4 quad .. + 3 of the item's pair, token row i.
 template <int NR, int NS, class ItemOf, class Origin, class Src, class Emit>
-__device__ __forceinline__ void lock_items(char* ring, int all, int stages, ItemOf item_of_pair, Origin origin, Src src, Emit emit) {
+__device__ __forceinline__ void lock_items(char* ring, int all, int stages, ItemOf item_of_pair, Origin origin, Src src,
+                                           Emit emit) {
   using namespace dma;
   using L = Lock<NR, NS>;
   constexpr int NT = L::NT;
@@ -503,8 +508,9 @@ __device__ __forceinline__ void lock_items(char* ring, int all, int stages, Item
         const char* st = ring + slot * L::kBytes;
         const int left = c.K - cs * 128;
         const char *mine = st + w * L::kMine, *shared = st + L::kRowsAt;
-        if (tiles <= NT / 2) consume_tiles<2, NT / 2, L::kRows>(acc, mine, 2048, shared, cs, left, []() __attribute__((always_inline)) {});
-        else consume_tiles<2, NT, L::kRows>(acc, mine, 2048, shared, cs, left, []() __attribute__((always_inline)) {});
+        auto free = []() __attribute__((always_inline)) {};
+        if (tiles <= NT / 2) consume_tiles<2, NT / 2, L::kRows>(acc, mine, 2048, shared, cs, left, free);
+        else consume_tiles<2, NT, L::kRows>(acc, mine, 2048, shared, cs, left, free);
         slot = slot == NS - 1 ? 0 : slot + 1;
       }
       if (c.live) {

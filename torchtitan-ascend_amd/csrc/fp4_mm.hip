@@ -8,6 +8,20 @@
 // Measured: 1 x 5120 x 8192 9.8 us (22 MB; 160 workgroups have rows), 13 x 1000 x 1440
 // 6.7, 96 rows of 68 of 128 matrices of 1536 x 2048 31.7 (114 MB, 4.5 TB/s between
 // start and end).
+//
+// A pass's token rows are 4, 8, 16, 32 or 64, chosen on the host from the rows that a
+// matrix gets on average; a matrix with more streams its weights again for every pass.
+// Both sides (captured, us, about 6 of them the graph's launch):
+//   grouped, 128 of 1536 x 2048    4 / 8 rows a pass, average 2: 48 / 42, 3: 61 / 48;
+//                                  8 / 32, 4: 52 / 50, 5: 57 / 53; 32 / 64, 24: 71 / 65, 32:
+//                                  93 / 76, 40: 102 / 78 (the hottest matrix has 1.5 times that)
+//   dense, 5120 x 8192             4 / 8, 2 to 4 rows: equal; 8 / 16, 9: 19 / 17; 16 / 32 in
+//                                  lock step, 16: 18 / 50, 17: 20 / 57; 16 / 64, 64: 28 / 87, 128:
+//                                  46 / 87; 16384 x 2048, 17: 19 / 21, 64: 19 / 29, 128: 33 / 30
+// so the lock step loses above 16 dense rows where N / 256 workgroups leave CUs idle,
+// and at 24 to 32 grouped ones.  A skewed load pays for the average: 200 rows of 128
+// matrices 47 us spread evenly, 197 with 96 of them on one; 4096 rows of 1024 matrices
+// of 256 x 512 20 us, 536 on one.
 #include <algorithm>
 
 #include "decode_stream.h"

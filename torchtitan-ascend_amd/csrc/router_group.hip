@@ -28,7 +28,7 @@
 //
 // What bounds it: few tokens, the latency of one launch (4 us); many tokens,
 // VALU issue (1140 instructions per wave of four tokens at E = 256, K = 8: 8 of
-// 13.6 us at 16384 tokens), not the logits' bytes (3.4 us).  The bias is 4 of
+// 13.6 us at 16384 tokens in a stream of launches), not the logits' bytes (3.4 us).  The bias is 4 of
 // the 13.6: a load per expert and lane, 88 instructions.  On the gate GEMM's
 // partials, with the histogram, 22 us.
 #include <type_traits>

@@ -41,20 +41,20 @@ class PackedWeights(NamedTuple):
     cols: int  # K
 
 
-_tracing, _mode = torch._C._get_tracing_state, torch._C._get_dispatch_mode
+_tracing, _mode = torch._C._is_tracing, torch._C._get_dispatch_mode
 _included, _mode_count = torch._C._dispatch_tls_is_dispatch_key_included, torch._C._len_torch_dispatch_stack
 _PRE_DISPATCH, _PROXY = torch._C.DispatchKey.PreDispatch, torch._C._TorchDispatchModeKey.PROXY
 
 
 def _seen() -> bool:
     """Whether a tracer or another dispatch mode is at work."""
-    return _mode_count() > 0 or _tracing() is not None or _included(_PRE_DISPATCH)
+    return _mode_count() > 0 or _tracing() or _included(_PRE_DISPATCH)
 
 
 def _direct(name: str) -> None:
     """Refuse a call under torch.jit.trace or make_fx, whose recording would hold the
     outputs' allocation and not the kernels."""
-    if _seen() and (_tracing() is not None or _included(_PRE_DISPATCH) or _mode(_PROXY) is not None):
+    if _seen() and (_tracing() or _included(_PRE_DISPATCH) or _mode(_PROXY) is not None):
         raise RuntimeError(f"decode.{name} cannot be recorded by a tracer: call functional.{name}")
 
 
@@ -149,9 +149,9 @@ def grouped_mm_e2m1(
     """out[m] = x[m] @ w[e]^T (+ bias) with 4-bit weights (ttamd_grouped_mm_e2m1):
     x bf16 [M, K] (without offs also [..., K]); expert e's rows end at offs[e]
     (int32 [E]) as in grouped_mm, or all rows take the one matrix of w.  bias [N]
-    bf16 or fp32, without offs.  For few rows: every 64 of an expert read its
-    weights again, so a prompt takes unpack_e2m1 and a matrix product.  Rows at or
-    past offs[-1] are not written."""
+    bf16 or fp32, without offs.  For few rows: an expert with more rows than a pass
+    holds (4 to 64, by the average) reads its weights again, so a prompt takes
+    unpack_e2m1 and a matrix product.  Rows at or past offs[-1] are not written."""
     dev = _gpu("x", x)
     _direct("grouped_mm_e2m1")
     _no_grad("grouped_mm_e2m1", x, bias)

@@ -442,9 +442,9 @@ def moe_decode(
     int64 [T, K]); arguments as decode.moe_decode.  At most 64 tokens stream the
     weights (decode.moe_decode; under a tracer ttamd::moe_decode); a prompt takes
     the router, the grouped GEMMs and the shared expert's pass, 4-bit weights
-    restored to bf16 for the call (D % 128 == 0 and H % 128 == 0 there).  The two sum
-    a logit in other orders, so tokens whose experts nearly tie may pick others.  No
-    backward."""
+    restored to bf16 for the call (D % 128 == 0 and H % 64 == 0 there, a shared
+    expert's H too).  The two sum a logit in other orders, so tokens whose experts
+    nearly tie may pick others.  No backward."""
     decode._no_grad("moe_decode", x, w_router, w13, w2, shared_w13, shared_w2, shared_gate)
     if x.dim() != 2 or x.dtype != _BF16:
         raise TypeError(f"x must be bfloat16 [T, D], got {x.dtype} {tuple(x.shape)}")
