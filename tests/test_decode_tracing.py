@@ -197,11 +197,12 @@ def test_layers_refuse_weights_on_another_device(tokens):
 def test_layers_take_and_refuse_the_same_forms_of_weights(library, tokens):
     t = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
     x, wr, w13, w2, s13, s2 = t(tokens, D), t(1, D), t(2 * H, D), t(D, H), t(64, D), t(D, 32)
-    p13, p2, q13, q2 = packed("cpu", 1, 2 * H, D), packed("cpu", 1, D, H), packed("cpu", 1, 64, D), packed("cpu", 1, D, 32)
+    p13, p2, q13, q2 = (packed("cpu", 1, *s) for s in ((2 * H, D), (D, H), (64, D), (D, 32)))
     with torch.no_grad():
         for w in ((w13, w2), (w13[None], w2), (p13, p2)):  # [N, K] is one expert
             shared = (q13, q2) if w[0] is p13 else (s13, s2[None])
-            assert functional.moe_decode(x, wr, *w, 1, shared_w13=shared[0], shared_w2=shared[1])[0].shape == (tokens, D)
+            out = functional.moe_decode(x, wr, *w, 1, shared_w13=shared[0], shared_w2=shared[1])[0]
+            assert out.shape == (tokens, D)
         for w in ((p13, w2), (w13, p2)):
             with pytest.raises(TypeError, match="both be bfloat16"):
                 functional.moe_decode(x, wr, *w, 1)

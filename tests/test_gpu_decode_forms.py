@@ -232,7 +232,8 @@ def call(name, *args):
 
 
 @pytest.mark.parametrize("counts,N,K", [
-    ([1], 40, 64), ([0, 3, 0, 1], 97, 1056), ([5, 0, 17, 64, 65, 2], 131, 512), ([0, 0, 0], 32, 32), ([1] * 60, 1536, 2048),
+    ([1], 40, 64), ([0, 3, 0, 1], 97, 1056), ([5, 0, 17, 64, 65, 2], 131, 512), ([0, 0, 0], 32, 32),
+    ([1] * 60, 1536, 2048),
     ([200, 1, 300], 31, 160), ([2] * 20, 18, 96), ([4, 3] * 8, 50, 288), ([30] * 5, 75, 544), ([100], 1003, 128)])
 @pytest.mark.parametrize("past", [0, 1, 5, 70])
 def test_rows_behind_the_last_run_stay(decode, counts, N, K, past):
@@ -265,8 +266,8 @@ def test_offsets_out_of_order_leave_rows(decode):
                        ([2 ** 31 - 1, -2 ** 31, 1, 3, 3], {0: (0, 12), 2: (0, 1), 3: (1, 3)})):
         announce(f"offsets {offs}")
         out = Guarded((M, N), BF16)
-        call("ttamd_grouped_mm_e2m1", x, p.codes, p.exponents, torch.tensor(offs, dtype=torch.int32, device=DEV), None, 0,
-             M, E, N, K, out.t)
+        ends = torch.tensor(offs, dtype=torch.int32, device=DEV)
+        call("ttamd_grouped_mm_e2m1", x, p.codes, p.exponents, ends, None, 0, M, E, N, K, out.t)
         rows = sorted({r for a, b in runs.values() for r in range(a, b)})
         out.check(rows)
         for e, (a, b) in runs.items():  # (rows of two runs hold either's)
@@ -275,8 +276,8 @@ def test_offsets_out_of_order_leave_rows(decode):
                 check_product(x[own], w[e], out.t[own])
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 5121, 160), (3, 17, 96), (13, 1001, 1440), (16, 33, 512), (17, 31, 288),
-                                   (40, 65, 96), (64, 15, 1056), (100, 130, 128)])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 5121, 160), (3, 17, 96), (13, 1001, 1440), (16, 33, 512),
+                                   (17, 31, 288), (40, 65, 96), (64, 15, 1056), (100, 130, 128)])
 def test_dense_products_write_their_rows_alone(decode, M, N, K):
     rng = np.random.default_rng(M + N)
     x, p, b = weights(rng, M, K, scale=1.0), decode.pack_e2m1(weights(rng, N, K)), Guarded((N,), BF16, 0x7F)
@@ -319,8 +320,8 @@ def test_the_layer_writes_its_rows_and_its_workspace_alone(decode, T, E, K, D, H
     out, scores, idx = Guarded((T, D), BF16), Guarded((T, K), torch.float32), Guarded((T, K), torch.int64)
     nbytes = lib.ttamd_moe_decode_workspace_bytes(T, D, H, E, K, shared)
     ws = Guarded((nbytes,), torch.uint8)
-    call("ttamd_moe_decode", x, T, D, H, E, K, wr, None, 1, 1, 0, 0, 0, 1e-20, 1.0, 0, float("nan"), *tensors[:4], shared,
-         *tensors[4:], None, scores.t, idx.t, out.t, ws.t, nbytes)
+    call("ttamd_moe_decode", x, T, D, H, E, K, wr, None, 1, 1, 0, 0, 0, 1e-20, 1.0, 0, float("nan"), *tensors[:4],
+         shared, *tensors[4:], None, scores.t, idx.t, out.t, ws.t, nbytes)
     for g in (out, scores, idx):
         g.check(slice(0, T))
     ws.check(slice(0, nbytes))
@@ -383,7 +384,8 @@ def test_every_stream(decode, bits, form, before):
 
 
 @pytest.mark.parametrize("T,E,K,groups", [
-    (61, 8, 1, None), (9, 64, 12, None), (32, 128, 8, None), (32, 128, 12, (4, 2)), (20, 160, 6, (8, 3)), (20, 192, 16, None),
+    (61, 8, 1, None), (9, 64, 12, None), (32, 128, 8, None), (32, 128, 12, (4, 2)), (20, 160, 6, (8, 3)),
+    (20, 192, 16, None),
     (17, 256, 8, (8, 4)), (17, 256, 16, None), (9, 200, 8, (8, 4)), (9, 256, 16, (64, 20)), (5, 300, 4, (3, 2)),
     (5, 512, 16, None), (33, 1024, 8, (64, 7)), (33, 1024, 16, None), (7, 990, 8, (33, 4)), (64, 1023, 16, (33, 20)),
     (2, 961, 3, (31, 1)), (64, 63, 3, (63, 5)),
