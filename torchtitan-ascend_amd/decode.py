@@ -51,18 +51,20 @@ def _seen() -> bool:
     return _mode_count() > 0 or _tracing() or _included(_PRE_DISPATCH)
 
 
-def _direct(name: str) -> None:
-    """Refuse a call under torch.jit.trace or make_fx, whose recording would hold the
-    outputs' allocation and not the kernels."""
-    if _seen() and (_tracing() or _included(_PRE_DISPATCH) or _mode(_PROXY) is not None):
-        raise RuntimeError(f"decode.{name} cannot be recorded by a tracer: call functional.{name}")
-
-
 def _no_grad(name: str, *tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
-            if t is not None and getattr(t, "requires_grad", False):
+            if t is not None and type(t) is not PackedWeights and getattr(t, "requires_grad", False):
                 raise RuntimeError(f"{name} is for inference (it has no backward); call it under torch.no_grad()")
+
+
+def _direct(name: str, *tensors) -> None:
+    """Refuse a call under torch.jit.trace or make_fx, whose recording would hold the
+    outputs' allocation and not the kernels, and one that asks for gradients."""
+    if (_mode_count() or _tracing() or _included(_PRE_DISPATCH)) and (
+            _tracing() or _included(_PRE_DISPATCH) or _mode(_PROXY) is not None):
+        raise RuntimeError(f"decode.{name} cannot be recorded by a tracer: call functional.{name}")
+    _no_grad(name, *tensors)
 
 
 def _shapes(E: int, N: int, K: int) -> tuple[tuple, tuple]:
@@ -93,8 +95,7 @@ def pack_e2m1(w: torch.Tensor) -> PackedWeights:
     magnitude, or within 2^-2 of a 32-column group's scale where that is more.
     A group that holds a NaN or an infinity becomes NaN."""
     dev = _gpu("w", w)
-    _direct("pack_e2m1")
-    _no_grad("pack_e2m1", w)
+    _direct("pack_e2m1", w)
     if w.dim() not in (2, 3):
         raise ValueError(f"w must be [E, N, K] or [N, K], got {tuple(w.shape)}")
     if w.dtype not in (_BF16, torch.float32):
@@ -102,9 +103,9 @@ def pack_e2m1(w: torch.Tensor) -> PackedWeights:
     w = w.contiguous()
     E, (N, K) = (w.shape[0] if w.dim() == 3 else 1), w.shape[-2:]
     codes_shape, exps_shape = _shapes(E, N, K)
-    codes = torch.empty(codes_shape, dtype=torch.uint8, device=dev)
-    exps = torch.empty(exps_shape, dtype=torch.uint8, device=dev)
-    _call(dev, "ttamd_pack_e2m1", _p(w), int(w.dtype == torch.float32), E, N, K, _p(codes), _p(exps), _stream(dev))
+    codes, exps = w.new_empty(codes_shape, dtype=_U8), w.new_empty(exps_shape, dtype=_U8)
+    _call(dev, "ttamd_pack_e2m1", w.data_ptr(), 1 if w.dtype is torch.float32 else 0, E, N, K, codes.data_ptr(),
+          exps.data_ptr(), _stream(dev))
     return PackedWeights(codes, exps, N, K)
 
 
@@ -114,8 +115,9 @@ def unpack_e2m1(w: PackedWeights) -> torch.Tensor:
     dev = _gpu("w.codes", w.codes)
     _direct("unpack_e2m1")
     codes, exps, E = _packed("w", w, dev)
-    out = torch.empty(E, w.rows, w.cols, dtype=_BF16, device=dev)
-    _call(dev, "ttamd_unpack_e2m1", _p(codes), _p(exps), E, w.rows, w.cols, _p(out), _stream(dev))
+    out = codes.new_empty((E, w.rows, w.cols), dtype=_BF16)
+    _call(dev, "ttamd_unpack_e2m1", codes.data_ptr(), exps.data_ptr(), E, w.rows, w.cols, out.data_ptr(),
+          _stream(dev))
     return out
 
 
@@ -153,8 +155,7 @@ def grouped_mm_e2m1(
     holds (4 to 64, by the average) reads its weights again, so a prompt takes
     unpack_e2m1 and a matrix product.  Rows at or past offs[-1] are not written."""
     dev = _gpu("x", x)
-    _direct("grouped_mm_e2m1")
-    _no_grad("grouped_mm_e2m1", x, bias)
+    _direct("grouped_mm_e2m1", x, bias)
     x = _want("x", x, _BF16)
     codes, exps, E = _packed("w", w, dev)
     N, K = w.rows, w.cols
@@ -273,8 +274,7 @@ def router_decode(
     ops.router_topk's with groups (one group without num_groups).  shared_gate [1,
     D] bf16: gate = sigmoid of the token's bf16 product with it."""
     dev = _gpu("x", x)
-    _direct("router_decode")
-    _no_grad("router_decode", x, w_router, shared_gate)
+    _direct("router_decode", x, w_router, shared_gate)
     x = _rows(x)
     w_router = _want("w_router", w_router, _BF16)
     _same_device(dev, w_router=w_router)
@@ -315,8 +315,7 @@ def experts_decode(
     packed.  A shared expert [2Hs, D] / [D, Hs] is added times shared_scale fp32 [T]
     (None: 1)."""
     dev = _gpu("x", x)
-    _direct("experts_decode")
-    _no_grad("experts_decode", x, top_scores, w13, w2, shared_w13, shared_w2, shared_scale)
+    _direct("experts_decode", x, top_scores, w13, w2, shared_w13, shared_w2, shared_scale)
     x = _rows(x)
     T, D = x.shape
     idx = selected_experts_indices
@@ -368,8 +367,7 @@ def moe_decode(
     experts_decode; shared_gate [1, D] scales the shared expert by sigmoid(x .
     shared_gate)."""
     dev = _gpu("x", x)
-    _direct("moe_decode")
-    _no_grad("moe_decode", x, w_router, w13, w2, shared_w13, shared_w2, shared_gate)
+    _direct("moe_decode", x, w_router, w13, w2, shared_w13, shared_w2, shared_gate)
     x = _rows(x)
     T, D = x.shape
     E, H, Hs, weights, shared, _keep = _experts(w13, w2, shared_w13, shared_w2, D, dev)
