@@ -246,25 +246,39 @@ def test_modes_and_subclasses_see_the_ops(library):
     assert library.names == ["ttamd_moe_decode"] and not mode.names[1:]
 
 
-def test_direct_calls_refuse_to_be_recorded(library):
-    x, wr = torch.zeros(9, D, dtype=BF16), torch.zeros(E, D, dtype=BF16)
+def direct_calls():
+    wr = torch.zeros(E, D, dtype=BF16)
     w = torch.zeros(E, 2 * H, D, dtype=BF16), torch.zeros(E, D, H, dtype=BF16)
     q = packed("cpu", 1, 2 * H, D)
     idx, scores = torch.zeros(9, K, dtype=torch.int64), torch.zeros(9, K)
-    for name, fn in {
+    return {
         "moe_decode": lambda x: decode.moe_decode(x, wr, *w, K)[0],
         "experts_decode": lambda x: decode.experts_decode(x, scores, idx, *w),
         "router_decode": lambda x: decode.router_decode(x, wr, K)[0],
         "grouped_mm_e2m1": lambda x: decode.grouped_mm_e2m1(x, q),
         "pack_e2m1": lambda x: decode.pack_e2m1(x).codes,
         "unpack_e2m1": lambda x: decode.unpack_e2m1(q),
-    }.items():
+    }
+
+
+def test_direct_calls_refuse_to_be_recorded(library):
+    x = torch.zeros(9, D, dtype=BF16)
+    for name, fn in direct_calls().items():
         with torch.no_grad():
             for trace in (make_fx(fn), make_fx(fn, pre_dispatch=True),
                           lambda x: torch.jit.trace(fn, (x,), check_trace=False)):
                 with pytest.raises(RuntimeError, match=f"functional.{name}"):
                     trace(x)
             fn(x)
+
+
+@pytest.mark.parametrize("name", list(direct_calls()))
+def test_direct_calls_end_a_compiled_graph(library, name):
+    fn = direct_calls()[name]
+    with torch.no_grad():
+        out = torch.compile(lambda x: fn(x + 1).float() + 1, backend="aot_eager")(torch.zeros(9, D, dtype=BF16))
+    torch._dynamo.reset()
+    assert library.names == [f"ttamd_{name}"] and out.dtype == F32
 
 
 @pytest.mark.parametrize("shape", [(9,), (3, 3), (1, 9), (0, 4)])

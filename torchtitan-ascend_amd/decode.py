@@ -61,7 +61,9 @@ def _no_grad(name: str, *tensors) -> None:
 def _direct(name: str, *tensors) -> None:
     """Refuse a call under torch.jit.trace or make_fx, whose recording would hold the
     outputs' allocation and not the kernels, and one that asks for gradients."""
-    if (_mode_count() or _tracing() or _included(_PRE_DISPATCH)) and (
+    if torch.compiler.is_dynamo_compiling():
+        pass  # (the graph ends in front of the C call)
+    elif (_mode_count() or _tracing() or _included(_PRE_DISPATCH)) and (
             _tracing() or _included(_PRE_DISPATCH) or _mode(_PROXY) is not None):
         raise RuntimeError(f"decode.{name} cannot be recorded by a tracer: call functional.{name}")
     _no_grad(name, *tensors)
